@@ -176,16 +176,20 @@ def prepare(c, seed):
 
 def _scale(amax, fmt):
     """fp32 scale of a block whose largest magnitude is amax."""
-    if fmt == "int8":
-        return (amax / 127.0).clamp(_LEAST, 1.0 / _LEAST)
+    if fmt == "int8":                             # a correctly rounded quotient
+        return (amax.double() / 127.0).float().clamp(_LEAST, 1.0 / _LEAST)
     m, e = torch.frexp(amax)                      # amax = m 2^e, m in [1/2, 1): m 2^9 <= 448 for m <= 7/8
     e = torch.where(m <= 0.875, e - 9, e - 8)
     return torch.where(amax > 0, torch.ldexp(torch.ones_like(amax), e), 0.0).clamp(_LEAST, 1.0 / _LEAST)
 
 
+def _inverse(scale):
+    return (1.0 / scale.double()).float()         # correctly rounded
+
+
 def _quantised(x, scale, fmt):
     """Codes (as bytes) of x over blocks of that scale."""
-    inv = 1.0 / scale
+    inv = _inverse(scale)
     if fmt == "int8":                             # the exact product, rounded half to even
         return (x.double() * inv.double()).round().clamp(-127, 127).to(torch.int8).view(torch.uint8)
     return (x.float() * inv).clamp(-448.0, 448.0).to(torch.float8_e4m3fn).view(torch.uint8)
@@ -217,7 +221,7 @@ def _plain_write(s):
         old = s["scales"][:, :, i]
         scale = torch.where(fresh[:, None], _scale(top, fmt), torch.maximum(old, torch.where(top > 0, _scale(top, fmt), 0.0)))
         # earlier tokens of a sequence's first page, under the page's new scale
-        ratio = (old * (1.0 / scale))[first][(...,) + (None,) * (codes.dim() - 2)]
+        ratio = (old * _inverse(scale))[first][(...,) + (None,) * (codes.dim() - 2)]
         was = codes[first]
         if fmt == "int8":
             now = (_values(was, fmt).double() * ratio.double()).round().clamp(-127, 127).to(torch.int8).view(torch.uint8)
