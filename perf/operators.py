@@ -183,16 +183,11 @@ def _scale(amax, fmt):
     return torch.where(amax > 0, torch.ldexp(torch.ones_like(amax), e), 0.0).clamp(_LEAST, 1.0 / _LEAST)
 
 
-def _inverse(scale):
-    return (1.0 / scale.double()).float()         # correctly rounded
-
-
 def _quantised(x, scale, fmt):
-    """Codes (as bytes) of x over blocks of that scale."""
-    inv = _inverse(scale)
-    if fmt == "int8":                             # the exact product, rounded half to even
-        return (x.double() * inv.double()).round().clamp(-127, 127).to(torch.int8).view(torch.uint8)
-    return (x.float() * inv).clamp(-448.0, 448.0).to(torch.float8_e4m3fn).view(torch.uint8)
+    """Codes (as bytes) of x over blocks of that scale: the nearest to the exact quotient."""
+    if fmt == "int8":
+        return (x.double() / scale.double()).round().clamp(-127, 127).to(torch.int8).view(torch.uint8)
+    return (x.float() / scale).clamp(-448.0, 448.0).to(torch.float8_e4m3fn).view(torch.uint8)
 
 
 def _values(codes, fmt):
@@ -221,14 +216,11 @@ def _plain_write(s):
         old = s["scales"][:, :, i]
         scale = torch.where(fresh[:, None], _scale(top, fmt), torch.maximum(old, torch.where(top > 0, _scale(top, fmt), 0.0)))
         # earlier tokens of a sequence's first page, under the page's new scale
-        ratio = (old * _inverse(scale))[first][(...,) + (None,) * (codes.dim() - 2)]
+        wide = (...,) + (None,) * (codes.dim() - 2)
         was = codes[first]
-        if fmt == "int8":
-            now = (_values(was, fmt).double() * ratio.double()).round().clamp(-127, 127).to(torch.int8).view(torch.uint8)
-        else:
-            now = (_values(was, fmt) * ratio).clamp(-448.0, 448.0).to(torch.float8_e4m3fn).view(torch.uint8)
+        now = _quantised(_values(was, fmt).double() * old[first][wide].double(), scale[first][wide], fmt)
         grown = (scale > old)[first] & ~fresh[first][:, None]
-        codes[first] = torch.where(grown[(...,) + (None,) * (codes.dim() - 2)], now, was)
+        codes[first] = torch.where(grown[wide], now, was)
         y = _quantised(x, scale[page][:, :, None], fmt)
         if i == 0:
             codes[page, :, slot] = y
@@ -356,7 +348,7 @@ def _rounded(y, fmt):
 
 def _exact_scale(a, fmt):
     s = a / 127 if fmt == "int8" else 2.0 ** torch.ceil(torch.log2(a.clamp(min=1e-300) / 448))
-    return s.clamp(_LEAST, 1 / _LEAST)
+    return s.clamp(_LEAST, 1 / _LEAST).float().double()      # a scale is an fp32 number
 
 
 def exact(c, seed):
