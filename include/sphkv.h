@@ -627,6 +627,110 @@ int32_t sphkv_work_pool_rows_per_item(const int32_t* row_start, int32_t num_sh, 
 int64_t sphkv_work_fill(const int32_t* row_start, int32_t num_sh, int32_t rows_per_item, int32_t interleave,
                         int32_t* work, int64_t max_items, int32_t* work_start);
 
+/*
+ * ---- 8-bit KV cache --------------------------------------------------------
+ * Keys and values as 8-bit codes in pages of page_size consecutive tokens of a
+ * sequence, with one fp32 scale per (page, kv head) for the keys and one for
+ * the values.  No reference counterpart: the reference stores keys as angle
+ * codes and values as fp16 (pagebuilder.py:8-42).  Keys are stored as given:
+ * RoPE is the caller's, as on the LayerPool path.
+ *
+ *   k_codes   uint8 [num_pages, num_kv, page_size, dh]
+ *   v_codes   uint8 [num_pages, num_kv, page_size/16, dh, 16]  (token-minor in
+ *             runs of 16 tokens)
+ *   scales    fp32 [num_pages, num_kv, 2]: the keys' and the values'
+ *   table     int32 [num_seqs, max_blocks], rows table_stride apart: the page
+ *             of each page_size tokens of a sequence.  A page outside
+ *             [0, num_pages) holds no token: nothing is written to it, it reads
+ *             as zeros and attention passes over it.
+ *   fmt       SPHKV_CACHE8_INT8: codes -127..127; SPHKV_CACHE8_E4M3: OCP fp8
+ *   types     SPHKV_FP16, SPHKV_BF16, SPHKV_FP32
+ * dh 64 or 128; page_size 16, 32, 64 or 128; max_blocks * page_size <= 2^30.
+ * k_codes, v_codes and scales 16-byte aligned.  Rows of k, v and q may have any
+ * row and head stride and alignment, their dh elements are contiguous (strides
+ * in elements).
+ *
+ * A token's code is the nearest to x / scale, half to even.  With a the largest
+ * finite magnitude among a (page, head)'s tokens, the scale is
+ *   int8   a / 127, correctly rounded;   e4m3   the least power of two with
+ *   a / scale <= 448;   both within [2^-60, 2^60] (beyond, values saturate).
+ * A NaN is stored as 0, an infinity as the largest code of its sign.
+ */
+#define SPHKV_CACHE8_INT8 0
+#define SPHKV_CACHE8_E4M3 1
+#define SPHKV_FP16 0
+#define SPHKV_BF16 1
+#define SPHKV_FP32 2
+
+/*
+ * Quantise new tokens into their pages.  k, v [num_rows, num_kv, dh] of
+ * in_type.  Sequence s's new tokens are rows cu_rows[s] .. cu_rows[s+1] - 1
+ * (cu_rows int32 [num_seqs + 1], cu_rows[0] = 0, non-decreasing; NULL: row s,
+ * one token each, num_rows = num_seqs) at positions start[s], start[s] + 1, ...
+ * Rows from cu_rows[num_seqs] on are not read; a token past the table, of a
+ * negative start or of an absent page is dropped.
+ *
+ * A page whose first slot is among the new tokens starts over: its scales are
+ * those of its new tokens.  Another page keeps its scale if that is enough for
+ * the new tokens; otherwise it gets theirs and the codes of its earlier tokens
+ * (slots before start[s]) become the nearest to code * old / new.  Slots past a
+ * sequence's last new token keep their bytes.  A written page belongs to one
+ * sequence (pages that several share may be read, not written).
+ */
+int sphkv_cache8_write(const void* k, const void* v, int32_t in_type, int64_t k_row_stride, int64_t k_head_stride,
+                       int64_t v_row_stride, int64_t v_head_stride, int64_t num_rows, const int32_t* cu_rows,
+                       const int32_t* start, const int32_t* table, int64_t table_stride, int32_t max_blocks,
+                       int32_t num_seqs, uint8_t* k_codes, uint8_t* v_codes, float* scales, int64_t num_pages,
+                       int32_t num_kv, int32_t dh, int32_t page_size, int32_t fmt, void* stream);
+
+/*
+ * Read tokens back: the fp32 product code * scale, rounded to out_type.  k_out, v_out
+ * [num_rows, num_kv, dh] contiguous, either may be NULL; rows and positions as
+ * sphkv_cache8_write's (cu_rows NULL: one token each).  Rows from
+ * cu_rows[num_seqs] on keep their contents; a token past the table, of a
+ * negative position or of an absent page is zeros.
+ */
+int sphkv_cache8_read(const uint8_t* k_codes, const uint8_t* v_codes, const float* scales, int64_t num_pages,
+                      int32_t num_kv, int32_t dh, int32_t page_size, int32_t fmt, const int32_t* cu_rows,
+                      const int32_t* start, const int32_t* table, int64_t table_stride, int32_t max_blocks,
+                      int32_t num_seqs, int64_t num_rows, void* k_out, void* v_out, int32_t out_type, void* stream);
+
+/*
+ * Attention of one query token per sequence over its first lens[s] tokens
+ * (its own among them, if it was written; lengths beyond the table count as the
+ * table's, negative ones as 0):
+ *   out = sum_t softmax_t(sm_scale <q, k_t>) v_t,  lse = ln sum_t exp(sm_scale <q, k_t>)
+ * q [num_seqs, num_kv*gqa, dh] fp16 or bf16; out of that type, contiguous; lse
+ * fp32 [num_seqs, num_kv*gqa] or NULL.  A sequence without a token gets zeros
+ * and -inf.  gqa 1..64.  workspace: device scratch of
+ * sphkv_cache8_decode_workspace_bytes() bytes, 16-byte aligned, contents
+ * irrelevant; calls that share one must not run concurrently.
+ */
+int64_t sphkv_cache8_decode_workspace_bytes(int32_t num_seqs, int32_t num_kv, int32_t gqa, int32_t dh);
+int sphkv_cache8_decode(const void* q, int32_t q_type, int64_t q_row_stride, int64_t q_head_stride,
+                        const int32_t* lens, const int32_t* table, int64_t table_stride, int32_t max_blocks,
+                        int32_t num_seqs, const uint8_t* k_codes, const uint8_t* v_codes, const float* scales,
+                        int64_t num_pages, int32_t num_kv, int32_t gqa, int32_t dh, int32_t page_size, int32_t fmt,
+                        float sm_scale, void* out, float* lse, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Attention of several query tokens per sequence, the last ones of its lens[s]
+ * tokens: rows cu_rows[s] + i (cu_rows as sphkv_cache8_write's, not NULL) at
+ * position lens[s] - n_s + i attends the positions up to its own (causal = 1)
+ * or all lens[s] (causal = 0).  A row that attends nothing (a negative
+ * position, an empty sequence) gets zeros and -inf; rows from
+ * cu_rows[num_seqs] on keep their contents.  q, out [num_rows, num_kv*gqa, dh],
+ * lse [num_rows, num_kv*gqa]; the rest as sphkv_cache8_decode.
+ */
+int64_t sphkv_cache8_prefill_workspace_bytes(int64_t num_rows, int32_t num_seqs, int32_t num_kv, int32_t gqa,
+                                             int32_t dh);
+int sphkv_cache8_prefill(const void* q, int32_t q_type, int64_t q_row_stride, int64_t q_head_stride,
+                         int64_t num_rows, const int32_t* cu_rows, const int32_t* lens, int32_t causal,
+                         const int32_t* table, int64_t table_stride, int32_t max_blocks, int32_t num_seqs,
+                         const uint8_t* k_codes, const uint8_t* v_codes, const float* scales, int64_t num_pages,
+                         int32_t num_kv, int32_t gqa, int32_t dh, int32_t page_size, int32_t fmt, float sm_scale,
+                         void* out, float* lse, void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -7,6 +7,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <cmath>
 #include <new>
 
 #include "../../include/sphkv.h"
@@ -1049,6 +1050,156 @@ int64_t sphkv_work_fill(const int32_t* row_start, int32_t num_sh, int32_t rows_p
   work_start[num_sh] = k;
   ok();
   return n;
+}
+
+}  // extern "C"
+
+// ---- 8-bit KV cache ---------------------------------------------------------
+
+namespace {
+
+// checks of what every cache call shares; fills c and b
+int cache8_checks(const char* fn, const uint8_t* k_codes, const uint8_t* v_codes, const float* scales, int64_t num_pages,
+                  int32_t num_kv, int32_t dh, int32_t page_size, int32_t fmt, const int32_t* table,
+                  int64_t table_stride, int32_t max_blocks, int32_t num_seqs, int64_t num_rows, sphkv::Cache8* c) {
+  if (!dh_ok(dh)) return fail(SPHKV_EINVAL, "%s: dh must be 64 or 128 (got %d)", fn, dh);
+  if (page_size != 16 && page_size != 32 && page_size != 64 && page_size != 128)
+    return fail(SPHKV_EINVAL, "%s: page_size must be 16, 32, 64 or 128 (got %d)", fn, page_size);
+  if (fmt != SPHKV_CACHE8_INT8 && fmt != SPHKV_CACHE8_E4M3) return fail(SPHKV_EINVAL, "%s: unknown fmt %d", fn, fmt);
+  if (num_seqs < 0 || num_rows < 0 || num_pages < 0 || max_blocks < 0 || num_kv < 1)
+    return fail(SPHKV_EINVAL, "%s: negative size", fn);
+  if (num_kv > 1024) return fail(SPHKV_EINVAL, "%s: num_kv must be at most 1024 (got %d)", fn, num_kv);
+  if (num_pages > INT32_MAX) return fail(SPHKV_EINVAL, "%s: num_pages exceeds int32", fn);
+  // (rows and sequences of one call: their workgroups fit a grid)
+  if (num_seqs > (1 << 20) || num_rows > (1 << 26))
+    return fail(SPHKV_EINVAL, "%s: at most 2^20 sequences and 2^26 rows", fn);
+  if (((num_rows >> 4) + 2 * (int64_t)num_seqs) * num_kv > (1 << 25))
+    return fail(SPHKV_EINVAL, "%s: (num_rows / 16 + 2 num_seqs) * num_kv exceeds 2^25", fn);
+  if ((int64_t)max_blocks * page_size > (1 << 30))
+    return fail(SPHKV_EINVAL, "%s: max_blocks * page_size exceeds 2^30", fn);
+  if (num_seqs > 1 && table_stride < max_blocks)
+    return fail(SPHKV_EINVAL, "%s: table_stride is less than max_blocks", fn);
+  if (((uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)scales) & 15)
+    return fail(SPHKV_EINVAL, "%s: k_codes, v_codes and scales must be 16-byte aligned", fn);
+  if (num_seqs > 0 && num_pages > 0 && (!k_codes || !v_codes || !scales))
+    return fail(SPHKV_EINVAL, "%s: null pointer argument", fn);
+  if (num_seqs > 0 && max_blocks > 0 && !table) return fail(SPHKV_EINVAL, "%s: null pointer argument", fn);
+  int shift = 4;
+  while ((1 << shift) < page_size) ++shift;
+  *c = {const_cast<uint8_t*>(k_codes), const_cast<uint8_t*>(v_codes), const_cast<float*>(scales), num_pages, num_kv, dh,
+        shift, fmt};
+  return SPHKV_OK;
+}
+
+int cache8_attend(const char* fn, bool decode, const void* q, int32_t q_type, int64_t q_row_stride,
+                  int64_t q_head_stride, int64_t num_rows, const int32_t* cu_rows, const int32_t* lens, int32_t causal,
+                  const int32_t* table, int64_t table_stride, int32_t max_blocks, int32_t num_seqs,
+                  const uint8_t* k_codes, const uint8_t* v_codes, const float* scales, int64_t num_pages,
+                  int32_t num_kv, int32_t gqa, int32_t dh, int32_t page_size, int32_t fmt, float sm_scale, void* out,
+                  float* lse, void* workspace, int64_t workspace_bytes, void* stream) {
+  sphkv::Cache8 c;
+  if (int rc = cache8_checks(fn, k_codes, v_codes, scales, num_pages, num_kv, dh, page_size, fmt, table, table_stride,
+                             max_blocks, num_seqs, num_rows, &c))
+    return rc;
+  if (gqa < 1 || gqa > sphkv::kCache8MaxGqa)
+    return fail(SPHKV_EINVAL, "%s: gqa must be in [1, %d] (got %d)", fn, sphkv::kCache8MaxGqa, gqa);
+  if (q_type != SPHKV_FP16 && q_type != SPHKV_BF16)
+    return fail(SPHKV_EINVAL, "%s: q must be fp16 or bf16 (type %d)", fn, q_type);
+  if (causal != 0 && causal != 1) return fail(SPHKV_EINVAL, "%s: causal must be 0 or 1 (got %d)", fn, causal);
+  if (!(sm_scale > 0.f) || !std::isfinite(sm_scale))
+    return fail(SPHKV_EINVAL, "%s: sm_scale must be positive and finite", fn);
+  if (num_rows * num_kv * gqa > (1LL << 31) - 1)
+    return fail(SPHKV_EINVAL, "%s: more than 2^31 - 1 (row, head) pairs", fn);
+  if (num_seqs == 0 || num_rows == 0) return ok();
+  if (!q || !lens || !out || (!decode && !cu_rows)) return fail(SPHKV_EINVAL, "%s: null pointer argument", fn);
+  const int64_t need = decode ? sphkv::cache8_decode_ws_bytes(num_seqs, num_kv, gqa, dh)
+                              : sphkv::cache8_prefill_ws_bytes(num_rows, num_seqs, num_kv, gqa, dh);
+  if (need > 0 && (!workspace || workspace_bytes < need))
+    return fail(SPHKV_EINVAL, "%s: workspace needs %lld bytes (got %lld)", fn, (long long)need,
+                (long long)workspace_bytes);
+  if ((uintptr_t)workspace & 15) return fail(SPHKV_EINVAL, "%s: workspace must be 16-byte aligned", fn);
+  sphkv::Cache8AttendLaunch L{c, {cu_rows, lens, table, table_stride, max_blocks, num_seqs, num_rows}, q, q_type,
+                              q_row_stride, q_head_stride, gqa, causal, sm_scale, out, lse, workspace};
+  return launch_status(sphkv::launch_cache8_attend(L, (hipStream_t)stream), fn);
+}
+
+}  // namespace
+
+extern "C" {
+
+int sphkv_cache8_write(const void* k, const void* v, int32_t in_type, int64_t k_row_stride, int64_t k_head_stride,
+                       int64_t v_row_stride, int64_t v_head_stride, int64_t num_rows, const int32_t* cu_rows,
+                       const int32_t* start, const int32_t* table, int64_t table_stride, int32_t max_blocks,
+                       int32_t num_seqs, uint8_t* k_codes, uint8_t* v_codes, float* scales, int64_t num_pages,
+                       int32_t num_kv, int32_t dh, int32_t page_size, int32_t fmt, void* stream) {
+  const char* fn = "sphkv_cache8_write";
+  sphkv::Cache8 c;
+  if (int rc = cache8_checks(fn, k_codes, v_codes, scales, num_pages, num_kv, dh, page_size, fmt, table, table_stride,
+                             max_blocks, num_seqs, num_rows, &c))
+    return rc;
+  if (in_type < SPHKV_FP16 || in_type > SPHKV_FP32) return fail(SPHKV_EINVAL, "%s: unknown type %d", fn, in_type);
+  if (!cu_rows && num_rows != num_seqs)
+    return fail(SPHKV_EINVAL, "%s: without cu_rows there is one row per sequence", fn);
+  if (num_seqs == 0 || num_rows == 0) return ok();
+  if (!k || !v || !start) return fail(SPHKV_EINVAL, "%s: null pointer argument", fn);
+  sphkv::Cache8RowsLaunch L{c, {cu_rows, start, table, table_stride, max_blocks, num_seqs, num_rows},
+                            const_cast<void*>(k), const_cast<void*>(v), in_type, k_row_stride, k_head_stride,
+                            v_row_stride, v_head_stride};
+  return launch_status(sphkv::launch_cache8_write(L, (hipStream_t)stream), fn);
+}
+
+int sphkv_cache8_read(const uint8_t* k_codes, const uint8_t* v_codes, const float* scales, int64_t num_pages,
+                      int32_t num_kv, int32_t dh, int32_t page_size, int32_t fmt, const int32_t* cu_rows,
+                      const int32_t* start, const int32_t* table, int64_t table_stride, int32_t max_blocks,
+                      int32_t num_seqs, int64_t num_rows, void* k_out, void* v_out, int32_t out_type, void* stream) {
+  const char* fn = "sphkv_cache8_read";
+  sphkv::Cache8 c;
+  if (int rc = cache8_checks(fn, k_codes, v_codes, scales, num_pages, num_kv, dh, page_size, fmt, table, table_stride,
+                             max_blocks, num_seqs, num_rows, &c))
+    return rc;
+  if (out_type < SPHKV_FP16 || out_type > SPHKV_FP32) return fail(SPHKV_EINVAL, "%s: unknown type %d", fn, out_type);
+  if (!cu_rows && num_rows != num_seqs)
+    return fail(SPHKV_EINVAL, "%s: without cu_rows there is one row per sequence", fn);
+  if (((uintptr_t)k_out | (uintptr_t)v_out) & 15)
+    return fail(SPHKV_EINVAL, "%s: k_out and v_out must be 16-byte aligned", fn);
+  if (num_seqs == 0 || num_rows == 0 || (!k_out && !v_out)) return ok();
+  if (!start) return fail(SPHKV_EINVAL, "%s: null pointer argument", fn);
+  sphkv::Cache8RowsLaunch L{c, {cu_rows, start, table, table_stride, max_blocks, num_seqs, num_rows}, k_out, v_out,
+                            out_type, (int64_t)num_kv * dh, dh, (int64_t)num_kv * dh, dh};
+  return launch_status(sphkv::launch_cache8_read(L, (hipStream_t)stream), fn);
+}
+
+int64_t sphkv_cache8_decode_workspace_bytes(int32_t num_seqs, int32_t num_kv, int32_t gqa, int32_t dh) {
+  if (num_seqs < 0 || num_kv < 1 || gqa < 1 || gqa > sphkv::kCache8MaxGqa || !dh_ok(dh)) return -1;
+  return sphkv::cache8_decode_ws_bytes(num_seqs, num_kv, gqa, dh);
+}
+
+int sphkv_cache8_decode(const void* q, int32_t q_type, int64_t q_row_stride, int64_t q_head_stride,
+                        const int32_t* lens, const int32_t* table, int64_t table_stride, int32_t max_blocks,
+                        int32_t num_seqs, const uint8_t* k_codes, const uint8_t* v_codes, const float* scales,
+                        int64_t num_pages, int32_t num_kv, int32_t gqa, int32_t dh, int32_t page_size, int32_t fmt,
+                        float sm_scale, void* out, float* lse, void* workspace, int64_t workspace_bytes,
+                        void* stream) {
+  return cache8_attend("sphkv_cache8_decode", true, q, q_type, q_row_stride, q_head_stride, num_seqs, nullptr, lens, 1,
+                       table, table_stride, max_blocks, num_seqs, k_codes, v_codes, scales, num_pages, num_kv, gqa, dh,
+                       page_size, fmt, sm_scale, out, lse, workspace, workspace_bytes, stream);
+}
+
+int64_t sphkv_cache8_prefill_workspace_bytes(int64_t num_rows, int32_t num_seqs, int32_t num_kv, int32_t gqa,
+                                             int32_t dh) {
+  if (num_rows < 0 || num_seqs < 0 || num_kv < 1 || gqa < 1 || gqa > sphkv::kCache8MaxGqa || !dh_ok(dh)) return -1;
+  return sphkv::cache8_prefill_ws_bytes(num_rows, num_seqs, num_kv, gqa, dh);
+}
+
+int sphkv_cache8_prefill(const void* q, int32_t q_type, int64_t q_row_stride, int64_t q_head_stride,
+                         int64_t num_rows, const int32_t* cu_rows, const int32_t* lens, int32_t causal,
+                         const int32_t* table, int64_t table_stride, int32_t max_blocks, int32_t num_seqs,
+                         const uint8_t* k_codes, const uint8_t* v_codes, const float* scales, int64_t num_pages,
+                         int32_t num_kv, int32_t gqa, int32_t dh, int32_t page_size, int32_t fmt, float sm_scale,
+                         void* out, float* lse, void* workspace, int64_t workspace_bytes, void* stream) {
+  return cache8_attend("sphkv_cache8_prefill", false, q, q_type, q_row_stride, q_head_stride, num_rows, cu_rows, lens,
+                       causal, table, table_stride, max_blocks, num_seqs, k_codes, v_codes, scales, num_pages, num_kv,
+                       gqa, dh, page_size, fmt, sm_scale, out, lse, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

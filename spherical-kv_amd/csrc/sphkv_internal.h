@@ -221,5 +221,34 @@ inline int64_t decode_workspace_bytes(int num_items, int gqa, int dh) {
   return (int64_t)num_items * partial_floats(gqa, dh) * 4 + kDecodeStatusBytes;
 }
 
+// 8-bit KV cache (sphkv_kv8.hip): codes in pages of a sequence's tokens, one
+// scale per (page, kv head) for the keys and one for the values.
+constexpr int kCache8Int8 = 0, kCache8E4M3 = 1;
+constexpr int kFp16 = 0, kBf16 = 1, kFp32 = 2;
+constexpr int kCache8MaxGqa = 64;
+struct Cache8 {
+  uint8_t* k; uint8_t* v; float* scales;   // [pages, num_kv, ps, dh], [pages, num_kv, ps/16, dh, 16], [pages, num_kv, 2]
+  int64_t num_pages; int32_t num_kv, dh, page_shift, fmt;
+};
+// where a batch's tokens are: rows cu[s].. of sequence s (cu null: row s) at
+// positions at[s].. (write, read: the first row's; attention: at = lens)
+struct Cache8Batch {
+  const int32_t* cu; const int32_t* at; const int32_t* table; int64_t table_stride;
+  int32_t max_blocks, num_seqs; int64_t num_rows;
+};
+struct Cache8RowsLaunch {                  // write: k, v are read; read: written (either may be null)
+  Cache8 c; Cache8Batch b;
+  void* k; void* v; int32_t type; int64_t k_row, k_head, v_row, v_head;
+};
+struct Cache8AttendLaunch {
+  Cache8 c; Cache8Batch b;                 // decode: cu null, one query row a sequence
+  const void* q; int32_t type; int64_t q_row, q_head; int32_t gqa, causal; float sm_scale;
+  void* out; float* lse; void* ws;
+};
+int launch_cache8_write(const Cache8RowsLaunch& L, hipStream_t stream);
+int launch_cache8_read(const Cache8RowsLaunch& L, hipStream_t stream);
+int launch_cache8_attend(const Cache8AttendLaunch& L, hipStream_t stream);
+int64_t cache8_decode_ws_bytes(int32_t num_seqs, int32_t num_kv, int32_t gqa, int32_t dh);
+int64_t cache8_prefill_ws_bytes(int64_t num_rows, int32_t num_seqs, int32_t num_kv, int32_t gqa, int32_t dh);
 
 }  // namespace sphkv

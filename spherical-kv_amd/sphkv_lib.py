@@ -80,6 +80,15 @@ SIGNATURES = {
     "sphkv_work_rows_per_item": (I32, [P, I32, I32, I32]),
     "sphkv_work_pool_rows_per_item": (I32, [P, I32, I32]),
     "sphkv_work_fill": (I64, [P, I32, I32, I32, P, I64, P]),
+    "sphkv_cache8_write": (ctypes.c_int, [P, P, I32, I64, I64, I64, I64, I64, P, P, P, I64, I32, I32, P, P, P, I64,
+                                          I32, I32, I32, I32, P]),
+    "sphkv_cache8_read": (ctypes.c_int, [P, P, P, I64, I32, I32, I32, I32, P, P, P, I64, I32, I32, I64, P, P, I32, P]),
+    "sphkv_cache8_decode_workspace_bytes": (I64, [I32, I32, I32, I32]),
+    "sphkv_cache8_decode": (ctypes.c_int, [P, I32, I64, I64, P, P, I64, I32, I32, P, P, P, I64, I32, I32, I32, I32,
+                                           I32, F32, P, P, P, I64, P]),
+    "sphkv_cache8_prefill_workspace_bytes": (I64, [I64, I32, I32, I32, I32]),
+    "sphkv_cache8_prefill": (ctypes.c_int, [P, I32, I64, I64, I64, P, P, I32, P, I64, I32, I32, P, P, P, I64, I32, I32,
+                                            I32, I32, I32, F32, P, P, P, I64, P]),
 }
 
 
