@@ -1071,8 +1071,8 @@ int cache8_checks(const char* fn, const uint8_t* k_codes, const uint8_t* v_codes
   if (num_kv > 1024) return fail(SPHKV_EINVAL, "%s: num_kv must be at most 1024 (got %d)", fn, num_kv);
   if (num_pages > INT32_MAX) return fail(SPHKV_EINVAL, "%s: num_pages exceeds int32", fn);
   // (rows and sequences of one call: their workgroups fit a grid)
-  if (num_seqs > (1 << 20) || num_rows > (1 << 26))
-    return fail(SPHKV_EINVAL, "%s: at most 2^20 sequences and 2^26 rows", fn);
+  if (num_seqs > (1 << 16) || num_rows > (1 << 26))
+    return fail(SPHKV_EINVAL, "%s: at most 2^16 sequences and 2^26 rows", fn);
   if (((num_rows >> 4) + 2 * (int64_t)num_seqs) * num_kv > (1 << 25))
     return fail(SPHKV_EINVAL, "%s: (num_rows / 16 + 2 num_seqs) * num_kv exceeds 2^25", fn);
   if ((int64_t)max_blocks * page_size > (1 << 30))
@@ -1108,8 +1108,8 @@ int cache8_attend(const char* fn, bool decode, const void* q, int32_t q_type, in
   if (causal != 0 && causal != 1) return fail(SPHKV_EINVAL, "%s: causal must be 0 or 1 (got %d)", fn, causal);
   if (!(sm_scale > 0.f) || !std::isfinite(sm_scale))
     return fail(SPHKV_EINVAL, "%s: sm_scale must be positive and finite", fn);
-  if (num_rows * num_kv * gqa > (1LL << 31) - 1)
-    return fail(SPHKV_EINVAL, "%s: more than 2^31 - 1 (row, head) pairs", fn);
+  if (num_rows * num_kv * gqa > (decode ? 1 << 25 : (1LL << 31) - 1))
+    return fail(SPHKV_EINVAL, "%s: too many (row, head) pairs", fn);
   if (num_seqs == 0 || num_rows == 0) return ok();
   if (!q || !lens || !out || (!decode && !cu_rows)) return fail(SPHKV_EINVAL, "%s: null pointer argument", fn);
   const int64_t need = decode ? sphkv::cache8_decode_ws_bytes(num_seqs, num_kv, gqa, dh)
@@ -1118,7 +1118,7 @@ int cache8_attend(const char* fn, bool decode, const void* q, int32_t q_type, in
     return fail(SPHKV_EINVAL, "%s: workspace needs %lld bytes (got %lld)", fn, (long long)need,
                 (long long)workspace_bytes);
   if ((uintptr_t)workspace & 15) return fail(SPHKV_EINVAL, "%s: workspace must be 16-byte aligned", fn);
-  sphkv::Cache8AttendLaunch L{c, {cu_rows, lens, table, table_stride, max_blocks, num_seqs, num_rows}, q, q_type,
+  sphkv::Cache8AttendLaunch L{c, {cu_rows, lens, table, table_stride, num_pages > 0 ? max_blocks : 0, num_seqs, num_rows}, q, q_type,
                               q_row_stride, q_head_stride, gqa, causal, sm_scale, out, lse, workspace};
   return launch_status(sphkv::launch_cache8_attend(L, (hipStream_t)stream), fn);
 }
@@ -1142,7 +1142,7 @@ int sphkv_cache8_write(const void* k, const void* v, int32_t in_type, int64_t k_
     return fail(SPHKV_EINVAL, "%s: without cu_rows there is one row per sequence", fn);
   if (num_seqs == 0 || num_rows == 0) return ok();
   if (!k || !v || !start) return fail(SPHKV_EINVAL, "%s: null pointer argument", fn);
-  sphkv::Cache8RowsLaunch L{c, {cu_rows, start, table, table_stride, max_blocks, num_seqs, num_rows},
+  sphkv::Cache8RowsLaunch L{c, {cu_rows, start, table, table_stride, num_pages > 0 ? max_blocks : 0, num_seqs, num_rows},
                             const_cast<void*>(k), const_cast<void*>(v), in_type, k_row_stride, k_head_stride,
                             v_row_stride, v_head_stride};
   return launch_status(sphkv::launch_cache8_write(L, (hipStream_t)stream), fn);
@@ -1164,7 +1164,7 @@ int sphkv_cache8_read(const uint8_t* k_codes, const uint8_t* v_codes, const floa
     return fail(SPHKV_EINVAL, "%s: k_out and v_out must be 16-byte aligned", fn);
   if (num_seqs == 0 || num_rows == 0 || (!k_out && !v_out)) return ok();
   if (!start) return fail(SPHKV_EINVAL, "%s: null pointer argument", fn);
-  sphkv::Cache8RowsLaunch L{c, {cu_rows, start, table, table_stride, max_blocks, num_seqs, num_rows}, k_out, v_out,
+  sphkv::Cache8RowsLaunch L{c, {cu_rows, start, table, table_stride, num_pages > 0 ? max_blocks : 0, num_seqs, num_rows}, k_out, v_out,
                             out_type, (int64_t)num_kv * dh, dh, (int64_t)num_kv * dh, dh};
   return launch_status(sphkv::launch_cache8_read(L, (hipStream_t)stream), fn);
 }

@@ -289,6 +289,404 @@ __global__ __launch_bounds__(256) void cache8_attend_kernel(Cache8AttendLaunch L
   }
 }
 
+// ---- decode ------------------------------------------------------------------
+//
+// out = sum_t w_t c_t / sum_t (w_t / sv_t),  w_t = 2^(s_t + log2 sv_t - R),
+// s_t = sm_scale log2(e) sk_t <q, k_t>, c_t the value codes, R a reference near
+// the largest s_t + log2 sv_t.  With the value scale inside the exponent, the
+// largest weight that meets the codes is near 2^8 wherever the scales lie, so
+// weights fit fp16 (11 bits) and the products run on raw codes.
+//
+// A tile is 64 tokens, one wave's step: S^T = K Q^T as four 16x16 blocks
+// (v_mfma_f32_16x16x32_f16: int8 and e4m3 are exact in fp16), O^T += V^T P^T as
+// DH/16 blocks of 32 tokens.  Token 16 g + 4 i + j of a tile is row 4 g + j of
+// score block i, so lane (g, column) ends up with the scores of the 16 tokens
+// 16 g .. 16 g + 15 of one page run, in order: they are its part of the second
+// product's B operand as they stand, and the 16 bytes that it loads per value
+// row are its part of the A operand.  Nothing passes through LDS.
+// A column is a query head; up to 8 heads use two columns each, the second one
+// for what the first one's fp16 weight leaves out.
+//
+// Work: the tiles of all (sequence, kv head) pairs in a row, cut into equal
+// runs, one per workgroup; its four waves take the tiles of a pair in turn and
+// join their sums in LDS.  A pair that one workgroup holds is written out there;
+// the others leave a partial per workgroup (two at most: its first and its last
+// pair) for the merge kernel.
+constexpr int kTileTokens = 64;
+constexpr int kDecodeGroups = 512;      // two workgroups of four waves per CU
+constexpr int kDecodeLeast = 4;         // tiles of a workgroup: one per wave
+constexpr float kTopWeight = 8.0f;      // log2 of the weight at the reference, ...
+constexpr float kSlackWeight = 4.0f;    // ... which moves once a weight passes 2^4 times that
+constexpr float kNoScore = -3.0e38f;    // reference before the first score
+
+typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
+
+// heads handled together: a kv head's first 16, next 16, ...
+__host__ __device__ __forceinline__ int head_parts(int gqa) { return (gqa + 15) / 16; }
+__host__ __device__ __forceinline__ int part_cols(int gqa, int part) { return gqa - part * 16 < 16 ? gqa - part * 16 : 16; }
+// floats of one partial: reference and sum per column, then acc[cols][DH]
+__host__ __device__ __forceinline__ int64_t partial8_floats(int gqa, int dh) { return 32 + (int64_t)(gqa < 16 ? gqa : 16) * dh; }
+__host__ __device__ __forceinline__ int64_t plan_bytes(int num_seqs) { return (16 + 8 * ((int64_t)num_seqs + 1) + 255) / 256 * 256; }
+
+__device__ __forceinline__ int seq_tokens(const Cache8& c, const Cache8Batch& b, int s) {
+  return clampi(b.at[s], 0, (int64_t)b.max_blocks << c.page_shift);
+}
+
+__device__ __forceinline__ int64_t shfl64(int64_t x, int lane) {
+  const int lo = __shfl((int)x, lane, kWave), hi = __shfl((int)(x >> 32), lane, kWave);
+  return ((int64_t)hi << 32) | (uint32_t)lo;
+}
+
+// inclusive scan over the wave
+__device__ __forceinline__ int64_t wave_scan(int64_t x) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1) {
+    const int64_t y = shfl64(x, lane - d);
+    if (lane >= d) x += y;
+  }
+  return x;
+}
+
+__device__ __forceinline__ int64_t uniform64(int64_t x) {
+  return ((int64_t)uniform((int)(x >> 32)) << 32) | (uint32_t)uniform((int)x);
+}
+
+// Four codes as two pairs of fp16 (exact).  int8: the byte + 128 below 1024,
+// whose fp16 last place is 1, less 1152.
+template <int FMT>
+__device__ __forceinline__ void codes4(uint32_t x, half2v& a, half2v& b) {
+  if constexpr (FMT == kCache8Int8) {
+    x ^= 0x80808080u;
+    const half2v off = {(_Float16)1152.f, (_Float16)1152.f};
+    a = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(0x64646464u, x, 0x04010400u)) - off;
+    b = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(0x64646464u, x, 0x04030402u)) - off;
+  } else {
+    a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, false);
+    b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, true);
+  }
+}
+
+template <int FMT>
+__device__ __forceinline__ half8 codes8(uint32_t x, uint32_t y) {
+  half2v a, b, c, d;
+  codes4<FMT>(x, a, b);
+  codes4<FMT>(y, c, d);
+  return half8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+__device__ __forceinline__ float log2_of(float x) { return __builtin_amdgcn_logf(x); }
+__device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// One query row's part in a lane: dims 64 j + 16 kb + 0..15, as fp16.  fp16 rows
+// as they are.  bf16 rows times a power of two that brings their largest
+// magnitude into [2^14, 2^15): what lies 2^-29 below it or higher is exact, the
+// rest within 2^-40 of it.  `back` undoes it on the scores.
+template <int TYPE, int DH>
+__device__ __forceinline__ void load_query(const void* q, int64_t at, bool live, int kb, half8 (&out)[DH / 32],
+                                           int& back) {
+  struct __attribute__((packed, aligned(2))) U4 { uintx4 v; };
+  uintx4 raw[DH / 32];
+#pragma unroll
+  for (int i = 0; i < DH / 32; ++i) {
+    raw[i] = uintx4{0, 0, 0, 0};
+    if (live) raw[i] = ((const U4*)((const uint16_t*)q + at + 64 * (i / 2) + 16 * kb + 8 * (i & 1)))->v;
+  }
+  back = 0;
+  if constexpr (TYPE == kFp16) {
+#pragma unroll
+    for (int i = 0; i < DH / 32; ++i) out[i] = __builtin_bit_cast(half8, raw[i]);
+  } else {
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < DH / 32; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        m = fmaxf(m, fabsf(__builtin_bit_cast(float, raw[i][e] << 16)));
+        m = fmaxf(m, fabsf(__builtin_bit_cast(float, raw[i][e] & 0xFFFF0000u)));
+      }
+    m = rows_max(m);
+    int e = 0;
+    frexpf(m, &e);                                    // m in [2^(e-1), 2^e)
+    back = m > 0.f && m < INFINITY ? e - 15 : 0;
+#pragma unroll
+    for (int i = 0; i < DH / 32; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        out[i][2 * k] = (_Float16)ldexpf(__builtin_bit_cast(float, raw[i][k] << 16), -back);
+        out[i][2 * k + 1] = (_Float16)ldexpf(__builtin_bit_cast(float, raw[i][k] & 0xFFFF0000u), -back);
+      }
+  }
+}
+
+// a tile's bytes in a lane
+template <int DH>
+struct Tile {
+  uintx4 k[4][DH / 64];       // score block i, dims 64 j + 16 kb ..: token 16 (r >> 2) + 4 i + (r & 3), r = lane & 15
+  uintx4 v[DH / 16];          // value row 16 d + (lane & 15), tokens 16 g .. 16 g + 15, g = lane >> 4
+  float sk, sv;               // the scales of the tokens of run g
+  int page;                   // their page, or -1
+};
+
+template <int FMT, int TYPE, int DH>
+__global__ __launch_bounds__(256, 2) void cache8_decode_kernel(Cache8AttendLaunch L, float* partials, int64_t* base_of) {
+  constexpr int DT = DH / 16;
+  __shared__ float s_ref[4][16], s_sum[4][16];
+  __shared__ float s_acc[4][16][DH + 4];
+  const Cache8& c = L.c;
+  const Cache8Batch& b = L.b;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
+  const int parts = head_parts(L.gqa), HV = c.num_kv * parts, n = b.num_seqs;
+
+  // this workgroup's tiles
+  int64_t total = 0;
+  for (int i = lane; i < n; i += kWave) total += (seq_tokens(c, b, i) + kTileTokens - 1) / kTileTokens;
+  total = uniform64(shfl64(wave_scan(total), 63)) * HV;
+  int64_t per = (total + kDecodeGroups - 1) / kDecodeGroups;
+  if (per < kDecodeLeast) per = kDecodeLeast;
+  int64_t p = (int64_t)blockIdx.x * per;
+  const int64_t pend = p + per < total ? p + per : total;
+  const bool writes_plan = blockIdx.x == 0 && wave == 3;
+  int s = 0;
+  int64_t sbase = 0;                                  // tile at which sequence s starts
+  if (p < pend || writes_plan) {
+    int64_t before = 0;
+    bool found = false;
+    for (int i0 = 0; i0 < n && (!found || writes_plan); i0 += kWave) {
+      const int i = i0 + lane;
+      const int64_t t = i < n ? (int64_t)((seq_tokens(c, b, i) + kTileTokens - 1) / kTileTokens) * HV : 0;
+      const int64_t incl = before + wave_scan(t);
+      if (writes_plan && i < n) base_of[1 + i] = incl - t;
+      const uint64_t past = __ballot(incl > p);
+      if (!found && past) {
+        const int l = __ffsll((unsigned long long)past) - 1;
+        found = true;
+        s = i0 + l;
+        sbase = uniform64(shfl64(incl - t, l));
+      }
+      before = uniform64(shfl64(incl, 63));
+    }
+    if (writes_plan && lane == 0) {
+      base_of[0] = per;
+      base_of[1 + n] = total;
+    }
+  }
+  const float qscale = L.sm_scale * 1.44269504088896f;
+  const bool twin = L.gqa <= 8;                       // heads in columns 0..7 and again in 8..15
+  const int64_t page_bytes = (int64_t)c.num_kv * DH << c.page_shift;
+
+  for (; p < pend; ++s) {
+    const int len = uniform(seq_tokens(c, b, s)), T = (len + kTileTokens - 1) / kTileTokens;
+    if (T == 0) continue;
+    const int32_t* table = b.table + s * b.table_stride;
+    while (p < pend && p < sbase + (int64_t)T * HV) {
+      const int hv = (int)((p - sbase) / T), h = hv / parts, part = hv - h * parts;
+      const int cols = part_cols(L.gqa, part);
+      const int64_t first = sbase + (int64_t)hv * T;
+      const int t0 = (int)(p - first), t1 = pend - first < T ? (int)(pend - first) : T;
+      const int mycol = twin ? (col & 7) : col;
+      const bool live = mycol < cols;
+
+      half8 q[DH / 32];
+      int back;
+      const int64_t row = (int64_t)s;
+      load_query<TYPE, DH>(L.q, row * L.q_row + (int64_t)(h * L.gqa + part * 16 + mycol) * L.q_head, live, g, q, back);
+      const float cq = ldexpf(qscale, back);
+
+      // pages of run `run` of tile t, or -1
+      auto page_at = [&](int t, int run) {
+        const int blk = (t * kTileTokens + run * 16) >> c.page_shift;
+        if (blk >= b.max_blocks || t * kTileTokens + run * 16 >= len) return -1;
+        const int pg = table[blk];
+        return pg >= 0 && pg < c.num_pages ? pg : -1;
+      };
+      Tile<DH> A;
+      auto load_k = [&](int t, int kpage) {
+        const int run = col >> 2, in = (t * kTileTokens + run * 16) & ((1 << c.page_shift) - 1);
+        const uint8_t* k = c.k + (kpage < 0 ? 0 : kpage) * page_bytes + ((int64_t)h * DH << c.page_shift) +
+                           (in + (col & 3)) * DH + 16 * g;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < DH / 64; ++j) A.k[i][j] = *(const uintx4*)(k + 4 * i * DH + 64 * j);
+      };
+      auto load_v = [&](int t, int vpage) {
+        const int in = (t * kTileTokens + g * 16) & ((1 << c.page_shift) - 1);
+        const int64_t pg = vpage < 0 ? 0 : vpage;
+        const uint8_t* v = c.v + pg * page_bytes + ((int64_t)h * DH << c.page_shift) + in * DH + 16 * col;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) A.v[d] = *(const uintx4*)(v + 256 * d);
+        const float2 sc = *(const float2*)(c.scales + 2 * (pg * c.num_kv + h));
+        A.sk = sc.x;
+        A.sv = sc.y;
+        A.page = vpage;
+      };
+
+      floatx4 acc[DT];
+#pragma unroll
+      for (int d = 0; d < DT; ++d) acc[d] = floatx4{0, 0, 0, 0};
+      float ref = kNoScore, sum = 0.f;
+
+      int t = t0 + wave;
+      int kp = -1, vp = -1, kp1 = -1, vp1 = -1;
+      if (t < t1) {
+        kp = page_at(t, col >> 2);
+        vp = page_at(t, g);
+        kp1 = t + 4 < t1 ? page_at(t + 4, col >> 2) : -1;
+        vp1 = t + 4 < t1 ? page_at(t + 4, g) : -1;
+        load_k(t, kp);
+        load_v(t, vp);
+      }
+      for (; t < t1; t += 4) {
+        const int kp2 = t + 8 < t1 ? page_at(t + 8, col >> 2) : -1, vp2 = t + 8 < t1 ? page_at(t + 8, g) : -1;
+        // scores
+        floatx4 sc[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          sc[i] = floatx4{0, 0, 0, 0};
+#pragma unroll
+          for (int j = 0; j < DH / 64; ++j) {
+            sc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8<FMT>(A.k[i][j].x, A.k[i][j].y), q[2 * j], sc[i], 0, 0, 0);
+            sc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8<FMT>(A.k[i][j].z, A.k[i][j].w), q[2 * j + 1], sc[i], 0, 0, 0);
+          }
+        }
+        if (t + 4 < t1) load_k(t + 4, kp1);
+        // tokens that are not there: behind the length, or of an absent page
+        const int have = A.page < 0 ? 0 : len - t * kTileTokens - 16 * g;     // of this lane's 16
+        if (__any(have < 16)) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) sc[e >> 2][e & 3] = e < have ? sc[e >> 2][e & 3] : -INFINITY;
+          uint32_t keep[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int m = have - 4 * k;
+            keep[k] = m >= 4 ? ~0u : (m <= 0 ? 0u : (1u << (8 * m)) - 1u);
+          }
+#pragma unroll
+          for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) A.v[d][k] &= keep[k];
+          if (have <= 0) A.sk = A.sv = 1.f;                                   // (an unwritten page's may be anything)
+        }
+        const float ck = fmaxf(cq * A.sk, 0x1p-126f), lsv = log2_of(A.sv);      // (never 0: 0 * -inf)
+        float top = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3]));
+#pragma unroll
+        for (int i = 1; i < 4; ++i) top = fmaxf(top, fmaxf(fmaxf(sc[i][0], sc[i][1]), fmaxf(sc[i][2], sc[i][3])));
+        top = fmaf(top, ck, lsv);
+        if (__any(top > ref + (kTopWeight + kSlackWeight))) {                 // (each column by its own scores)
+          top = rows_max(top);
+          const float to = top > ref + (kTopWeight + kSlackWeight) ? top - kTopWeight : ref;
+          const float f = exp2_of(ref - to);
+          ref = to;
+          sum *= f;
+#pragma unroll
+          for (int d = 0; d < DT; ++d) acc[d] *= f;
+        }
+        // weights
+        const float off = lsv - ref;
+        float wsum = 0.f;
+        half8 w[2];
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) {
+          const float x = exp2_of(fmaf(sc[e >> 2][e & 3], ck, off)), y = exp2_of(fmaf(sc[e >> 2][(e & 3) + 1], ck, off));
+          wsum += x + y;
+          _Float16 hx = (_Float16)x, hy = (_Float16)y;
+          if (twin && col >= 8) {
+            hx = (_Float16)(x - (float)hx);
+            hy = (_Float16)(y - (float)hy);
+          }
+          w[e >> 3][e & 7] = hx;
+          w[e >> 3][(e & 7) + 1] = hy;
+        }
+        sum = fmaf(wsum, exp2_of(-lsv), sum);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8<FMT>(A.v[d].x, A.v[d].y), w[0], acc[d], 0, 0, 0);
+          acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8<FMT>(A.v[d].z, A.v[d].w), w[1], acc[d], 0, 0, 0);
+        }
+        if (t + 4 < t1) load_v(t + 4, vp1);
+        kp1 = kp2;
+        vp1 = vp2;
+      }
+
+      // the waves' sums, joined: reference, sum, then acc under the common reference
+      sum = rows_sum(sum);
+      if (g == 0) {
+        s_ref[wave][col] = ref;
+        s_sum[wave][col] = sum;
+      }
+      __syncthreads();
+      const float R = fmaxf(fmaxf(s_ref[0][col], s_ref[1][col]), fmaxf(s_ref[2][col], s_ref[3][col]));
+      const float f = exp2_of(ref - R);
+#pragma unroll
+      for (int d = 0; d < DT; ++d) *(floatx4*)&s_acc[wave][col][16 * d + 4 * g] = acc[d] * f;
+      __syncthreads();
+      const bool whole = t0 == 0 && t1 == T;
+      float* part_out = partials + (2 * (int64_t)blockIdx.x + (t0 == 0)) * partial8_floats(L.gqa, DH);
+      for (int i = threadIdx.x; i < cols * DH; i += 256) {
+        const int cc = i / DH, d = i % DH;
+        float o = s_acc[0][cc][d] + s_acc[1][cc][d] + s_acc[2][cc][d] + s_acc[3][cc][d];
+        if (twin) o += s_acc[0][cc + 8][d] + s_acc[1][cc + 8][d] + s_acc[2][cc + 8][d] + s_acc[3][cc + 8][d];
+        const float Rc = fmaxf(fmaxf(s_ref[0][cc], s_ref[1][cc]), fmaxf(s_ref[2][cc], s_ref[3][cc]));
+        float l = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) l = fmaf(s_sum[w][cc], exp2_of(s_ref[w][cc] - Rc), l);
+        const int64_t at = row * c.num_kv * L.gqa + h * L.gqa + part * 16 + cc;
+        if (whole) {
+          store1<TYPE>(L.out, at * DH + d, l == 0.f ? 0.f : o / l);
+          if (L.lse && d == 0) L.lse[at] = l == 0.f ? -INFINITY : (Rc + log2_of(l)) * 0.693147180559945f;
+        } else {
+          part_out[32 + cc * DH + d] = o;
+          if (d == 0) {
+            part_out[cc] = Rc;
+            part_out[16 + cc] = l;
+          }
+        }
+      }
+      __syncthreads();
+      p = first + t1;
+    }
+    sbase += (int64_t)T * HV;
+  }
+}
+
+// Joins the partials of each (sequence, kv head) that several workgroups hold,
+// and writes the rows of sequences without a token.  One wave per query head.
+template <int TYPE, int DH>
+__global__ __launch_bounds__(64) void cache8_decode_merge_kernel(Cache8AttendLaunch L, const float* partials,
+                                                                 const int64_t* base_of) {
+  const Cache8& c = L.c;
+  const int heads = c.num_kv * L.gqa, s = blockIdx.x / heads, hq = blockIdx.x % heads, lane = threadIdx.x;
+  const int h = hq / L.gqa, part = (hq - h * L.gqa) / 16, cc = (hq - h * L.gqa) % 16, parts = head_parts(L.gqa);
+  const int64_t per = base_of[0], a = base_of[1 + s], T = (base_of[2 + s] - a) / (c.num_kv * parts);
+  const int64_t at = (int64_t)s * heads + hq;
+  constexpr int DPL = DH / 64;
+  if (T == 0) {
+    for (int i = 0; i < DPL; ++i) store1<TYPE>(L.out, at * DH + lane * DPL + i, 0.f);
+    if (L.lse && lane == 0) L.lse[at] = -INFINITY;
+    return;
+  }
+  const int64_t first = a + (int64_t)(h * parts + part) * T, g0 = first / per, g1 = (first + T - 1) / per;
+  if (g0 == g1) return;
+  const int64_t floats = partial8_floats(L.gqa, DH);
+  auto partial = [&](int64_t g) { return partials + (2 * g + (g == g0)) * floats; };
+  float R = kNoScore;
+  for (int64_t g = g0 + lane; g <= g1; g += kWave) R = fmaxf(R, partial(g)[cc]);
+  R = wave_max(R);
+  float l = 0.f, acc[DPL] = {};
+#pragma unroll 8
+  for (int64_t g = g0; g <= g1; ++g) {
+    const float* x = partial(g);
+    const float f = exp2_of(x[cc] - R);
+    l = fmaf(x[16 + cc], f, l);
+#pragma unroll
+    for (int i = 0; i < DPL; ++i) acc[i] = fmaf(x[32 + cc * DH + lane * DPL + i], f, acc[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < DPL; ++i) store1<TYPE>(L.out, at * DH + lane * DPL + i, l == 0.f ? 0.f : acc[i] / l);
+  if (L.lse && lane == 0) L.lse[at] = l == 0.f ? -INFINITY : (R + log2_of(l)) * 0.693147180559945f;
+}
+
 template <template <int, int, int> class K, class... A>
 int pick(int type, int fmt, int dh, A... a) {
 #define SPHKV_PICK(T, F, D) if (type == T && fmt == F && dh == D) return K<T, F, D>::go(a...)
@@ -331,6 +729,20 @@ template <int T, int F, int D> struct Attend {
   }
 };
 
+template <int T, int F, int D> struct Decode {
+  static int go(const Cache8AttendLaunch& L, hipStream_t st) {
+    if constexpr (T == kFp32) {
+      return -1;
+    } else {
+      int64_t* plan = (int64_t*)L.ws;
+      float* partials = (float*)((uint8_t*)L.ws + plan_bytes(L.b.num_seqs));
+      cache8_decode_kernel<F, T, D><<<kDecodeGroups, 256, 0, st>>>(L, partials, plan);
+      cache8_decode_merge_kernel<T, D><<<L.b.num_seqs * L.c.num_kv * L.gqa, 64, 0, st>>>(L, partials, plan);
+      return hipPeekAtLastError() == hipSuccess ? 0 : -1;
+    }
+  }
+};
+
 }  // namespace
 
 int launch_cache8_write(const Cache8RowsLaunch& L, hipStream_t stream) {
@@ -340,9 +752,11 @@ int launch_cache8_read(const Cache8RowsLaunch& L, hipStream_t stream) {
   return pick<Read>(L.type, L.c.fmt, L.c.dh, L, stream);
 }
 int launch_cache8_attend(const Cache8AttendLaunch& L, hipStream_t stream) {
-  return pick<Attend>(L.type, L.c.fmt, L.c.dh, L, stream);
+  return L.b.cu ? pick<Attend>(L.type, L.c.fmt, L.c.dh, L, stream) : pick<Decode>(L.type, L.c.fmt, L.c.dh, L, stream);
 }
-int64_t cache8_decode_ws_bytes(int32_t, int32_t, int32_t, int32_t) { return 0; }
+int64_t cache8_decode_ws_bytes(int32_t num_seqs, int32_t, int32_t gqa, int32_t dh) {
+  return plan_bytes(num_seqs) + 2 * kDecodeGroups * 4 * partial8_floats(gqa, dh);
+}
 int64_t cache8_prefill_ws_bytes(int64_t, int32_t, int32_t, int32_t, int32_t) { return 0; }
 
 }  // namespace sphkv

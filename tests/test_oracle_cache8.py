@@ -119,8 +119,8 @@ _SHARED = [
     (dict(pages=-1), "negative size"), (dict(num_kv=0), "negative size"), (dict(num_kv=1025), "num_kv must be"),
     (dict(pages=1 << 31), "exceeds int32"), (dict(mb=1 << 27, ts=1 << 27), "exceeds 2^30"),
     (dict(ts=7), "table_stride"), (dict(kc=_FAKE + 8), "16-byte aligned"), (dict(sc=_FAKE + 4), "16-byte aligned"),
-    (dict(vc=None), "null pointer"), (dict(table=None), "null pointer"), (dict(num_seqs=(1 << 20) + 1), "at most 2^20"),
-    (dict(num_seqs=1 << 20, num_kv=64), "exceeds 2^25"),
+    (dict(vc=None), "null pointer"), (dict(table=None), "null pointer"), (dict(num_seqs=(1 << 16) + 1), "at most 2^16"),
+    (dict(num_seqs=1 << 16, num_kv=1024), "exceeds 2^25"),
 ]
 
 
@@ -162,7 +162,7 @@ def test_attention_refusals(decode, kw, msg):
 def test_prefill_refusals():
     lib = sphkv_lib.load()
     for kw, msg in ((dict(cu=None), "null pointer"), (dict(causal=2), "causal must be"), (dict(num_rows=-1), "negative"),
-                    (dict(num_rows=1 << 22, num_kv=16, gqa=64), "2^31 - 1")):
+                    (dict(num_rows=1 << 22, num_kv=16, gqa=64), "too many")):
         assert lib.sphkv_cache8_prefill(*_attend_args(False, **kw)) == -1
         assert msg in lib.sphkv_last_error().decode()
 
