@@ -111,21 +111,23 @@ class Cache:
         return k, v, present
 
     def attend(self, q, table, lens, cu_rows=None, causal=True, sm_scale=None):
-        """(out, lse, bound): bound[row, head] = (per dim sum_t p_t |v_t|, largest sum_d |q_d k_d| sm_scale,
-        largest |score|) for tolerances.  q [rows, num_q, dh] float64."""
+        """(out, lse, mass, reach, under), the last three for tolerances: sum_t p_t |v_t| of each output, the
+        largest sum_d |q_d k_d| sm_scale of each row, and of each output max_t (p_t sv_t) sum_t |value code of t|.
+        q [rows, num_q, dh] float64."""
         n = len(lens)
         cu = np.arange(n + 1) if cu_rows is None else cu_rows
         H = self.num_kv
         gqa = q.shape[1] // H
         sm = 1.0 / np.sqrt(self.dh) if sm_scale is None else sm_scale
         out, lse = np.zeros(q.shape), np.full(q.shape[:2], -np.inf)
-        mass, reach = np.zeros(q.shape), np.zeros(q.shape[:2])
+        mass, reach, under = np.zeros(q.shape), np.zeros(q.shape[:2]), np.zeros(q.shape)
         for s in range(n):
             m = int(cu[s + 1]) - int(cu[s])
             L = min(max(int(lens[s]), 0), table.shape[1] * self.ps)
             if m <= 0 or L <= 0:
                 continue
             k, v, present = self.tokens(table, s, 0, L)
+            pages = np.repeat([max(self.page(table, s, b), 0) for b in range(-(-L // self.ps))], self.ps)[:L]
             for h in range(H):
                 rows = q[cu[s]:cu[s + 1], h * gqa:(h + 1) * gqa]                       # [m, gqa, dh]
                 x = np.einsum("mgd,td->mgt", rows, k[:, h]) * sm
@@ -139,7 +141,10 @@ class Cache:
                 at = (slice(int(cu[s]), int(cu[s + 1])), slice(h * gqa, (h + 1) * gqa))
                 out[at] = p @ v[:, h]
                 mass[at] = p @ np.abs(v[:, h])
+                sv = self.scales[pages, h, 1]
+                codes = np.abs(v[:, h]) / np.where(sv > 0, sv, 1)[:, None]
+                under[at] = (p * sv).max(-1, keepdims=True) * (see[:, None] @ codes)
                 with np.errstate(divide="ignore"):
                     lse[at] = (np.where(np.isfinite(top), top, 0.0) + np.log(l))[..., 0]
                 reach[at] = np.where(see[:, None], r, 0).max(-1)
-        return out, lse, mass, reach
+        return out, lse, mass, reach, under

@@ -221,74 +221,6 @@ __global__ __launch_bounds__(256) void cache8_read_kernel(Cache8RowsLaunch L, in
   }
 }
 
-// One workgroup per (query row, q head), 256 tokens at a time.
-template <int TYPE, int FMT, int DH>
-__global__ __launch_bounds__(256) void cache8_attend_kernel(Cache8AttendLaunch L) {
-  __shared__ float sq[DH], sw[256], red[8], accs[256];
-  const Cache8& c = L.c;
-  const Cache8Batch& b = L.b;
-  const int hq = blockIdx.x, h = hq / L.gqa, tid = threadIdx.x, ps = 1 << c.page_shift;
-  const int64_t row = blockIdx.y + (int64_t)blockIdx.z * 32768;
-  if (row >= b.num_rows) return;
-  const int s = b.cu ? seq_of_slot(b, row, 1, 0, 0) : (int)row;
-  int begin, end;
-  rows_of(b, s, begin, end);
-  if (row < begin || row >= end) return;
-  int n = clampi(b.at[s], 0, (int64_t)b.max_blocks << c.page_shift);      // tokens attended
-  if (L.causal) n = clampi((int64_t)n - (end - begin) + (row - begin) + 1, 0, n);
-  for (int d = tid; d < DH; d += 256) sq[d] = load1<TYPE>(L.q, row * L.q_row + hq * L.q_head + d);
-  __syncthreads();
-  float m = -INFINITY, l = 0.f, acc = 0.f;
-  const int d = tid % DH, part = tid / DH, parts = 256 / DH;
-  for (int t0 = 0; t0 < n; t0 += 256) {
-    const int t = t0 + tid;
-    float x = -INFINITY, sv = 0.f;
-    if (t < n) {
-      const int page = page_of(c, b, s, t >> c.page_shift);
-      if (page >= 0) {
-        const int64_t ph = (int64_t)page * c.num_kv + h;
-        const uint8_t* kc = c.k + (ph * ps + (t & (ps - 1))) * DH;
-        x = 0.f;
-        for (int i = 0; i < DH; ++i) x = fmaf(sq[i], decode1<FMT>(kc[i]), x);
-        x *= c.scales[2 * ph] * L.sm_scale;
-        sv = c.scales[2 * ph + 1];
-      }
-    }
-    float top = wave_max(x);
-    if ((tid & 63) == 0) red[tid >> 6] = top;
-    __syncthreads();
-    top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    const float M = fmaxf(m, top);
-    const float R = M == -INFINITY ? 0.f : M;                         // (a NaN score stays one)
-    const float f = expf(m - R), w = expf(x - R);
-    l = l * f + w;                                                    // this thread's tokens
-    sw[tid] = w * sv;
-    m = M;
-    __syncthreads();
-    acc *= f;
-    const int lim = n - t0 < 256 ? n - t0 : 256;
-    for (int i = part; i < lim; i += parts) {
-      const int page = page_of(c, b, s, (t0 + i) >> c.page_shift);
-      if (page < 0) continue;
-      const int r = (t0 + i) & (ps - 1);
-      acc = fmaf(sw[i], decode1<FMT>(c.v[((int64_t)page * c.num_kv + h) * ps * DH + (r >> 4) * 16 * DH + d * 16 + (r & 15)]), acc);
-    }
-    __syncthreads();
-  }
-  for (int k = 1; k < 64; k <<= 1) l += shfl_xor(l, k);
-  if ((tid & 63) == 0) red[tid >> 6] = l;
-  accs[tid] = acc;
-  __syncthreads();
-  l = red[0] + red[1] + red[2] + red[3];
-  if (tid < DH) {
-    float o = 0.f;
-    for (int p = 0; p < parts; ++p) o += accs[p * DH + tid];
-    const int64_t at = row * c.num_kv * L.gqa + hq;
-    store1<TYPE>(L.out, at * DH + tid, l > 0.f ? o / l : (l == 0.f ? 0.f : NAN));
-    if (L.lse && tid == 0) L.lse[at] = l == 0.f ? -INFINITY : m + logf(l);
-  }
-}
-
 // ---- decode ------------------------------------------------------------------
 //
 // out = sum_t w_t c_t / sum_t (w_t / sv_t),  w_t = 2^(s_t + log2 sv_t - R),
@@ -378,39 +310,31 @@ __device__ __forceinline__ half8 codes8(uint32_t x, uint32_t y) {
 __device__ __forceinline__ float log2_of(float x) { return __builtin_amdgcn_logf(x); }
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// One query row's part in a lane: dims 64 j + 16 kb + 0..15, as fp16.  fp16 rows
-// as they are.  bf16 rows times a power of two that brings their largest
-// magnitude into [2^14, 2^15): what lies 2^-29 below it or higher is exact, the
-// rest within 2^-40 of it.  `back` undoes it on the scores.
-template <int TYPE, int DH>
-__device__ __forceinline__ void load_query(const void* q, int64_t at, bool live, int kb, half8 (&out)[DH / 32],
-                                           int& back) {
-  struct __attribute__((packed, aligned(2))) U4 { uintx4 v; };
-  uintx4 raw[DH / 32];
-#pragma unroll
-  for (int i = 0; i < DH / 32; ++i) {
-    raw[i] = uintx4{0, 0, 0, 0};
-    if (live) raw[i] = ((const U4*)((const uint16_t*)q + at + 64 * (i / 2) + 16 * kb + 8 * (i & 1)))->v;
-  }
+// A query row's part in a lane as fp16.  fp16 rows as they are.  bf16 rows times
+// a power of two that brings their largest magnitude (row_max joins the lanes
+// that share a row) into [2^14, 2^15): what lies 2^-29 below it or higher is
+// exact, the rest within 2^-40 of it.  `back` undoes it on the scores.
+template <int TYPE, int N, class MAX>
+__device__ __forceinline__ void query_fp16(const uintx4 (&raw)[N], MAX row_max, half8 (&out)[N], int& back) {
   back = 0;
   if constexpr (TYPE == kFp16) {
 #pragma unroll
-    for (int i = 0; i < DH / 32; ++i) out[i] = __builtin_bit_cast(half8, raw[i]);
+    for (int i = 0; i < N; ++i) out[i] = __builtin_bit_cast(half8, raw[i]);
   } else {
     float m = 0.f;
 #pragma unroll
-    for (int i = 0; i < DH / 32; ++i)
+    for (int i = 0; i < N; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         m = fmaxf(m, fabsf(__builtin_bit_cast(float, raw[i][e] << 16)));
         m = fmaxf(m, fabsf(__builtin_bit_cast(float, raw[i][e] & 0xFFFF0000u)));
       }
-    m = rows_max(m);
+    m = row_max(m);
     int e = 0;
     frexpf(m, &e);                                    // m in [2^(e-1), 2^e)
     back = m > 0.f && m < INFINITY ? e - 15 : 0;
 #pragma unroll
-    for (int i = 0; i < DH / 32; ++i)
+    for (int i = 0; i < N; ++i)
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         out[i][2 * k] = (_Float16)ldexpf(__builtin_bit_cast(float, raw[i][k] << 16), -back);
@@ -487,10 +411,21 @@ __global__ __launch_bounds__(256, 2) void cache8_decode_kernel(Cache8AttendLaunc
       const int mycol = twin ? (col & 7) : col;
       const bool live = mycol < cols;
 
+      // a column's query: dims 64 j + 16 g + 0..15 in lane group g
       half8 q[DH / 32];
       int back;
       const int64_t row = (int64_t)s;
-      load_query<TYPE, DH>(L.q, row * L.q_row + (int64_t)(h * L.gqa + part * 16 + mycol) * L.q_head, live, g, q, back);
+      {
+        struct __attribute__((packed, aligned(2))) U4 { uintx4 v; };
+        const uint16_t* src = (const uint16_t*)L.q + row * L.q_row + (int64_t)(h * L.gqa + part * 16 + mycol) * L.q_head + 16 * g;
+        uintx4 raw[DH / 32];
+#pragma unroll
+        for (int i = 0; i < DH / 32; ++i) {
+          raw[i] = uintx4{0, 0, 0, 0};
+          if (live) raw[i] = ((const U4*)(src + 64 * (i / 2) + 8 * (i & 1)))->v;
+        }
+        query_fp16<TYPE, DH / 32>(raw, [](float m) { return rows_max(m); }, q, back);
+      }
       const float cq = ldexpf(qscale, back);
 
       // pages of run `run` of tile t, or -1
@@ -687,6 +622,323 @@ __global__ __launch_bounds__(64) void cache8_decode_merge_kernel(Cache8AttendLau
   if (L.lse && lane == 0) L.lse[at] = l == 0.f ? -INFINITY : (R + log2_of(l)) * 0.693147180559945f;
 }
 
+// ---- prefill -----------------------------------------------------------------
+//
+// The same sums for many query rows.  A kv head's rows are its gqa heads of each
+// token in turn: a workgroup takes 128 of them, 32 per wave, and walks the tiles
+// of 64 tokens that the last of them sees.  Codes become fp16 once per workgroup,
+// on their way into LDS (two buffers: the next tile's bytes are on the way while
+// this one is multiplied).  S^T = K Q^T as two 32x32 blocks per wave
+// (v_mfma_f32_32x32x16_f16), O^T += V^T P^T.  Token 16 x + 8 h + y of a block is
+// score row 16 x + 4 h + y for y < 4 and 16 x + 4 h + y + 4 above, so that lane
+// (h, row) holds its part of the second product's B operand, and every group of 8
+// scores lies in one 16-token run, whose scales are the same for the wave.
+// LDS rows are 16-byte chunks, exclusive-or'ed with the row so that the 16 rows
+// that a read touches at once lie in different banks.
+//
+// With few row tiles the keys of each are split over workgroups, whose partials a
+// second kernel joins.
+constexpr int kRowTile = 128;
+constexpr int kPrefillGroups = 512;     // workgroups that run at once: two per CU
+constexpr int kSplitLeast = 4;          // tiles of a split
+constexpr int kSplitMost = 64;
+
+__host__ __device__ __forceinline__ int64_t row_tiles(int64_t num_rows, int num_seqs, int gqa) {
+  return ((num_rows * gqa) >> 7) + num_seqs;
+}
+__host__ __device__ __forceinline__ int prefill_splits(int64_t num_rows, int num_seqs, int num_kv, int gqa) {
+  const int64_t wgs = row_tiles(num_rows, num_seqs, gqa) * num_kv, s = kPrefillGroups / wgs;
+  return (int)(s < 1 ? 1 : (s > kSplitMost ? kSplitMost : s));
+}
+// floats of one split's partial: reference and sum per row, then acc[rows][DH]
+__host__ __device__ __forceinline__ int64_t split_floats(int dh) { return (int64_t)kRowTile * (dh + 2); }
+
+// tokens that a sequence's row of token `last_token` sees, and the splits that
+// so many are worth
+__device__ __forceinline__ int tile_seen(const Cache8AttendLaunch& L, int len, int n, int last_token) {
+  return L.causal ? clampi((int64_t)len - n + last_token + 1, 0, len) : len;
+}
+__device__ __forceinline__ int splits_of(int seen, int splits) {
+  const int most = (seen + kTileTokens - 1) / kTileTokens / kSplitLeast;
+  return most < 1 ? 1 : (most < splits ? most : splits);
+}
+
+template <int DH>
+__device__ __forceinline__ int k_at(int token, int chunk) {        // fp16 elements
+  return token * DH + 8 * (DH == 128 ? (chunk ^ (token & 15)) : (chunk ^ ((token >> 1) & 7)));
+}
+__device__ __forceinline__ int v_at(int d, int chunk) { return d * kTileTokens + 8 * (chunk ^ ((d >> 1) & 7)); }
+
+__device__ __forceinline__ float halves_max(float x) {
+  float a = x, b = x;
+  swap32(a, b);
+  return fmaxf(a, b);
+}
+__device__ __forceinline__ float halves_sum(float x) {
+  float a = x, b = x;
+  swap32(a, b);
+  return a + b;
+}
+
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+
+template <int FMT, int TYPE, int DH>
+__global__ __launch_bounds__(256, 2) void cache8_prefill_kernel(Cache8AttendLaunch L, int splits, float* partials) {
+  constexpr int KS = DH / 16, DB = DH / 32, PER = DH / 64;         // k-steps, value blocks, 16-byte loads of a thread
+  __shared__ __align__(16) _Float16 s_k[2][kTileTokens * DH], s_v[2][kTileTokens * DH];
+  __shared__ float s_sk[2][4], s_lsv[2][4], s_inv[2][4];
+  const Cache8& c = L.c;
+  const Cache8Batch& b = L.b;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
+  // neighbours take different heads (eight of them: one per XCD and its L2), and
+  // the longest rows of a sequence come first
+  const int h = blockIdx.x % c.num_kv, z = blockIdx.y, gqa = L.gqa;
+  const int64_t slot = (gridDim.x - 1 - blockIdx.x) / c.num_kv;
+  const int s = uniform(seq_of_slot(b, slot, gqa, 7, 1));
+  int begin, end;
+  rows_of(b, s, begin, end);
+  begin = uniform(begin);
+  const int n = uniform(end) - begin;
+  const int64_t r0 = (slot - first_slot(b, s, gqa, 7, 1)) * kRowTile, rows_all = (int64_t)n * gqa;
+  if (r0 >= rows_all) return;
+  const int len = uniform(seq_tokens(c, b, s));
+  const int last = (int)((r0 + kRowTile < rows_all ? r0 + kRowTile : rows_all) - 1);
+  const int seen = tile_seen(L, len, n, last / gqa);
+  const int parts = splits_of(seen, splits);
+  if (z >= parts) return;
+  const int NT = (seen + kTileTokens - 1) / kTileTokens;
+  const int tbeg = (int)((int64_t)NT * z / parts), tend = (int)((int64_t)NT * (z + 1) / parts);
+
+  // this lane's row
+  const int64_t r = r0 + wave * 32 + col;
+  const bool live = r < rows_all;
+  const int tok = live ? (int)(r / gqa) : 0, hd = live ? (int)(r - (int64_t)tok * gqa) : 0;
+  const int lim = live ? tile_seen(L, len, n, tok) : 0;
+  int lim_min = live ? lim : 0x7FFFFFFF, lim_max = lim;
+#pragma unroll
+  for (int m = 1; m < 32; m <<= 1) {
+    lim_min = min(lim_min, __shfl_xor(lim_min, m, kWave));
+    lim_max = max(lim_max, __shfl_xor(lim_max, m, kWave));
+  }
+  lim_min = uniform(lim_min);
+  lim_max = uniform(lim_max);
+
+  half8 q[KS];
+  int back = 0;
+  {
+    struct __attribute__((packed, aligned(2))) U4 { uintx4 v; };
+    const uint16_t* src = (const uint16_t*)L.q + (int64_t)(begin + tok) * L.q_row + (int64_t)(h * gqa + hd) * L.q_head + 8 * half;
+    uintx4 raw[KS];
+#pragma unroll
+    for (int i = 0; i < KS; ++i) {
+      raw[i] = uintx4{0, 0, 0, 0};
+      if (live) raw[i] = ((const U4*)(src + 16 * i))->v;
+    }
+    query_fp16<TYPE, KS>(raw, [](float m) { return halves_max(m); }, q, back);
+  }
+  const float cq = ldexpf(L.sm_scale * 1.44269504088896f, back);
+
+  const int32_t* table = b.table + s * b.table_stride;
+  const int64_t page_bytes = (int64_t)c.num_kv * DH << c.page_shift;
+  const int ps_mask = (1 << c.page_shift) - 1;
+  // A wave's part of a tile: 16 codes of DH/64 key rows and as many value rows a
+  // thread, of runs that are the same for the wave.
+  uintx4 kraw[PER], vraw[PER];
+  auto run_of = [&](int i) { return DH == 128 ? 2 * i + (wave >> 1) : wave; };
+  auto fetch = [&](int t) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int run = run_of(i), at = t * kTileTokens + run * 16;
+      kraw[i] = vraw[i] = uintx4{0, 0, 0, 0};
+      const int blk = at >> c.page_shift;
+      int pg = at < len && blk < b.max_blocks ? uniform(table[blk]) : -1;
+      if (pg >= c.num_pages) pg = -1;
+      float sk = 1.f, lsv = -INFINITY, inv = 0.f;
+      if (pg >= 0) {
+        const int64_t base = pg * page_bytes + ((int64_t)h * DH << c.page_shift) + (at & ps_mask) * DH;
+        const int in = DH == 128 ? tid & 127 : lane;               // this thread's 16 bytes of the run's DH * 16
+        kraw[i] = *(const uintx4*)(c.k + base + 16 * in);
+        vraw[i] = *(const uintx4*)(c.v + base + 16 * in);
+        const float2 sc = *(const float2*)(c.scales + 2 * ((int64_t)pg * c.num_kv + h));
+        sk = sc.x;
+        lsv = log2_of(sc.y);
+        inv = exp2_of(-lsv);
+        const int have = len - at;                                  // tokens of the run that are there
+        if (have < 16) {
+          const int token = in / (DH / 16);
+          if (token >= have) kraw[i] = uintx4{0, 0, 0, 0};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int m = have - 4 * k;
+            vraw[i][k] &= m >= 4 ? ~0u : (m <= 0 ? 0u : (1u << (8 * m)) - 1u);
+          }
+        }
+      }
+      if ((DH == 128 ? tid & 127 : lane) == 0) {
+        const int bf = t & 1;
+        s_sk[bf][run] = sk;
+        s_lsv[bf][run] = lsv;
+        s_inv[bf][run] = inv;
+      }
+    }
+  };
+  auto stage = [&](int t) {
+    const int bf = t & 1;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int run = run_of(i), in = DH == 128 ? tid & 127 : lane;
+      const int token = run * 16 + in / (DH / 16), chunk = 2 * (in % (DH / 16));
+      *(half8*)&s_k[bf][k_at<DH>(token, chunk)] = codes8<FMT>(kraw[i].x, kraw[i].y);
+      *(half8*)&s_k[bf][k_at<DH>(token, chunk + 1)] = codes8<FMT>(kraw[i].z, kraw[i].w);
+      *(half8*)&s_v[bf][v_at(in, 2 * run)] = codes8<FMT>(vraw[i].x, vraw[i].y);
+      *(half8*)&s_v[bf][v_at(in, 2 * run + 1)] = codes8<FMT>(vraw[i].z, vraw[i].w);
+    }
+  };
+
+  floatx16 acc[DB];
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
+  float ref = kNoScore, sum = 0.f;
+  const int ktok = 16 * (col >> 4) + 8 * ((col >> 2) & 1) + 4 * ((col >> 3) & 1) + (col & 3);   // token of score row `col`
+
+  if (tbeg < tend) {
+    fetch(tbeg);
+    stage(tbeg);
+  }
+  __syncthreads();
+  for (int t = tbeg; t < tend; ++t) {
+    const int bf = t & 1, t0 = t * kTileTokens;
+    if (t + 1 < tend) fetch(t + 1);
+    if (t0 < lim_max) {
+      floatx16 sc[2];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sc[x][i] = 0.f;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          const half8 a = *(const half8*)&s_k[bf][k_at<DH>(32 * x + ktok, 2 * k + half)];
+          sc[x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, q[k], sc[x], 0, 0, 0);
+        }
+      }
+      if (t0 + kTileTokens > lim_min) {
+        const int left = lim - t0 - 8 * half;
+#pragma unroll
+        for (int e = 0; e < 32; ++e)
+          sc[e >> 4][e & 15] = 16 * (e >> 3) + (e & 7) < left ? sc[e >> 4][e & 15] : -INFINITY;
+      }
+      float ck[4], lsv[4], top = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        ck[u] = fmaxf(cq * s_sk[bf][u], 0x1p-126f);                   // (never 0: 0 * -inf)
+        lsv[u] = s_lsv[bf][u];
+        float m = sc[u >> 1][8 * (u & 1)];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) m = fmaxf(m, sc[u >> 1][8 * (u & 1) + i]);
+        top = fmaxf(top, fmaf(m, ck[u], lsv[u]));
+      }
+      if (__any(top > ref + (kTopWeight + kSlackWeight))) {           // (each row by its own scores)
+        top = halves_max(top);
+        const float to = top > ref + (kTopWeight + kSlackWeight) ? top - kTopWeight : ref;
+        const float f = exp2_of(ref - to);
+        ref = to;
+        sum *= f;
+#pragma unroll
+        for (int d = 0; d < DB; ++d) acc[d] *= f;
+      }
+      half8 w[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const float off = lsv[u] - ref;
+        float ws = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float x = exp2_of(fmaf(sc[u >> 1][8 * (u & 1) + i], ck[u], off));
+          ws += x;
+          w[u][i] = (_Float16)x;
+        }
+        sum = fmaf(ws, s_inv[bf][u], sum);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int d = 0; d < DB; ++d) {
+          const half8 a = *(const half8*)&s_v[bf][v_at(32 * d + col, 2 * u + half)];
+          acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, w[u], acc[d], 0, 0, 0);
+        }
+    }
+    if (t + 1 < tend) stage(t + 1);
+    __syncthreads();
+  }
+
+  sum = halves_sum(sum);
+  if (!live) return;
+  const int64_t at = (int64_t)(begin + tok) * c.num_kv * gqa + h * gqa + hd;
+  if (parts == 1) {
+    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        store1<TYPE>(L.out, at * DH + 32 * d + 8 * (i >> 2) + 4 * half + (i & 3), sum == 0.f ? 0.f : acc[d][i] * inv);
+    if (L.lse && half == 0) L.lse[at] = sum == 0.f ? -INFINITY : (ref + log2_of(sum)) * 0.693147180559945f;
+  } else {
+    float* o = partials + ((slot * c.num_kv + h) * splits + z) * split_floats(DH);
+    const int row = wave * 32 + col;
+    if (half == 0) {
+      o[row] = ref;
+      o[kRowTile + row] = sum;
+    }
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *(floatx4*)&o[2 * kRowTile + row * DH + 32 * d + 8 * i + 4 * half] =
+            floatx4{acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]};
+  }
+}
+
+// Joins the splits of each row; one wave per (row, query head).
+template <int TYPE, int DH>
+__global__ __launch_bounds__(256) void cache8_prefill_merge_kernel(Cache8AttendLaunch L, int splits, const float* partials) {
+  const Cache8& c = L.c;
+  const Cache8Batch& b = L.b;
+  const int heads = c.num_kv * L.gqa, lane = threadIdx.x & 63;
+  const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), row = at / heads;
+  if (row >= b.num_rows) return;
+  const int hq = (int)(at - row * heads), h = hq / L.gqa;
+  const int s = seq_of_slot(b, row, 1, 0, 0);
+  int begin, end;
+  rows_of(b, s, begin, end);
+  if (row < begin || row >= end) return;
+  const int n = end - begin, len = seq_tokens(c, b, s);
+  const int64_t r = (row - begin) * L.gqa + hq - h * L.gqa, rows_all = (int64_t)n * L.gqa, r0 = r & ~(int64_t)(kRowTile - 1);
+  const int last = (int)((r0 + kRowTile < rows_all ? r0 + kRowTile : rows_all) - 1);
+  const int parts = splits_of(tile_seen(L, len, n, last / L.gqa), splits);
+  if (parts == 1) return;
+  const int64_t slot = first_slot(b, s, L.gqa, 7, 1) + (r >> 7);
+  const int in = (int)(r & (kRowTile - 1));
+  const float* x = partials + (slot * c.num_kv + h) * splits * split_floats(DH);
+  constexpr int DPL = DH / 64;
+  float R = kNoScore;
+  for (int z = lane; z < parts; z += kWave) R = fmaxf(R, x[z * split_floats(DH) + in]);
+  R = wave_max(R);
+  float l = 0.f, acc[DPL] = {};
+#pragma unroll 4
+  for (int z = 0; z < parts; ++z) {
+    const float* p = x + z * split_floats(DH);
+    const float f = exp2_of(p[in] - R);
+    l = fmaf(p[kRowTile + in], f, l);
+#pragma unroll
+    for (int i = 0; i < DPL; ++i) acc[i] = fmaf(p[2 * kRowTile + in * DH + lane * DPL + i], f, acc[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < DPL; ++i) store1<TYPE>(L.out, at * DH + lane * DPL + i, l == 0.f ? 0.f : acc[i] / l);
+  if (L.lse && lane == 0) L.lse[at] = l == 0.f ? -INFINITY : (R + log2_of(l)) * 0.693147180559945f;
+}
+
 template <template <int, int, int> class K, class... A>
 int pick(int type, int fmt, int dh, A... a) {
 #define SPHKV_PICK(T, F, D) if (type == T && fmt == F && dh == D) return K<T, F, D>::go(a...)
@@ -719,16 +971,6 @@ template <int T, int F, int D> struct Read {
     return hipPeekAtLastError() == hipSuccess ? 0 : -1;
   }
 };
-template <int T, int F, int D> struct Attend {
-  static int go(const Cache8AttendLaunch& L, hipStream_t st) {
-    const int64_t rows = L.b.num_rows;
-    const dim3 grid(L.c.num_kv * L.gqa, (unsigned)(rows < 32768 ? rows : 32768), (unsigned)((rows + 32767) / 32768));
-    if constexpr (T == kFp32) return -1;
-    else cache8_attend_kernel<T, F, D><<<grid, 256, 0, st>>>(L);
-    return hipPeekAtLastError() == hipSuccess ? 0 : -1;
-  }
-};
-
 template <int T, int F, int D> struct Decode {
   static int go(const Cache8AttendLaunch& L, hipStream_t st) {
     if constexpr (T == kFp32) {
@@ -743,6 +985,23 @@ template <int T, int F, int D> struct Decode {
   }
 };
 
+template <int T, int F, int D> struct Prefill {
+  static int go(const Cache8AttendLaunch& L, hipStream_t st) {
+    if constexpr (T == kFp32) {
+      return -1;
+    } else {
+      const int64_t tiles = row_tiles(L.b.num_rows, L.b.num_seqs, L.gqa);
+      const int splits = prefill_splits(L.b.num_rows, L.b.num_seqs, L.c.num_kv, L.gqa);
+      cache8_prefill_kernel<F, T, D><<<dim3((unsigned)(tiles * L.c.num_kv), splits), 256, 0, st>>>(L, splits, (float*)L.ws);
+      if (splits > 1) {
+        const int64_t waves = L.b.num_rows * L.c.num_kv * L.gqa;
+        cache8_prefill_merge_kernel<T, D><<<(unsigned)((waves + 3) / 4), 256, 0, st>>>(L, splits, (const float*)L.ws);
+      }
+      return hipPeekAtLastError() == hipSuccess ? 0 : -1;
+    }
+  }
+};
+
 }  // namespace
 
 int launch_cache8_write(const Cache8RowsLaunch& L, hipStream_t stream) {
@@ -752,11 +1011,15 @@ int launch_cache8_read(const Cache8RowsLaunch& L, hipStream_t stream) {
   return pick<Read>(L.type, L.c.fmt, L.c.dh, L, stream);
 }
 int launch_cache8_attend(const Cache8AttendLaunch& L, hipStream_t stream) {
-  return L.b.cu ? pick<Attend>(L.type, L.c.fmt, L.c.dh, L, stream) : pick<Decode>(L.type, L.c.fmt, L.c.dh, L, stream);
+  return L.b.cu ? pick<Prefill>(L.type, L.c.fmt, L.c.dh, L, stream) : pick<Decode>(L.type, L.c.fmt, L.c.dh, L, stream);
 }
 int64_t cache8_decode_ws_bytes(int32_t num_seqs, int32_t, int32_t gqa, int32_t dh) {
   return plan_bytes(num_seqs) + 2 * kDecodeGroups * 4 * partial8_floats(gqa, dh);
 }
-int64_t cache8_prefill_ws_bytes(int64_t, int32_t, int32_t, int32_t, int32_t) { return 0; }
+int64_t cache8_prefill_ws_bytes(int64_t num_rows, int32_t num_seqs, int32_t num_kv, int32_t gqa, int32_t dh) {
+  if (num_rows == 0 || num_seqs == 0) return 0;
+  const int splits = prefill_splits(num_rows, num_seqs, num_kv, gqa);
+  return splits == 1 ? 0 : row_tiles(num_rows, num_seqs, gqa) * num_kv * splits * split_floats(dh) * 4;
+}
 
 }  // namespace sphkv

@@ -63,17 +63,21 @@ def same_cache(cache, want, what):
         assert np.array_equal(a, b, equal_nan=True), f"{what}: {(a != b).sum()} {name} codes differ"
 
 
-def check_attention(out, lse, want, want_lse, mass, reach, dtype, dh, what):
+def check_attention(out, lse, want, want_lse, mass, reach, under, dtype, dh, what):
     """|out - want| against the roundings that the operator makes.  A score's sum
     of dh products, its scaling and its exponent in fp32 are off by at most
     delta = 2^-24 ((dh + 16) sum|q k| + 8 |score|) + 2^-21 (|score| is at most
     sum|q k|), which moves a weight by that factor, above and below the
-    division; a weight is rounded to fp16 (2^-11 of it, or half of the
-    smallest fp16 of a range whose top weights are over 2^8: under 2^-32 of
-    them a token); the output is rounded once more, by half a step."""
+    division.  A weight w_t ~ p_t sv_t is rounded to fp16: by 2^-11 of it, or by
+    2^-25, half of the smallest fp16 step.  The largest weight is at least 2^8
+    then, so w = 1 is at most 2^-8 max(p sv), and 2^-25 for every token and its
+    code moves an output by at most 2^-33 max_t(p_t sv_t) sum_t |code_t|
+    (`under`).  The output is rounded once more, by half a step (2^-25 at least
+    in fp16)."""
     out, lse = out.double().cpu().numpy(), lse.double().cpu().numpy()
     delta = 2.0 ** -24 * (dh + 24) * reach + 2.0 ** -21
-    tol = (2.0 ** -11 + 2.2 * delta)[..., None] * mass + torch.finfo(dtype).eps / 2 * np.abs(want) + 2.0 ** -25
+    tol = (2.0 ** -11 + 2.2 * delta)[..., None] * mass + 2.0 ** -33 * under \
+        + torch.finfo(dtype).eps / 2 * np.abs(want) + 2.0 ** -25
     err = np.abs(out - want)
     log(f"  {what}: max err {err.max(initial=0):.3g}, {(err / tol).max(initial=0):.3f} of the bound")
     assert (err <= tol).all(), f"{what}: {(err > tol).sum()} outputs off"

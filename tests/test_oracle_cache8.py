@@ -74,12 +74,12 @@ def test_attention_of_the_oracle_is_softmax():
     x = rng.standard_normal((60, 2, 64))
     c.write(x, x[::-1], table, [0, 0], [0, 40, 60])
     q = rng.standard_normal((5, 4, 64))
-    out, lse, _, _ = c.attend(q, table, [40, 20], [0, 3, 5])
+    out, lse, *_ = c.attend(q, table, [40, 20], [0, 3, 5])
     k, v, _ = c.tokens(table, 0, 0, 39)                          # row 1 of sequence 0: positions 0..38
     s = k[:, 1] @ q[1, 3] / 8.0
     p = np.exp(s - s.max())
     assert np.allclose(out[1, 3], p @ v[:, 1] / p.sum(), rtol=1e-12) and np.isclose(lse[1, 3], np.log(np.exp(s).sum()))
-    out, lse, _, _ = c.attend(q[:2], table, [0, 7])
+    out, lse, *_ = c.attend(q[:2], table, [0, 7])
     assert (out[0] == 0).all() and (lse[0] == -np.inf).all() and np.isfinite(lse[1]).all()
 
 
