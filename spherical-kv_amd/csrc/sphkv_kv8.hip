@@ -10,6 +10,8 @@
 namespace sphkv {
 namespace {
 
+typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
+
 constexpr float kLeastScale = 0x1p-60f, kMostScale = 0x1p60f;
 
 __device__ __forceinline__ int clampi(int64_t x, int64_t lo, int64_t hi) {
@@ -57,13 +59,6 @@ __device__ __forceinline__ int page_of(const Cache8& c, const Cache8Batch& b, in
 }
 
 template <int TYPE>
-__device__ __forceinline__ float load1(const void* p, int64_t i) {
-  if constexpr (TYPE == kFp16) return (float)((const _Float16*)p)[i];
-  if constexpr (TYPE == kBf16) return __builtin_bit_cast(float, (uint32_t)((const uint16_t*)p)[i] << 16);
-  return ((const float*)p)[i];
-}
-
-template <int TYPE>
 __device__ __forceinline__ void store1(void* p, int64_t i, float x) {
   if constexpr (TYPE == kFp16) ((_Float16*)p)[i] = (_Float16)x;
   else if constexpr (TYPE == kBf16) ((__bf16*)p)[i] = (__bf16)x;
@@ -74,6 +69,18 @@ template <int FMT>
 __device__ __forceinline__ float decode1(uint8_t c) {
   if constexpr (FMT == kCache8Int8) return (float)(int8_t)c;
   return __builtin_amdgcn_cvt_f32_fp8(c, 0);
+}
+
+// byte k (a constant after unrolling) of four codes
+template <int FMT>
+__device__ __forceinline__ float decode_byte(uint32_t x, int k) {
+  if constexpr (FMT == kCache8Int8) return (float)(int8_t)(x >> (8 * k));
+  switch (k) {
+    case 0: return __builtin_amdgcn_cvt_f32_fp8(x, 0);
+    case 1: return __builtin_amdgcn_cvt_f32_fp8(x, 1);
+    case 2: return __builtin_amdgcn_cvt_f32_fp8(x, 2);
+    default: return __builtin_amdgcn_cvt_f32_fp8(x, 3);
+  }
 }
 
 // The scale of a block whose largest finite magnitude is a.
@@ -97,16 +104,26 @@ __device__ __forceinline__ float block_scale(float a) {
 // comparison with s / 2 puts r right.  e4m3: s is a power of two, so x * inv is
 // exact and rounded once.
 template <int FMT>
-__device__ __forceinline__ uint8_t code_of(float x, float s, float inv) {
-  if (!(x == x)) return 0;
+__device__ __forceinline__ float scaled(float x, float s, float inv) {
+  x = x == x ? x : 0.f;
   if constexpr (FMT == kCache8Int8) {
     float r = fminf(fmaxf(rintf(x * inv), -127.f), 127.f);
-    const float d = fmaf(-r, s, x), h = 0.5f * s;
-    if (fabsf(d) > h || (fabsf(d) == h && ((int)r & 1))) r += d > 0.f ? 1.f : -1.f;
-    return (uint8_t)(int)fminf(fmaxf(r, -127.f), 127.f);
+    const float d = fmaf(-r, s, x), h = 0.5f * s, a = fabsf(d);
+    const bool off = (a > h) | ((a == h) & ((int)r & 1));
+    r += off ? __builtin_copysignf(1.f, d) : 0.f;
+    return fminf(fmaxf(r, -127.f), 127.f);
   }
-  const float y = fminf(fmaxf(x * inv, -448.f), 448.f);
-  return (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(y, y, 0, false);
+  return fminf(fmaxf(x * inv, -448.f), 448.f);
+}
+template <int FMT>
+__device__ __forceinline__ uint32_t code4(float x, float y, float z, float w, float s, float inv) {
+  x = scaled<FMT>(x, s, inv);
+  y = scaled<FMT>(y, s, inv);
+  z = scaled<FMT>(z, s, inv);
+  w = scaled<FMT>(w, s, inv);
+  if constexpr (FMT == kCache8Int8)
+    return ((uint32_t)(int)x & 255u) | ((uint32_t)(int)y & 255u) << 8 | ((uint32_t)(int)z & 255u) << 16 | (uint32_t)(int)w << 24;
+  return __builtin_amdgcn_cvt_pk_fp8_f32(z, w, __builtin_amdgcn_cvt_pk_fp8_f32(x, y, 0, false), true);
 }
 
 // A code of scale s as a code of scale t > s (both exact in 64 bits).
@@ -117,106 +134,354 @@ __device__ __forceinline__ uint8_t recode(uint8_t c, float s, float t) {
   return (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32((float)y, (float)y, 0, false);
 }
 
+// over the 16 lanes of each row by rotation, then over the rows
+template <int N>
+__device__ __forceinline__ float row_rotated(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), 0x120 + N, 0xF, 0xF, true));
+}
 __device__ __forceinline__ float wave_max(float x) {
-  for (int m = 1; m < kWave; m <<= 1) x = fmaxf(x, shfl_xor(x, m));
-  return x;
+  x = fmaxf(x, row_rotated<8>(x));
+  x = fmaxf(x, row_rotated<4>(x));
+  x = fmaxf(x, row_rotated<2>(x));
+  x = fmaxf(x, row_rotated<1>(x));
+  return rows_max(x);
 }
 
-// One wave per (touched page, kv head).
-template <int TYPE, int FMT, int DH>
-__global__ __launch_bounds__(256) void cache8_write_kernel(Cache8RowsLaunch L, int64_t slots) {
-  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63;
+// ---- write and read ------------------------------------------------------------
+//
+// Both move bytes: 2 * 16 * DH elements of a run of 16 tokens in and out per
+// wave, once.  A lane takes 16 bytes of a key row at a time; of the values, which
+// lie token-minor, two dims of all its tokens (of 8 at DH 64, the lane's half
+// saying which), so that the transposition is the lane's own.
+
+template <int TYPE> struct Elem { typedef uint16_t T; static constexpr int kVec = 8; };
+template <> struct Elem<kFp32> { typedef float T; static constexpr int kVec = 4; };
+
+template <int TYPE>
+__device__ __forceinline__ float value_of(typename Elem<TYPE>::T x) {
+  if constexpr (TYPE == kFp16) return (float)__builtin_bit_cast(_Float16, x);
+  else if constexpr (TYPE == kBf16) return __builtin_bit_cast(float, (uint32_t)x << 16);
+  else return x;
+}
+template <int TYPE>
+__device__ __forceinline__ typename Elem<TYPE>::T element_of(float x) {
+  if constexpr (TYPE == kFp16) return __builtin_bit_cast(uint16_t, (_Float16)x);
+  else if constexpr (TYPE == kBf16) return __builtin_bit_cast(uint16_t, (__bf16)x);
+  else return x;
+}
+
+// N consecutive elements at any alignment that theirs allows
+template <class T, int N>
+struct __attribute__((packed, aligned(sizeof(T)))) Unaligned { T x[N]; };
+
+// |x|, or 0 where x is not finite
+__device__ __forceinline__ float finite_abs(float x) {
+  x = fabsf(x);
+  return x < INFINITY ? x : 0.f;
+}
+
+// Largest magnitude of a lane's elements by their bits (two at a time where they
+// have 16), infinities and NaN at the top.
+typedef uint16_t ushort2v __attribute__((ext_vector_type(2)));
+template <int TYPE>
+struct Top {
+  uint32_t bits = 0;
+  template <int N>
+  __device__ __forceinline__ void add(const typename Elem<TYPE>::T (&x)[N]) {
+    if constexpr (TYPE == kFp32) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) bits = max(bits, __builtin_bit_cast(uint32_t, x[i]) & 0x7FFFFFFFu);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; i += 2) {
+        const uint32_t y = ((uint32_t)x[i] | (uint32_t)x[i + 1] << 16) & 0x7FFF7FFFu;
+        bits = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(ushort2v, bits), __builtin_bit_cast(ushort2v, y)));
+      }
+    }
+  }
+  __device__ __forceinline__ float value() const {
+    if constexpr (TYPE == kFp32) return __builtin_bit_cast(float, bits);
+    else return value_of<TYPE>((uint16_t)max(bits & 0xFFFFu, bits >> 16));
+  }
+};
+
+// Four codes in the plain case (finite values that the scale reaches), and
+// `worst`, to which they raise |x - code s|.  int8: x / s + 1.5 * 2^23 has the
+// rounded quotient in its low byte; where `worst` stays below s / 2 by more than
+// the product can be off, all are the nearest.  e4m3: exact.
+constexpr float kRoundInt = 12582912.f;
+template <int FMT>
+__device__ __forceinline__ uint32_t plain_code4(const float (&x)[4], float s, float inv, float& worst) {
+  if constexpr (FMT == kCache8Int8) {
+    uint32_t y[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float r = fmaf(x[i], inv, kRoundInt);
+      y[i] = __builtin_bit_cast(uint32_t, r);
+      worst = fmaxf(worst, fabsf(fmaf(kRoundInt - r, s, x[i])));
+    }
+    return __builtin_amdgcn_perm(__builtin_amdgcn_perm(y[3], y[2], 0x0C0C0400u), __builtin_amdgcn_perm(y[1], y[0], 0x0C0C0400u), 0x05040100u);
+  }
+  return __builtin_amdgcn_cvt_pk_fp8_f32(x[2] * inv, x[3] * inv, __builtin_amdgcn_cvt_pk_fp8_f32(x[0] * inv, x[1] * inv, 0, false), true);
+}
+// whether plain_code4's codes hold
+template <int FMT>
+__device__ __forceinline__ bool plain_holds(float top, float s, float worst) {
+  return top < INFINITY && s < kMostScale && (FMT == kCache8E4M3 || worst < s * (0.5f - 0x1p-14f));
+}
+
+// Workgroups of whole pages: RUNS waves a page, at least four waves.
+template <int TYPE, int FMT, int DH, int RUNS>
+__global__ __launch_bounds__(RUNS == 8 ? 512 : 256) void cache8_write_kernel(Cache8RowsLaunch L, uint32_t items) {
+  constexpr int kWaves = RUNS == 8 ? 8 : 4, kPages = kWaves / RUNS;
+  constexpr int VEC = Elem<TYPE>::kVec, LPR = DH / VEC, RPL = 64 / LPR, KN = 16 / RPL;   // lanes a row, rows a load, loads
+  constexpr int VT = DH / 8;                                         // tokens of a lane's values: 16 (DH 128) or 8
+  typedef typename Elem<TYPE>::T E;
+  __shared__ float s_top[2][kWaves];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, run = wave % RUNS;
   const Cache8& c = L.c;
   const Cache8Batch& b = L.b;
-  if (w >= slots * c.num_kv) return;
-  const int64_t j = w / c.num_kv;
-  const int h = (int)(w - j * c.num_kv), ps = 1 << c.page_shift;
-  int s, begin, end;
-  int64_t jj = 0;
-  if (b.cu) {
-    s = seq_of_slot(b, j, 1, c.page_shift, 2);
-    jj = j - first_slot(b, s, 1, c.page_shift, 2);
-  } else {
-    s = (int)j;
+  const uint32_t item = blockIdx.x * kPages + wave / RUNS;
+  const uint32_t j = item / c.num_kv;
+  const int h = (int)(item - j * c.num_kv);
+  constexpr int ps = 16 * RUNS;
+  int o = 0, e = 0, page = -1;                                        // the page's new slots o .. e - 1
+  int64_t row0 = 0;                                                   // row of slot o
+  if (item < items) {
+    int s = (int)j, begin, end;
+    int64_t jj = 0;
+    if (b.cu) {
+      s = uniform(seq_of_slot(b, j, 1, c.page_shift, 2));
+      jj = j - first_slot(b, s, 1, c.page_shift, 2);
+    }
+    rows_of(b, s, begin, end);
+    const int64_t start = b.at[s], blk = start / ps + jj, left = start + (end - begin) - blk * ps;
+    if (start >= 0 && left > 0) {
+      o = jj ? 0 : (int)(start & (ps - 1));
+      e = left < ps ? (int)left : ps;
+      if (o < e) page = uniform(page_of(c, b, s, blk));
+      row0 = begin + (blk * ps + o - start);
+    }
   }
-  rows_of(b, s, begin, end);
-  const int64_t start = b.at[s];
-  if (start < 0) return;
-  const int64_t blk = (start >> c.page_shift) + jj, pos0 = blk << c.page_shift;
-  const int o = jj ? 0 : (int)(start & (ps - 1));                     // first new slot of the page
-  const int64_t left = start + (end - begin) - pos0;
-  const int e = left < ps ? (int)left : ps;                           // one past the last
-  const int page = page_of(c, b, s, blk);
-  if (page < 0 || o >= e) return;
-  const int64_t row0 = begin + (pos0 + o - start);                    // row of slot o
-  const int64_t ph = (int64_t)page * c.num_kv + h;
-  uint8_t* kc = c.k + ph * ps * DH;
-  uint8_t* vc = c.v + ph * ps * DH;
-  for (int which = 0; which < 2; ++which) {
-    const void* x = which ? L.v : L.k;
-    const int64_t rs = which ? L.v_row : L.k_row, at = h * (which ? L.v_head : L.k_head);
-    float a = 0.f;
-    for (int t = o; t < e; ++t)
-      for (int d = lane; d < DH; d += 64) {
-        const float y = fabsf(load1<TYPE>(x, (row0 + t - o) * rs + at + d));
-        if (y < INFINITY) a = fmaxf(a, y);
-      }
-    a = wave_max(a);
-    const float old = c.scales[2 * ph + which];
-    float sc = block_scale<FMT>(a);
-    if (o > 0 && !(sc > old)) sc = old;
-    const float inv = __fdiv_rn(1.0f, sc);
-    if (o > 0 && sc > old)
-      for (int t = 0; t < o; ++t)
-        for (int d = lane; d < DH; d += 64) {
-          uint8_t* p = which ? vc + (t >> 4) * 16 * DH + d * 16 + (t & 15) : kc + t * DH + d;
-          *p = recode<FMT>(*p, old, sc);
+  const bool any = page >= 0 && o < e;
+  const int lo = any ? min(max(o - 16 * run, 0), 16) : 0, hi = any ? min(max(e - 16 * run, 0), 16) : 0;
+  const int64_t ph = (int64_t)(any ? page : 0) * c.num_kv + h;
+  const int64_t first = row0;
+  row0 += 16 * run - o;                                               // row of this run's token 0
+  uint8_t* kc = c.k + (ph * ps + 16 * run) * DH;
+  uint8_t* vc = c.v + (ph * ps + 16 * run) * DH;
+  const int krow = lane / LPR, kdim = VEC * (lane % LPR);             // key rows krow + RPL i, dims kdim ..
+  const int vdim = 2 * (lane & (DH / 2 - 1)), vtok = DH == 128 ? 0 : 8 * (lane >> 5);
+  // every lane loads, the page's first new row where its own is none (a branch
+  // around a load would wait for each, and that row changes no maximum)
+  const int64_t other = any ? first : 0;
+  Unaligned<E, VEC> kx[KN];
+  Unaligned<E, 2> vx[VT];
+#pragma unroll
+  for (int i = 0; i < KN; ++i) {
+    const int t = krow + RPL * i;
+    const int64_t row = t >= lo && t < hi ? row0 + t : other;
+    kx[i] = *(const Unaligned<E, VEC>*)((const E*)L.k + row * L.k_row + h * L.k_head + kdim);
+  }
+#pragma unroll
+  for (int i = 0; i < VT; ++i) {
+    const int t = vtok + i;
+    const int64_t row = t >= lo && t < hi ? row0 + t : other;
+    vx[i] = *(const Unaligned<E, 2>*)((const E*)L.v + row * L.v_row + h * L.v_head + vdim);
+  }
+  float kold = 0.f, vold = 0.f;
+  if (any) {
+    kold = c.scales[2 * ph];
+    vold = c.scales[2 * ph + 1];
+  }
+  Top<TYPE> km, vm;
+#pragma unroll
+  for (int i = 0; i < KN; ++i) km.add(kx[i].x);
+#pragma unroll
+  for (int i = 0; i < VT; ++i) vm.add(vx[i].x);
+  float ktop = km.value(), vtop = vm.value();
+  const bool kfine = !__any(!(ktop < INFINITY)), vfine = !__any(!(vtop < INFINITY));
+  if (!kfine) {
+    ktop = 0.f;
+#pragma unroll
+    for (int i = 0; i < KN; ++i)
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) ktop = fmaxf(ktop, finite_abs(value_of<TYPE>(kx[i].x[v])));
+  }
+  if (!vfine) {
+    vtop = 0.f;
+#pragma unroll
+    for (int i = 0; i < VT; ++i) vtop = fmaxf(vtop, fmaxf(finite_abs(value_of<TYPE>(vx[i].x[0])), finite_abs(value_of<TYPE>(vx[i].x[1]))));
+  }
+  ktop = wave_max(ktop);
+  vtop = wave_max(vtop);
+  if constexpr (RUNS > 1) {
+    if (lane == 0) {
+      s_top[0][wave] = ktop;
+      s_top[1][wave] = vtop;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < RUNS; ++w) {
+      ktop = fmaxf(ktop, s_top[0][wave - run + w]);
+      vtop = fmaxf(vtop, s_top[1][wave - run + w]);
+    }
+  }
+  if (!any) return;
+  float ks = block_scale<FMT>(ktop), vs = block_scale<FMT>(vtop);
+  if (o > 0 && !(ks > kold)) ks = kold;
+  if (o > 0 && !(vs > vold)) vs = vold;
+  if (run == 0 && lane == 0) *(float2*)(c.scales + 2 * ph) = float2{ks, vs};
+  // (every wave of a page has read the old scales: before the barrier, or itself)
+  const float kinv = __fdiv_rn(1.0f, ks), vinv = __fdiv_rn(1.0f, vs);
+  uint32_t ky[KN][VEC / 4], vy[2][VT / 4];
+  float kworst = 0.f, vworst = 0.f;
+#pragma unroll
+  for (int i = 0; i < KN; ++i)
+#pragma unroll
+    for (int k = 0; k < VEC / 4; ++k) {
+      const float x[4] = {value_of<TYPE>(kx[i].x[4 * k]), value_of<TYPE>(kx[i].x[4 * k + 1]),
+                          value_of<TYPE>(kx[i].x[4 * k + 2]), value_of<TYPE>(kx[i].x[4 * k + 3])};
+      ky[i][k] = plain_code4<FMT>(x, ks, kinv, kworst);
+    }
+#pragma unroll
+  for (int d = 0; d < 2; ++d)
+#pragma unroll
+    for (int k = 0; k < VT / 4; ++k) {
+      const float x[4] = {value_of<TYPE>(vx[4 * k].x[d]), value_of<TYPE>(vx[4 * k + 1].x[d]),
+                          value_of<TYPE>(vx[4 * k + 2].x[d]), value_of<TYPE>(vx[4 * k + 3].x[d])};
+      vy[d][k] = plain_code4<FMT>(x, vs, vinv, vworst);
+    }
+  if (!kfine || __any(!plain_holds<FMT>(ktop, ks, kworst)))
+#pragma unroll
+    for (int i = 0; i < KN; ++i)
+#pragma unroll
+      for (int k = 0; k < VEC / 4; ++k)
+        ky[i][k] = code4<FMT>(value_of<TYPE>(kx[i].x[4 * k]), value_of<TYPE>(kx[i].x[4 * k + 1]),
+                              value_of<TYPE>(kx[i].x[4 * k + 2]), value_of<TYPE>(kx[i].x[4 * k + 3]), ks, kinv);
+  if (!vfine || __any(!plain_holds<FMT>(vtop, vs, vworst)))
+#pragma unroll
+    for (int d = 0; d < 2; ++d)
+#pragma unroll
+      for (int k = 0; k < VT / 4; ++k)
+        vy[d][k] = code4<FMT>(value_of<TYPE>(vx[4 * k].x[d]), value_of<TYPE>(vx[4 * k + 1].x[d]),
+                              value_of<TYPE>(vx[4 * k + 2].x[d]), value_of<TYPE>(vx[4 * k + 3].x[d]), vs, vinv);
+#pragma unroll
+  for (int i = 0; i < KN; ++i) {
+    const int t = krow + RPL * i;
+    if (t < lo || t >= hi) continue;
+    if constexpr (VEC == 8) *(uint2*)(kc + t * DH + kdim) = uint2{ky[i][0], ky[i][1]};
+    else *(uint32_t*)(kc + t * DH + kdim) = ky[i][0];
+  }
+  // codes held before, under a larger scale: rare
+  if (lo > 0 && ks > kold)
+#pragma unroll 1
+    for (int i = lane; i < lo * DH; i += kWave) kc[i] = recode<FMT>(kc[i], kold, ks);
+  if (lo > 0 && vs > vold)
+#pragma unroll 1
+    for (int i = 0; i < 2 * VT; ++i) {
+      uint8_t* p = vc + (vdim + i / VT) * 16 + vtok + i % VT;
+      if (vtok + i % VT < lo) *p = recode<FMT>(*p, vold, vs);
+    }
+  if (lo < hi) {
+#pragma unroll
+    for (int d = 0; d < 2; ++d) {
+      uint32_t (&y)[VT / 4] = vy[d];
+      uint32_t* p = (uint32_t*)(vc + (vdim + d) * 16 + vtok);
+      if (lo > 0 || hi < 16) {                                        // the run's other tokens keep their bytes
+#pragma unroll
+        for (int k = 0; k < VT / 4; ++k) {
+          const uint32_t was = p[k];
+          const int a = lo - vtok - 4 * k, z = hi - vtok - 4 * k;    // the dword's new bytes: a .. z - 1
+          const uint32_t upto = z >= 4 ? ~0u : (z <= 0 ? 0u : (1u << (8 * z)) - 1u);
+          const uint32_t from = a >= 4 ? 0u : (a <= 0 ? ~0u : ~((1u << (8 * a)) - 1u));
+          y[k] = (y[k] & upto & from) | (was & ~(upto & from));
         }
-    for (int t = o; t < e; ++t)
-      for (int d = lane; d < DH; d += 64) {
-        uint8_t* p = which ? vc + (t >> 4) * 16 * DH + d * 16 + (t & 15) : kc + t * DH + d;
-        *p = code_of<FMT>(load1<TYPE>(x, (row0 + t - o) * rs + at + d), sc, inv);
       }
-    if (lane == 0) c.scales[2 * ph + which] = sc;
+      if constexpr (VT == 16) *(uintx4*)p = uintx4{y[0], y[1], y[2], y[3]};
+      else *(uint2*)p = uint2{y[0], y[1]};
+    }
   }
 }
 
 // One wave per (16-token run, kv head).
 template <int TYPE, int FMT, int DH>
-__global__ __launch_bounds__(256) void cache8_read_kernel(Cache8RowsLaunch L, int64_t slots) {
-  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+__global__ __launch_bounds__(256) void cache8_read_kernel(Cache8RowsLaunch L, uint32_t items) {
+  constexpr int LPR = DH / 16, RPL = 64 / LPR, KN = 16 / RPL, VT = DH / 8;
+  typedef typename Elem<TYPE>::T E;
+  const uint32_t item = blockIdx.x * 4 + (threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   const Cache8& c = L.c;
   const Cache8Batch& b = L.b;
-  if (w >= slots * c.num_kv) return;
-  const int64_t j = w / c.num_kv;
-  const int h = (int)(w - j * c.num_kv), ps = 1 << c.page_shift;
-  int s, begin, end;
+  if (item >= items) return;
+  const uint32_t j = item / c.num_kv;
+  const int h = (int)(item - j * c.num_kv), ps = 1 << c.page_shift;
+  int s = (int)j, begin, end;
   int64_t jj = 0;
   if (b.cu) {
-    s = seq_of_slot(b, j, 1, 4, 2);
+    s = uniform(seq_of_slot(b, j, 1, 4, 2));
     jj = j - first_slot(b, s, 1, 4, 2);
-  } else {
-    s = (int)j;
   }
   rows_of(b, s, begin, end);
-  const int64_t start = b.at[s], pos0 = ((start >> 4) + jj) << 4;
-  const int o = jj ? 0 : (int)(start & 15);
-  const int64_t left = start + (end - begin) - pos0;
-  const int e = left < 16 ? (int)left : 16;
-  if (o >= e) return;
-  const int page = page_of(c, b, s, pos0 >> c.page_shift);
-  const int64_t ph = (int64_t)page * c.num_kv + h;
-  const int run = (int)(pos0 & (ps - 1)) >> 4;
-  const uint8_t* kc = c.k + (ph * ps + run * 16) * DH;
-  const uint8_t* vc = c.v + (ph * ps + run * 16) * DH;
-  const float sk = page < 0 ? 0.f : c.scales[2 * ph], sv = page < 0 ? 0.f : c.scales[2 * ph + 1];
-  for (int t = o; t < e; ++t) {
-    const int64_t row = begin + (pos0 + t - start);
-    for (int d = lane; d < DH; d += 64) {
-      if (L.k) store1<TYPE>(L.k, row * L.k_row + h * L.k_head + d, page < 0 ? 0.f : decode1<FMT>(kc[t * DH + d]) * sk);
-      if (L.v) store1<TYPE>(L.v, row * L.v_row + h * L.v_head + d, page < 0 ? 0.f : decode1<FMT>(vc[d * 16 + t]) * sv);
+  const int64_t start = b.at[s], pos0 = ((start >> 4) + jj) << 4, left = start + (end - begin) - pos0;
+  const int lo = jj ? 0 : (int)(start & 15), hi = left < 16 ? (int)left : 16;
+  if (lo >= hi) return;
+  const int page = uniform(page_of(c, b, s, pos0 >> c.page_shift));
+  const int64_t row0 = begin + (pos0 - start);                        // row of the run's token 0
+  uintx4 kx[KN], vx[2];
+  float sk = 0.f, sv = 0.f;
+  const int krow = lane / LPR, kdim = 16 * (lane % LPR);
+  const int vdim = 2 * (lane & (DH / 2 - 1)), vtok = DH == 128 ? 0 : 8 * (lane >> 5);
+#pragma unroll
+  for (int i = 0; i < KN; ++i) kx[i] = uintx4{0, 0, 0, 0};
+  vx[0] = vx[1] = uintx4{0, 0, 0, 0};
+  if (page >= 0) {
+    const int64_t ph = (int64_t)page * c.num_kv + h, at = (ph * ps + (pos0 & (ps - 1))) * DH;
+    if (L.k)
+#pragma unroll
+      for (int i = 0; i < KN; ++i) kx[i] = *(const uintx4*)(c.k + at + (krow + RPL * i) * DH + kdim);
+    if (L.v) {
+      if constexpr (VT == 16) {
+#pragma unroll
+        for (int d = 0; d < 2; ++d) vx[d] = *(const uintx4*)(c.v + at + (vdim + d) * 16);
+      } else {
+#pragma unroll
+        for (int d = 0; d < 2; ++d) {
+          const uint2 x = *(const uint2*)(c.v + at + (vdim + d) * 16 + vtok);
+          vx[d].x = x.x;
+          vx[d].y = x.y;
+        }
+      }
+    }
+    const float2 sc = *(const float2*)(c.scales + 2 * ph);
+    sk = sc.x;
+    sv = sc.y;
+  }
+  if (L.k) {
+#pragma unroll
+    for (int i = 0; i < KN; ++i) {
+      const int t = krow + RPL * i;
+      if (t < lo || t >= hi) continue;
+      constexpr int N = 16 / sizeof(E);                               // elements of a 16-byte store
+      E* p = (E*)L.k + (row0 + t) * L.k_row + h * L.k_head + kdim;
+#pragma unroll
+      for (int k = 0; k < 16 / N; ++k) {
+        struct __attribute__((aligned(16))) { E x[N]; } y;
+#pragma unroll
+        for (int n = 0; n < N; ++n) y.x[n] = element_of<TYPE>(decode_byte<FMT>(kx[i][(k * N + n) / 4], n & 3) * sk);
+        *(decltype(y)*)(p + k * N) = y;
+      }
+    }
+  }
+  if (L.v) {
+#pragma unroll
+    for (int i = 0; i < VT; ++i) {
+      const int t = vtok + i;
+      if (t < lo || t >= hi) continue;
+      struct __attribute__((aligned(2 * sizeof(E)))) { E x[2]; } y;
+#pragma unroll
+      for (int d = 0; d < 2; ++d) y.x[d] = element_of<TYPE>(decode_byte<FMT>(vx[d][i / 4], i & 3) * sv);
+      *(decltype(y)*)((E*)L.v + (row0 + t) * L.v_row + h * L.v_head + vdim) = y;
     }
   }
 }
@@ -251,7 +516,6 @@ constexpr float kTopWeight = 8.0f;      // log2 of the weight at the reference, 
 constexpr float kSlackWeight = 4.0f;    // ... which moves once a weight passes 2^4 times that
 constexpr float kNoScore = -3.0e38f;    // reference before the first score
 
-typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
 
 // heads handled together: a kv head's first 16, next 16, ...
 __host__ __device__ __forceinline__ int head_parts(int gqa) { return (gqa + 15) / 16; }
@@ -959,15 +1223,20 @@ int64_t row_slots(const Cache8Batch& b, int shift) {
 
 template <int T, int F, int D> struct Write {
   static int go(const Cache8RowsLaunch& L, hipStream_t st) {
-    const int64_t slots = row_slots(L.b, L.c.page_shift), waves = slots * L.c.num_kv;
-    cache8_write_kernel<T, F, D><<<dim3((unsigned)((waves + 3) / 4)), 256, 0, st>>>(L, slots);
+    const uint32_t items = (uint32_t)(row_slots(L.b, L.c.page_shift) * L.c.num_kv);
+    switch (L.c.page_shift) {
+      case 4: cache8_write_kernel<T, F, D, 1><<<(items + 3) / 4, 256, 0, st>>>(L, items); break;
+      case 5: cache8_write_kernel<T, F, D, 2><<<(items + 1) / 2, 256, 0, st>>>(L, items); break;
+      case 6: cache8_write_kernel<T, F, D, 4><<<items, 256, 0, st>>>(L, items); break;
+      default: cache8_write_kernel<T, F, D, 8><<<items, 512, 0, st>>>(L, items);
+    }
     return hipPeekAtLastError() == hipSuccess ? 0 : -1;
   }
 };
 template <int T, int F, int D> struct Read {
   static int go(const Cache8RowsLaunch& L, hipStream_t st) {
-    const int64_t slots = row_slots(L.b, 4), waves = slots * L.c.num_kv;
-    cache8_read_kernel<T, F, D><<<dim3((unsigned)((waves + 3) / 4)), 256, 0, st>>>(L, slots);
+    const uint32_t items = (uint32_t)(row_slots(L.b, 4) * L.c.num_kv);
+    cache8_read_kernel<T, F, D><<<(items + 3) / 4, 256, 0, st>>>(L, items);
     return hipPeekAtLastError() == hipSuccess ? 0 : -1;
   }
 };
