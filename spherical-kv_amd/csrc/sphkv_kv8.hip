@@ -1008,49 +1008,49 @@ __global__ __launch_bounds__(256, 2) void cache8_prefill_kernel(Cache8AttendLaun
   // A wave's part of a tile: 16 codes of DH/64 key rows and as many value rows a
   // thread, of runs that are the same for the wave.
   uintx4 kraw[PER], vraw[PER];
+  float2 scraw[PER];
+  int page[PER], ahead[PER];                                        // of the tile that is fetched next, and of the one after it
   auto run_of = [&](int i) { return DH == 128 ? 2 * i + (wave >> 1) : wave; };
+  const int in = DH == 128 ? tid & 127 : lane;                       // this thread's 16 bytes of a run's DH * 16
+  auto find = [&](int t) {                                           // (waited for a tile later)
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int at = t * kTileTokens + run_of(i) * 16, blk = at >> c.page_shift;
+      ahead[i] = t < tend && at < len && blk < b.max_blocks ? table[blk] : -1;
+    }
+  };
   auto fetch = [&](int t) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int run = run_of(i), at = t * kTileTokens + run * 16;
-      kraw[i] = vraw[i] = uintx4{0, 0, 0, 0};
-      const int blk = at >> c.page_shift;
-      int pg = at < len && blk < b.max_blocks ? uniform(table[blk]) : -1;
-      if (pg >= c.num_pages) pg = -1;
-      float sk = 1.f, lsv = -INFINITY, inv = 0.f;
-      if (pg >= 0) {
-        const int64_t base = pg * page_bytes + ((int64_t)h * DH << c.page_shift) + (at & ps_mask) * DH;
-        const int in = DH == 128 ? tid & 127 : lane;               // this thread's 16 bytes of the run's DH * 16
-        kraw[i] = *(const uintx4*)(c.k + base + 16 * in);
-        vraw[i] = *(const uintx4*)(c.v + base + 16 * in);
-        const float2 sc = *(const float2*)(c.scales + 2 * ((int64_t)pg * c.num_kv + h));
-        sk = sc.x;
-        lsv = log2_of(sc.y);
-        inv = exp2_of(-lsv);
-        const int have = len - at;                                  // tokens of the run that are there
-        if (have < 16) {
-          const int token = in / (DH / 16);
-          if (token >= have) kraw[i] = uintx4{0, 0, 0, 0};
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int m = have - 4 * k;
-            vraw[i][k] &= m >= 4 ? ~0u : (m <= 0 ? 0u : (1u << (8 * m)) - 1u);
-          }
-        }
-      }
-      if ((DH == 128 ? tid & 127 : lane) == 0) {
-        const int bf = t & 1;
-        s_sk[bf][run] = sk;
-        s_lsv[bf][run] = lsv;
-        s_inv[bf][run] = inv;
-      }
+      const int at = t * kTileTokens + run_of(i) * 16;
+      int pg = uniform(ahead[i]);
+      if (pg < 0 || pg >= c.num_pages) pg = -1;
+      page[i] = pg;
+      const int64_t p = pg < 0 ? 0 : pg, base = p * page_bytes + ((int64_t)h * DH << c.page_shift) + (at & ps_mask) * DH;
+      kraw[i] = *(const uintx4*)(c.k + base + 16 * in);
+      vraw[i] = *(const uintx4*)(c.v + base + 16 * in);
+      scraw[i] = *(const float2*)(c.scales + 2 * (p * c.num_kv + h));
     }
   };
   auto stage = [&](int t) {
     const int bf = t & 1;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int run = run_of(i), in = DH == 128 ? tid & 127 : lane;
+      const int run = run_of(i), have = page[i] < 0 ? 0 : len - t * kTileTokens - run * 16;   // tokens of the run that are there
+      if (have < 16) {
+        if (in / (DH / 16) >= have) kraw[i] = uintx4{0, 0, 0, 0};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int m = have - 4 * k;
+          vraw[i][k] &= m >= 4 ? ~0u : (m <= 0 ? 0u : (1u << (8 * m)) - 1u);
+        }
+      }
+      if (in == 0) {
+        const float lsv = have > 0 ? log2_of(scraw[i].y) : -INFINITY;
+        s_sk[bf][run] = have > 0 ? scraw[i].x : 1.f;
+        s_lsv[bf][run] = lsv;
+        s_inv[bf][run] = have > 0 ? exp2_of(-lsv) : 0.f;
+      }
       const int token = run * 16 + in / (DH / 16), chunk = 2 * (in % (DH / 16));
       *(half8*)&s_k[bf][k_at<DH>(token, chunk)] = codes8<FMT>(kraw[i].x, kraw[i].y);
       *(half8*)&s_k[bf][k_at<DH>(token, chunk + 1)] = codes8<FMT>(kraw[i].z, kraw[i].w);
@@ -1068,13 +1068,18 @@ __global__ __launch_bounds__(256, 2) void cache8_prefill_kernel(Cache8AttendLaun
   const int ktok = 16 * (col >> 4) + 8 * ((col >> 2) & 1) + 4 * ((col >> 3) & 1) + (col & 3);   // token of score row `col`
 
   if (tbeg < tend) {
+    find(tbeg);
     fetch(tbeg);
+    find(tbeg + 1);
     stage(tbeg);
   }
   __syncthreads();
   for (int t = tbeg; t < tend; ++t) {
     const int bf = t & 1, t0 = t * kTileTokens;
-    if (t + 1 < tend) fetch(t + 1);
+    if (t + 1 < tend) {
+      fetch(t + 1);
+      find(t + 2);
+    }
     if (t0 < lim_max) {
       floatx16 sc[2];
 #pragma unroll
