@@ -623,7 +623,7 @@ __global__ __launch_bounds__(256, 2) void cache8_decode_kernel(Cache8AttendLaunc
   __shared__ float s_acc[4][16][DH + 4];
   const Cache8& c = L.c;
   const Cache8Batch& b = L.b;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
   const int parts = head_parts(L.gqa), HV = c.num_kv * parts, n = b.num_seqs;
 
   // this workgroup's tiles
@@ -673,7 +673,6 @@ __global__ __launch_bounds__(256, 2) void cache8_decode_kernel(Cache8AttendLaunc
       const int64_t first = sbase + (int64_t)hv * T;
       const int t0 = (int)(p - first), t1 = pend - first < T ? (int)(pend - first) : T;
       const int mycol = twin ? (col & 7) : col;
-      const bool live = mycol < cols;
 
       // a column's query: dims 64 j + 16 g + 0..15 in lane group g
       half8 q[DH / 32];
@@ -681,23 +680,19 @@ __global__ __launch_bounds__(256, 2) void cache8_decode_kernel(Cache8AttendLaunc
       const int64_t row = (int64_t)s;
       {
         struct __attribute__((packed, aligned(2))) U4 { uintx4 v; };
-        const uint16_t* src = (const uint16_t*)L.q + row * L.q_row + (int64_t)(h * L.gqa + part * 16 + mycol) * L.q_head + 16 * g;
+        const int mine = mycol < cols ? mycol : 0;                           // (columns over: the first again, dropped at the end)
+        const uint16_t* src = (const uint16_t*)L.q + row * L.q_row + (int64_t)(h * L.gqa + part * 16 + mine) * L.q_head + 16 * g;
         uintx4 raw[DH / 32];
 #pragma unroll
-        for (int i = 0; i < DH / 32; ++i) {
-          raw[i] = uintx4{0, 0, 0, 0};
-          if (live) raw[i] = ((const U4*)(src + 64 * (i / 2) + 8 * (i & 1)))->v;
-        }
+        for (int i = 0; i < DH / 32; ++i) raw[i] = ((const U4*)(src + 64 * (i / 2) + 8 * (i & 1)))->v;
         query_fp16<TYPE, DH / 32>(raw, [](float m) { return rows_max(m); }, q, back);
       }
       const float cq = ldexpf(qscale, back);
 
-      // pages of run `run` of tile t, or -1
+      // page of run `run` of tile t, or -1
       auto page_at = [&](int t, int run) {
-        const int blk = (t * kTileTokens + run * 16) >> c.page_shift;
-        if (blk >= b.max_blocks || t * kTileTokens + run * 16 >= len) return -1;
-        const int pg = table[blk];
-        return pg >= 0 && pg < c.num_pages ? pg : -1;
+        const int at = t * kTileTokens + run * 16, blk = at >> c.page_shift, pg = table[min(blk, b.max_blocks - 1)];
+        return at < len && blk < b.max_blocks && pg < c.num_pages ? pg : -1;
       };
       Tile<DH> A;
       auto load_k = [&](int t, int kpage) {
@@ -727,17 +722,21 @@ __global__ __launch_bounds__(256, 2) void cache8_decode_kernel(Cache8AttendLaunc
       float ref = kNoScore, sum = 0.f;
 
       int t = t0 + wave;
-      int kp = -1, vp = -1, kp1 = -1, vp1 = -1;
+      // Every turn issues the same loads in the same order, so that it waits for
+      // this tile's and none of the next (a branch around a load makes the waits
+      // wait for all); the last one's are this tile's again.
+      int kp1, vp1;
       if (t < t1) {
-        kp = page_at(t, col >> 2);
-        vp = page_at(t, g);
-        kp1 = t + 4 < t1 ? page_at(t + 4, col >> 2) : -1;
-        vp1 = t + 4 < t1 ? page_at(t + 4, g) : -1;
+        const int kp = page_at(t, col >> 2), vp = page_at(t, g);
+        const int tn = t + 4 < t1 ? t + 4 : t;
+        kp1 = page_at(tn, col >> 2);
+        vp1 = page_at(tn, g);
         load_k(t, kp);
         load_v(t, vp);
       }
       for (; t < t1; t += 4) {
-        const int kp2 = t + 8 < t1 ? page_at(t + 8, col >> 2) : -1, vp2 = t + 8 < t1 ? page_at(t + 8, g) : -1;
+        const int tn = t + 4 < t1 ? t + 4 : t, t2 = t + 8 < t1 ? t + 8 : t;
+        const int kp2 = page_at(t2, col >> 2), vp2 = page_at(t2, g);
         // scores
         floatx4 sc[4];
 #pragma unroll
@@ -749,7 +748,7 @@ __global__ __launch_bounds__(256, 2) void cache8_decode_kernel(Cache8AttendLaunc
             sc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8<FMT>(A.k[i][j].z, A.k[i][j].w), q[2 * j + 1], sc[i], 0, 0, 0);
           }
         }
-        if (t + 4 < t1) load_k(t + 4, kp1);
+        load_k(tn, kp1);
         // tokens that are not there: behind the length, or of an absent page
         const int have = A.page < 0 ? 0 : len - t * kTileTokens - 16 * g;     // of this lane's 16
         if (__any(have < 16)) {
@@ -803,7 +802,7 @@ __global__ __launch_bounds__(256, 2) void cache8_decode_kernel(Cache8AttendLaunc
           acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8<FMT>(A.v[d].x, A.v[d].y), w[0], acc[d], 0, 0, 0);
           acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8<FMT>(A.v[d].z, A.v[d].w), w[1], acc[d], 0, 0, 0);
         }
-        if (t + 4 < t1) load_v(t + 4, vp1);
+        load_v(tn, vp1);
         kp1 = kp2;
         vp1 = vp2;
       }
@@ -953,7 +952,7 @@ __global__ __launch_bounds__(256, 2) void cache8_prefill_kernel(Cache8AttendLaun
   __shared__ float s_sk[2][4], s_lsv[2][4], s_inv[2][4];
   const Cache8& c = L.c;
   const Cache8Batch& b = L.b;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), col = lane & 31, half = lane >> 5;
   // neighbours take different heads (eight of them: one per XCD and its L2), and
   // the longest rows of a sequence come first
   const int h = blockIdx.x % c.num_kv, z = blockIdx.y, gqa = L.gqa;
@@ -992,12 +991,9 @@ __global__ __launch_bounds__(256, 2) void cache8_prefill_kernel(Cache8AttendLaun
   {
     struct __attribute__((packed, aligned(2))) U4 { uintx4 v; };
     const uint16_t* src = (const uint16_t*)L.q + (int64_t)(begin + tok) * L.q_row + (int64_t)(h * gqa + hd) * L.q_head + 8 * half;
-    uintx4 raw[KS];
+    uintx4 raw[KS];                                                 // (a lane without a row takes the first: dropped at the end)
 #pragma unroll
-    for (int i = 0; i < KS; ++i) {
-      raw[i] = uintx4{0, 0, 0, 0};
-      if (live) raw[i] = ((const U4*)(src + 16 * i))->v;
-    }
+    for (int i = 0; i < KS; ++i) raw[i] = ((const U4*)(src + 16 * i))->v;
     query_fp16<TYPE, KS>(raw, [](float m) { return halves_max(m); }, q, back);
   }
   const float cq = ldexpf(L.sm_scale * 1.44269504088896f, back);
@@ -1007,55 +1003,66 @@ __global__ __launch_bounds__(256, 2) void cache8_prefill_kernel(Cache8AttendLaun
   const int ps_mask = (1 << c.page_shift) - 1;
   // A wave's part of a tile: 16 codes of DH/64 key rows and as many value rows a
   // thread, of runs that are the same for the wave.
-  uintx4 kraw[PER], vraw[PER];
-  float2 scraw[PER];
-  int page[PER], ahead[PER];                                        // of the tile that is fetched next, and of the one after it
+  struct Raw {
+    uintx4 k[PER], v[PER];
+    float sk[PER], sv[PER];
+    int page[PER];
+  } raw[2];                                                         // of even and of odd tiles: two are on the way
+  int pages[2][PER];                                                // of the next even and odd tile to fetch
   auto run_of = [&](int i) { return DH == 128 ? 2 * i + (wave >> 1) : wave; };
   const int in = DH == 128 ? tid & 127 : lane;                       // this thread's 16 bytes of a run's DH * 16
-  auto find = [&](int t) {                                           // (waited for a tile later)
+  // Every step issues the same loads in the same order, so that it waits for those
+  // of two tiles before and no later ones: beyond the last tile, and of absent
+  // pages, they have no bytes to read.  (Loads return in order: a tile's pages are
+  // looked up before the tile before it is fetched.)
+  auto find = [&](int t, int (&to)[PER]) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int at = t * kTileTokens + run_of(i) * 16, blk = at >> c.page_shift;
-      ahead[i] = t < tend && at < len && blk < b.max_blocks ? table[blk] : -1;
+      to[i] = table[min(blk, b.max_blocks - 1)];
+      if (t >= tend || at >= len || blk >= b.max_blocks) to[i] = -1;
     }
   };
-  auto fetch = [&](int t) {
+  auto fetch = [&](int t, const int (&from)[PER], Raw& to) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int at = t * kTileTokens + run_of(i) * 16;
-      int pg = uniform(ahead[i]);
-      if (pg < 0 || pg >= c.num_pages) pg = -1;
-      page[i] = pg;
+      int pg = uniform(from[i]);
+      if (pg >= c.num_pages) pg = -1;
+      to.page[i] = pg;
       const int64_t p = pg < 0 ? 0 : pg, base = p * page_bytes + ((int64_t)h * DH << c.page_shift) + (at & ps_mask) * DH;
-      kraw[i] = *(const uintx4*)(c.k + base + 16 * in);
-      vraw[i] = *(const uintx4*)(c.v + base + 16 * in);
-      scraw[i] = *(const float2*)(c.scales + 2 * (p * c.num_kv + h));
+      const int bytes = pg < 0 ? 0 : 16 * DH;
+      to.k[i] = __builtin_amdgcn_raw_buffer_load_b128(make_rsrc(c.k + base, bytes), 16 * in, 0, 0);
+      to.v[i] = __builtin_amdgcn_raw_buffer_load_b128(make_rsrc(c.v + base, bytes), 16 * in, 0, 0);
+      const rsrc_t sc = make_rsrc(c.scales + 2 * (p * c.num_kv + h), pg < 0 ? 0 : 8);
+      to.sk[i] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(sc, 0, 0, 0));
+      to.sv[i] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(sc, 4, 0, 0));
     }
   };
-  auto stage = [&](int t) {
+  auto stage = [&](int t, Raw& of) {
     const int bf = t & 1;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int run = run_of(i), have = page[i] < 0 ? 0 : len - t * kTileTokens - run * 16;   // tokens of the run that are there
+      const int run = run_of(i), have = of.page[i] < 0 ? 0 : len - t * kTileTokens - run * 16;   // tokens of the run that are there
       if (have < 16) {
-        if (in / (DH / 16) >= have) kraw[i] = uintx4{0, 0, 0, 0};
+        if (in / (DH / 16) >= have) of.k[i] = uintx4{0, 0, 0, 0};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const int m = have - 4 * k;
-          vraw[i][k] &= m >= 4 ? ~0u : (m <= 0 ? 0u : (1u << (8 * m)) - 1u);
+          of.v[i][k] &= m >= 4 ? ~0u : (m <= 0 ? 0u : (1u << (8 * m)) - 1u);
         }
       }
       if (in == 0) {
-        const float lsv = have > 0 ? log2_of(scraw[i].y) : -INFINITY;
-        s_sk[bf][run] = have > 0 ? scraw[i].x : 1.f;
+        const float lsv = have > 0 ? log2_of(of.sv[i]) : -INFINITY;
+        s_sk[bf][run] = have > 0 ? of.sk[i] : 1.f;
         s_lsv[bf][run] = lsv;
         s_inv[bf][run] = have > 0 ? exp2_of(-lsv) : 0.f;
       }
       const int token = run * 16 + in / (DH / 16), chunk = 2 * (in % (DH / 16));
-      *(half8*)&s_k[bf][k_at<DH>(token, chunk)] = codes8<FMT>(kraw[i].x, kraw[i].y);
-      *(half8*)&s_k[bf][k_at<DH>(token, chunk + 1)] = codes8<FMT>(kraw[i].z, kraw[i].w);
-      *(half8*)&s_v[bf][v_at(in, 2 * run)] = codes8<FMT>(vraw[i].x, vraw[i].y);
-      *(half8*)&s_v[bf][v_at(in, 2 * run + 1)] = codes8<FMT>(vraw[i].z, vraw[i].w);
+      *(half8*)&s_k[bf][k_at<DH>(token, chunk)] = codes8<FMT>(of.k[i].x, of.k[i].y);
+      *(half8*)&s_k[bf][k_at<DH>(token, chunk + 1)] = codes8<FMT>(of.k[i].z, of.k[i].w);
+      *(half8*)&s_v[bf][v_at(in, 2 * run)] = codes8<FMT>(of.v[i].x, of.v[i].y);
+      *(half8*)&s_v[bf][v_at(in, 2 * run + 1)] = codes8<FMT>(of.v[i].z, of.v[i].w);
     }
   };
 
@@ -1067,19 +1074,11 @@ __global__ __launch_bounds__(256, 2) void cache8_prefill_kernel(Cache8AttendLaun
   float ref = kNoScore, sum = 0.f;
   const int ktok = 16 * (col >> 4) + 8 * ((col >> 2) & 1) + 4 * ((col >> 3) & 1) + (col & 3);   // token of score row `col`
 
-  if (tbeg < tend) {
-    find(tbeg);
-    fetch(tbeg);
-    find(tbeg + 1);
-    stage(tbeg);
-  }
-  __syncthreads();
-  for (int t = tbeg; t < tend; ++t) {
+  // tile t: in LDS; t + 1: on the way or here, in `next`; t + 2: fetched into `then`
+  auto step = [&](int t, Raw& next, Raw& then, int (&pages_next)[PER], const int (&pages_then)[PER]) {
     const int bf = t & 1, t0 = t * kTileTokens;
-    if (t + 1 < tend) {
-      fetch(t + 1);
-      find(t + 2);
-    }
+    find(t + 3, pages_next);
+    fetch(t + 2, pages_then, then);
     if (t0 < lim_max) {
       floatx16 sc[2];
 #pragma unroll
@@ -1138,8 +1137,21 @@ __global__ __launch_bounds__(256, 2) void cache8_prefill_kernel(Cache8AttendLaun
           acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, w[u], acc[d], 0, 0, 0);
         }
     }
-    if (t + 1 < tend) stage(t + 1);
+    stage(t + 1, next);
     __syncthreads();
+  };
+  if (tbeg < tend) {
+    find(tbeg, pages[0]);
+    find(tbeg + 1, pages[1]);
+    fetch(tbeg, pages[0], raw[0]);
+    find(tbeg + 2, pages[0]);
+    fetch(tbeg + 1, pages[1], raw[1]);
+    stage(tbeg, raw[0]);
+  }
+  __syncthreads();
+  for (int t = tbeg; t < tend; t += 2) {
+    step(t, raw[1], raw[0], pages[1], pages[0]);
+    if (t + 1 < tend) step(t + 1, raw[0], raw[1], pages[0], pages[1]);
   }
 
   sum = halves_sum(sum);
