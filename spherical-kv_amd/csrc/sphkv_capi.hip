@@ -1108,7 +1108,7 @@ int cache8_attend(const char* fn, bool decode, const void* q, int32_t q_type, in
   if (causal != 0 && causal != 1) return fail(SPHKV_EINVAL, "%s: causal must be 0 or 1 (got %d)", fn, causal);
   if (!(sm_scale > 0.f) || !std::isfinite(sm_scale))
     return fail(SPHKV_EINVAL, "%s: sm_scale must be positive and finite", fn);
-  if (decode ? num_rows * num_kv * gqa > 1 << 25 : (((num_rows * gqa) >> 7) + num_seqs) * num_kv > 1 << 23)
+  if (decode ? num_rows * num_kv * gqa > 1 << 23 : (((num_rows * gqa) >> 7) + num_seqs) * num_kv > 1 << 23)
     return fail(SPHKV_EINVAL, "%s: too many (row, head) pairs", fn);
   if (num_seqs == 0 || num_rows == 0) return ok();
   if (!q || !lens || !out || (!decode && !cu_rows)) return fail(SPHKV_EINVAL, "%s: null pointer argument", fn);

@@ -71,6 +71,12 @@ __device__ __forceinline__ float decode1(uint8_t c) {
   return __builtin_amdgcn_cvt_f32_fp8(c, 0);
 }
 
+// the lowest n bytes of a dword (none below 1, all from 4 on)
+__device__ __forceinline__ uint32_t low_bytes(int n) {
+  n = min(max(n, 0), 4);
+  return (uint32_t)((1ull << (8 * n)) - 1);
+}
+
 // byte k (a constant after unrolling) of four codes
 template <int FMT>
 __device__ __forceinline__ float decode_byte(uint32_t x, int k) {
@@ -393,9 +399,8 @@ __global__ __launch_bounds__(RUNS == 8 ? 512 : 256) void cache8_write_kernel(Cac
         for (int k = 0; k < VT / 4; ++k) {
           const uint32_t was = p[k];
           const int a = lo - vtok - 4 * k, z = hi - vtok - 4 * k;    // the dword's new bytes: a .. z - 1
-          const uint32_t upto = z >= 4 ? ~0u : (z <= 0 ? 0u : (1u << (8 * z)) - 1u);
-          const uint32_t from = a >= 4 ? 0u : (a <= 0 ? ~0u : ~((1u << (8 * a)) - 1u));
-          y[k] = (y[k] & upto & from) | (was & ~(upto & from));
+          const uint32_t fresh = low_bytes(z) & ~low_bytes(a);
+          y[k] = (y[k] & fresh) | (was & ~fresh);
         }
       }
       if constexpr (VT == 16) *(uintx4*)p = uintx4{y[0], y[1], y[2], y[3]};
@@ -692,7 +697,8 @@ __global__ __launch_bounds__(256, 2) void cache8_decode_kernel(Cache8AttendLaunc
       // page of run `run` of tile t, or -1
       auto page_at = [&](int t, int run) {
         const int at = t * kTileTokens + run * 16, blk = at >> c.page_shift, pg = table[min(blk, b.max_blocks - 1)];
-        return at < len && blk < b.max_blocks && pg < c.num_pages ? pg : -1;
+        const int has = (at < len) & (blk < b.max_blocks) & (pg < (int)c.num_pages);   // (no branch around the load)
+        return pg | (has - 1);
       };
       Tile<DH> A;
       auto load_k = [&](int t, int kpage) {
@@ -722,21 +728,17 @@ __global__ __launch_bounds__(256, 2) void cache8_decode_kernel(Cache8AttendLaunc
       float ref = kNoScore, sum = 0.f;
 
       int t = t0 + wave;
-      // Every turn issues the same loads in the same order, so that it waits for
-      // this tile's and none of the next (a branch around a load makes the waits
-      // wait for all); the last one's are this tile's again.
-      int kp1, vp1;
+      int kp1 = 0, vp1 = 0;                           // the pages of the wave's next tile
       if (t < t1) {
         const int kp = page_at(t, col >> 2), vp = page_at(t, g);
-        const int tn = t + 4 < t1 ? t + 4 : t;
-        kp1 = page_at(tn, col >> 2);
-        vp1 = page_at(tn, g);
+        kp1 = page_at(t + 4, col >> 2);
+        vp1 = page_at(t + 4, g);
         load_k(t, kp);
+        __builtin_amdgcn_sched_barrier(0);            // (in the loop's order, for its waits)
         load_v(t, vp);
       }
       for (; t < t1; t += 4) {
-        const int tn = t + 4 < t1 ? t + 4 : t, t2 = t + 8 < t1 ? t + 8 : t;
-        const int kp2 = page_at(t2, col >> 2), vp2 = page_at(t2, g);
+        const int kp2 = page_at(t + 8, col >> 2), vp2 = page_at(t + 8, g);
         // scores
         floatx4 sc[4];
 #pragma unroll
@@ -748,7 +750,7 @@ __global__ __launch_bounds__(256, 2) void cache8_decode_kernel(Cache8AttendLaunc
             sc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8<FMT>(A.k[i][j].z, A.k[i][j].w), q[2 * j + 1], sc[i], 0, 0, 0);
           }
         }
-        load_k(tn, kp1);
+        if (t + 4 < t1) load_k(t + 4, kp1);
         // tokens that are not there: behind the length, or of an absent page
         const int have = A.page < 0 ? 0 : len - t * kTileTokens - 16 * g;     // of this lane's 16
         if (__any(have < 16)) {
@@ -757,8 +759,7 @@ __global__ __launch_bounds__(256, 2) void cache8_decode_kernel(Cache8AttendLaunc
           uint32_t keep[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const int m = have - 4 * k;
-            keep[k] = m >= 4 ? ~0u : (m <= 0 ? 0u : (1u << (8 * m)) - 1u);
+            keep[k] = low_bytes(have - 4 * k);
           }
 #pragma unroll
           for (int d = 0; d < DT; ++d)
@@ -802,7 +803,7 @@ __global__ __launch_bounds__(256, 2) void cache8_decode_kernel(Cache8AttendLaunc
           acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8<FMT>(A.v[d].x, A.v[d].y), w[0], acc[d], 0, 0, 0);
           acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8<FMT>(A.v[d].z, A.v[d].w), w[1], acc[d], 0, 0, 0);
         }
-        load_v(tn, vp1);
+        if (t + 4 < t1) load_v(t + 4, vp1);
         kp1 = kp2;
         vp1 = vp2;
       }
@@ -848,41 +849,113 @@ __global__ __launch_bounds__(256, 2) void cache8_decode_kernel(Cache8AttendLaunc
   }
 }
 
+__device__ __forceinline__ float wave_sum(float x) {
+  x += row_rotated<8>(x);
+  x += row_rotated<4>(x);
+  x += row_rotated<2>(x);
+  x += row_rotated<1>(x);
+  return rows_sum(x);
+}
+
+// Partials first, first + step, ... before end of one output row, joined by the
+// wave, CH (up to 16) at a time whose loads are all on the way at once: R, l and
+// the lane's DH / 64 outputs.  `at(i)`: partial i's reference (its sum `sums` floats on) and
+// its row.
+template <int DPL, int CH, class AT>
+__device__ __forceinline__ void join(int64_t first, int64_t end, int64_t step, int sums, AT at, float& R, float& l,
+                                     float (&acc)[DPL]) {
+  const int lane = threadIdx.x & 63;
+  R = kNoScore;
+  l = 0.f;
+#pragma unroll
+  for (int i = 0; i < DPL; ++i) acc[i] = 0.f;
+  for (int64_t g = first; g < end; g += CH * step) {
+    float a[CH][DPL], r = kNoScore, ls = 0.f;
+    if (lane < CH && g + lane * step < end) {
+      const float* ref = at(g + lane * step).ref;
+      r = ref[0];
+      ls = ref[sums];
+    }
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const int64_t k = g + i * step;
+      const float* row = at(k < end ? k : g).row + lane * DPL;        // (a missing one's weight is 0)
+#pragma unroll
+      for (int d = 0; d < DPL; ++d) a[i][d] = row[d];
+    }
+    const float M = fmaxf(R, wave_max(r)), f = exp2_of(r - M), was = exp2_of(R - M);
+    const bool has = lane < CH && g + lane * step < end;
+    const float w = has ? f : 0.f;
+    l = fmaf(l, was, wave_sum(ls * w));
+#pragma unroll
+    for (int d = 0; d < DPL; ++d) acc[d] *= was;
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const float wi = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), i));
+      if (g + i * step < end)
+#pragma unroll
+        for (int d = 0; d < DPL; ++d) acc[d] = fmaf(a[i][d], wi, acc[d]);
+    }
+    R = M;
+  }
+}
+struct Partial { const float* ref; const float* row; };
+
 // Joins the partials of each (sequence, kv head) that several workgroups hold,
-// and writes the rows of sequences without a token.  One wave per query head.
-template <int TYPE, int DH>
-__global__ __launch_bounds__(64) void cache8_decode_merge_kernel(Cache8AttendLaunch L, const float* partials,
-                                                                 const int64_t* base_of) {
+// and writes the rows of sequences without a token.  WAVES waves per query head
+// share its partials: four where there are few pairs and many partials of each
+// (one document of 32K tokens, 64 of each head: 3.9 us, 7.8 with one wave), one
+// where there are many pairs of one or two (64 short contexts: 4.4 us, 7.3 with
+// four).
+template <int TYPE, int DH, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void cache8_decode_merge_kernel(Cache8AttendLaunch L, const float* partials,
+                                                                  const int64_t* base_of) {
+  constexpr int DPL = DH / 64;
+  __shared__ float s_r[WAVES], s_l[WAVES], s_a[WAVES][DH];
   const Cache8& c = L.c;
-  const int heads = c.num_kv * L.gqa, s = blockIdx.x / heads, hq = blockIdx.x % heads, lane = threadIdx.x;
+  const int heads = c.num_kv * L.gqa, s = blockIdx.x / heads, hq = blockIdx.x % heads;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int h = hq / L.gqa, part = (hq - h * L.gqa) / 16, cc = (hq - h * L.gqa) % 16, parts = head_parts(L.gqa);
   const int64_t per = base_of[0], a = base_of[1 + s], T = (base_of[2 + s] - a) / (c.num_kv * parts);
   const int64_t at = (int64_t)s * heads + hq;
-  constexpr int DPL = DH / 64;
   if (T == 0) {
-    for (int i = 0; i < DPL; ++i) store1<TYPE>(L.out, at * DH + lane * DPL + i, 0.f);
-    if (L.lse && lane == 0) L.lse[at] = -INFINITY;
+    for (int d = threadIdx.x; d < DH; d += 64 * WAVES) store1<TYPE>(L.out, at * DH + d, 0.f);
+    if (L.lse && threadIdx.x == 0) L.lse[at] = -INFINITY;
     return;
   }
   const int64_t first = a + (int64_t)(h * parts + part) * T, g0 = first / per, g1 = (first + T - 1) / per;
   if (g0 == g1) return;
   const int64_t floats = partial8_floats(L.gqa, DH);
-  auto partial = [&](int64_t g) { return partials + (2 * g + (g == g0)) * floats; };
-  float R = kNoScore;
-  for (int64_t g = g0 + lane; g <= g1; g += kWave) R = fmaxf(R, partial(g)[cc]);
-  R = wave_max(R);
-  float l = 0.f, acc[DPL] = {};
-#pragma unroll 8
-  for (int64_t g = g0; g <= g1; ++g) {
-    const float* x = partial(g);
-    const float f = exp2_of(x[cc] - R);
-    l = fmaf(x[16 + cc], f, l);
+  float R, l, acc[DPL];
+  join<DPL, WAVES == 4 ? 16 : 4>(g0 + wave, g1 + 1, WAVES, 16, [&](int64_t g) {
+    const float* p = partials + (2 * g + (g == g0)) * floats;
+    return Partial{p + cc, p + 32 + cc * DH};
+  }, R, l, acc);
+  if constexpr (WAVES == 1) {
 #pragma unroll
-    for (int i = 0; i < DPL; ++i) acc[i] = fmaf(x[32 + cc * DH + lane * DPL + i], f, acc[i]);
+    for (int d = 0; d < DPL; ++d) store1<TYPE>(L.out, at * DH + lane * DPL + d, l == 0.f ? 0.f : acc[d] / l);
+    if (L.lse && lane == 0) L.lse[at] = l == 0.f ? -INFINITY : (R + log2_of(l)) * 0.693147180559945f;
+  } else {
+    if (lane == 0) {
+      s_r[wave] = R;
+      s_l[wave] = l;
+    }
+#pragma unroll
+    for (int d = 0; d < DPL; ++d) s_a[wave][lane * DPL + d] = acc[d];
+    __syncthreads();
+    if (threadIdx.x >= DH) return;
+    float M = s_r[0], o = 0.f, sum = 0.f;
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) M = fmaxf(M, s_r[w]);
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      const float f = exp2_of(s_r[w] - M);
+      sum = fmaf(s_l[w], f, sum);
+      o = fmaf(s_a[w][threadIdx.x], f, o);
+    }
+    store1<TYPE>(L.out, at * DH + threadIdx.x, sum == 0.f ? 0.f : o / sum);
+    if (L.lse && threadIdx.x == 0) L.lse[at] = sum == 0.f ? -INFINITY : (M + log2_of(sum)) * 0.693147180559945f;
   }
-#pragma unroll
-  for (int i = 0; i < DPL; ++i) store1<TYPE>(L.out, at * DH + lane * DPL + i, l == 0.f ? 0.f : acc[i] / l);
-  if (L.lse && lane == 0) L.lse[at] = l == 0.f ? -INFINITY : (R + log2_of(l)) * 0.693147180559945f;
 }
 
 // ---- prefill -----------------------------------------------------------------
@@ -1048,8 +1121,7 @@ __global__ __launch_bounds__(256, 2) void cache8_prefill_kernel(Cache8AttendLaun
         if (in / (DH / 16) >= have) of.k[i] = uintx4{0, 0, 0, 0};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const int m = have - 4 * k;
-          of.v[i][k] &= m >= 4 ? ~0u : (m <= 0 ? 0u : (1u << (8 * m)) - 1u);
+          of.v[i][k] &= low_bytes(have - 4 * k);
         }
       }
       if (in == 0) {
@@ -1203,18 +1275,11 @@ __global__ __launch_bounds__(256) void cache8_prefill_merge_kernel(Cache8AttendL
   const int in = (int)(r & (kRowTile - 1));
   const float* x = partials + (slot * c.num_kv + h) * splits * split_floats(DH);
   constexpr int DPL = DH / 64;
-  float R = kNoScore;
-  for (int z = lane; z < parts; z += kWave) R = fmaxf(R, x[z * split_floats(DH) + in]);
-  R = wave_max(R);
-  float l = 0.f, acc[DPL] = {};
-#pragma unroll 4
-  for (int z = 0; z < parts; ++z) {
+  float R, l, acc[DPL];
+  join<DPL, 16>(0, parts, 1, kRowTile, [&](int64_t z) {
     const float* p = x + z * split_floats(DH);
-    const float f = exp2_of(p[in] - R);
-    l = fmaf(p[kRowTile + in], f, l);
-#pragma unroll
-    for (int i = 0; i < DPL; ++i) acc[i] = fmaf(p[2 * kRowTile + in * DH + lane * DPL + i], f, acc[i]);
-  }
+    return Partial{p + in, p + 2 * kRowTile + in * DH};
+  }, R, l, acc);
 #pragma unroll
   for (int i = 0; i < DPL; ++i) store1<TYPE>(L.out, at * DH + lane * DPL + i, l == 0.f ? 0.f : acc[i] / l);
   if (L.lse && lane == 0) L.lse[at] = l == 0.f ? -INFINITY : (R + log2_of(l)) * 0.693147180559945f;
@@ -1265,7 +1330,11 @@ template <int T, int F, int D> struct Decode {
       int64_t* plan = (int64_t*)L.ws;
       float* partials = (float*)((uint8_t*)L.ws + plan_bytes(L.b.num_seqs));
       cache8_decode_kernel<F, T, D><<<kDecodeGroups, 256, 0, st>>>(L, partials, plan);
-      cache8_decode_merge_kernel<T, D><<<L.b.num_seqs * L.c.num_kv * L.gqa, 64, 0, st>>>(L, partials, plan);
+      const int heads = L.b.num_seqs * L.c.num_kv * L.gqa;
+      if (L.b.num_seqs * L.c.num_kv * head_parts(L.gqa) < kDecodeGroups / 4)
+        cache8_decode_merge_kernel<T, D, 4><<<heads, 256, 0, st>>>(L, partials, plan);
+      else
+        cache8_decode_merge_kernel<T, D, 1><<<heads, 64, 0, st>>>(L, partials, plan);
       return hipPeekAtLastError() == hipSuccess ? 0 : -1;
     }
   }
