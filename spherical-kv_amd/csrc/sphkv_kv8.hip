@@ -1017,6 +1017,7 @@ __device__ __forceinline__ float halves_sum(float x) {
 }
 
 typedef float floatx16 __attribute__((ext_vector_type(16)));
+template <int N> struct Int { static constexpr int value = N; };
 
 template <int FMT, int TYPE, int DH>
 __global__ __launch_bounds__(256, 2) void cache8_prefill_kernel(Cache8AttendLaunch L, int splits, float* partials) {
@@ -1080,14 +1081,14 @@ __global__ __launch_bounds__(256, 2) void cache8_prefill_kernel(Cache8AttendLaun
     uintx4 k[PER], v[PER];
     float sk[PER], sv[PER];
     int page[PER];
-  } raw[2];                                                         // of even and of odd tiles: two are on the way
-  int pages[2][PER];                                                // of the next even and odd tile to fetch
+  } raw;
+  int pages[2][PER];                                                // of the next tiles of either parity
   auto run_of = [&](int i) { return DH == 128 ? 2 * i + (wave >> 1) : wave; };
   const int in = DH == 128 ? tid & 127 : lane;                       // this thread's 16 bytes of a run's DH * 16
-  // Every step issues the same loads in the same order, so that it waits for those
-  // of two tiles before and no later ones: beyond the last tile, and of absent
-  // pages, they have no bytes to read.  (Loads return in order: a tile's pages are
-  // looked up before the tile before it is fetched.)
+  // Every step issues the same loads in the same order, so that its waits are for
+  // the ones it needs: beyond the last tile, and of absent pages, they have no bytes
+  // to read.  (Loads return in order: a tile's pages are looked up before the tile
+  // before it is fetched.)
   auto find = [&](int t, int (&to)[PER]) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
@@ -1096,45 +1097,44 @@ __global__ __launch_bounds__(256, 2) void cache8_prefill_kernel(Cache8AttendLaun
       if (t >= tend || at >= len || blk >= b.max_blocks) to[i] = -1;
     }
   };
-  auto fetch = [&](int t, const int (&from)[PER], Raw& to) {
+  auto fetch = [&](int t, const int (&from)[PER]) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int at = t * kTileTokens + run_of(i) * 16;
       int pg = uniform(from[i]);
       if (pg >= c.num_pages) pg = -1;
-      to.page[i] = pg;
+      raw.page[i] = pg;
       const int64_t p = pg < 0 ? 0 : pg, base = p * page_bytes + ((int64_t)h * DH << c.page_shift) + (at & ps_mask) * DH;
       const int bytes = pg < 0 ? 0 : 16 * DH;
-      to.k[i] = __builtin_amdgcn_raw_buffer_load_b128(make_rsrc(c.k + base, bytes), 16 * in, 0, 0);
-      to.v[i] = __builtin_amdgcn_raw_buffer_load_b128(make_rsrc(c.v + base, bytes), 16 * in, 0, 0);
+      raw.k[i] = __builtin_amdgcn_raw_buffer_load_b128(make_rsrc(c.k + base, bytes), 16 * in, 0, 0);
+      raw.v[i] = __builtin_amdgcn_raw_buffer_load_b128(make_rsrc(c.v + base, bytes), 16 * in, 0, 0);
       const rsrc_t sc = make_rsrc(c.scales + 2 * (p * c.num_kv + h), pg < 0 ? 0 : 8);
-      to.sk[i] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(sc, 0, 0, 0));
-      to.sv[i] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(sc, 4, 0, 0));
+      raw.sk[i] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(sc, 0, 0, 0));
+      raw.sv[i] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(sc, 4, 0, 0));
     }
   };
-  auto stage = [&](int t, Raw& of) {
-    const int bf = t & 1;
+  auto stage = [&](int t, int bf) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int run = run_of(i), have = of.page[i] < 0 ? 0 : len - t * kTileTokens - run * 16;   // tokens of the run that are there
+      const int run = run_of(i), have = raw.page[i] < 0 ? 0 : len - t * kTileTokens - run * 16;   // tokens of the run that are there
       if (have < 16) {
-        if (in / (DH / 16) >= have) of.k[i] = uintx4{0, 0, 0, 0};
+        if (in / (DH / 16) >= have) raw.k[i] = uintx4{0, 0, 0, 0};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          of.v[i][k] &= low_bytes(have - 4 * k);
+          raw.v[i][k] &= low_bytes(have - 4 * k);
         }
       }
       if (in == 0) {
-        const float lsv = have > 0 ? log2_of(of.sv[i]) : -INFINITY;
-        s_sk[bf][run] = have > 0 ? of.sk[i] : 1.f;
+        const float lsv = have > 0 ? log2_of(raw.sv[i]) : -INFINITY;
+        s_sk[bf][run] = have > 0 ? raw.sk[i] : 1.f;
         s_lsv[bf][run] = lsv;
         s_inv[bf][run] = have > 0 ? exp2_of(-lsv) : 0.f;
       }
       const int token = run * 16 + in / (DH / 16), chunk = 2 * (in % (DH / 16));
-      *(half8*)&s_k[bf][k_at<DH>(token, chunk)] = codes8<FMT>(of.k[i].x, of.k[i].y);
-      *(half8*)&s_k[bf][k_at<DH>(token, chunk + 1)] = codes8<FMT>(of.k[i].z, of.k[i].w);
-      *(half8*)&s_v[bf][v_at(in, 2 * run)] = codes8<FMT>(of.v[i].x, of.v[i].y);
-      *(half8*)&s_v[bf][v_at(in, 2 * run + 1)] = codes8<FMT>(of.v[i].z, of.v[i].w);
+      *(half8*)&s_k[bf][k_at<DH>(token, chunk)] = codes8<FMT>(raw.k[i].x, raw.k[i].y);
+      *(half8*)&s_k[bf][k_at<DH>(token, chunk + 1)] = codes8<FMT>(raw.k[i].z, raw.k[i].w);
+      *(half8*)&s_v[bf][v_at(in, 2 * run)] = codes8<FMT>(raw.v[i].x, raw.v[i].y);
+      *(half8*)&s_v[bf][v_at(in, 2 * run + 1)] = codes8<FMT>(raw.v[i].z, raw.v[i].w);
     }
   };
 
@@ -1146,11 +1146,11 @@ __global__ __launch_bounds__(256, 2) void cache8_prefill_kernel(Cache8AttendLaun
   float ref = kNoScore, sum = 0.f;
   const int ktok = 16 * (col >> 4) + 8 * ((col >> 2) & 1) + 4 * ((col >> 3) & 1) + (col & 3);   // token of score row `col`
 
-  // tile t: in LDS; t + 1: on the way or here, in `next`; t + 2: fetched into `then`
-  auto step = [&](int t, Raw& next, Raw& then, int (&pages_next)[PER], const int (&pages_then)[PER]) {
-    const int bf = t & 1, t0 = t * kTileTokens;
-    find(t + 3, pages_next);
-    fetch(t + 2, pages_then, then);
+  // Tile t, from LDS buffer bf (a constant); then tile t + 1, whose loads had the
+  // whole step, into the other, and the loads of t + 2.
+  auto step = [&](int t, auto parity) {
+    constexpr int bf = parity.value;
+    const int t0 = t * kTileTokens;
     if (t0 < lim_max) {
       floatx16 sc[2];
 #pragma unroll
@@ -1209,21 +1209,23 @@ __global__ __launch_bounds__(256, 2) void cache8_prefill_kernel(Cache8AttendLaun
           acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, w[u], acc[d], 0, 0, 0);
         }
     }
-    stage(t + 1, next);
+    stage(t + 1, 1 - bf);
+    find(t + 3, pages[1 - bf]);
+    fetch(t + 2, pages[bf]);
     __syncthreads();
   };
   if (tbeg < tend) {
     find(tbeg, pages[0]);
     find(tbeg + 1, pages[1]);
-    fetch(tbeg, pages[0], raw[0]);
+    fetch(tbeg, pages[0]);
+    stage(tbeg, 0);
     find(tbeg + 2, pages[0]);
-    fetch(tbeg + 1, pages[1], raw[1]);
-    stage(tbeg, raw[0]);
+    fetch(tbeg + 1, pages[1]);
   }
   __syncthreads();
   for (int t = tbeg; t < tend; t += 2) {
-    step(t, raw[1], raw[0], pages[1], pages[0]);
-    if (t + 1 < tend) step(t + 1, raw[0], raw[1], pages[0], pages[1]);
+    step(t, Int<0>{});
+    if (t + 1 < tend) step(t + 1, Int<1>{});
   }
 
   sum = halves_sum(sum);
