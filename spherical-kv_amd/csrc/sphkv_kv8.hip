@@ -587,8 +587,14 @@ template <int TYPE, int N, class MAX>
 __device__ __forceinline__ void query_fp16(const uintx4 (&raw)[N], MAX row_max, half8 (&out)[N], int& back) {
   back = 0;
   if constexpr (TYPE == kFp16) {
+    // (used here, so that their wait is here: a wait at the first product, inside
+    // the loop, would in every turn be for the loads of the next tile too)
 #pragma unroll
-    for (int i = 0; i < N; ++i) out[i] = __builtin_bit_cast(half8, raw[i]);
+    for (int i = 0; i < N; ++i) {
+      uintx4 x = raw[i];
+      asm volatile("" : "+v"(x));
+      out[i] = __builtin_bit_cast(half8, x);
+    }
   } else {
     float m = 0.f;
 #pragma unroll
@@ -1019,6 +1025,19 @@ __device__ __forceinline__ float halves_sum(float x) {
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 template <int N> struct Int { static constexpr int value = N; };
 
+// N LDS reads that feed N matrix instructions: kAhead of them in flight
+constexpr int kAhead = 6;
+template <int N>
+__device__ __forceinline__ void reads_ahead() {
+  __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+#pragma unroll
+  for (int i = 0; i < N - kAhead; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(0x008, kAhead, 0);
+}
+
 template <int FMT, int TYPE, int DH>
 __global__ __launch_bounds__(256, 2) void cache8_prefill_kernel(Cache8AttendLaunch L, int splits, float* partials) {
   constexpr int KS = DH / 16, DB = DH / 32, PER = DH / 64;         // k-steps, value blocks, 16-byte loads of a thread
@@ -1163,6 +1182,7 @@ __global__ __launch_bounds__(256, 2) void cache8_prefill_kernel(Cache8AttendLaun
           sc[x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, q[k], sc[x], 0, 0, 0);
         }
       }
+      reads_ahead<2 * KS>();
       if (t0 + kTileTokens > lim_min) {
         const int left = lim - t0 - 8 * half;
 #pragma unroll
@@ -1208,6 +1228,7 @@ __global__ __launch_bounds__(256, 2) void cache8_prefill_kernel(Cache8AttendLaun
           const half8 a = *(const half8*)&s_v[bf][v_at(32 * d + col, 2 * u + half)];
           acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, w[u], acc[d], 0, 0, 0);
         }
+      reads_ahead<4 * DB>();
     }
     stage(t + 1, 1 - bf);
     find(t + 3, pages[1 - bf]);
