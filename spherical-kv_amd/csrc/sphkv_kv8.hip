@@ -980,20 +980,24 @@ __global__ __launch_bounds__(64 * WAVES) void cache8_decode_merge_kernel(Cache8A
 //
 // With few row tiles the keys of each are split over workgroups, whose partials a
 // second kernel joins.
-constexpr int kRowTile = 128;
-constexpr int kPrefillGroups = 512;     // workgroups that run at once: two per CU
+// Waves of a workgroup, 32 rows each, and the workgroups that run at once: at
+// DH 128 eight waves share a tile and fill a CU's registers; at DH 64 four do, and
+// three workgroups fit.
 constexpr int kSplitLeast = 4;          // tiles of a split
 constexpr int kSplitMost = 64;
+__host__ __device__ constexpr int row_waves(int dh) { return dh == 128 ? 8 : 4; }
+__host__ __device__ constexpr int row_shift(int dh) { return dh == 128 ? 8 : 7; }       // log2 of a tile's rows
+__host__ __device__ constexpr int prefill_groups(int dh) { return dh == 128 ? 256 : 768; }
 
-__host__ __device__ __forceinline__ int64_t row_tiles(int64_t num_rows, int num_seqs, int gqa) {
-  return ((num_rows * gqa) >> 7) + num_seqs;
+__host__ __device__ __forceinline__ int64_t row_tiles(int64_t num_rows, int num_seqs, int gqa, int dh) {
+  return ((num_rows * gqa) >> row_shift(dh)) + num_seqs;
 }
-__host__ __device__ __forceinline__ int prefill_splits(int64_t num_rows, int num_seqs, int num_kv, int gqa) {
-  const int64_t wgs = row_tiles(num_rows, num_seqs, gqa) * num_kv, s = kPrefillGroups / wgs;
+__host__ __device__ __forceinline__ int prefill_splits(int64_t num_rows, int num_seqs, int num_kv, int gqa, int dh) {
+  const int64_t wgs = row_tiles(num_rows, num_seqs, gqa, dh) * num_kv, s = prefill_groups(dh) / wgs;
   return (int)(s < 1 ? 1 : (s > kSplitMost ? kSplitMost : s));
 }
 // floats of one split's partial: reference and sum per row, then acc[rows][DH]
-__host__ __device__ __forceinline__ int64_t split_floats(int dh) { return (int64_t)kRowTile * (dh + 2); }
+__host__ __device__ __forceinline__ int64_t split_floats(int dh) { return (int64_t)(dh + 2) << row_shift(dh); }
 
 // tokens that a sequence's row of token `last_token` sees, and the splits that
 // so many are worth
@@ -1039,8 +1043,8 @@ __device__ __forceinline__ void reads_ahead() {
 }
 
 template <int FMT, int TYPE, int DH>
-__global__ __launch_bounds__(256, 2) void cache8_prefill_kernel(Cache8AttendLaunch L, int splits, float* partials) {
-  constexpr int KS = DH / 16, DB = DH / 32, PER = DH / 64;         // k-steps, value blocks, 16-byte loads of a thread
+__global__ __launch_bounds__(64 * row_waves(DH), 2) void cache8_prefill_kernel(Cache8AttendLaunch L, int splits, float* partials) {
+  constexpr int KS = DH / 16, DB = DH / 32, RS = row_shift(DH), kRowTile = 1 << RS;      // k-steps, value blocks
   __shared__ __align__(16) _Float16 s_k[2][kTileTokens * DH], s_v[2][kTileTokens * DH];
   __shared__ float s_sk[2][4], s_lsv[2][4], s_inv[2][4];
   const Cache8& c = L.c;
@@ -1050,12 +1054,12 @@ __global__ __launch_bounds__(256, 2) void cache8_prefill_kernel(Cache8AttendLaun
   // the longest rows of a sequence come first
   const int h = blockIdx.x % c.num_kv, z = blockIdx.y, gqa = L.gqa;
   const int64_t slot = (gridDim.x - 1 - blockIdx.x) / c.num_kv;
-  const int s = uniform(seq_of_slot(b, slot, gqa, 7, 1));
+  const int s = uniform(seq_of_slot(b, slot, gqa, RS, 1));
   int begin, end;
   rows_of(b, s, begin, end);
   begin = uniform(begin);
   const int n = uniform(end) - begin;
-  const int64_t r0 = (slot - first_slot(b, s, gqa, 7, 1)) * kRowTile, rows_all = (int64_t)n * gqa;
+  const int64_t r0 = (slot - first_slot(b, s, gqa, RS, 1)) * kRowTile, rows_all = (int64_t)n * gqa;
   if (r0 >= rows_all) return;
   const int len = uniform(seq_tokens(c, b, s));
   const int last = (int)((r0 + kRowTile < rows_all ? r0 + kRowTile : rows_all) - 1);
@@ -1092,69 +1096,53 @@ __global__ __launch_bounds__(256, 2) void cache8_prefill_kernel(Cache8AttendLaun
   const float cq = ldexpf(L.sm_scale * 1.44269504088896f, back);
 
   const int32_t* table = b.table + s * b.table_stride;
-  const int64_t page_bytes = (int64_t)c.num_kv * DH << c.page_shift;
-  const int ps_mask = (1 << c.page_shift) - 1;
-  // A wave's part of a tile: 16 codes of DH/64 key rows and as many value rows a
-  // thread, of runs that are the same for the wave.
+  // A thread's part of a tile: 16 codes of a key row and 16 of a value row, of a run
+  // that is the same for the wave.
+  const int run = DH == 128 ? wave >> 1 : wave, in = DH == 128 ? tid & 127 : lane;
   struct Raw {
-    uintx4 k[PER], v[PER];
-    float sk[PER], sv[PER];
-    int page[PER];
-  } raw;
-  int pages[2][PER];                                                // of the next tiles of either parity
-  auto run_of = [&](int i) { return DH == 128 ? 2 * i + (wave >> 1) : wave; };
-  const int in = DH == 128 ? tid & 127 : lane;                       // this thread's 16 bytes of a run's DH * 16
+    uintx4 k, v;
+    float2 sc;
+    int page;
+  } raws[2];                                                        // of even and odd tiles
+  int pages[2];
+  const int64_t page_bytes = (int64_t)c.num_kv * DH << c.page_shift;
+  const uint8_t* kbase = c.k + ((int64_t)h * DH << c.page_shift);
+  const uint8_t* vbase = c.v + ((int64_t)h * DH << c.page_shift);
+  const float* scbase = c.scales + 2 * h;
+  const int ps_mask = (1 << c.page_shift) - 1, last_blk = b.max_blocks - 1;
   // Every step issues the same loads in the same order, so that its waits are for
-  // the ones it needs: beyond the last tile, and of absent pages, they have no bytes
-  // to read.  (Loads return in order: a tile's pages are looked up before the tile
-  // before it is fetched.)
-  auto find = [&](int t, int (&to)[PER]) {
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int at = t * kTileTokens + run_of(i) * 16, blk = at >> c.page_shift;
-      to[i] = table[min(blk, b.max_blocks - 1)];
-      if (t >= tend || at >= len || blk >= b.max_blocks) to[i] = -1;
-    }
+  // the ones it needs (loads return in order: a tile's pages are looked up before
+  // the tile before it is fetched).  Beyond the last tile, and of absent pages, they
+  // read page 0, whose tokens are dropped.
+  auto find = [&](int t) { return table[min((t * kTileTokens + run * 16) >> c.page_shift, last_blk)]; };
+  auto fetch = [&](int t, int found, Raw& raw) {
+    const int at = t * kTileTokens + run * 16;
+    int pg = uniform(found);
+    pg = t < tend && at < len && pg < (int)c.num_pages ? pg : -1;
+    raw.page = pg;
+    const int64_t p = max(pg, 0), base = p * page_bytes + (at & ps_mask) * DH;
+    raw.k = *(const uintx4*)(kbase + base + 16 * in);
+    raw.v = *(const uintx4*)(vbase + base + 16 * in);
+    raw.sc = *(const float2*)(scbase + p * (2 * c.num_kv));
   };
-  auto fetch = [&](int t, const int (&from)[PER]) {
+  auto stage = [&](int t, int bf, Raw raw) {
+    const int have = raw.page < 0 ? 0 : len - t * kTileTokens - run * 16;   // tokens of the run that are there
+    if (have < 16) {
+      if (in / (DH / 16) >= have) raw.k = uintx4{0, 0, 0, 0};
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int at = t * kTileTokens + run_of(i) * 16;
-      int pg = uniform(from[i]);
-      if (pg >= c.num_pages) pg = -1;
-      raw.page[i] = pg;
-      const int64_t p = pg < 0 ? 0 : pg, base = p * page_bytes + ((int64_t)h * DH << c.page_shift) + (at & ps_mask) * DH;
-      const int bytes = pg < 0 ? 0 : 16 * DH;
-      raw.k[i] = __builtin_amdgcn_raw_buffer_load_b128(make_rsrc(c.k + base, bytes), 16 * in, 0, 0);
-      raw.v[i] = __builtin_amdgcn_raw_buffer_load_b128(make_rsrc(c.v + base, bytes), 16 * in, 0, 0);
-      const rsrc_t sc = make_rsrc(c.scales + 2 * (p * c.num_kv + h), pg < 0 ? 0 : 8);
-      raw.sk[i] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(sc, 0, 0, 0));
-      raw.sv[i] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(sc, 4, 0, 0));
+      for (int k = 0; k < 4; ++k) raw.v[k] &= low_bytes(have - 4 * k);
     }
-  };
-  auto stage = [&](int t, int bf) {
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int run = run_of(i), have = raw.page[i] < 0 ? 0 : len - t * kTileTokens - run * 16;   // tokens of the run that are there
-      if (have < 16) {
-        if (in / (DH / 16) >= have) raw.k[i] = uintx4{0, 0, 0, 0};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          raw.v[i][k] &= low_bytes(have - 4 * k);
-        }
-      }
-      if (in == 0) {
-        const float lsv = have > 0 ? log2_of(raw.sv[i]) : -INFINITY;
-        s_sk[bf][run] = have > 0 ? raw.sk[i] : 1.f;
-        s_lsv[bf][run] = lsv;
-        s_inv[bf][run] = have > 0 ? exp2_of(-lsv) : 0.f;
-      }
-      const int token = run * 16 + in / (DH / 16), chunk = 2 * (in % (DH / 16));
-      *(half8*)&s_k[bf][k_at<DH>(token, chunk)] = codes8<FMT>(raw.k[i].x, raw.k[i].y);
-      *(half8*)&s_k[bf][k_at<DH>(token, chunk + 1)] = codes8<FMT>(raw.k[i].z, raw.k[i].w);
-      *(half8*)&s_v[bf][v_at(in, 2 * run)] = codes8<FMT>(raw.v[i].x, raw.v[i].y);
-      *(half8*)&s_v[bf][v_at(in, 2 * run + 1)] = codes8<FMT>(raw.v[i].z, raw.v[i].w);
+    if (in == 0) {
+      const float lsv = have > 0 ? log2_of(raw.sc.y) : -INFINITY;
+      s_sk[bf][run] = have > 0 ? raw.sc.x : 1.f;
+      s_lsv[bf][run] = lsv;
+      s_inv[bf][run] = have > 0 ? exp2_of(-lsv) : 0.f;
     }
+    const int token = run * 16 + in / (DH / 16), chunk = 2 * (in % (DH / 16));
+    *(half8*)&s_k[bf][k_at<DH>(token, chunk)] = codes8<FMT>(raw.k.x, raw.k.y);
+    *(half8*)&s_k[bf][k_at<DH>(token, chunk + 1)] = codes8<FMT>(raw.k.z, raw.k.w);
+    *(half8*)&s_v[bf][v_at(in, 2 * run)] = codes8<FMT>(raw.v.x, raw.v.y);
+    *(half8*)&s_v[bf][v_at(in, 2 * run + 1)] = codes8<FMT>(raw.v.z, raw.v.w);
   };
 
   floatx16 acc[DB];
@@ -1165,8 +1153,8 @@ __global__ __launch_bounds__(256, 2) void cache8_prefill_kernel(Cache8AttendLaun
   float ref = kNoScore, sum = 0.f;
   const int ktok = 16 * (col >> 4) + 8 * ((col >> 2) & 1) + 4 * ((col >> 3) & 1) + (col & 3);   // token of score row `col`
 
-  // Tile t, from LDS buffer bf (a constant); then tile t + 1, whose loads had the
-  // whole step, into the other, and the loads of t + 2.
+  // Tile t, from LDS buffer bf (a constant); then tile t + 1, whose loads had two
+  // steps, into the other, and the loads of t + 3.
   auto step = [&](int t, auto parity) {
     constexpr int bf = parity.value;
     const int t0 = t * kTileTokens;
@@ -1230,23 +1218,33 @@ __global__ __launch_bounds__(256, 2) void cache8_prefill_kernel(Cache8AttendLaun
         }
       reads_ahead<4 * DB>();
     }
-    stage(t + 1, 1 - bf);
-    find(t + 3, pages[1 - bf]);
-    fetch(t + 2, pages[bf]);
+    stage(t + 1, 1 - bf, raws[1 - bf]);
+    __builtin_amdgcn_sched_barrier(0);
+    pages[bf] = find(t + 4);
+    __builtin_amdgcn_sched_barrier(0);
+    fetch(t + 3, pages[1 - bf], raws[1 - bf]);
+    __builtin_amdgcn_sched_barrier(0);
     __syncthreads();
   };
   if (tbeg < tend) {
-    find(tbeg, pages[0]);
-    find(tbeg + 1, pages[1]);
-    fetch(tbeg, pages[0]);
-    stage(tbeg, 0);
-    find(tbeg + 2, pages[0]);
-    fetch(tbeg + 1, pages[1]);
-  }
-  __syncthreads();
-  for (int t = tbeg; t < tend; t += 2) {
-    step(t, Int<0>{});
-    if (t + 1 < tend) step(t + 1, Int<1>{});
+    pages[0] = find(tbeg);
+    pages[1] = find(tbeg + 1);
+    fetch(tbeg, pages[0], raws[0]);
+    pages[0] = find(tbeg + 2);
+    __builtin_amdgcn_sched_barrier(0);                               // (in the loop's order, for its waits)
+    fetch(tbeg + 1, pages[1], raws[1]);
+    stage(tbeg, 0, raws[0]);
+    __builtin_amdgcn_sched_barrier(0);
+    pages[1] = find(tbeg + 3);
+    fetch(tbeg + 2, pages[0], raws[0]);
+    __builtin_amdgcn_sched_barrier(0);
+    __syncthreads();
+    for (int t = tbeg;;) {                                           // (exits that let every step know what is on the way)
+      step(t, Int<0>{});
+      if (++t >= tend) break;
+      step(t, Int<1>{});
+      if (++t >= tend) break;
+    }
   }
 
   sum = halves_sum(sum);
@@ -1279,6 +1277,7 @@ __global__ __launch_bounds__(256, 2) void cache8_prefill_kernel(Cache8AttendLaun
 // Joins the splits of each row; one wave per (row, query head).
 template <int TYPE, int DH>
 __global__ __launch_bounds__(256) void cache8_prefill_merge_kernel(Cache8AttendLaunch L, int splits, const float* partials) {
+  constexpr int RS = row_shift(DH), kRowTile = 1 << RS;
   const Cache8& c = L.c;
   const Cache8Batch& b = L.b;
   const int heads = c.num_kv * L.gqa, lane = threadIdx.x & 63;
@@ -1294,7 +1293,7 @@ __global__ __launch_bounds__(256) void cache8_prefill_merge_kernel(Cache8AttendL
   const int last = (int)((r0 + kRowTile < rows_all ? r0 + kRowTile : rows_all) - 1);
   const int parts = splits_of(tile_seen(L, len, n, last / L.gqa), splits);
   if (parts == 1) return;
-  const int64_t slot = first_slot(b, s, L.gqa, 7, 1) + (r >> 7);
+  const int64_t slot = first_slot(b, s, L.gqa, RS, 1) + (r >> RS);
   const int in = (int)(r & (kRowTile - 1));
   const float* x = partials + (slot * c.num_kv + h) * splits * split_floats(DH);
   constexpr int DPL = DH / 64;
@@ -1368,9 +1367,9 @@ template <int T, int F, int D> struct Prefill {
     if constexpr (T == kFp32) {
       return -1;
     } else {
-      const int64_t tiles = row_tiles(L.b.num_rows, L.b.num_seqs, L.gqa);
-      const int splits = prefill_splits(L.b.num_rows, L.b.num_seqs, L.c.num_kv, L.gqa);
-      cache8_prefill_kernel<F, T, D><<<dim3((unsigned)(tiles * L.c.num_kv), splits), 256, 0, st>>>(L, splits, (float*)L.ws);
+      const int64_t tiles = row_tiles(L.b.num_rows, L.b.num_seqs, L.gqa, D);
+      const int splits = prefill_splits(L.b.num_rows, L.b.num_seqs, L.c.num_kv, L.gqa, D);
+      cache8_prefill_kernel<F, T, D><<<dim3((unsigned)(tiles * L.c.num_kv), splits), 64 * row_waves(D), 0, st>>>(L, splits, (float*)L.ws);
       if (splits > 1) {
         const int64_t waves = L.b.num_rows * L.c.num_kv * L.gqa;
         cache8_prefill_merge_kernel<T, D><<<(unsigned)((waves + 3) / 4), 256, 0, st>>>(L, splits, (const float*)L.ws);
@@ -1396,8 +1395,8 @@ int64_t cache8_decode_ws_bytes(int32_t num_seqs, int32_t, int32_t gqa, int32_t d
 }
 int64_t cache8_prefill_ws_bytes(int64_t num_rows, int32_t num_seqs, int32_t num_kv, int32_t gqa, int32_t dh) {
   if (num_rows == 0 || num_seqs == 0) return 0;
-  const int splits = prefill_splits(num_rows, num_seqs, num_kv, gqa);
-  return splits == 1 ? 0 : row_tiles(num_rows, num_seqs, gqa) * num_kv * splits * split_floats(dh) * 4;
+  const int splits = prefill_splits(num_rows, num_seqs, num_kv, gqa, dh);
+  return splits == 1 ? 0 : row_tiles(num_rows, num_seqs, gqa, dh) * num_kv * splits * split_floats(dh) * 4;
 }
 
 }  // namespace sphkv
