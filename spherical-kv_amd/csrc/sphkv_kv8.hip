@@ -1117,6 +1117,7 @@ __global__ __launch_bounds__(64 * row_waves(DH), 2) void cache8_prefill_kernel(C
   auto find = [&](int t) { return table[min((t * kTileTokens + run * 16) >> c.page_shift, last_blk)]; };
   auto fetch = [&](int t, int found, Raw& raw) {
     const int at = t * kTileTokens + run * 16;
+    asm volatile("" : "+v"(found));                                 // (waited for here and no earlier)
     int pg = uniform(found);
     pg = t < tend && at < len && pg < (int)c.num_pages ? pg : -1;
     raw.page = pg;
@@ -1158,7 +1159,7 @@ __global__ __launch_bounds__(64 * row_waves(DH), 2) void cache8_prefill_kernel(C
   auto step = [&](int t, auto parity) {
     constexpr int bf = parity.value;
     const int t0 = t * kTileTokens;
-    if (t0 < lim_max) {
+    if (t0 < lim_max && t < tend) {
       floatx16 sc[2];
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
@@ -1236,14 +1237,15 @@ __global__ __launch_bounds__(64 * row_waves(DH), 2) void cache8_prefill_kernel(C
     stage(tbeg, 0, raws[0]);
     __builtin_amdgcn_sched_barrier(0);
     pages[1] = find(tbeg + 3);
-    fetch(tbeg + 2, pages[0], raws[0]);
     __builtin_amdgcn_sched_barrier(0);
+    fetch(tbeg + 2, pages[0], raws[0]);
+    // (nothing on the way into the loop: its waits are then for its own loads, not
+    // for registers that only the loads before it used)
+    __builtin_amdgcn_s_waitcnt(0x0F70);                              // vmcnt(0)
     __syncthreads();
-    for (int t = tbeg;;) {                                           // (exits that let every step know what is on the way)
+    for (int t = tbeg; t < tend; t += 2) {                           // (one exit: every step knows what is on the way)
       step(t, Int<0>{});
-      if (++t >= tend) break;
-      step(t, Int<1>{});
-      if (++t >= tend) break;
+      step(t + 1, Int<1>{});
     }
   }
 
