@@ -980,24 +980,32 @@ __global__ __launch_bounds__(64 * WAVES) void cache8_decode_merge_kernel(Cache8A
 //
 // With few row tiles the keys of each are split over workgroups, whose partials a
 // second kernel joins.
-// Waves of a workgroup, 32 rows each, and the workgroups that run at once: at
-// DH 128 eight waves share a tile and fill a CU's registers; at DH 64 four do, and
-// three workgroups fit.
+// A workgroup's shape.  At DH 128 eight waves fill a CU's registers and share its
+// tiles: 256 rows; or, where the sequences have 128 rows or fewer on average, 128
+// rows by two groups of four waves that take the tiles in turn (a tile's step is
+// then a wave's 600 instructions, whatever the rows: four long documents of 20 to 96
+// rows a head 82.6 us with all waves on the same tile, 75.3 in turn).  At DH 64 four
+// waves, 128 rows, and three workgroups to a CU.
+struct PrefillShape {
+  int row_shift, groups, turns;         // log2 of a tile's rows, workgroups at once, wave groups that take turns
+};
+__host__ __device__ __forceinline__ PrefillShape prefill_shape(int64_t num_rows, int num_seqs, int gqa, int dh) {
+  if (dh == 64) return {7, 768, 1};
+  return num_rows * gqa <= 128 * (int64_t)num_seqs ? PrefillShape{7, 256, 2} : PrefillShape{8, 256, 1};
+}
 constexpr int kSplitLeast = 4;          // tiles of a split
 constexpr int kSplitMost = 64;
-__host__ __device__ constexpr int row_waves(int dh) { return dh == 128 ? 8 : 4; }
-__host__ __device__ constexpr int row_shift(int dh) { return dh == 128 ? 8 : 7; }       // log2 of a tile's rows
-__host__ __device__ constexpr int prefill_groups(int dh) { return dh == 128 ? 256 : 768; }
 
-__host__ __device__ __forceinline__ int64_t row_tiles(int64_t num_rows, int num_seqs, int gqa, int dh) {
-  return ((num_rows * gqa) >> row_shift(dh)) + num_seqs;
+__host__ __device__ __forceinline__ int64_t row_tiles(int64_t num_rows, int num_seqs, int gqa, int row_shift) {
+  return ((num_rows * gqa) >> row_shift) + num_seqs;
 }
-__host__ __device__ __forceinline__ int prefill_splits(int64_t num_rows, int num_seqs, int num_kv, int gqa, int dh) {
-  const int64_t wgs = row_tiles(num_rows, num_seqs, gqa, dh) * num_kv, s = prefill_groups(dh) / wgs;
+__host__ __device__ __forceinline__ int prefill_splits(int64_t num_rows, int num_seqs, int num_kv, int gqa, PrefillShape p) {
+  // (sequences of few rows have a tile each, and their slots are up to twice as many)
+  const int64_t tiles = p.turns == 2 ? num_seqs : row_tiles(num_rows, num_seqs, gqa, p.row_shift), s = p.groups / (tiles * num_kv);
   return (int)(s < 1 ? 1 : (s > kSplitMost ? kSplitMost : s));
 }
 // floats of one split's partial: reference and sum per row, then acc[rows][DH]
-__host__ __device__ __forceinline__ int64_t split_floats(int dh) { return (int64_t)(dh + 2) << row_shift(dh); }
+__host__ __device__ __forceinline__ int64_t split_floats(int dh, int row_shift) { return (int64_t)(dh + 2) << row_shift; }
 
 // tokens that a sequence's row of token `last_token` sees, and the splits that
 // so many are worth
@@ -1042,18 +1050,25 @@ __device__ __forceinline__ void reads_ahead() {
   __builtin_amdgcn_sched_group_barrier(0x008, kAhead, 0);
 }
 
-template <int FMT, int TYPE, int DH>
-__global__ __launch_bounds__(64 * row_waves(DH), 2) void cache8_prefill_kernel(Cache8AttendLaunch L, int splits, float* partials) {
-  constexpr int KS = DH / 16, DB = DH / 32, RS = row_shift(DH), kRowTile = 1 << RS;      // k-steps, value blocks
-  __shared__ __align__(16) _Float16 s_k[2][kTileTokens * DH], s_v[2][kTileTokens * DH];
-  __shared__ float s_sk[2][4], s_lsv[2][4], s_inv[2][4];
+template <int FMT, int TYPE, int DH, int TURNS>
+__global__ __launch_bounds__(DH == 128 ? 512 : 256, 2) void cache8_prefill_kernel(Cache8AttendLaunch L, int splits, float* partials) {
+  constexpr int KS = DH / 16, DB = DH / 32;                        // k-steps, value blocks
+  constexpr int kRowWaves = (DH == 128 ? 8 : 4) / TURNS, kRowTile = 32 * kRowWaves, RS = kRowTile == 256 ? 8 : 7;
+  constexpr int NB = 2 * TURNS, HALF = TURNS;                      // tiles in LDS; half of them between two barriers
+  constexpr int NR = 2;                                    // tiles on the way
+  __shared__ __align__(16) _Float16 s_k[NB][kTileTokens * DH], s_v[NB][kTileTokens * DH];
+  __shared__ float s_sk[NB][4], s_lsv[NB][4], s_inv[NB][4];
   const Cache8& c = L.c;
   const Cache8Batch& b = L.b;
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), col = lane & 31, half = lane >> 5;
-  // neighbours take different heads (eight of them: one per XCD and its L2), and
-  // the longest rows of a sequence come first
-  const int h = blockIdx.x % c.num_kv, z = blockIdx.y, gqa = L.gqa;
-  const int64_t slot = (gridDim.x - 1 - blockIdx.x) / c.num_kv;
+  // Neighbours take the splits of one row tile, then different heads (unsplit and
+  // eight of them: one per XCD and its L2, which the row tiles of a head share; with
+  // a row tile per sequence nothing is shared, and a head per XCD reads half of
+  // each L2's channels: 122 us, 76 with the splits first).  The longest rows of a
+  // sequence come first.
+  const uint32_t pair = blockIdx.x / splits;
+  const int h = pair % c.num_kv, z = blockIdx.x % splits, gqa = L.gqa;
+  const int64_t slot = (gridDim.x / splits - 1 - pair) / c.num_kv;
   const int s = uniform(seq_of_slot(b, slot, gqa, RS, 1));
   int begin, end;
   rows_of(b, s, begin, end);
@@ -1070,7 +1085,8 @@ __global__ __launch_bounds__(64 * row_waves(DH), 2) void cache8_prefill_kernel(C
   const int tbeg = (int)((int64_t)NT * z / parts), tend = (int)((int64_t)NT * (z + 1) / parts);
 
   // this lane's row
-  const int64_t r = r0 + wave * 32 + col;
+  const int row_wave = wave % kRowWaves, turn = wave / kRowWaves;
+  const int64_t r = r0 + row_wave * 32 + col;
   const bool live = r < rows_all;
   const int tok = live ? (int)(r / gqa) : 0, hd = live ? (int)(r - (int64_t)tok * gqa) : 0;
   const int lim = live ? tile_seen(L, len, n, tok) : 0;
@@ -1103,7 +1119,7 @@ __global__ __launch_bounds__(64 * row_waves(DH), 2) void cache8_prefill_kernel(C
     uintx4 k, v;
     float2 sc;
     int page;
-  } raws[2];                                                        // of even and odd tiles
+  } raws[NR];
   int pages[2];
   const int64_t page_bytes = (int64_t)c.num_kv * DH << c.page_shift;
   const uint8_t* kbase = c.k + ((int64_t)h * DH << c.page_shift);
@@ -1154,12 +1170,13 @@ __global__ __launch_bounds__(64 * row_waves(DH), 2) void cache8_prefill_kernel(C
   float ref = kNoScore, sum = 0.f;
   const int ktok = 16 * (col >> 4) + 8 * ((col >> 2) & 1) + 4 * ((col >> 3) & 1) + (col & 3);   // token of score row `col`
 
-  // Tile t, from LDS buffer bf (a constant); then tile t + 1, whose loads had two
-  // steps, into the other, and the loads of t + 3.
-  auto step = [&](int t, auto parity) {
-    constexpr int bf = parity.value;
+  // Tile t from LDS buffer bf (a constant), by the waves whose turn it is; then tile
+  // t + HALF, whose loads had NR steps, into its own, and the loads of the tile NR
+  // later.
+  auto step = [&](int t, auto buffer) {
+    constexpr int bf = buffer.value, nx = (bf + HALF) % NR, px = nx & 1;
     const int t0 = t * kTileTokens;
-    if (t0 < lim_max && t < tend) {
+    if (t0 < lim_max && t < tend && (TURNS == 1 || turn == bf % TURNS)) {
       floatx16 sc[2];
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
@@ -1219,37 +1236,73 @@ __global__ __launch_bounds__(64 * row_waves(DH), 2) void cache8_prefill_kernel(C
         }
       reads_ahead<4 * DB>();
     }
-    stage(t + 1, 1 - bf, raws[1 - bf]);
+    stage(t + HALF, (bf + HALF) % NB, raws[nx]);
     __builtin_amdgcn_sched_barrier(0);
-    pages[bf] = find(t + 4);
+    pages[1 - px] = find(t + HALF + NR + 1);
     __builtin_amdgcn_sched_barrier(0);
-    fetch(t + 3, pages[1 - bf], raws[1 - bf]);
+    fetch(t + HALF + NR, pages[px], raws[nx]);
     __builtin_amdgcn_sched_barrier(0);
-    __syncthreads();
+    if (bf % HALF == HALF - 1) __syncthreads();
   };
   if (tbeg < tend) {
     pages[0] = find(tbeg);
-    pages[1] = find(tbeg + 1);
-    fetch(tbeg, pages[0], raws[0]);
-    pages[0] = find(tbeg + 2);
-    __builtin_amdgcn_sched_barrier(0);                               // (in the loop's order, for its waits)
-    fetch(tbeg + 1, pages[1], raws[1]);
-    stage(tbeg, 0, raws[0]);
-    __builtin_amdgcn_sched_barrier(0);
-    pages[1] = find(tbeg + 3);
-    __builtin_amdgcn_sched_barrier(0);
-    fetch(tbeg + 2, pages[0], raws[0]);
+#pragma unroll
+    for (int i = 0; i < NR; ++i) {
+      pages[(i + 1) & 1] = find(tbeg + i + 1);
+      fetch(tbeg + i, pages[i & 1], raws[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < HALF; ++i) {
+      stage(tbeg + i, i, raws[i]);
+      pages[(NR + i + 1) & 1] = find(tbeg + NR + i + 1);
+      fetch(tbeg + NR + i, pages[(NR + i) & 1], raws[i]);
+    }
     // (nothing on the way into the loop: its waits are then for its own loads, not
     // for registers that only the loads before it used)
     __builtin_amdgcn_s_waitcnt(0x0F70);                              // vmcnt(0)
     __syncthreads();
-    for (int t = tbeg; t < tend; t += 2) {                           // (one exit: every step knows what is on the way)
+    for (int t = tbeg; t < tend; t += NB) {                          // (one exit: every step knows what is on the way)
       step(t, Int<0>{});
       step(t + 1, Int<1>{});
+      if constexpr (NB == 4) {
+        step(t + 2, Int<2>{});
+        step(t + 3, Int<3>{});
+      }
     }
   }
 
   sum = halves_sum(sum);
+  if constexpr (TURNS == 2) {                                         // the second group's sums, through LDS, to the first
+    float* o = (float*)s_k;                                           // [DH / 4][kRowTile][4]
+    float* rs = (float*)s_v;                                          // references, sums
+    const int row = row_wave * 32 + col;
+    static_assert(sizeof(s_k) >= sizeof(float) * kRowTile * DH && sizeof(s_v) >= sizeof(float) * 2 * kRowTile, "");
+    if (turn == 1) {
+      if (half == 0) {
+        rs[row] = ref;
+        rs[kRowTile + row] = sum;
+      }
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *(floatx4*)&o[((8 * d + 2 * i + half) * kRowTile + row) * 4] =
+              floatx4{acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]};
+    }
+    __syncthreads();
+    if (turn == 1) return;
+    const float other = rs[row], R = fmaxf(ref, other), f = exp2_of(ref - R), g = exp2_of(other - R);
+    ref = R;
+    sum = fmaf(sum, f, rs[kRowTile + row] * g);
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const floatx4 x = *(const floatx4*)&o[((8 * d + 2 * i + half) * kRowTile + row) * 4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[d][4 * i + e] = fmaf(acc[d][4 * i + e], f, x[e] * g);
+      }
+  }
   if (!live) return;
   const int64_t at = (int64_t)(begin + tok) * c.num_kv * gqa + h * gqa + hd;
   if (parts == 1) {
@@ -1261,8 +1314,8 @@ __global__ __launch_bounds__(64 * row_waves(DH), 2) void cache8_prefill_kernel(C
         store1<TYPE>(L.out, at * DH + 32 * d + 8 * (i >> 2) + 4 * half + (i & 3), sum == 0.f ? 0.f : acc[d][i] * inv);
     if (L.lse && half == 0) L.lse[at] = sum == 0.f ? -INFINITY : (ref + log2_of(sum)) * 0.693147180559945f;
   } else {
-    float* o = partials + ((slot * c.num_kv + h) * splits + z) * split_floats(DH);
-    const int row = wave * 32 + col;
+    float* o = partials + ((slot * c.num_kv + h) * splits + z) * split_floats(DH, RS);
+    const int row = row_wave * 32 + col;
     if (half == 0) {
       o[row] = ref;
       o[kRowTile + row] = sum;
@@ -1278,8 +1331,9 @@ __global__ __launch_bounds__(64 * row_waves(DH), 2) void cache8_prefill_kernel(C
 
 // Joins the splits of each row; one wave per (row, query head).
 template <int TYPE, int DH>
-__global__ __launch_bounds__(256) void cache8_prefill_merge_kernel(Cache8AttendLaunch L, int splits, const float* partials) {
-  constexpr int RS = row_shift(DH), kRowTile = 1 << RS;
+__global__ __launch_bounds__(256) void cache8_prefill_merge_kernel(Cache8AttendLaunch L, int RS, int splits,
+                                                                   const float* partials) {
+  const int kRowTile = 1 << RS;
   const Cache8& c = L.c;
   const Cache8Batch& b = L.b;
   const int heads = c.num_kv * L.gqa, lane = threadIdx.x & 63;
@@ -1297,11 +1351,11 @@ __global__ __launch_bounds__(256) void cache8_prefill_merge_kernel(Cache8AttendL
   if (parts == 1) return;
   const int64_t slot = first_slot(b, s, L.gqa, RS, 1) + (r >> RS);
   const int in = (int)(r & (kRowTile - 1));
-  const float* x = partials + (slot * c.num_kv + h) * splits * split_floats(DH);
+  const float* x = partials + (slot * c.num_kv + h) * splits * split_floats(DH, RS);
   constexpr int DPL = DH / 64;
   float R, l, acc[DPL];
   join<DPL, 16>(0, parts, 1, kRowTile, [&](int64_t z) {
-    const float* p = x + z * split_floats(DH);
+    const float* p = x + z * split_floats(DH, RS);
     return Partial{p + in, p + 2 * kRowTile + in * DH};
   }, R, l, acc);
 #pragma unroll
@@ -1369,12 +1423,19 @@ template <int T, int F, int D> struct Prefill {
     if constexpr (T == kFp32) {
       return -1;
     } else {
-      const int64_t tiles = row_tiles(L.b.num_rows, L.b.num_seqs, L.gqa, D);
-      const int splits = prefill_splits(L.b.num_rows, L.b.num_seqs, L.c.num_kv, L.gqa, D);
-      cache8_prefill_kernel<F, T, D><<<dim3((unsigned)(tiles * L.c.num_kv), splits), 64 * row_waves(D), 0, st>>>(L, splits, (float*)L.ws);
+      const PrefillShape shape = prefill_shape(L.b.num_rows, L.b.num_seqs, L.gqa, D);
+      const int64_t tiles = row_tiles(L.b.num_rows, L.b.num_seqs, L.gqa, shape.row_shift);
+      const int splits = prefill_splits(L.b.num_rows, L.b.num_seqs, L.c.num_kv, L.gqa, shape);
+      const unsigned grid = (unsigned)(tiles * L.c.num_kv * splits);
+      if constexpr (D == 128) {
+        if (shape.turns == 2) cache8_prefill_kernel<F, T, D, 2><<<grid, 512, 0, st>>>(L, splits, (float*)L.ws);
+        else cache8_prefill_kernel<F, T, D, 1><<<grid, 512, 0, st>>>(L, splits, (float*)L.ws);
+      } else {
+        cache8_prefill_kernel<F, T, D, 1><<<grid, 256, 0, st>>>(L, splits, (float*)L.ws);
+      }
       if (splits > 1) {
         const int64_t waves = L.b.num_rows * L.c.num_kv * L.gqa;
-        cache8_prefill_merge_kernel<T, D><<<(unsigned)((waves + 3) / 4), 256, 0, st>>>(L, splits, (const float*)L.ws);
+        cache8_prefill_merge_kernel<T, D><<<(unsigned)((waves + 3) / 4), 256, 0, st>>>(L, shape.row_shift, splits, (const float*)L.ws);
       }
       return hipPeekAtLastError() == hipSuccess ? 0 : -1;
     }
@@ -1397,8 +1458,9 @@ int64_t cache8_decode_ws_bytes(int32_t num_seqs, int32_t, int32_t gqa, int32_t d
 }
 int64_t cache8_prefill_ws_bytes(int64_t num_rows, int32_t num_seqs, int32_t num_kv, int32_t gqa, int32_t dh) {
   if (num_rows == 0 || num_seqs == 0) return 0;
-  const int splits = prefill_splits(num_rows, num_seqs, num_kv, gqa, dh);
-  return splits == 1 ? 0 : row_tiles(num_rows, num_seqs, gqa, dh) * num_kv * splits * split_floats(dh) * 4;
+  const PrefillShape p = prefill_shape(num_rows, num_seqs, gqa, dh);
+  const int splits = prefill_splits(num_rows, num_seqs, num_kv, gqa, p);
+  return splits == 1 ? 0 : row_tiles(num_rows, num_seqs, gqa, p.row_shift) * num_kv * splits * split_floats(dh, p.row_shift) * 4;
 }
 
 }  // namespace sphkv
