@@ -19,8 +19,8 @@ that share one must not run concurrently.  No CPU or torch fallback exists.
 """
 from __future__ import annotations
 
-import contextlib
 import math
+from functools import lru_cache
 from typing import Optional, Tuple
 
 import torch
@@ -32,8 +32,10 @@ _lib = sphkv_lib.load()
 
 FORMATS = {"int8": 0, "e4m3": 1}                # SPHKV_CACHE8_*
 _TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+_FLOAT, _INT = torch.float32, torch.int32
+# torch's raw accessors where this build has them: half a microsecond a call less
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-_NOTHING = contextlib.nullcontext()
+_device_index = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _need(t: torch.Tensor, dtype, name: str, device=None) -> None:
@@ -55,7 +57,7 @@ class Cache8:
     values), contiguous and 16-byte aligned; fmt "int8" or "e4m3"."""
 
     __slots__ = ("k_codes", "v_codes", "scales", "fmt", "num_pages", "num_kv", "page_size", "dh", "device", "_tail",
-                 "_ptrs", "_index")
+                 "_ptrs", "_index", "_sm")
 
     def __init__(self, k_codes: torch.Tensor, v_codes: torch.Tensor, scales: torch.Tensor, fmt: str = "int8"):
         if fmt not in FORMATS:
@@ -82,6 +84,7 @@ class Cache8:
         self._index = dev.index
         self._ptrs = (k_codes.data_ptr(), v_codes.data_ptr(), scales.data_ptr(), num_pages, num_kv)
         self._tail = (dh, page_size, FORMATS[fmt])
+        self._sm = 1.0 / math.sqrt(dh)
 
     @staticmethod
     def allocate(num_pages: int, num_kv: int, dh: int, page_size: int = 16, fmt: str = "int8",
@@ -91,40 +94,48 @@ class Cache8:
         v = torch.zeros((num_pages, num_kv, max(page_size // 16, 1), dh, 16), dtype=torch.uint8, device=device)
         return Cache8(k, v, torch.zeros((num_pages, num_kv, 2), dtype=torch.float32, device=device), fmt)
 
-    def _on_device(self):
-        """A context in which launches go to the cache's device."""
-        return _NOTHING if torch.cuda.current_device() == self._index else torch.cuda.device(self.device)
-
-    def _stream(self) -> int:
-        """Raw handle of torch's current stream on the cache's device."""
-        return _raw_stream(self._index) if _raw_stream else torch.cuda.current_stream(self.device).cuda_stream
+    def _call(self, fn, *args) -> None:
+        """Launch on torch's current stream of the cache's device, that device current."""
+        if _device_index() != self._index:
+            with torch.cuda.device(self.device):
+                return self._call(fn, *args)
+        rc = fn(*args, _raw_stream(self._index) if _raw_stream else torch.cuda.current_stream(self.device).cuda_stream)
+        if rc:
+            check(rc, fn.__name__)
 
 
 def _seq_args(cache: Cache8, table: torch.Tensor, at: torch.Tensor, cu_rows: Optional[torch.Tensor], name: str):
-    """Checks of a batch's page table, per-sequence int32 values and row starts."""
+    """Checks of a batch's page table, per-sequence int32 values and row starts;
+    (table, row stride, blocks, sequences) for the call."""
     dev = cache.device
-    _need(table, torch.int32, "table", dev)
-    _need(at, torch.int32, name, dev)
-    if table.dim() != 2 or at.dim() != 1 or at.shape[0] != table.shape[0]:
+    _need(table, _INT, "table", dev)
+    _need(at, _INT, name, dev)
+    if table.dim() != 2 or at.dim() != 1:
         raise ValueError(f"table must be [num_seqs, max_blocks] and {name} [num_seqs]")
-    if (table.shape[1] > 1 and table.stride(1) != 1) or not at.is_contiguous():
+    n, blocks = table.shape
+    row, one = table.stride()
+    if at.shape[0] != n:
+        raise ValueError(f"table must be [num_seqs, max_blocks] and {name} [num_seqs]")
+    if (blocks > 1 and one != 1) or (n > 1 and at.stride(0) != 1):
         raise ValueError(f"table's rows and {name} must be contiguous")
-    if table.shape[0] > 1 and table.stride(0) < table.shape[1]:
+    if n > 1 and row < blocks:
         raise ValueError("table's rows must not overlap")
     if cu_rows is not None:
-        _need(cu_rows, torch.int32, "cu_rows", dev)
-        if cu_rows.dim() != 1 or cu_rows.shape[0] != at.shape[0] + 1 or not cu_rows.is_contiguous():
+        _need(cu_rows, _INT, "cu_rows", dev)
+        if cu_rows.dim() != 1 or cu_rows.shape[0] != n + 1 or cu_rows.stride(0) != 1:
             raise ValueError("cu_rows must be a contiguous [num_seqs + 1]")
+    return table.data_ptr(), row, blocks, n
 
 
-def _rows(t: torch.Tensor, name: str, heads: int, cache: Cache8):
-    """Checks of [rows, heads, dh] rows of any row and head stride."""
-    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != cache.dh:
-        raise ValueError(f"{name} must be [rows, {heads}, {cache.dh}], got {tuple(t.shape)}")
-    if t.stride(2) != 1:
-        raise ValueError(f"the {cache.dh} elements of a row of {name} must be contiguous")
-    if t.stride(0) < 0 or t.stride(1) < 0:
-        raise ValueError(f"{name} must not have negative strides")
+def _rows(t: torch.Tensor, name: str, heads: int, dh: int):
+    """Checks of [rows, heads, dh] rows of any row and head stride; (row, head) strides."""
+    shape = t.shape
+    if len(shape) != 3 or shape[1] != heads or shape[2] != dh:
+        raise ValueError(f"{name} must be [rows, {heads}, {dh}], got {tuple(shape)}")
+    row, head, one = t.stride()
+    if one != 1:
+        raise ValueError(f"the {dh} elements of a row of {name} must be contiguous")
+    return row, head
 
 
 def _out(t: Optional[torch.Tensor], shape, dtype, name: str, cache: Cache8) -> torch.Tensor:
@@ -149,23 +160,21 @@ def cache8_write(cache: Cache8, k: torch.Tensor, v: torch.Tensor, table: torch.T
     held are rounded to the new scale.  A written page belongs to one sequence.
     Tokens past the table, of a negative start or of a page outside the cache
     are dropped."""
-    _seq_args(cache, table, start, cu_rows, "start")
+    tab, stride, blocks, n = _seq_args(cache, table, start, cu_rows, "start")
     if not isinstance(k, torch.Tensor) or k.dtype not in _TYPES:
         raise TypeError("k must be an fp16, bf16 or fp32 tensor")
     _need(k, k.dtype, "k", cache.device)
     _need(v, k.dtype, "v", cache.device)
-    _rows(k, "k", cache.num_kv, cache)
-    _rows(v, "v", cache.num_kv, cache)
-    if v.shape != k.shape:
+    k_row, k_head = _rows(k, "k", cache.num_kv, cache.dh)
+    v_row, v_head = _rows(v, "v", cache.num_kv, cache.dh)
+    rows = k.shape[0]
+    if v.shape[0] != rows:
         raise ValueError("k and v must have as many rows")
-    if cu_rows is None and k.shape[0] != start.shape[0]:
+    if cu_rows is None and rows != n:
         raise ValueError("without cu_rows there is one row per sequence")
-    with cache._on_device():
-        rc = _lib.sphkv_cache8_write(
-            k.data_ptr(), v.data_ptr(), _TYPES[k.dtype], k.stride(0), k.stride(1), v.stride(0), v.stride(1), k.shape[0],
-            None if cu_rows is None else cu_rows.data_ptr(), start.data_ptr(), table.data_ptr(), table.stride(0),
-            table.shape[1], table.shape[0], *cache._ptrs, *cache._tail, cache._stream())
-    check(rc, "cache8_write")
+    cache._call(_lib.sphkv_cache8_write, k.data_ptr(), v.data_ptr(), _TYPES[k.dtype], k_row, k_head, v_row, v_head, rows,
+                None if cu_rows is None else cu_rows.data_ptr(), start.data_ptr(), tab, stride, blocks, n, *cache._ptrs,
+                *cache._tail)
 
 
 def cache8_read(cache: Cache8, table: torch.Tensor, start: torch.Tensor, cu_rows: Optional[torch.Tensor] = None,
@@ -178,35 +187,31 @@ def cache8_read(cache: Cache8, table: torch.Tensor, start: torch.Tensor, cu_rows
     token each, num_seqs).  Rows behind the last sequence are left as they were
     in k_out and v_out.  Tokens past the table, of a negative position or of a
     page outside the cache read as zeros."""
-    _seq_args(cache, table, start, cu_rows, "start")
+    tab, stride, blocks, n = _seq_args(cache, table, start, cu_rows, "start")
     if dtype not in _TYPES:
         raise TypeError("dtype must be fp16, bf16 or fp32")
     if cu_rows is None:
-        if num_rows is not None and num_rows != start.shape[0]:
+        if num_rows is not None and num_rows != n:
             raise ValueError("without cu_rows there is one row per sequence")
-        num_rows = start.shape[0]
+        num_rows = n
     elif num_rows is None or num_rows < 0:
         raise ValueError("num_rows (cu_rows' last value, or more) is needed with cu_rows")
     shape = (int(num_rows), cache.num_kv, cache.dh)
     k_out, v_out = _out(k_out, shape, dtype, "k_out", cache), _out(v_out, shape, dtype, "v_out", cache)
-    with cache._on_device():
-        rc = _lib.sphkv_cache8_read(
-            *cache._ptrs, *cache._tail, None if cu_rows is None else cu_rows.data_ptr(), start.data_ptr(),
-            table.data_ptr(), table.stride(0), table.shape[1], table.shape[0], shape[0], k_out.data_ptr(),
-            v_out.data_ptr(), _TYPES[dtype], cache._stream())
-    check(rc, "cache8_read")
+    cache._call(_lib.sphkv_cache8_read, *cache._ptrs, *cache._tail, None if cu_rows is None else cu_rows.data_ptr(),
+                start.data_ptr(), tab, stride, blocks, n, shape[0], k_out.data_ptr(), v_out.data_ptr(), _TYPES[dtype])
     return k_out, v_out
 
 
-def _query(cache: Cache8, q: torch.Tensor) -> int:
-    """q heads per kv head of a checked q."""
-    if not isinstance(q, torch.Tensor) or q.dtype not in (torch.float16, torch.bfloat16):
+def _query(cache: Cache8, q: torch.Tensor):
+    """Checks of q; (shape, q heads per kv head, row stride, head stride)."""
+    if not isinstance(q, torch.Tensor) or (q.dtype is not torch.float16 and q.dtype is not torch.bfloat16):
         raise TypeError("q must be an fp16 or bf16 tensor")
     _need(q, q.dtype, "q", cache.device)
-    if q.dim() != 3 or q.shape[1] == 0 or q.shape[1] % cache.num_kv:
+    shape = q.shape
+    if len(shape) != 3 or shape[1] == 0 or shape[1] % cache.num_kv:
         raise ValueError("q must be [rows, num_kv * gqa, dh]")
-    _rows(q, "q", q.shape[1], cache)
-    return q.shape[1] // cache.num_kv
+    return shape, shape[1] // cache.num_kv, *_rows(q, "q", shape[1], cache.dh)
 
 
 def _workspace(cache: Cache8, need: int, workspace: Optional[torch.Tensor]):
@@ -222,19 +227,29 @@ def _workspace(cache: Cache8, need: int, workspace: Optional[torch.Tensor]):
     return workspace.data_ptr(), workspace.numel(), workspace
 
 
+@lru_cache(maxsize=256)
+def _decode_bytes(num_seqs: int, num_kv: int, gqa: int, dh: int) -> int:
+    return _lib.sphkv_cache8_decode_workspace_bytes(num_seqs, num_kv, gqa, dh)
+
+
+@lru_cache(maxsize=256)
+def _prefill_bytes(num_rows: int, num_seqs: int, num_kv: int, gqa: int, dh: int) -> int:
+    return _lib.sphkv_cache8_prefill_workspace_bytes(num_rows, num_seqs, num_kv, gqa, dh)
+
+
 def decode_workspace_bytes(cache: Cache8, num_seqs: int, gqa: int) -> int:
     """Bytes of a workspace for cache8_decode of num_seqs sequences."""
-    n = _lib.sphkv_cache8_decode_workspace_bytes(int(num_seqs), cache.num_kv, int(gqa), cache.dh)
+    n = _decode_bytes(int(num_seqs), cache.num_kv, int(gqa), cache.dh)
     if n < 0:
-        raise ValueError("bad num_seqs or gqa for the decode workspace")
+        raise ValueError("bad num_seqs or gqa (1..64) for the decode workspace")
     return n
 
 
 def prefill_workspace_bytes(cache: Cache8, num_rows: int, num_seqs: int, gqa: int) -> int:
     """Bytes of a workspace for cache8_prefill of num_rows rows of num_seqs sequences."""
-    n = _lib.sphkv_cache8_prefill_workspace_bytes(int(num_rows), int(num_seqs), cache.num_kv, int(gqa), cache.dh)
+    n = _prefill_bytes(int(num_rows), int(num_seqs), cache.num_kv, int(gqa), cache.dh)
     if n < 0:
-        raise ValueError("bad num_rows, num_seqs or gqa for the prefill workspace")
+        raise ValueError("bad num_rows, num_seqs or gqa (1..64) for the prefill workspace")
     return n
 
 
@@ -247,21 +262,17 @@ def cache8_decode(cache: Cache8, q: torch.Tensor, table: torch.Tensor, lens: tor
     given.  Returns out (q's shape and type), with return_lse (out, lse):
     lse fp32 [num_seqs, num_kv * gqa] is the natural log of the softmax's sum.
     A sequence without tokens gets zeros and -inf."""
-    _seq_args(cache, table, lens, None, "lens")
-    gqa = _query(cache, q)
-    if q.shape[0] != lens.shape[0]:
+    tab, stride, blocks, n = _seq_args(cache, table, lens, None, "lens")
+    shape, gqa, q_row, q_head = _query(cache, q)
+    if shape[0] != n:
         raise ValueError("q must have one row per sequence")
-    out = _out(out, q.shape, q.dtype, "out", cache)
+    out = _out(out, shape, q.dtype, "out", cache)
     if return_lse or lse is not None:
-        lse = _out(lse, q.shape[:2], torch.float32, "lse", cache)
-    ws, nbytes, _keep = _workspace(cache, decode_workspace_bytes(cache, q.shape[0], gqa), workspace)
-    with cache._on_device():
-        rc = _lib.sphkv_cache8_decode(
-            q.data_ptr(), _TYPES[q.dtype], q.stride(0), q.stride(1), lens.data_ptr(), table.data_ptr(),
-            table.stride(0), table.shape[1], table.shape[0], *cache._ptrs, gqa, *cache._tail,
-            1.0 / math.sqrt(cache.dh) if sm_scale is None else float(sm_scale), out.data_ptr(),
-            None if lse is None else lse.data_ptr(), ws, nbytes, cache._stream())
-    check(rc, "cache8_decode")
+        lse = _out(lse, shape[:2], _FLOAT, "lse", cache)
+    ws, nbytes, _keep = _workspace(cache, decode_workspace_bytes(cache, n, gqa), workspace)
+    cache._call(_lib.sphkv_cache8_decode, q.data_ptr(), _TYPES[q.dtype], q_row, q_head, lens.data_ptr(), tab, stride, blocks,
+                n, *cache._ptrs, gqa, *cache._tail, cache._sm if sm_scale is None else float(sm_scale), out.data_ptr(),
+                None if lse is None else lse.data_ptr(), ws, nbytes)
     return (out, lse) if return_lse else out
 
 
@@ -275,19 +286,16 @@ def cache8_prefill(cache: Cache8, q: torch.Tensor, cu_rows: torch.Tensor, table:
     its own (causal) or all lens[s].  Write the tokens first.  Rows that attend
     nothing get zeros and -inf; rows behind the last sequence are left as they
     were in out and lse.  The rest as cache8_decode."""
-    _seq_args(cache, table, lens, cu_rows, "lens")
     if cu_rows is None:
         raise TypeError("cu_rows must be a torch.Tensor")
-    gqa = _query(cache, q)
-    out = _out(out, q.shape, q.dtype, "out", cache)
+    tab, stride, blocks, n = _seq_args(cache, table, lens, cu_rows, "lens")
+    shape, gqa, q_row, q_head = _query(cache, q)
+    out = _out(out, shape, q.dtype, "out", cache)
     if return_lse or lse is not None:
-        lse = _out(lse, q.shape[:2], torch.float32, "lse", cache)
-    ws, nbytes, _keep = _workspace(cache, prefill_workspace_bytes(cache, q.shape[0], table.shape[0], gqa), workspace)
-    with cache._on_device():
-        rc = _lib.sphkv_cache8_prefill(
-            q.data_ptr(), _TYPES[q.dtype], q.stride(0), q.stride(1), q.shape[0], cu_rows.data_ptr(), lens.data_ptr(),
-            1 if causal else 0, table.data_ptr(), table.stride(0), table.shape[1], table.shape[0], *cache._ptrs, gqa,
-            *cache._tail, 1.0 / math.sqrt(cache.dh) if sm_scale is None else float(sm_scale), out.data_ptr(),
-            None if lse is None else lse.data_ptr(), ws, nbytes, cache._stream())
-    check(rc, "cache8_prefill")
+        lse = _out(lse, shape[:2], _FLOAT, "lse", cache)
+    ws, nbytes, _keep = _workspace(cache, prefill_workspace_bytes(cache, shape[0], n, gqa), workspace)
+    cache._call(_lib.sphkv_cache8_prefill, q.data_ptr(), _TYPES[q.dtype], q_row, q_head, shape[0], cu_rows.data_ptr(),
+                lens.data_ptr(), 1 if causal else 0, tab, stride, blocks, n, *cache._ptrs, gqa, *cache._tail,
+                cache._sm if sm_scale is None else float(sm_scale), out.data_ptr(),
+                None if lse is None else lse.data_ptr(), ws, nbytes)
     return (out, lse) if return_lse else out
