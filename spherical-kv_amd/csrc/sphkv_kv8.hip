@@ -515,8 +515,11 @@ __global__ __launch_bounds__(256) void cache8_read_kernel(Cache8RowsLaunch L, ui
 // the others leave a partial per workgroup (two at most: its first and its last
 // pair) for the merge kernel.
 constexpr int kTileTokens = 64;
-constexpr int kDecodeGroups = 512;      // two workgroups of four waves per CU
-constexpr int kDecodeLeast = 4;         // tiles of a workgroup: one per wave
+// Workgroups: two of four waves per CU at DH 128, three at DH 64, whose registers
+// allow it (256 contexts of 100 to 900 tokens 50.7 us, 58.0 with two).  Their tiles
+// are a multiple of their waves.
+__host__ __device__ constexpr int decode_groups(int dh) { return dh == 128 ? 512 : 768; }
+constexpr int kDecodeWaves = 4;
 constexpr float kTopWeight = 8.0f;      // log2 of the weight at the reference, ...
 constexpr float kSlackWeight = 4.0f;    // ... which moves once a weight passes 2^4 times that
 constexpr float kNoScore = -3.0e38f;    // reference before the first score
@@ -641,8 +644,8 @@ __global__ __launch_bounds__(256, 2) void cache8_decode_kernel(Cache8AttendLaunc
   int64_t total = 0;
   for (int i = lane; i < n; i += kWave) total += (seq_tokens(c, b, i) + kTileTokens - 1) / kTileTokens;
   total = uniform64(shfl64(wave_scan(total), 63)) * HV;
-  int64_t per = (total + kDecodeGroups - 1) / kDecodeGroups;
-  if (per < kDecodeLeast) per = kDecodeLeast;
+  constexpr int64_t kShare = (int64_t)decode_groups(DH) * kDecodeWaves;
+  const int64_t per = total > kShare ? (total + kShare - 1) / kShare * kDecodeWaves : kDecodeWaves;
   int64_t p = (int64_t)blockIdx.x * per;
   const int64_t pend = p + per < total ? p + per : total;
   const bool writes_plan = blockIdx.x == 0 && wave == 3;
@@ -1407,9 +1410,9 @@ template <int T, int F, int D> struct Decode {
     } else {
       int64_t* plan = (int64_t*)L.ws;
       float* partials = (float*)((uint8_t*)L.ws + plan_bytes(L.b.num_seqs));
-      cache8_decode_kernel<F, T, D><<<kDecodeGroups, 256, 0, st>>>(L, partials, plan);
+      cache8_decode_kernel<F, T, D><<<decode_groups(D), 256, 0, st>>>(L, partials, plan);
       const int heads = L.b.num_seqs * L.c.num_kv * L.gqa;
-      if (L.b.num_seqs * L.c.num_kv * head_parts(L.gqa) < kDecodeGroups / 4)
+      if (L.b.num_seqs * L.c.num_kv * head_parts(L.gqa) < 128)
         cache8_decode_merge_kernel<T, D, 4><<<heads, 256, 0, st>>>(L, partials, plan);
       else
         cache8_decode_merge_kernel<T, D, 1><<<heads, 64, 0, st>>>(L, partials, plan);
@@ -1454,7 +1457,7 @@ int launch_cache8_attend(const Cache8AttendLaunch& L, hipStream_t stream) {
   return L.b.cu ? pick<Prefill>(L.type, L.c.fmt, L.c.dh, L, stream) : pick<Decode>(L.type, L.c.fmt, L.c.dh, L, stream);
 }
 int64_t cache8_decode_ws_bytes(int32_t num_seqs, int32_t, int32_t gqa, int32_t dh) {
-  return plan_bytes(num_seqs) + 2 * kDecodeGroups * 4 * partial8_floats(gqa, dh);
+  return plan_bytes(num_seqs) + 2 * decode_groups(dh) * 4 * partial8_floats(gqa, dh);
 }
 int64_t cache8_prefill_ws_bytes(int64_t num_rows, int32_t num_seqs, int32_t num_kv, int32_t gqa, int32_t dh) {
   if (num_rows == 0 || num_seqs == 0) return 0;
