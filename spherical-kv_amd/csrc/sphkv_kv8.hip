@@ -262,7 +262,7 @@ __global__ __launch_bounds__(RUNS == 8 ? 512 : 256) void cache8_write_kernel(Cac
     }
     rows_of(b, s, begin, end);
     const int64_t start = b.at[s], blk = start / ps + jj, left = start + (end - begin) - blk * ps;
-    if (start >= 0 && left > 0) {
+    if (start >= 0 && jj >= 0 && left > 0) {                          // (jj < 0: row starts that decrease)
       o = jj ? 0 : (int)(start & (ps - 1));
       e = left < ps ? (int)left : ps;
       if (o < e) page = uniform(page_of(c, b, s, blk));
@@ -335,8 +335,8 @@ __global__ __launch_bounds__(RUNS == 8 ? 512 : 256) void cache8_write_kernel(Cac
   }
   if (!any) return;
   float ks = block_scale<FMT>(ktop), vs = block_scale<FMT>(vtop);
-  if (o > 0 && !(ks > kold)) ks = kold;
-  if (o > 0 && !(vs > vold)) vs = vold;
+  if (o > 0 && kold >= ks) ks = kold;
+  if (o > 0 && vold >= vs) vs = vold;
   if (run == 0 && lane == 0) *(float2*)(c.scales + 2 * ph) = float2{ks, vs};
   // (every wave of a page has read the old scales: before the barrier, or itself)
   const float kinv = __fdiv_rn(1.0f, ks), vinv = __fdiv_rn(1.0f, vs);
@@ -430,7 +430,7 @@ __global__ __launch_bounds__(256) void cache8_read_kernel(Cache8RowsLaunch L, ui
   rows_of(b, s, begin, end);
   const int64_t start = b.at[s], pos0 = ((start >> 4) + jj) << 4, left = start + (end - begin) - pos0;
   const int lo = jj ? 0 : (int)(start & 15), hi = left < 16 ? (int)left : 16;
-  if (lo >= hi) return;
+  if (lo >= hi || jj < 0) return;                                     // (jj < 0: row starts that decrease)
   const int page = uniform(page_of(c, b, s, pos0 >> c.page_shift));
   const int64_t row0 = begin + (pos0 - start);                        // row of the run's token 0
   uintx4 kx[KN], vx[2];
@@ -523,7 +523,11 @@ constexpr int kDecodeWaves = 4;
 constexpr float kTopWeight = 8.0f;      // log2 of the weight at the reference, ...
 constexpr float kSlackWeight = 4.0f;    // ... which moves once a weight passes 2^4 times that
 constexpr float kNoScore = -3.0e38f;    // reference before the first score
-
+// An exponent is one multiply-add, s_t + (log2 sv_t - R), whose rounding differs
+// from that of R by up to 2^-24 R: from this on they are rounded alike, s_t + log2
+// sv_t first, so that the largest weight is exactly that at any magnitude (always: 3
+// to 5 % of the prefill).
+constexpr float kPlainScore = 0x1p18f;
 
 // heads handled together: a kv head's first 16, next 16, ...
 __host__ __device__ __forceinline__ int head_parts(int gqa) { return (gqa + 15) / 16; }
@@ -677,7 +681,7 @@ __global__ __launch_bounds__(256, 2) void cache8_decode_kernel(Cache8AttendLaunc
   const bool twin = L.gqa <= 8;                       // heads in columns 0..7 and again in 8..15
   const int64_t page_bytes = (int64_t)c.num_kv * DH << c.page_shift;
 
-  for (; p < pend; ++s) {
+  for (; p < pend && s < n; ++s) {
     const int len = uniform(seq_tokens(c, b, s)), T = (len + kTileTokens - 1) / kTileTokens;
     if (T == 0) continue;
     const int32_t* table = b.table + s * b.table_stride;
@@ -791,12 +795,18 @@ __global__ __launch_bounds__(256, 2) void cache8_decode_kernel(Cache8AttendLaunc
           for (int d = 0; d < DT; ++d) acc[d] *= f;
         }
         // weights
-        const float off = lsv - ref;
+        float cw = ck, off = lsv - ref;
+        if (__any((fabsf(ref) > kPlainScore) & (ref > kNoScore))) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) sc[e >> 2][e & 3] = fmaf(sc[e >> 2][e & 3], ck, lsv) - ref;
+          cw = 1.f;
+          off = 0.f;
+        }
         float wsum = 0.f;
         half8 w[2];
 #pragma unroll
         for (int e = 0; e < 16; e += 2) {
-          const float x = exp2_of(fmaf(sc[e >> 2][e & 3], ck, off)), y = exp2_of(fmaf(sc[e >> 2][(e & 3) + 1], ck, off));
+          const float x = exp2_of(fmaf(sc[e >> 2][e & 3], cw, off)), y = exp2_of(fmaf(sc[e >> 2][(e & 3) + 1], cw, off));
           wsum += x + y;
           _Float16 hx = (_Float16)x, hy = (_Float16)y;
           if (twin && col >= 8) {
@@ -1078,7 +1088,7 @@ __global__ __launch_bounds__(DH == 128 ? 512 : 256, 2) void cache8_prefill_kerne
   begin = uniform(begin);
   const int n = uniform(end) - begin;
   const int64_t r0 = (slot - first_slot(b, s, gqa, RS, 1)) * kRowTile, rows_all = (int64_t)n * gqa;
-  if (r0 >= rows_all) return;
+  if (r0 < 0 || r0 >= rows_all) return;                             // (r0 < 0: row starts that decrease)
   const int len = uniform(seq_tokens(c, b, s));
   const int last = (int)((r0 + kRowTile < rows_all ? r0 + kRowTile : rows_all) - 1);
   const int seen = tile_seen(L, len, n, last / gqa);
@@ -1217,14 +1227,25 @@ __global__ __launch_bounds__(DH == 128 ? 512 : 256, 2) void cache8_prefill_kerne
 #pragma unroll
         for (int d = 0; d < DB; ++d) acc[d] *= f;
       }
+      float off[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) off[u] = lsv[u] - ref;
+      if (__any((fabsf(ref) > kPlainScore) & (ref > kNoScore))) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) sc[u >> 1][8 * (u & 1) + i] = fmaf(sc[u >> 1][8 * (u & 1) + i], ck[u], lsv[u]) - ref;
+          ck[u] = 1.f;
+          off[u] = 0.f;
+        }
+      }
       half8 w[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        const float off = lsv[u] - ref;
         float ws = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float x = exp2_of(fmaf(sc[u >> 1][8 * (u & 1) + i], ck[u], off));
+          const float x = exp2_of(fmaf(sc[u >> 1][8 * (u & 1) + i], ck[u], off[u]));
           ws += x;
           w[u][i] = (_Float16)x;
         }

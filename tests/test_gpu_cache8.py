@@ -100,6 +100,7 @@ WRITES = [
     ("e4m3", "fp16", 128, 32, 8, [(0, 0), (40, 9), (0, 0)]),
     ("int8", "fp16", 64, 64, 5, [(i, 1) for i in range(0, 140, 7)]),
     ("int8", "fp32", 128, 16, 2, [(3, 1)] * 1 + [(0, 5)] * 70),          # more than 64 sequences
+    ("e4m3", "bf16", 64, 16, 1, [(i % 23, i % 4) for i in range(5000)]), # more than 64 * 64
 ]
 
 
@@ -260,6 +261,7 @@ DECODES = [
     ("int8", "fp16", 128, 16, 2, 3, [(i * 37) % 200 for i in range(150)]),
     ("e4m3", "bf16", 128, 32, 8, 5, [12000]),
     ("int8", "fp16", 64, 16, 1, 1, [20000, 1]),
+    ("e4m3", "fp16", 64, 16, 1, 2, [(i * 7) % 40 for i in range(3000)]),
 ]
 
 
@@ -360,6 +362,57 @@ def test_decode_peaked_and_flat_softmax(gpu):
             assert torch.isfinite(out).all() and (np.abs(rows_np(lse) - want[1]) <= tol).all()
 
 
+@pytest.mark.parametrize("dh", [64, 128])
+def test_scores_of_any_size(gpu, dh):
+    """Scores up to 2^36, whose fp32 spacing is 2^13: the largest takes all, and its weight is exactly its own."""
+    n, ps = 100, 16
+    k = torch.zeros(8, 1, ps, dh, dtype=torch.uint8, device=gpu)
+    table = tables(70, 8, [7])
+    for t in range(n):
+        k[int(table[0, t // ps]), 0, t % ps, 0] = t + 1
+    cache = random_cache(gpu, 71, 8, 1, dh, ps, "int8")
+    cache.k_codes.copy_(k)
+    cache.scales[..., 0] = 512.0
+    q = torch.zeros(3, 2, dh, dtype=torch.float16, device=gpu)
+    q[:, 0, 0], q[:, 1, 0] = 65504.0, -65504.0
+    o = oracle_of(cache)
+    _, v, _ = o.tokens(table, 0, 0, n)
+    td, lens = i32(table, gpu), i32([n], gpu)
+    outs = [kv8.cache8_decode(cache, q[:1], td, lens, return_lse=True),
+            kv8.cache8_prefill(cache, q, i32([0, 3], gpu), td, lens, False, return_lse=True)]
+    for out, lse in outs:
+        for row in range(out.shape[0]):
+            for head, token in ((0, n - 1), (1, 0)):
+                want = v[token, 0]
+                got = out[row, head].double().cpu().numpy()
+                # one weight: rounded to fp16 in the product and not in the sum, and the output's own rounding
+                assert (np.abs(got - want) <= 2.0 ** -10 * np.abs(want) + 2.0 ** -25).all()
+                score = (1 if head == 0 else -1) * 65504.0 * 512.0 * (token + 1) / math.sqrt(dh)
+                assert abs(lse[row, head].item() - score) <= 2.0 ** -21 * abs(score)
+
+
+def test_empty_caches_and_tables(gpu):
+    """A cache of no page, tables of no block, no sequence at all: zeros and -inf, and nothing written."""
+    q = torch.randn(2, 4, 64, device=gpu).half()
+    cu = i32([0, 1, 2], gpu)
+    for cache, table in ((kv8.Cache8.allocate(0, 2, 64, 16, "int8", gpu), i32([[0, 1], [5, -1]], gpu)),
+                         (random_cache(gpu, 72, 3, 2, 64, 16, "int8"), torch.empty(2, 0, dtype=torch.int32, device=gpu))):
+        lens = i32([5, 20], gpu)
+        before = cache.k_codes.clone()
+        kv8.cache8_write(cache, q[:, :2], q[:, :2], table, i32([0, 3], gpu))
+        assert torch.equal(cache.k_codes, before)
+        k, v = kv8.cache8_read(cache, table, i32([0, 3], gpu))
+        assert (k == 0).all() and (v == 0).all()
+        for out, lse in (kv8.cache8_decode(cache, q, table, lens, return_lse=True),
+                         kv8.cache8_prefill(cache, q, cu, table, lens, return_lse=True)):
+            assert (out == 0).all() and torch.isneginf(lse).all()
+    none = torch.empty(0, 2, dtype=torch.int32, device=gpu)
+    assert kv8.cache8_decode(cache, q[:0], none, i32([], gpu)).shape == (0, 4, 64)
+    assert kv8.cache8_prefill(cache, q[:0], i32([0], gpu), none, i32([], gpu)).shape == (0, 4, 64)
+    kv8.cache8_write(cache, q[:0, :2], q[:0, :2], none, i32([], gpu))
+    assert kv8.cache8_read(cache, none, i32([], gpu))[0].shape == (0, 2, 64)
+
+
 def test_decode_nan_query_stays_in_its_row(gpu):
     lens = [300, 300]
     cache, table, q = attention_case(gpu, 28, "e4m3", "bf16", 128, 16, 2, 4, lens, 2, absent=False)
@@ -423,6 +476,9 @@ PREFILLS = [
     ("int8", "bf16", 128, 16, 2, 2, [(5, 9), (30, 30), (-4, 3), (17, 20)], True),      # more rows than tokens
     ("e4m3", "fp16", 128, 32, 1, 4, [(3 * i, i) for i in range(70)], True),
     ("int8", "fp16", 128, 16, 1, 4, [(6000, 3), (4000, 24)], True),                    # few rows, many keys
+    ("e4m3", "bf16", 128, 16, 1, 4, [(3000, 100)], True),                              # split, more rows than a tile
+    ("int8", "bf16", 64, 16, 1, 4, [(2500, 20), (40, 40)], True),
+    ("e4m3", "fp16", 128, 64, 8, 4, [(1100, 1100)], True),                             # whole tiles, no split
 ]
 
 
