@@ -1022,9 +1022,12 @@ constexpr int kSplitMost = 64;
 __host__ __device__ __forceinline__ int64_t row_tiles(int64_t num_rows, int num_seqs, int gqa, int row_shift) {
   return ((num_rows * gqa) >> row_shift) + num_seqs;
 }
+// Splits of each row tile: the workgroups at once over the fewest tiles that the
+// rows can make (twice as many at most, whose workgroups then take two rounds of
+// half the keys; by the most they can make, eight chunks of 64 tokens on 4K ran on
+// half of the CUs).
 __host__ __device__ __forceinline__ int prefill_splits(int64_t num_rows, int num_seqs, int num_kv, int gqa, PrefillShape p) {
-  // (sequences of few rows have a tile each, and their slots are up to twice as many)
-  const int64_t tiles = p.turns == 2 ? num_seqs : row_tiles(num_rows, num_seqs, gqa, p.row_shift), s = p.groups / (tiles * num_kv);
+  const int64_t whole = (num_rows * gqa) >> p.row_shift, s = p.groups / ((whole > num_seqs ? whole : num_seqs) * num_kv);
   return (int)(s < 1 ? 1 : (s > kSplitMost ? kSplitMost : s));
 }
 // floats of one split's partial: reference and sum per row, then acc[rows][DH]
