@@ -656,7 +656,8 @@ int64_t sphkv_work_fill(const int32_t* row_start, int32_t num_sh, int32_t rows_p
  *   a / scale <= 448;   both within [2^-60, 2^60] (beyond, values saturate).
  * A NaN is stored as 0, an infinity as the largest code of its sign (so no NaN
  * code of e4m3 is ever written; one that a caller puts there makes NaN of the
- * rows that share its tile of 64 tokens).  Scales are positive.  `stream` belongs
+ * rows that share its tile of 64 tokens).  Scales are positive; in attention a value
+ * scale below 2^-60 counts as that.  `stream` belongs
  * to the current device, as the pointers do; batches have at most 2^16 sequences.
  */
 #define SPHKV_CACHE8_INT8 0

@@ -783,7 +783,7 @@ __global__ __launch_bounds__(256, 2) void cache8_decode_kernel(Cache8AttendLaunc
             for (int k = 0; k < 4; ++k) A.v[d][k] &= keep[k];
           if (have <= 0) A.sk = A.sv = 1.f;                                   // (an unwritten page's may be anything)
         }
-        const float ck = fmaxf(cq * A.sk, 0x1p-126f), lsv = log2_of(A.sv);      // (never 0: 0 * -inf)
+        const float ck = fmaxf(cq * A.sk, 0x1p-126f), lsv = log2_of(fmaxf(A.sv, kLeastScale));   // (never 0: 0 * -inf, -inf)
         float top = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3]));
 #pragma unroll
         for (int i = 1; i < 4; ++i) top = fmaxf(top, fmaxf(fmaxf(sc[i][0], sc[i][1]), fmaxf(sc[i][2], sc[i][3])));
@@ -1176,7 +1176,7 @@ __global__ __launch_bounds__(DH == 128 ? 512 : 256, 2) void cache8_prefill_kerne
       for (int k = 0; k < 4; ++k) raw.v[k] &= low_bytes(have - 4 * k);
     }
     if (in == 0) {
-      const float lsv = have > 0 ? log2_of(raw.sc.y) : -INFINITY;
+      const float lsv = have > 0 ? log2_of(fmaxf(raw.sc.y, kLeastScale)) : -INFINITY;
       s_sk[bf][run] = have > 0 ? raw.sc.x : 1.f;
       s_lsv[bf][run] = lsv;
       s_inv[bf][run] = have > 0 ? exp2_of(-lsv) : 0.f;

@@ -413,6 +413,20 @@ def test_empty_caches_and_tables(gpu):
     assert kv8.cache8_read(cache, none, i32([], gpu))[0].shape == (0, 2, 64)
 
 
+def test_tokens_never_written(gpu):
+    """A new cache holds zeros under scales of zero: they count as tokens of zeros."""
+    cache = kv8.Cache8.allocate(3, 2, 64, 16, "e4m3", gpu)
+    q = torch.randn(4, 4, 64, device=gpu).bfloat16()
+    table, lens = i32([[2, 0]], gpu), i32([20], gpu)
+    for out, lse in (kv8.cache8_decode(cache, q[:1], table, lens, return_lse=True),
+                     kv8.cache8_prefill(cache, q, i32([0, 4], gpu), table, lens, False, return_lse=True)):
+        assert (out == 0).all()
+        # Scores of zero, ln 20.  A value scale below 2^-60 counts as that: the reference is -60 - 8 and the sum
+        # 20 * 2^68, whose log2 is 72.3, with an fp32 spacing of 2^-17: one spacing for the logarithm (1 ulp) and
+        # half of one for the addition, times ln 2
+        assert (lse - math.log(20)).abs().max().item() <= 1.5 * 2.0 ** -17 * math.log(2)
+
+
 def test_decode_nan_query_stays_in_its_row(gpu):
     lens = [300, 300]
     cache, table, q = attention_case(gpu, 28, "e4m3", "bf16", 128, 16, 2, 4, lens, 2, absent=False)
