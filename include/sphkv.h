@@ -706,7 +706,8 @@ int sphkv_cache8_read(const uint8_t* k_codes, const uint8_t* v_codes, const floa
  *   out = sum_t softmax_t(sm_scale <q, k_t>) v_t,  lse = ln sum_t exp(sm_scale <q, k_t>)
  * q [num_seqs, num_kv*gqa, dh] fp16 or bf16; out of that type, contiguous; lse
  * fp32 [num_seqs, num_kv*gqa] or NULL.  A sequence without a token gets zeros
- * and -inf.  gqa 1..64.  workspace: device scratch of
+ * and -inf.  gqa 1..64.  Scores, sums and outputs are held in fp32, a weight meets
+ * its value with 22 bits.  workspace: device scratch of
  * sphkv_cache8_decode_workspace_bytes() bytes, 16-byte aligned, contents
  * irrelevant; calls that share one must not run concurrently.
  */

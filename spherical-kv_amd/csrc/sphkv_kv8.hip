@@ -509,7 +509,10 @@ __global__ __launch_bounds__(256) void cache8_read_kernel(Cache8RowsLaunch L, ui
 // product's B operand as they stand, and the 16 bytes that it loads per value
 // row are its part of the A operand.  Nothing passes through LDS.
 // A column is a query head; up to 8 heads use two columns each, the second one
-// for what the first one's fp16 weight leaves out.
+// for what the first one's fp16 weight leaves out.  More heads fill the columns, and
+// that rest is a product of its own, hidden behind the loads (32 contexts of 2K to 8K
+// tokens, 4 heads x 16 queries x 128, 45.5 us with it and 45.9 without; 16 contexts
+// of 2K to 16K, 2 x 64, 55.2 and 56.3).
 //
 // Work: the tiles of all (sequence, kv head) pairs in a row, cut into equal
 // runs, one per workgroup; its four waves take the tiles of a pair in turn and
@@ -637,7 +640,8 @@ struct Tile {
   int page;                   // their page, or -1
 };
 
-template <int FMT, int TYPE, int DH>
+// TWIN: up to 8 heads, in columns 0..7 and again in 8..15
+template <int FMT, int TYPE, int DH, bool TWIN>
 __global__ __launch_bounds__(256, 2) void cache8_decode_kernel(Cache8AttendLaunch L, float* partials, int64_t* base_of) {
   constexpr int DT = DH / 16;
   __shared__ float s_ref[4][16], s_sum[4][16];
@@ -681,7 +685,6 @@ __global__ __launch_bounds__(256, 2) void cache8_decode_kernel(Cache8AttendLaunc
     }
   }
   const float qscale = L.sm_scale * 1.44269504088896f;
-  const bool twin = L.gqa <= 8;                       // heads in columns 0..7 and again in 8..15
   const int64_t page_bytes = (int64_t)c.num_kv * DH << c.page_shift;
 
   for (; p < pend && s < n; ++s) {
@@ -693,7 +696,7 @@ __global__ __launch_bounds__(256, 2) void cache8_decode_kernel(Cache8AttendLaunc
       const int cols = part_cols(L.gqa, part);
       const int64_t first = sbase + (int64_t)hv * T;
       const int t0 = (int)(p - first), t1 = pend - first < T ? (int)(pend - first) : T;
-      const int mycol = twin ? (col & 7) : col;
+      const int mycol = TWIN ? (col & 7) : col;
 
       // a column's query: dims 64 j + 16 g + 0..15 in lane group g
       half8 q[DH / 32];
@@ -806,24 +809,32 @@ __global__ __launch_bounds__(256, 2) void cache8_decode_kernel(Cache8AttendLaunc
           off = 0.f;
         }
         float wsum = 0.f;
-        half8 w[2];
+        half8 w[2], rest[2];                                                  // fp16 numbers, and what they leave out
 #pragma unroll
         for (int e = 0; e < 16; e += 2) {
           const float x = exp2_of(fmaf(sc[e >> 2][e & 3], cw, off)), y = exp2_of(fmaf(sc[e >> 2][(e & 3) + 1], cw, off));
           wsum += x + y;
           _Float16 hx = (_Float16)x, hy = (_Float16)y;
-          if (twin && col >= 8) {
-            hx = (_Float16)(x - (float)hx);
-            hy = (_Float16)(y - (float)hy);
+          const _Float16 rx = (_Float16)(x - (float)hx), ry = (_Float16)(y - (float)hy);
+          if (TWIN && col >= 8) {
+            hx = rx;
+            hy = ry;
           }
           w[e >> 3][e & 7] = hx;
           w[e >> 3][(e & 7) + 1] = hy;
+          rest[e >> 3][e & 7] = rx;
+          rest[e >> 3][(e & 7) + 1] = ry;
         }
         sum = fmaf(wsum, exp2_of(-lsv), sum);
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
-          acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8<FMT>(A.v[d].x, A.v[d].y), w[0], acc[d], 0, 0, 0);
-          acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8<FMT>(A.v[d].z, A.v[d].w), w[1], acc[d], 0, 0, 0);
+          const half8 lo = codes8<FMT>(A.v[d].x, A.v[d].y), hi = codes8<FMT>(A.v[d].z, A.v[d].w);
+          acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, w[0], acc[d], 0, 0, 0);
+          acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, w[1], acc[d], 0, 0, 0);
+          if constexpr (!TWIN) {
+            acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, rest[0], acc[d], 0, 0, 0);
+            acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, rest[1], acc[d], 0, 0, 0);
+          }
         }
         if (t + 4 < t1) load_v(t + 4, vp1);
         kp1 = kp2;
@@ -847,7 +858,7 @@ __global__ __launch_bounds__(256, 2) void cache8_decode_kernel(Cache8AttendLaunc
       for (int i = threadIdx.x; i < cols * DH; i += 256) {
         const int cc = i / DH, d = i % DH;
         float o = s_acc[0][cc][d] + s_acc[1][cc][d] + s_acc[2][cc][d] + s_acc[3][cc][d];
-        if (twin) o += s_acc[0][cc + 8][d] + s_acc[1][cc + 8][d] + s_acc[2][cc + 8][d] + s_acc[3][cc + 8][d];
+        if constexpr (TWIN) o += s_acc[0][cc + 8][d] + s_acc[1][cc + 8][d] + s_acc[2][cc + 8][d] + s_acc[3][cc + 8][d];
         const float Rc = fmaxf(fmaxf(s_ref[0][cc], s_ref[1][cc]), fmaxf(s_ref[2][cc], s_ref[3][cc]));
         float l = 0.f;
 #pragma unroll
@@ -1444,7 +1455,8 @@ template <int T, int F, int D> struct Decode {
     } else {
       int64_t* plan = (int64_t*)L.ws;
       float* partials = (float*)((uint8_t*)L.ws + plan_bytes(L.b.num_seqs));
-      cache8_decode_kernel<F, T, D><<<decode_groups(D), 256, 0, st>>>(L, partials, plan);
+      if (L.gqa <= 8) cache8_decode_kernel<F, T, D, true><<<decode_groups(D), 256, 0, st>>>(L, partials, plan);
+      else cache8_decode_kernel<F, T, D, false><<<decode_groups(D), 256, 0, st>>>(L, partials, plan);
       const int heads = L.b.num_seqs * L.c.num_kv * L.gqa;
       if (L.b.num_seqs * L.c.num_kv * head_parts(L.gqa) < 128)
         cache8_decode_merge_kernel<T, D, 4><<<heads, 256, 0, st>>>(L, partials, plan);

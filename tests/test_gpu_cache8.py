@@ -672,3 +672,45 @@ def test_offsets_past_32_bits(gpu):
         assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
     assert torch.equal(kv8.cache8_decode(cache, q[:1], t_far, n), kv8.cache8_decode(low, q[:1], t_low, n))
     assert torch.equal(kv8.cache8_prefill(cache, q, cu, t_far, n), kv8.cache8_prefill(low, q, cu, t_low, n))
+
+
+# ---- weights of the second product -------------------------------------------------------
+
+def check_residual(out, want, mass, reach, under, dtype, dh, n, what):
+    """check_attention's bound for weights held as two fp16 numbers: a weight is off by 2^-22 of it (the second
+    number holds what the first leaves out, to 2^-11 of that) or by half of the smallest fp16 step.  The products
+    are summed in fp32: n of them in each of two numbers' sums, of which a partial sum is at most the mass, and 64
+    more steps (rescales, joins of waves, splits and workgroups, the division), each by at most 2^-24 of it."""
+    out = out.double().cpu().numpy()
+    delta = 2.0 ** -24 * (dh + 24) * reach + 2.0 ** -21
+    tol = (2.0 ** -22 + 2.2 * delta + 2.0 ** -24 * (2 * n + 64))[..., None] * mass + 2.0 ** -33 * under \
+        + torch.finfo(dtype).eps / 2 * np.abs(want) + 2.0 ** -25
+    err = np.abs(out - want)
+    log(f"  {what}: max err {err.max():.3g}, {(err / tol).max():.3f} of the bound")
+    assert (err <= tol).all(), f"{what}: {(err > tol).sum()} of {err.size} outputs off"
+
+
+def cancelling_cache(gpu, seed, fmt, dh, num_kv, lens):
+    """Values of +-1 and 2, in some dims of random signs: outputs far below sum p|v| that show a weight's rounding."""
+    ps = 16
+    cache, table, _ = attention_case(gpu, seed, fmt, "fp16", dh, ps, num_kv, 1, lens, len(lens), spread=0.5, absent=False)
+    codes = {"int8": [1, 2, 255, 254], "e4m3": [0x38, 0x40, 0xB8, 0xC0]}[fmt]
+    g = np.random.default_rng(seed)
+    cache.v_codes.copy_(torch.from_numpy(np.array(codes, np.uint8)[g.integers(0, 4, tuple(cache.v_codes.shape))]))
+    cache.scales[..., 0] = 1 / 128 if fmt == "int8" else 1 / 512          # small scores, whose own errors stay below
+    cache.scales[..., 1] = 1 / 64
+    return cache, table
+
+
+@pytest.mark.parametrize("fmt, dtype, dh, num_kv, gqa", [
+    ("int8", "fp16", 128, 2, 1), ("e4m3", "fp16", 64, 2, 8), ("int8", "bf16", 128, 1, 4),
+    ("int8", "fp16", 128, 2, 9), ("e4m3", "fp16", 128, 1, 16), ("int8", "fp16", 64, 1, 33), ("e4m3", "bf16", 64, 1, 64),
+    ("int8", "bf16", 128, 2, 16),
+])
+def test_decode_weights_hold_22_bits(gpu, fmt, dtype, dh, num_kv, gqa):
+    lens = [16, 5, 33, 2, 64, 90]
+    cache, table = cancelling_cache(gpu, 80, fmt, dh, num_kv, lens)
+    q = (torch.randn(6, num_kv * gqa, dh, device=gpu, generator=torch.Generator(gpu).manual_seed(81)) / 8).to(TYPES[dtype])
+    out = kv8.cache8_decode(cache, q, i32(table, gpu), i32(lens, gpu))
+    want, _, *bounds = clean(oracle_of(cache)).attend(rows_np(q), table, lens)
+    check_residual(out, want, *bounds, TYPES[dtype], dh, np.array(lens)[:, None], f"decode gqa {gqa}")
