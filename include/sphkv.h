@@ -725,7 +725,8 @@ int sphkv_cache8_decode(const void* q, int32_t q_type, int64_t q_row_stride, int
  * or all lens[s] (causal = 0).  A row that attends nothing (a negative
  * position, an empty sequence) gets zeros and -inf; rows from
  * cu_rows[num_seqs] on keep their contents.  q, out [num_rows, num_kv*gqa, dh],
- * lse [num_rows, num_kv*gqa]; the rest as sphkv_cache8_decode.
+ * lse [num_rows, num_kv*gqa]; the rest as sphkv_cache8_decode, but that a weight
+ * meets its value with 11 bits for bf16 (whose outputs have 8), with 22 for fp16.
  */
 int64_t sphkv_cache8_prefill_workspace_bytes(int64_t num_rows, int32_t num_seqs, int32_t num_kv, int32_t gqa,
                                              int32_t dh);

@@ -589,6 +589,12 @@ __device__ __forceinline__ half8 codes8(uint32_t x, uint32_t y) {
   return half8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
+// two numbers as fp16, half to even
+__device__ __forceinline__ half2v fp16_pair(float x, float y) {
+  typedef float float2v __attribute__((ext_vector_type(2)));
+  return __builtin_convertvector(float2v{x, y}, half2v);
+}
+
 __device__ __forceinline__ float log2_of(float x) { return __builtin_amdgcn_logf(x); }
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 
@@ -1005,6 +1011,14 @@ __global__ __launch_bounds__(64 * WAVES) void cache8_decode_merge_kernel(Cache8A
 // LDS rows are 16-byte chunks, exclusive-or'ed with the row so that the 16 rows
 // that a read touches at once lie in different banks.
 //
+// A weight meets its value as one fp16 number where outputs are bf16, and as two, the
+// second for what the first leaves out, where they are fp16.  One number's 2^-11 is an
+// eighth of bf16's own step and not seen beside it: 1.627e-3 from the 64-bit
+// definition, the plain form 1.623e-3 (8 prompts of 100 to 500 tokens, relative
+// norm).  fp16's step is as fine as the weight's: 2.35e-4 with one, the plain form and
+// two 2.03e-4.  The second product is matrix work, half as much again: 4 prompts of 1K
+// 64.9 us with one, 76.7 with two; 8K in bf16 would take 720 us for 553.
+//
 // With few row tiles the keys of each are split over workgroups, whose partials a
 // second kernel joins.
 //
@@ -1074,17 +1088,17 @@ __device__ __forceinline__ float halves_sum(float x) {
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 template <int N> struct Int { static constexpr int value = N; };
 
-// N LDS reads that feed N matrix instructions: kAhead of them in flight
+// N LDS reads that feed M matrix instructions each: kAhead of them in flight
 constexpr int kAhead = 6;
-template <int N>
+template <int N, int M>
 __device__ __forceinline__ void reads_ahead() {
   __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
 #pragma unroll
   for (int i = 0; i < N - kAhead; ++i) {
-    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x008, M, 0);
     __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
   }
-  __builtin_amdgcn_sched_group_barrier(0x008, kAhead, 0);
+  __builtin_amdgcn_sched_group_barrier(0x008, kAhead * M, 0);
 }
 
 template <int FMT, int TYPE, int DH, int TURNS>
@@ -1093,6 +1107,7 @@ __global__ __launch_bounds__(DH == 128 ? 512 : 256, 2) void cache8_prefill_kerne
   constexpr int kRowWaves = (DH == 128 ? 8 : 4) / TURNS, kRowTile = 32 * kRowWaves, RS = kRowTile == 256 ? 8 : 7;
   constexpr int NB = 2 * TURNS, HALF = TURNS;                      // tiles in LDS; half of them between two barriers
   constexpr int NR = 2;                                    // tiles on the way
+  constexpr bool kRest = TYPE == kFp16;                            // weights as two fp16 numbers (above)
   __shared__ __align__(16) _Float16 s_k[NB][kTileTokens * DH], s_v[NB][kTileTokens * DH];
   __shared__ float s_sk[NB][4], s_lsv[NB][4], s_inv[NB][4];
   const Cache8& c = L.c;
@@ -1225,7 +1240,7 @@ __global__ __launch_bounds__(DH == 128 ? 512 : 256, 2) void cache8_prefill_kerne
           sc[x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, q[k], sc[x], 0, 0, 0);
         }
       }
-      reads_ahead<2 * KS>();
+      reads_ahead<2 * KS, 1>();
       if (t0 + kTileTokens > lim_min) {
         const int left = lim - t0 - 8 * half;
 #pragma unroll
@@ -1263,15 +1278,24 @@ __global__ __launch_bounds__(DH == 128 ? 512 : 256, 2) void cache8_prefill_kerne
           off[u] = 0.f;
         }
       }
-      half8 w[4];
+      half8 w[4], rest[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         float ws = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < 8; i += 2) {
           const float x = exp2_of(fmaf(sc[u >> 1][8 * (u & 1) + i], ck[u], off[u]));
+          const float y = exp2_of(fmaf(sc[u >> 1][8 * (u & 1) + i + 1], ck[u], off[u]));
           ws += x;
-          w[u][i] = (_Float16)x;
+          ws += y;
+          const half2v a = fp16_pair(x, y);
+          w[u][i] = a[0];
+          w[u][i + 1] = a[1];
+          if constexpr (kRest) {
+            const half2v r = fp16_pair(x - (float)a[0], y - (float)a[1]);
+            rest[u][i] = r[0];
+            rest[u][i + 1] = r[1];
+          }
         }
         sum = fmaf(ws, s_inv[bf][u], sum);
       }
@@ -1281,8 +1305,9 @@ __global__ __launch_bounds__(DH == 128 ? 512 : 256, 2) void cache8_prefill_kerne
         for (int d = 0; d < DB; ++d) {
           const half8 a = *(const half8*)&s_v[bf][v_at(32 * d + col, 2 * u + half)];
           acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, w[u], acc[d], 0, 0, 0);
+          if constexpr (kRest) acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, rest[u], acc[d], 0, 0, 0);
         }
-      reads_ahead<4 * DB>();
+      reads_ahead<4 * DB, kRest ? 2 : 1>();
     }
     stage(t + HALF, (bf + HALF) % NB, raws[nx]);
     __builtin_amdgcn_sched_barrier(0);

@@ -714,3 +714,19 @@ def test_decode_weights_hold_22_bits(gpu, fmt, dtype, dh, num_kv, gqa):
     out = kv8.cache8_decode(cache, q, i32(table, gpu), i32(lens, gpu))
     want, _, *bounds = clean(oracle_of(cache)).attend(rows_np(q), table, lens)
     check_residual(out, want, *bounds, TYPES[dtype], dh, np.array(lens)[:, None], f"decode gqa {gqa}")
+
+
+@pytest.mark.parametrize("fmt, dh, num_kv, gqa, new", [
+    ("int8", 128, 2, 4, [16, 5, 33, 1, 64, 90]),          # a row tile of 256, unsplit
+    ("e4m3", 128, 1, 8, [1, 2, 3, 1, 4, 5]),              # few rows: two groups of waves take turns
+    ("e4m3", 64, 2, 2, [16, 5, 33, 2, 64, 90]),
+    ("int8", 64, 1, 33, [2, 5, 1, 2, 3, 1]),
+])
+def test_prefill_fp16_weights_hold_22_bits(gpu, fmt, dh, num_kv, gqa, new):
+    lens = [16, 5, 33, 2, 64, 90]
+    cu = np.cumsum([0] + new)
+    cache, table = cancelling_cache(gpu, 82, fmt, dh, num_kv, lens)
+    q = (torch.randn(int(cu[-1]), num_kv * gqa, dh, device=gpu, generator=torch.Generator(gpu).manual_seed(83)) / 8).half()
+    out = kv8.cache8_prefill(cache, q, i32(cu, gpu), i32(table, gpu), i32(lens, gpu))
+    want, _, *bounds = clean(oracle_of(cache)).attend(rows_np(q), table, lens, cu)
+    check_residual(out, want, *bounds, torch.float16, dh, np.repeat(lens, new)[:, None], f"prefill gqa {gqa}")
