@@ -21,6 +21,7 @@ from __future__ import annotations
 
 import math
 from functools import lru_cache
+from operator import attrgetter
 from typing import Optional, Tuple
 
 import torch
@@ -54,10 +55,16 @@ class Cache8:
 
     k_codes uint8 [num_pages, num_kv, page_size, dh], v_codes uint8 [num_pages,
     num_kv, page_size/16, dh, 16], scales fp32 [num_pages, num_kv, 2] (keys,
-    values), contiguous and 16-byte aligned; fmt "int8" or "e4m3"."""
+    values), contiguous and 16-byte aligned; fmt "int8" or "e4m3".  The tensors
+    and what follows from them are read-only: a cache over others is another
+    Cache8."""
 
-    __slots__ = ("k_codes", "v_codes", "scales", "fmt", "num_pages", "num_kv", "page_size", "dh", "device", "_tail",
-                 "_ptrs", "_index", "_sm")
+    __slots__ = ("_k_codes", "_v_codes", "_scales", "_fmt", "_num_pages", "_num_kv", "_page_size", "_dh", "_device",
+                 "_tail", "_index", "_sm")
+    k_codes, v_codes, scales = (property(attrgetter(n)) for n in ("_k_codes", "_v_codes", "_scales"))
+    fmt, device = property(attrgetter("_fmt")), property(attrgetter("_device"))
+    num_pages, num_kv = property(attrgetter("_num_pages")), property(attrgetter("_num_kv"))
+    page_size, dh = property(attrgetter("_page_size")), property(attrgetter("_dh"))
 
     def __init__(self, k_codes: torch.Tensor, v_codes: torch.Tensor, scales: torch.Tensor, fmt: str = "int8"):
         if fmt not in FORMATS:
@@ -79,10 +86,9 @@ class Cache8:
             raise ValueError("scales must be [num_pages, num_kv, 2]")
         if not (k_codes.is_contiguous() and v_codes.is_contiguous() and scales.is_contiguous()):
             raise ValueError("k_codes, v_codes and scales must be contiguous")
-        self.k_codes, self.v_codes, self.scales, self.fmt = k_codes, v_codes, scales, fmt
-        self.num_pages, self.num_kv, self.page_size, self.dh, self.device = num_pages, num_kv, page_size, dh, dev
+        self._k_codes, self._v_codes, self._scales, self._fmt = k_codes, v_codes, scales, fmt
+        self._num_pages, self._num_kv, self._page_size, self._dh, self._device = num_pages, num_kv, page_size, dh, dev
         self._index = dev.index
-        self._ptrs = (k_codes.data_ptr(), v_codes.data_ptr(), scales.data_ptr(), num_pages, num_kv)
         self._tail = (dh, page_size, FORMATS[fmt])
         self._sm = 1.0 / math.sqrt(dh)
 
@@ -94,12 +100,16 @@ class Cache8:
         v = torch.zeros((num_pages, num_kv, max(page_size // 16, 1), dh, 16), dtype=torch.uint8, device=device)
         return Cache8(k, v, torch.zeros((num_pages, num_kv, 2), dtype=torch.float32, device=device), fmt)
 
+    def _ptrs(self):
+        """The call's arguments from k_codes to num_kv."""
+        return (self._k_codes.data_ptr(), self._v_codes.data_ptr(), self._scales.data_ptr(), self._num_pages, self._num_kv)
+
     def _call(self, fn, *args) -> None:
         """Launch on torch's current stream of the cache's device, that device current."""
         if _device_index() != self._index:
-            with torch.cuda.device(self.device):
+            with torch.cuda.device(self._device):
                 return self._call(fn, *args)
-        rc = fn(*args, _raw_stream(self._index) if _raw_stream else torch.cuda.current_stream(self.device).cuda_stream)
+        rc = fn(*args, _raw_stream(self._index) if _raw_stream else torch.cuda.current_stream(self._device).cuda_stream)
         if rc:
             check(rc, fn.__name__)
 
@@ -107,7 +117,7 @@ class Cache8:
 def _seq_args(cache: Cache8, table: torch.Tensor, at: torch.Tensor, cu_rows: Optional[torch.Tensor], name: str):
     """Checks of a batch's page table, per-sequence int32 values and row starts;
     (table, row stride, blocks, sequences) for the call."""
-    dev = cache.device
+    dev = cache._device
     _need(table, _INT, "table", dev)
     _need(at, _INT, name, dev)
     if table.dim() != 2 or at.dim() != 1:
@@ -140,8 +150,8 @@ def _rows(t: torch.Tensor, name: str, heads: int, dh: int):
 
 def _out(t: Optional[torch.Tensor], shape, dtype, name: str, cache: Cache8) -> torch.Tensor:
     if t is None:
-        return torch.empty(shape, dtype=dtype, device=cache.device)
-    _need(t, dtype, name, cache.device)
+        return torch.empty(shape, dtype=dtype, device=cache._device)
+    _need(t, dtype, name, cache._device)
     if tuple(t.shape) != tuple(shape) or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {tuple(shape)}")
     return t
@@ -163,17 +173,17 @@ def cache8_write(cache: Cache8, k: torch.Tensor, v: torch.Tensor, table: torch.T
     tab, stride, blocks, n = _seq_args(cache, table, start, cu_rows, "start")
     if not isinstance(k, torch.Tensor) or k.dtype not in _TYPES:
         raise TypeError("k must be an fp16, bf16 or fp32 tensor")
-    _need(k, k.dtype, "k", cache.device)
-    _need(v, k.dtype, "v", cache.device)
-    k_row, k_head = _rows(k, "k", cache.num_kv, cache.dh)
-    v_row, v_head = _rows(v, "v", cache.num_kv, cache.dh)
+    _need(k, k.dtype, "k", cache._device)
+    _need(v, k.dtype, "v", cache._device)
+    k_row, k_head = _rows(k, "k", cache._num_kv, cache._dh)
+    v_row, v_head = _rows(v, "v", cache._num_kv, cache._dh)
     rows = k.shape[0]
     if v.shape[0] != rows:
         raise ValueError("k and v must have as many rows")
     if cu_rows is None and rows != n:
         raise ValueError("without cu_rows there is one row per sequence")
     cache._call(_lib.sphkv_cache8_write, k.data_ptr(), v.data_ptr(), _TYPES[k.dtype], k_row, k_head, v_row, v_head, rows,
-                None if cu_rows is None else cu_rows.data_ptr(), start.data_ptr(), tab, stride, blocks, n, *cache._ptrs,
+                None if cu_rows is None else cu_rows.data_ptr(), start.data_ptr(), tab, stride, blocks, n, *cache._ptrs(),
                 *cache._tail)
 
 
@@ -196,9 +206,9 @@ def cache8_read(cache: Cache8, table: torch.Tensor, start: torch.Tensor, cu_rows
         num_rows = n
     elif num_rows is None or num_rows < 0:
         raise ValueError("num_rows (cu_rows' last value, or more) is needed with cu_rows")
-    shape = (int(num_rows), cache.num_kv, cache.dh)
+    shape = (int(num_rows), cache._num_kv, cache._dh)
     k_out, v_out = _out(k_out, shape, dtype, "k_out", cache), _out(v_out, shape, dtype, "v_out", cache)
-    cache._call(_lib.sphkv_cache8_read, *cache._ptrs, *cache._tail, None if cu_rows is None else cu_rows.data_ptr(),
+    cache._call(_lib.sphkv_cache8_read, *cache._ptrs(), *cache._tail, None if cu_rows is None else cu_rows.data_ptr(),
                 start.data_ptr(), tab, stride, blocks, n, shape[0], k_out.data_ptr(), v_out.data_ptr(), _TYPES[dtype])
     return k_out, v_out
 
@@ -207,11 +217,11 @@ def _query(cache: Cache8, q: torch.Tensor):
     """Checks of q; (shape, q heads per kv head, row stride, head stride)."""
     if not isinstance(q, torch.Tensor) or (q.dtype is not torch.float16 and q.dtype is not torch.bfloat16):
         raise TypeError("q must be an fp16 or bf16 tensor")
-    _need(q, q.dtype, "q", cache.device)
+    _need(q, q.dtype, "q", cache._device)
     shape = q.shape
-    if len(shape) != 3 or shape[1] == 0 or shape[1] % cache.num_kv:
+    if len(shape) != 3 or shape[1] == 0 or shape[1] % cache._num_kv:
         raise ValueError("q must be [rows, num_kv * gqa, dh]")
-    return shape, shape[1] // cache.num_kv, *_rows(q, "q", shape[1], cache.dh)
+    return shape, shape[1] // cache._num_kv, *_rows(q, "q", shape[1], cache._dh)
 
 
 def _workspace(cache: Cache8, need: int, workspace: Optional[torch.Tensor]):
@@ -219,9 +229,9 @@ def _workspace(cache: Cache8, need: int, workspace: Optional[torch.Tensor]):
     if workspace is None:
         if need <= 0:
             return None, 0, None
-        workspace = torch.empty(need, dtype=torch.uint8, device=cache.device)
+        workspace = torch.empty(need, dtype=torch.uint8, device=cache._device)
     else:
-        _need(workspace, torch.uint8, "workspace", cache.device)
+        _need(workspace, torch.uint8, "workspace", cache._device)
         if not workspace.is_contiguous() or workspace.numel() < need:
             raise ValueError(f"workspace must be contiguous and hold {need} bytes, got {workspace.numel()}")
     return workspace.data_ptr(), workspace.numel(), workspace
@@ -239,7 +249,7 @@ def _prefill_bytes(num_rows: int, num_seqs: int, num_kv: int, gqa: int, dh: int)
 
 def decode_workspace_bytes(cache: Cache8, num_seqs: int, gqa: int) -> int:
     """Bytes of a workspace for cache8_decode of num_seqs sequences."""
-    n = _decode_bytes(int(num_seqs), cache.num_kv, int(gqa), cache.dh)
+    n = _decode_bytes(int(num_seqs), cache._num_kv, int(gqa), cache._dh)
     if n < 0:
         raise ValueError("bad num_seqs or gqa (1..64) for the decode workspace")
     return n
@@ -247,7 +257,7 @@ def decode_workspace_bytes(cache: Cache8, num_seqs: int, gqa: int) -> int:
 
 def prefill_workspace_bytes(cache: Cache8, num_rows: int, num_seqs: int, gqa: int) -> int:
     """Bytes of a workspace for cache8_prefill of num_rows rows of num_seqs sequences."""
-    n = _prefill_bytes(int(num_rows), int(num_seqs), cache.num_kv, int(gqa), cache.dh)
+    n = _prefill_bytes(int(num_rows), int(num_seqs), cache._num_kv, int(gqa), cache._dh)
     if n < 0:
         raise ValueError("bad num_rows, num_seqs or gqa (1..64) for the prefill workspace")
     return n
@@ -271,7 +281,7 @@ def cache8_decode(cache: Cache8, q: torch.Tensor, table: torch.Tensor, lens: tor
         lse = _out(lse, shape[:2], _FLOAT, "lse", cache)
     ws, nbytes, _keep = _workspace(cache, decode_workspace_bytes(cache, n, gqa), workspace)
     cache._call(_lib.sphkv_cache8_decode, q.data_ptr(), _TYPES[q.dtype], q_row, q_head, lens.data_ptr(), tab, stride, blocks,
-                n, *cache._ptrs, gqa, *cache._tail, cache._sm if sm_scale is None else float(sm_scale), out.data_ptr(),
+                n, *cache._ptrs(), gqa, *cache._tail, cache._sm if sm_scale is None else float(sm_scale), out.data_ptr(),
                 None if lse is None else lse.data_ptr(), ws, nbytes)
     return (out, lse) if return_lse else out
 
@@ -295,7 +305,7 @@ def cache8_prefill(cache: Cache8, q: torch.Tensor, cu_rows: torch.Tensor, table:
         lse = _out(lse, shape[:2], _FLOAT, "lse", cache)
     ws, nbytes, _keep = _workspace(cache, prefill_workspace_bytes(cache, shape[0], n, gqa), workspace)
     cache._call(_lib.sphkv_cache8_prefill, q.data_ptr(), _TYPES[q.dtype], q_row, q_head, shape[0], cu_rows.data_ptr(),
-                lens.data_ptr(), 1 if causal else 0, tab, stride, blocks, n, *cache._ptrs, gqa, *cache._tail,
+                lens.data_ptr(), 1 if causal else 0, tab, stride, blocks, n, *cache._ptrs(), gqa, *cache._tail,
                 cache._sm if sm_scale is None else float(sm_scale), out.data_ptr(),
                 None if lse is None else lse.data_ptr(), ws, nbytes)
     return (out, lse) if return_lse else out

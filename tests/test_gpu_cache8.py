@@ -730,3 +730,24 @@ def test_prefill_fp16_weights_hold_22_bits(gpu, fmt, dh, num_kv, gqa, new):
     out = kv8.cache8_prefill(cache, q, i32(cu, gpu), i32(table, gpu), i32(lens, gpu))
     want, _, *bounds = clean(oracle_of(cache)).attend(rows_np(q), table, lens, cu)
     check_residual(out, want, *bounds, torch.float16, dh, np.repeat(lens, new)[:, None], f"prefill gqa {gqa}")
+
+
+# ---- the cache's own tensors -------------------------------------------------------------
+
+def test_calls_follow_the_tensors_storage(gpu):
+    """Storage that a caller puts under the cache's tensors is what the next call reads and writes."""
+    lens = [40, 17]
+    cache, table, q = attention_case(gpu, 84, "int8", "fp16", 64, 16, 2, 2, lens, 2, absent=False)
+    other, _, _ = attention_case(gpu, 85, "int8", "fp16", 64, 16, 2, 2, lens, 2, absent=False)
+    t, n = i32(table, gpu), i32(lens, gpu)
+    first, second = kv8.cache8_decode(cache, q, t, n), kv8.cache8_decode(other, q, t, n)
+    assert not torch.equal(first, second)
+    held = [x.data for x in (cache.k_codes, cache.v_codes, cache.scales)]
+    before = [x.clone() for x in held]
+    cache.k_codes.data, cache.v_codes.data, cache.scales.data = (x.clone() for x in (other.k_codes, other.v_codes, other.scales))
+    assert torch.equal(kv8.cache8_decode(cache, q, t, n), second)
+    k = torch.randn(2, 2, 64, device=gpu).half()
+    for c in (cache, other):
+        kv8.cache8_write(c, k, k, t, i32([0, 0], gpu))
+    assert torch.equal(cache.k_codes, other.k_codes) and torch.equal(cache.scales, other.scales)
+    assert all(torch.equal(a, b) for a, b in zip(held, before))

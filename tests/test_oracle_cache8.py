@@ -199,3 +199,13 @@ def test_python_refuses_cpu_tensors_and_bad_formats():
         kv8.Cache8(k.to(torch.int8), v, s)
     with pytest.raises(TypeError, match="torch.Tensor"):
         kv8.Cache8(None, v, s)
+
+
+def test_what_a_cache_consists_of_is_read_only():
+    """Another tensor or format in an existing cache would be checked against nothing."""
+    c = object.__new__(kv8.Cache8)
+    for name in ("k_codes", "v_codes", "scales", "fmt", "num_pages", "num_kv", "page_size", "dh", "device"):
+        with pytest.raises(AttributeError):
+            setattr(c, name, None)
+    with pytest.raises(AttributeError):
+        c.other = None
