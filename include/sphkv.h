@@ -658,7 +658,11 @@ int64_t sphkv_work_fill(const int32_t* row_start, int32_t num_sh, int32_t rows_p
  * code of e4m3 is ever written; one that a caller puts there makes NaN of the
  * rows that share its tile of 64 tokens).  Scales are positive; in attention a value
  * scale below 2^-60 counts as that.  `stream` belongs
- * to the current device, as the pointers do; batches have at most 2^16 sequences.
+ * to the current device, as the pointers do.  A call has at most 2^16 sequences and
+ * 2^26 rows, (num_rows / 16 + 2 num_seqs) * num_kv at most 2^25, in a write
+ * (num_rows / page_size + 2 num_seqs) * num_kv below 2^30 / page_size, in decode
+ * num_seqs * num_kv * gqa at most 2^23 and in prefill (num_rows * gqa / 128 +
+ * num_seqs) * num_kv below 2^23; what passes these is refused.
  */
 #define SPHKV_CACHE8_INT8 0
 #define SPHKV_CACHE8_E4M3 1

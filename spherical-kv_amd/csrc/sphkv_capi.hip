@@ -1108,7 +1108,8 @@ int cache8_attend(const char* fn, bool decode, const void* q, int32_t q_type, in
   if (causal != 0 && causal != 1) return fail(SPHKV_EINVAL, "%s: causal must be 0 or 1 (got %d)", fn, causal);
   if (!(sm_scale > 0.f) || !std::isfinite(sm_scale))
     return fail(SPHKV_EINVAL, "%s: sm_scale must be positive and finite", fn);
-  if (decode ? num_rows * num_kv * gqa > 1 << 23 : (((num_rows * gqa) >> 7) + num_seqs) * num_kv > 1 << 23)
+  // (a grid holds fewer than 2^32 threads: a merge wave or four per (row, head), 512 per (row tile, kv head))
+  if (decode ? num_rows * num_kv * gqa > 1 << 23 : (((num_rows * gqa) >> 7) + num_seqs) * num_kv >= 1 << 23)
     return fail(SPHKV_EINVAL, "%s: too many (row, head) pairs", fn);
   if (num_seqs == 0 || num_rows == 0) return ok();
   if (!q || !lens || !out || (!decode && !cu_rows)) return fail(SPHKV_EINVAL, "%s: null pointer argument", fn);
@@ -1140,6 +1141,9 @@ int sphkv_cache8_write(const void* k, const void* v, int32_t in_type, int64_t k_
   if (in_type < SPHKV_FP16 || in_type > SPHKV_FP32) return fail(SPHKV_EINVAL, "%s: unknown type %d", fn, in_type);
   if (!cu_rows && num_rows != num_seqs)
     return fail(SPHKV_EINVAL, "%s: without cu_rows there is one row per sequence", fn);
+  // (a wave of 64 threads per 16 tokens of a page: fewer than 2^32 in a grid)
+  if ((cu_rows ? (num_rows >> c.page_shift) + 2 * (int64_t)num_seqs : num_seqs) * num_kv >= (1 << 30) / page_size)
+    return fail(SPHKV_EINVAL, "%s: (num_rows / page_size + 2 num_seqs) * num_kv must be below 2^30 / page_size", fn);
   if (num_seqs == 0 || num_rows == 0) return ok();
   if (!k || !v || !start) return fail(SPHKV_EINVAL, "%s: null pointer argument", fn);
   sphkv::Cache8RowsLaunch L{c, {cu_rows, start, table, table_stride, num_pages > 0 ? max_blocks : 0, num_seqs, num_rows},

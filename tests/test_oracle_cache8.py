@@ -209,3 +209,15 @@ def test_what_a_cache_consists_of_is_read_only():
             setattr(c, name, None)
     with pytest.raises(AttributeError):
         c.other = None
+
+
+def test_grids_past_32_bits_are_refused():
+    """Calls whose workgroups would hold 2^32 threads or more, which no launch takes: each fills its grid to 2^32."""
+    lib = sphkv_lib.load()
+    n = 1 << 16
+    for ps, kw in ((32, dict(num_kv=256)), (64, dict(num_kv=128)), (128, dict(num_kv=64)),
+                   (128, dict(num_kv=128, cu=None, num_rows=n))):
+        assert lib.sphkv_cache8_write(*_write_args(**{**dict(ps=ps, num_seqs=n), **kw})) == -1
+        assert "below 2^30 / page_size" in lib.sphkv_last_error().decode()
+    assert lib.sphkv_cache8_prefill(*_attend_args(False, num_rows=16, num_seqs=n, num_kv=128, gqa=1)) == -1
+    assert "too many (row, head) pairs" in lib.sphkv_last_error().decode()
