@@ -749,5 +749,117 @@ def test_calls_follow_the_tensors_storage(gpu):
     k = torch.randn(2, 2, 64, device=gpu).half()
     for c in (cache, other):
         kv8.cache8_write(c, k, k, t, i32([0, 0], gpu))
-    assert torch.equal(cache.k_codes, other.k_codes) and torch.equal(cache.scales, other.scales)
-    assert all(torch.equal(a, b) for a, b in zip(held, before))
+    pairs = [(cache.k_codes, other.k_codes), (cache.v_codes, other.v_codes), (cache.scales, other.scales), *zip(held, before)]
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in pairs)     # (by bytes: poisoned scales are NaN)
+
+
+# ---- decode beyond one tile a wave -------------------------------------------------------
+
+LONG_DECODES = [
+    # (fmt, dtype, dh, page, num_kv, gqa, lens)
+    ("int8", "fp16", 128, 16, 1, 64, [40000, 777, 3]),
+    ("e4m3", "bf16", 128, 64, 8, 8, [30000, 5000, 70]),
+    ("e4m3", "fp16", 64, 32, 8, 1, [30000, 5000, 0, 130]),
+    ("int8", "bf16", 64, 16, 8, 7, [40000, 9000, 1]),
+    ("int8", "fp16", 128, 128, 4, 12, [50000, 300, 20000]),
+]
+
+
+def decode_shape(cache, lens, gqa):
+    """(workgroups, tiles of each, all tiles): the workspace has two partials a workgroup; its four waves take turns."""
+    groups = kv8.decode_workspace_bytes(cache, 0, gqa) // (8 * (32 + min(gqa, 16) * cache.dh))
+    tiles = sum(-(-n // 64) for n in lens) * cache.num_kv * (-(-gqa // 16))
+    return groups, 4 * -(-tiles // (4 * groups)), tiles
+
+
+@pytest.mark.parametrize("fmt, dtype, dh, ps, num_kv, gqa, lens", LONG_DECODES)
+def test_decode_many_tiles_a_wave(gpu, fmt, dtype, dh, ps, num_kv, gqa, lens):
+    """Waves that take several tiles of a pair: the next tile's loads, page ids looked up ahead, a reference that
+    moves with sums in hand, lengths and absent pages in later tiles.  Even heads have small queries, whose flat
+    softmax shows a single wrong tile; odd ones large queries, whose scores keep rising."""
+    cache, table, q = attention_case(gpu, 90, fmt, dtype, dh, ps, num_kv, gqa, lens, len(lens))
+    table[0, 5:lens[0] // ps:37] = -1                                    # absent pages all along the longest
+    table[0, lens[0] // ps // 2] = cache.num_pages + 3
+    table[0, (lens[0] - 1) // ps] = -1                                   # and its last one
+    size = torch.tensor([1 / 16, 4.0], device=gpu).repeat(num_kv * gqa)[:num_kv * gqa]
+    q = (q.float() * size[None, :, None]).to(q.dtype)
+    groups, per, tiles = decode_shape(cache, lens, gqa)
+    assert groups in (512, 768) and per >= 8 and tiles > 4 * groups      # two tiles a wave and more
+    out, lse = kv8.cache8_decode(cache, q, i32(table, gpu), i32(lens, gpu), return_lse=True)
+    o = clean(oracle_of(cache))
+    want = o.attend(rows_np(q), table, lens)
+    check_attention(out, lse, *want, TYPES[dtype], dh, "decode")
+    # sums: the tokens of a wave, then the partials of a pair
+    pair = -(-max(lens) // 64)
+    check_residual(out, want[0], *want[2:], TYPES[dtype], dh, np.array([[per // 4 * 64 + pair // per + 2]]), "decode")
+    assert torch.equal(kv8.cache8_decode(cache, q, i32(table, gpu), i32(lens, gpu)), out)
+    # the reference moves by a rise of 2^4 and more: there is one between tiles of the same wave
+    head = min(1, gqa - 1) if num_kv == 1 or gqa > 1 else 1              # a head of large queries
+    k, _, present = o.tokens(table, 0, 0, lens[0])
+    x = k[:, head // gqa] @ rows_np(q)[0, head] / math.sqrt(dh) * math.log2(math.e)
+    sv = np.repeat(o.scales[np.maximum(np.where(table[0] < cache.num_pages, table[0], 0), 0), head // gqa, 1], ps)[:lens[0]]
+    x = np.where(present, x + np.log2(np.where(present, sv, 1)), -np.inf)
+    x = np.pad(x, (0, -lens[0] % 64), constant_values=-np.inf).reshape(-1, 64).max(1)
+    first = (head // gqa) * (-(-gqa // 16)) * pair                       # the pair's first tile among all
+    t = np.arange(pair - 4)
+    same = (first + t) // per == (first + t + 4) // per
+    assert ((x[4:] > x[:-4] + 4) & np.isfinite(x[:-4]) & same).sum() > 3
+
+
+@pytest.mark.parametrize("fmt, dtype, dh", [("int8", "fp16", 128), ("e4m3", "bf16", 64)])
+def test_decode_one_long_among_many_short(gpu, fmt, dtype, dh):
+    """One wave joins all partials of a long pair where there are 128 pairs and more."""
+    lens = [30000] + [(i * 7) % 50 for i in range(69)]
+    num_kv, gqa = 2, 4
+    cache, table, q = attention_case(gpu, 92, fmt, dtype, dh, 16, num_kv, gqa, lens, len(lens))
+    _, per, _ = decode_shape(cache, lens, gqa)
+    assert len(lens) * num_kv >= 128 and 30000 // 64 // per > 100        # partials of the long pair
+    q[:, ::2] /= 16
+    out, lse = kv8.cache8_decode(cache, q, i32(table, gpu), i32(lens, gpu), return_lse=True)
+    want = clean(oracle_of(cache)).attend(rows_np(q), table, lens)
+    check_attention(out, lse, *want, TYPES[dtype], dh, "one long")
+    check_residual(out, want[0], *want[2:], TYPES[dtype], dh, np.array([[64 + 469 // per + 2]]), "one long")
+
+
+# ---- masks inside a tile, row starts that are none ---------------------------------------
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("dh", [64, 128])
+def test_prefill_mask_inside_a_tile(gpu, fmt, dh):
+    """A page from the middle of a tile of 64 tokens takes the largest finite codes: rows before it keep their bits,
+    those of the same tile among them (a NaN code there would make them NaN, by the product with a weight of 0)."""
+    cache, table, q = attention_case(gpu, 94, fmt, "fp16", dh, 16, 2, 4, [400], 400)
+    t, cu, n = i32(table, gpu), i32([0, 400], gpu), i32([400], gpu)
+    want = kv8.cache8_prefill(cache, q, cu, t, n)
+    largest = 127 if fmt == "int8" else 0x7E
+    cache.k_codes[int(table[0, 21])] = largest                           # tokens 336 .. 351 of the tile 320 .. 383
+    cache.v_codes[int(table[0, 21])] = largest
+    got = kv8.cache8_prefill(cache, q, cu, t, n)
+    assert torch.isfinite(got).all()
+    assert torch.equal(got[:336], want[:336]) and not torch.equal(got[336:], want[336:])
+
+
+@pytest.mark.parametrize("ps", [16, 64])
+@pytest.mark.parametrize("cu", [[0, 40, 10, 60], [50, 0, 60, 20], [-5, 1000, 3, 60], [60, 40, 20, 0], [2 ** 31 - 1, -2 ** 31, 30, 31]])
+def test_row_starts_out_of_order(gpu, cu, ps):
+    """Which rows such row starts stand for is not defined; every call ends, and no row outside 0 .. num_rows - 1 and
+    no page outside the tables is touched."""
+    rows, num_kv, gqa, dh = 60, 2, 4, 64
+    cache = random_cache(gpu, 96, 20, num_kv, dh, ps, "int8")
+    table = tables(97, 16, [4, 4, 4])
+    spare = np.setdiff1d(np.arange(20), table)
+    before = [x[spare].clone() for x in (cache.k_codes, cache.v_codes, cache.scales)]
+    td, start, lens, c = i32(table, gpu), i32([0, 3, 20], gpu), i32([64, 30, 50], gpu), i32(cu, gpu)
+    k = torch.full((rows + 8, num_kv, dh), float("inf"), device=gpu)     # rows around the given ones: would fill pages
+    k[4:-4] = torch.rand(rows, num_kv, dh, device=gpu)
+    kv8.cache8_write(cache, k[4:-4], k[4:-4], td, start, c)
+    assert all(torch.equal(x[spare], y) for x, y in zip((cache.k_codes, cache.v_codes, cache.scales), before))
+    assert torch.isfinite(cache.scales).all()
+    ko, vo = (torch.full((rows + 8, num_kv, dh), 7.0, dtype=torch.float16, device=gpu) for _ in range(2))
+    kv8.cache8_read(cache, td, start, c, rows, torch.float16, ko[4:-4], vo[4:-4])
+    q = torch.randn(rows, num_kv * gqa, dh, device=gpu).half()
+    out = torch.full((rows + 8, num_kv * gqa, dh), 7.0, dtype=torch.float16, device=gpu)
+    lse = torch.full((rows + 8, num_kv * gqa), 7.0, device=gpu)
+    kv8.cache8_prefill(cache, q, c, td, lens, out=out[4:-4], lse=lse[4:-4])
+    for x in (ko, vo, out, lse):
+        assert (x[:4] == 7).all() and (x[-4:] == 7).all()
