@@ -76,6 +76,8 @@ class Cache8:
         if k_codes.dim() != 4:
             raise ValueError("k_codes must be [num_pages, num_kv, page_size, dh]")
         num_pages, num_kv, page_size, dh = k_codes.shape
+        if not 1 <= num_kv <= 1024:
+            raise ValueError(f"num_kv must be in [1, 1024], got {num_kv}")
         if page_size not in (16, 32, 64, 128):
             raise ValueError(f"page_size must be 16, 32, 64 or 128, got {page_size}")
         if dh not in (64, 128):

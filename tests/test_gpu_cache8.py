@@ -863,3 +863,9 @@ def test_row_starts_out_of_order(gpu, cu, ps):
     kv8.cache8_prefill(cache, q, c, td, lens, out=out[4:-4], lse=lse[4:-4])
     for x in (ko, vo, out, lse):
         assert (x[:4] == 7).all() and (x[-4:] == 7).all()
+
+
+def test_head_counts_that_no_call_takes_are_refused(gpu):
+    for num_kv in (0, 1025):
+        with pytest.raises(ValueError, match="num_kv must be"):
+            kv8.Cache8.allocate(1, num_kv, 64, 16, "int8", gpu)
