@@ -159,8 +159,8 @@ __device__ __forceinline__ float wave_max(float x) {
 // wave, once.  A lane takes 16 bytes of a key row at a time; of the values, which
 // lie token-minor, two dims of all its tokens (of 8 at DH 64, the lane's half
 // saying which), so that the transposition is the lane's own.  100K fp16 tokens of
-// 8 heads x 128 are written as int8 in 140 us and read back in 118 (626 MB each way:
-// 4.5 and 5.3 TB/s, a large copy has 4.9).
+// 8 heads x 128 are written as int8 in 136 us and read back in 122 (626 MB each way:
+// 4.6 and 5.1 TB/s, a large copy has 4.9).
 
 template <int TYPE> struct Elem { typedef uint16_t T; static constexpr int kVec = 8; };
 template <> struct Elem<kFp32> { typedef float T; static constexpr int kVec = 4; };
@@ -381,7 +381,10 @@ __global__ __launch_bounds__(RUNS == 8 ? 512 : 256) void cache8_write_kernel(Cac
     if constexpr (VEC == 8) *(uint2*)(kc + t * DH + kdim) = uint2{ky[i][0], ky[i][1]};
     else *(uint32_t*)(kc + t * DH + kdim) = ky[i][0];
   }
-  // codes held before, under a larger scale: rare
+  // Codes held before, under a larger scale, a byte a lane at a time.  int8 tokens
+  // alike in size grow 16 % of the scales per token appended to pages of 16, so most
+  // calls wait for a wave that does this (256 sequences of 8 heads: 13.4 us a call, 8.0
+  // where no scale grows); e4m3's powers of two grow 2.5 % at pages of 32 (17.1 and 8.9).
   if (lo > 0 && ks > kold)
 #pragma unroll 1
     for (int i = lane; i < lo * DH; i += kWave) kc[i] = recode<FMT>(kc[i], kold, ks);
@@ -519,7 +522,8 @@ __global__ __launch_bounds__(256) void cache8_read_kernel(Cache8RowsLaunch L, ui
 // join their sums in LDS.  A pair that one workgroup holds is written out there;
 // the others leave a partial per workgroup (two at most: its first and its last
 // pair) for the merge kernel.  HBM-bound: 64 contexts of 2K..32K tokens, 8 heads x
-// 128 in e4m3, 2.28 GB in 400 us (5.7 TB/s); one of 32K in int8 17.6 us + 4 of merge.
+// 128 in e4m3, 2.28 GB in 400 us (5.7 TB/s); one of 32K in int8 20 us, about 4 of them
+// the merge.
 constexpr int kTileTokens = 64;
 // Workgroups: two of four waves per CU at DH 128, three at DH 64, whose registers
 // allow it (256 contexts of 100 to 900 tokens 50.7 us, 58.0 with two).  Their tiles
@@ -943,9 +947,9 @@ struct Partial { const float* ref; const float* row; };
 // Joins the partials of each (sequence, kv head) that several workgroups hold,
 // and writes the rows of sequences without a token.  WAVES waves per query head
 // share its partials: four where there are few pairs and many partials of each
-// (one document of 32K tokens, 64 of each head: 3.9 us, 7.8 with one wave), one
-// where there are many pairs of one or two (64 short contexts: 4.4 us, 7.3 with
-// four).
+// (one document of 32K tokens, 8 pairs, 64 of each head: 3.9 us, 7.8 with one wave),
+// one where there are many pairs of one or two (64 short contexts, 512 pairs: 4.4 us,
+// 7.3 with four).
 template <int TYPE, int DH, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void cache8_decode_merge_kernel(Cache8AttendLaunch L, const float* partials,
                                                                   const int64_t* base_of) {
@@ -1022,18 +1026,20 @@ __global__ __launch_bounds__(64 * WAVES) void cache8_decode_merge_kernel(Cache8A
 // With few row tiles the keys of each are split over workgroups, whose partials a
 // second kernel joins.
 //
-// A prompt of 8K tokens, 32 heads on 8 of 128: 0.55 TFLOP in 550 us (1.0 PFLOP/s; a
-// library product of 8192^3 has 1.21), the matrix cores 47 % busy beside 8 vector
-// instructions for each of theirs.  A wave of 64 rows would halve the LDS reads, but
+// A bf16 prompt of 8K tokens, 32 heads on 8 of 128: 0.55 TFLOP in 550 to 580 us over
+// cards (1.0 to 0.95 PFLOP/s; a library product of 8192^3 has 1.21), the matrix cores
+// 47 % and the vector units 55 % busy, 8 vector instructions for each matrix one.  At
+// head dim 64 a score has half the products: 14 vector instructions for each matrix
+// one, vector units 70 %, matrix cores 34 %.  A wave of 64 rows would halve the LDS reads, but
 // sums, scores, queries and weights alone are 288 registers: one wave per SIMD, with
 // nothing beside its products.
 
 // A workgroup's shape.  At DH 128 eight waves fill a CU's registers and share its
 // tiles: 256 rows; or, where the sequences have 128 rows or fewer on average, 128
 // rows by two groups of four waves that take the tiles in turn (a tile's step is
-// then a wave's 600 instructions, whatever the rows: four long documents of 20 to 96
-// rows a head 82.6 us with all waves on the same tile, 75.3 in turn).  At DH 64 four
-// waves, 128 rows, and three workgroups to a CU.
+// then a wave's 600 instructions, whatever the rows: four long documents of 28 to 72
+// rows a head 85.7 us with all waves on the same tile, 75.4 in turn; in fp16 98.4 and
+// 87.3).  At DH 64 four waves, 128 rows, and three workgroups to a CU.
 struct PrefillShape {
   int row_shift, groups, turns;         // log2 of a tile's rows, workgroups at once, wave groups that take turns
 };
@@ -1050,7 +1056,9 @@ __host__ __device__ __forceinline__ int64_t row_tiles(int64_t num_rows, int num_
 // Splits of each row tile: the workgroups at once over the fewest tiles that the
 // rows can make (twice as many at most, whose workgroups then take two rounds of
 // half the keys; by the most they can make, eight chunks of 64 tokens on 4K ran on
-// half of the CUs).
+// half of the CUs).  The lengths, which the host does not know, have no part in it: 16
+// tokens on 100K take 66 us alone and 1,940 beside 15 prompts of 500, whose rows
+// leave the long one a single workgroup per head.
 __host__ __device__ __forceinline__ int prefill_splits(int64_t num_rows, int num_seqs, int num_kv, int gqa, PrefillShape p) {
   const int64_t whole = (num_rows * gqa) >> p.row_shift, s = p.groups / ((whole > num_seqs ? whole : num_seqs) * num_kv);
   return (int)(s < 1 ? 1 : (s > kSplitMost ? kSplitMost : s));
@@ -1115,9 +1123,8 @@ __global__ __launch_bounds__(DH == 128 ? 512 : 256, 2) void cache8_prefill_kerne
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), col = lane & 31, half = lane >> 5;
   // Neighbours take the splits of one row tile, then different heads (unsplit and
   // eight of them: one per XCD and its L2, which the row tiles of a head share; with
-  // a row tile per sequence nothing is shared, and a head per XCD reads half of
-  // each L2's channels: 122 us, 76 with the splits first).  The longest rows of a
-  // sequence come first.
+  // splits the heads could as well come first: four long documents 75.1 us, 75.4).
+  // The longest rows of a sequence come first.
   const uint32_t pair = blockIdx.x / splits;
   const int h = pair % c.num_kv, z = blockIdx.x % splits, gqa = L.gqa;
   const int64_t slot = (gridDim.x / splits - 1 - pair) / c.num_kv;

@@ -297,7 +297,10 @@ def cache8_prefill(cache: Cache8, q: torch.Tensor, cu_rows: torch.Tensor, table:
     * gqa, dh] is at position lens[s] - n_s + i and attends the tokens up to
     its own (causal) or all lens[s].  Write the tokens first.  Rows that attend
     nothing get zeros and -inf; rows behind the last sequence are left as they
-    were in out and lse.  The rest as cache8_decode."""
+    were in out and lse.  A softmax weight meets its value with 22 bits for fp16
+    q, with 11 for bf16.  Few tokens on a long context are slow beside many short
+    sequences (the keys are split evenly over a batch): give them a call of their
+    own.  The rest as cache8_decode."""
     if cu_rows is None:
         raise TypeError("cu_rows must be a torch.Tensor")
     tab, stride, blocks, n = _seq_args(cache, table, lens, cu_rows, "lens")
