@@ -2,67 +2,19 @@
 // KV cache").  No reference counterpart: the reference keeps angle codes and
 // fp16 values.
 #include <hip/hip_runtime.h>
-#include <hip/hip_bf16.h>
 
-#include "sphkv_common.h"
-#include "sphkv_internal.h"
+#include "sphkv_attend.h"
 
 namespace sphkv {
 namespace {
 
-typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
-
 constexpr float kLeastScale = 0x1p-60f, kMostScale = 0x1p60f;
-
-__device__ __forceinline__ int clampi(int64_t x, int64_t lo, int64_t hi) {
-  return (int)(x < lo ? lo : (x > hi ? hi : x));
-}
-
-// rows of sequence s, whatever the list holds: begin..end within [0, num_rows]
-__device__ __forceinline__ void rows_of(const Cache8Batch& b, int s, int& begin, int& end) {
-  if (!b.cu) {
-    begin = s;
-    end = s + 1;
-    return;
-  }
-  begin = clampi(b.cu[s], 0, b.num_rows);
-  end = clampi(b.cu[s + 1], begin, b.num_rows);
-}
-
-// Work slots of a ragged batch without its lengths on the host: sequence s
-// starts at slot (cu[s] * mul >> shift) + extra * s, so n rows get more than
-// n * mul / 2^shift - 1 + extra slots.  The last sequence whose first slot is
-// at most j: 64 probes at a time, one step up to 64 sequences.  j is uniform
-// over the wave.
-__device__ __forceinline__ int64_t first_slot(const Cache8Batch& b, int s, int mul, int shift, int extra) {
-  return (((int64_t)clampi(b.cu[s], 0, b.num_rows) * mul) >> shift) + (int64_t)extra * s;
-}
-
-__device__ __forceinline__ int seq_of_slot(const Cache8Batch& b, int64_t j, int mul, int shift, int extra) {
-  const int lane = threadIdx.x & (kWave - 1);
-  int lo = 0, hi = b.num_seqs;
-  while (hi - lo > 1) {
-    const int step = (hi - lo + kWave - 1) / kWave, p = lo + lane * step;
-    const bool le = p < hi && first_slot(b, p < hi ? p : lo, mul, shift, extra) <= j;
-    const int cnt = __popcll(__ballot(le));
-    lo += (cnt > 0 ? cnt - 1 : 0) * step;
-    hi = lo + step < hi ? lo + step : hi;
-  }
-  return lo;
-}
 
 // the page of block blk of sequence s, or -1
 __device__ __forceinline__ int page_of(const Cache8& c, const Cache8Batch& b, int s, int64_t blk) {
   if (blk < 0 || blk >= b.max_blocks) return -1;
   const int p = b.table[s * b.table_stride + blk];
   return p >= 0 && p < c.num_pages ? p : -1;
-}
-
-template <int TYPE>
-__device__ __forceinline__ void store1(void* p, int64_t i, float x) {
-  if constexpr (TYPE == kFp16) ((_Float16*)p)[i] = (_Float16)x;
-  else if constexpr (TYPE == kBf16) ((__bf16*)p)[i] = (__bf16)x;
-  else ((float*)p)[i] = x;
 }
 
 template <int FMT>
@@ -140,19 +92,6 @@ __device__ __forceinline__ uint8_t recode(uint8_t c, float s, float t) {
   return (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32((float)y, (float)y, 0, false);
 }
 
-// over the 16 lanes of each row by rotation, then over the rows
-template <int N>
-__device__ __forceinline__ float row_rotated(float x) {
-  return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), 0x120 + N, 0xF, 0xF, true));
-}
-__device__ __forceinline__ float wave_max(float x) {
-  x = fmaxf(x, row_rotated<8>(x));
-  x = fmaxf(x, row_rotated<4>(x));
-  x = fmaxf(x, row_rotated<2>(x));
-  x = fmaxf(x, row_rotated<1>(x));
-  return rows_max(x);
-}
-
 // ---- write and read ------------------------------------------------------------
 //
 // Both move bytes: 2 * 16 * DH elements of a run of 16 tokens in and out per
@@ -161,26 +100,6 @@ __device__ __forceinline__ float wave_max(float x) {
 // saying which), so that the transposition is the lane's own.  100K fp16 tokens of
 // 8 heads x 128 are written as int8 in 136 us and read back in 122 (626 MB each way:
 // 4.6 and 5.1 TB/s, a large copy has 4.9).
-
-template <int TYPE> struct Elem { typedef uint16_t T; static constexpr int kVec = 8; };
-template <> struct Elem<kFp32> { typedef float T; static constexpr int kVec = 4; };
-
-template <int TYPE>
-__device__ __forceinline__ float value_of(typename Elem<TYPE>::T x) {
-  if constexpr (TYPE == kFp16) return (float)__builtin_bit_cast(_Float16, x);
-  else if constexpr (TYPE == kBf16) return __builtin_bit_cast(float, (uint32_t)x << 16);
-  else return x;
-}
-template <int TYPE>
-__device__ __forceinline__ typename Elem<TYPE>::T element_of(float x) {
-  if constexpr (TYPE == kFp16) return __builtin_bit_cast(uint16_t, (_Float16)x);
-  else if constexpr (TYPE == kBf16) return __builtin_bit_cast(uint16_t, (__bf16)x);
-  else return x;
-}
-
-// N consecutive elements at any alignment that theirs allows
-template <class T, int N>
-struct __attribute__((packed, aligned(sizeof(T)))) Unaligned { T x[N]; };
 
 // |x|, or 0 where x is not finite
 __device__ __forceinline__ float finite_abs(float x) {
@@ -530,9 +449,6 @@ constexpr int kTileTokens = 64;
 // are a multiple of their waves.
 __host__ __device__ constexpr int decode_groups(int dh) { return dh == 128 ? 512 : 768; }
 constexpr int kDecodeWaves = 4;
-constexpr float kTopWeight = 8.0f;      // log2 of the weight at the reference, ...
-constexpr float kSlackWeight = 4.0f;    // ... which moves once a weight passes 2^4 times that
-constexpr float kNoScore = -3.0e38f;    // reference before the first score
 // An exponent is one multiply-add, s_t + (log2 sv_t - R), whose rounding differs
 // from that of R by up to 2^-24 R: from this on they are rounded alike, s_t + log2
 // sv_t first, so that the largest weight is exactly that at any magnitude (always: 3
@@ -548,26 +464,6 @@ __host__ __device__ __forceinline__ int64_t plan_bytes(int num_seqs) { return (1
 
 __device__ __forceinline__ int seq_tokens(const Cache8& c, const Cache8Batch& b, int s) {
   return clampi(b.at[s], 0, (int64_t)b.max_blocks << c.page_shift);
-}
-
-__device__ __forceinline__ int64_t shfl64(int64_t x, int lane) {
-  const int lo = __shfl((int)x, lane, kWave), hi = __shfl((int)(x >> 32), lane, kWave);
-  return ((int64_t)hi << 32) | (uint32_t)lo;
-}
-
-// inclusive scan over the wave
-__device__ __forceinline__ int64_t wave_scan(int64_t x) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int d = 1; d < kWave; d <<= 1) {
-    const int64_t y = shfl64(x, lane - d);
-    if (lane >= d) x += y;
-  }
-  return x;
-}
-
-__device__ __forceinline__ int64_t uniform64(int64_t x) {
-  return ((int64_t)uniform((int)(x >> 32)) << 32) | (uint32_t)uniform((int)x);
 }
 
 // Four codes as two pairs of fp16 (exact).  int8: the byte + 128 below 1024,
@@ -592,15 +488,6 @@ __device__ __forceinline__ half8 codes8(uint32_t x, uint32_t y) {
   codes4<FMT>(y, c, d);
   return half8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
-
-// two numbers as fp16, half to even
-__device__ __forceinline__ half2v fp16_pair(float x, float y) {
-  typedef float float2v __attribute__((ext_vector_type(2)));
-  return __builtin_convertvector(float2v{x, y}, half2v);
-}
-
-__device__ __forceinline__ float log2_of(float x) { return __builtin_amdgcn_logf(x); }
-__device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // A query row's part in a lane as fp16.  fp16 rows as they are.  bf16 rows times
 // a power of two that brings their largest magnitude (row_max joins the lanes
@@ -892,58 +779,6 @@ __global__ __launch_bounds__(256, 2) void cache8_decode_kernel(Cache8AttendLaunc
   }
 }
 
-__device__ __forceinline__ float wave_sum(float x) {
-  x += row_rotated<8>(x);
-  x += row_rotated<4>(x);
-  x += row_rotated<2>(x);
-  x += row_rotated<1>(x);
-  return rows_sum(x);
-}
-
-// Partials first, first + step, ... before end of one output row, joined by the
-// wave, CH (up to 16) at a time whose loads are all on the way at once: R, l and
-// the lane's DH / 64 outputs.  `at(i)`: partial i's reference (its sum `sums` floats on) and
-// its row.
-template <int DPL, int CH, class AT>
-__device__ __forceinline__ void join(int64_t first, int64_t end, int64_t step, int sums, AT at, float& R, float& l,
-                                     float (&acc)[DPL]) {
-  const int lane = threadIdx.x & 63;
-  R = kNoScore;
-  l = 0.f;
-#pragma unroll
-  for (int i = 0; i < DPL; ++i) acc[i] = 0.f;
-  for (int64_t g = first; g < end; g += CH * step) {
-    float a[CH][DPL], r = kNoScore, ls = 0.f;
-    if (lane < CH && g + lane * step < end) {
-      const float* ref = at(g + lane * step).ref;
-      r = ref[0];
-      ls = ref[sums];
-    }
-#pragma unroll
-    for (int i = 0; i < CH; ++i) {
-      const int64_t k = g + i * step;
-      const float* row = at(k < end ? k : g).row + lane * DPL;        // (a missing one's weight is 0)
-#pragma unroll
-      for (int d = 0; d < DPL; ++d) a[i][d] = row[d];
-    }
-    const float M = fmaxf(R, wave_max(r)), f = exp2_of(r - M), was = exp2_of(R - M);
-    const bool has = lane < CH && g + lane * step < end;
-    const float w = has ? f : 0.f;
-    l = fmaf(l, was, wave_sum(ls * w));
-#pragma unroll
-    for (int d = 0; d < DPL; ++d) acc[d] *= was;
-#pragma unroll
-    for (int i = 0; i < CH; ++i) {
-      const float wi = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), i));
-      if (g + i * step < end)
-#pragma unroll
-        for (int d = 0; d < DPL; ++d) acc[d] = fmaf(a[i][d], wi, acc[d]);
-    }
-    R = M;
-  }
-}
-struct Partial { const float* ref; const float* row; };
-
 // Joins the partials of each (sequence, kv head) that several workgroups hold,
 // and writes the rows of sequences without a token.  WAVES waves per query head
 // share its partials: four where there are few pairs and many partials of each
@@ -1081,33 +916,6 @@ __device__ __forceinline__ int k_at(int token, int chunk) {        // fp16 eleme
   return token * DH + 8 * (DH == 128 ? (chunk ^ (token & 15)) : (chunk ^ ((token >> 1) & 7)));
 }
 __device__ __forceinline__ int v_at(int d, int chunk) { return d * kTileTokens + 8 * (chunk ^ ((d >> 1) & 7)); }
-
-__device__ __forceinline__ float halves_max(float x) {
-  float a = x, b = x;
-  swap32(a, b);
-  return fmaxf(a, b);
-}
-__device__ __forceinline__ float halves_sum(float x) {
-  float a = x, b = x;
-  swap32(a, b);
-  return a + b;
-}
-
-typedef float floatx16 __attribute__((ext_vector_type(16)));
-template <int N> struct Int { static constexpr int value = N; };
-
-// N LDS reads that feed M matrix instructions each: kAhead of them in flight
-constexpr int kAhead = 6;
-template <int N, int M>
-__device__ __forceinline__ void reads_ahead() {
-  __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
-#pragma unroll
-  for (int i = 0; i < N - kAhead; ++i) {
-    __builtin_amdgcn_sched_group_barrier(0x008, M, 0);
-    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-  }
-  __builtin_amdgcn_sched_group_barrier(0x008, kAhead * M, 0);
-}
 
 template <int FMT, int TYPE, int DH, int TURNS>
 __global__ __launch_bounds__(DH == 128 ? 512 : 256, 2) void cache8_prefill_kernel(Cache8AttendLaunch L, int splits, float* partials) {
