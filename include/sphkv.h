@@ -741,6 +741,115 @@ int sphkv_cache8_prefill(const void* q, int32_t q_type, int64_t q_row_stride, in
                          int32_t num_kv, int32_t gqa, int32_t dh, int32_t page_size, int32_t fmt, float sm_scale,
                          void* out, float* lse, void* workspace, int64_t workspace_bytes, void* stream);
 
+/*
+ * ---- 16-bit KV cache ---------------------------------------------------------
+ * Keys and values as fp16 or bf16 numbers in pages of page_size consecutive
+ * tokens of a sequence.  No reference counterpart.  Pages, heads and tokens may
+ * lie in any order: element (page, head, token, d) of the keys is k[page * k_page
+ * + head * k_head + token * k_token + d], strides in elements, non-negative and
+ * multiples of 8, page_size * k_token at most 2^28; the values likewise.  k and v
+ * are 16-byte aligned, type is SPHKV_FP16 or SPHKV_BF16, dh 64 or 128, page_size
+ * 16, 32, 64 or 128, num_kv at most 1024.  The struct is read during the call.
+ *
+ * table, cu_rows, start, lens, num_rows, num_seqs, workspace, stream and their
+ * limits are those of the 8-bit cache above: a page outside [0, num_pages) holds
+ * no token.  Rows of k, v, q and q_out may have any row and head stride and the
+ * alignment of their elements, their dh elements are contiguous.
+ */
+typedef struct sphkv_cache16 {
+  void* k;
+  void* v;
+  int64_t k_page, k_head, k_token;
+  int64_t v_page, v_head, v_token;
+  int64_t num_pages;
+  int32_t num_kv, dh, page_size, type;
+} sphkv_cache16;
+#define SPHKV_FP64 3
+
+/*
+ * Append new tokens: keys rotated by their positions, values as they are, each
+ * rounded once to the cache's type, and, unless q is NULL (gqa 0 then), the same
+ * tokens' queries rotated into q_out (of the cache's type; q_out may be q itself
+ * where their types and strides agree).  k, v [num_rows, num_kv, dh] and q
+ * [num_rows, num_kv*gqa, dh] of in_type (fp16, bf16 or fp32).  Sequence s's tokens
+ * are rows cu_rows[s] .. cu_rows[s+1] - 1 (NULL: row s, one token each, num_rows =
+ * num_seqs) at positions start[s], start[s] + 1, ...
+ *
+ * A head is `parts` (1 or 2) equal parts.  In each, the first 2 num_freqs
+ * elements are num_freqs pairs: (j, j + num_freqs), or (2j, 2j + 1) if interleaved;
+ * pair j turns by position * inv_freq[j] radians (formed in 64 bits; inv_freq fp32
+ * or fp64, by freq_type).  2 num_freqs is a multiple of 16 and at most dh / parts;
+ * the rest of a part stays.  num_freqs 0 (inv_freq NULL): nothing turns.
+ *
+ * Keys and values of a token past the table, of a sequence with a negative start
+ * or of an absent page are dropped (its queries are rotated all the same); rows
+ * from cu_rows[num_seqs] on are not read, and keep their contents in q_out.  A
+ * written page belongs to one sequence.
+ */
+int sphkv_cache16_append(const sphkv_cache16* cache, const void* k, const void* v, const void* q, int32_t in_type,
+                         int64_t k_row_stride, int64_t k_head_stride, int64_t v_row_stride, int64_t v_head_stride,
+                         int64_t q_row_stride, int64_t q_head_stride, int32_t gqa, void* q_out,
+                         int64_t q_out_row_stride, int64_t q_out_head_stride, int64_t num_rows, const int32_t* cu_rows,
+                         const int32_t* start, const int32_t* table, int64_t table_stride, int32_t max_blocks,
+                         int32_t num_seqs, const void* inv_freq, int32_t freq_type, int32_t num_freqs, int32_t parts,
+                         int32_t interleaved, void* stream);
+
+/*
+ * Attention of one query token per sequence, at position lens[s] - 1, over the
+ * last `window` of its first lens[s] tokens (0: all of them), its own among them:
+ *   out = sum_t softmax_t(sm_scale <q, k_t>) v_t,  lse = ln sum_t exp(sm_scale <q, k_t>)
+ * q [num_seqs, num_kv*gqa, dh] and out (contiguous) of the cache's type, lse fp32
+ * [num_seqs, num_kv*gqa] or NULL, gqa 1..64.  A sequence without a token gets zeros
+ * and -inf.  Scores, sums and outputs are held in fp32; a weight meets its value as
+ * two numbers of the cache's type (22 bits for fp16, 16 for bf16).  A value that
+ * is not finite makes that element of the rows that see its token an infinity or
+ * NaN, and of no other row.
+ */
+int64_t sphkv_cache16_decode_workspace_bytes(int32_t num_seqs, int32_t num_kv, int32_t gqa, int32_t dh,
+                                             int32_t differential);
+int sphkv_cache16_decode(const sphkv_cache16* cache, const void* q, int64_t q_row_stride, int64_t q_head_stride,
+                         int32_t gqa, const int32_t* lens, int32_t window, const int32_t* table, int64_t table_stride,
+                         int32_t max_blocks, int32_t num_seqs, float sm_scale, void* out, float* lse, void* workspace,
+                         int64_t workspace_bytes, void* stream);
+
+/*
+ * Differential attention of one query token per sequence: a head's first dh/2
+ * elements of q and k make one softmax map, the last dh/2 another, and
+ *   x = sum_t (softmax_t(sm_scale <q1, k1_t>) - lambda[h] softmax_t(sm_scale <q2, k2_t>)) v_t
+ *   out = x, or x / sqrt(mean(x^2) + norm_eps) * norm_weight where that is not NULL
+ * lambda fp32 [num_kv*gqa], norm_weight fp32 [dh], gqa 1..32, lse fp32 [num_seqs,
+ * num_kv*gqa, 2] (of both maps) or NULL; the rest as sphkv_cache16_decode.
+ */
+int sphkv_cache16_diff_decode(const sphkv_cache16* cache, const void* q, int64_t q_row_stride, int64_t q_head_stride,
+                              int32_t gqa, const float* lambda, const float* norm_weight, float norm_eps,
+                              const int32_t* lens, int32_t window, const int32_t* table, int64_t table_stride,
+                              int32_t max_blocks, int32_t num_seqs, float sm_scale, void* out, float* lse,
+                              void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Attention of several query tokens per sequence, the last ones of its lens[s]
+ * tokens: rows cu_rows[s] + i at position p = lens[s] - n_s + i attend the
+ * positions up to p (causal = 1; with a window w > 0 those above p - w) or all
+ * lens[s] (causal = 0, window 0).  A row that attends nothing gets zeros and
+ * -inf; rows from cu_rows[num_seqs] on keep their contents.  q, out [num_rows,
+ * num_kv*gqa, dh], lse [num_rows, num_kv*gqa].  A weight meets its value as two
+ * numbers of the cache's type in fp16 and in differential attention, as one bf16
+ * number otherwise.  The rest as the calls above.
+ */
+int64_t sphkv_cache16_prefill_workspace_bytes(int64_t num_rows, int32_t num_seqs, int32_t num_kv, int32_t gqa,
+                                              int32_t dh, int32_t differential);
+int sphkv_cache16_prefill(const sphkv_cache16* cache, const void* q, int64_t q_row_stride, int64_t q_head_stride,
+                          int32_t gqa, int64_t num_rows, const int32_t* cu_rows, const int32_t* lens, int32_t causal,
+                          int32_t window, const int32_t* table, int64_t table_stride, int32_t max_blocks,
+                          int32_t num_seqs, float sm_scale, void* out, float* lse, void* workspace,
+                          int64_t workspace_bytes, void* stream);
+int sphkv_cache16_diff_prefill(const sphkv_cache16* cache, const void* q, int64_t q_row_stride, int64_t q_head_stride,
+                               int32_t gqa, const float* lambda, const float* norm_weight, float norm_eps,
+                               int64_t num_rows, const int32_t* cu_rows, const int32_t* lens, int32_t causal,
+                               int32_t window, const int32_t* table, int64_t table_stride, int32_t max_blocks,
+                               int32_t num_seqs, float sm_scale, void* out, float* lse, void* workspace,
+                               int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

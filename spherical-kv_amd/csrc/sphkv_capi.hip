@@ -1124,6 +1124,81 @@ int cache8_attend(const char* fn, bool decode, const void* q, int32_t q_type, in
   return launch_status(sphkv::launch_cache8_attend(L, (hipStream_t)stream), fn);
 }
 
+// ---- 16-bit KV cache
+
+int cache16_checks(const char* fn, const sphkv_cache16* cache, const int32_t* table, int64_t table_stride,
+                   int32_t max_blocks, int32_t num_seqs, int64_t num_rows, sphkv::Cache16* c) {
+  if (!cache) return fail(SPHKV_EINVAL, "%s: null pointer argument", fn);
+  const sphkv_cache16& x = *cache;
+  if (!dh_ok(x.dh)) return fail(SPHKV_EINVAL, "%s: dh must be 64 or 128 (got %d)", fn, x.dh);
+  if (x.page_size != 16 && x.page_size != 32 && x.page_size != 64 && x.page_size != 128)
+    return fail(SPHKV_EINVAL, "%s: page_size must be 16, 32, 64 or 128 (got %d)", fn, x.page_size);
+  if (x.type != SPHKV_FP16 && x.type != SPHKV_BF16) return fail(SPHKV_EINVAL, "%s: the cache must be fp16 or bf16 (type %d)", fn, x.type);
+  if (num_seqs < 0 || num_rows < 0 || x.num_pages < 0 || max_blocks < 0 || x.num_kv < 1)
+    return fail(SPHKV_EINVAL, "%s: negative size", fn);
+  if (x.num_kv > 1024) return fail(SPHKV_EINVAL, "%s: num_kv must be at most 1024 (got %d)", fn, x.num_kv);
+  if (x.num_pages > INT32_MAX) return fail(SPHKV_EINVAL, "%s: num_pages exceeds int32", fn);
+  const int64_t strides[6] = {x.k_page, x.k_head, x.k_token, x.v_page, x.v_head, x.v_token};
+  for (int64_t st : strides)
+    if (st < 0 || (st & 7)) return fail(SPHKV_EINVAL, "%s: the cache's strides must be non-negative multiples of 8", fn);
+  if (x.k_token > (1 << 28) / x.page_size || x.v_token > (1 << 28) / x.page_size)
+    return fail(SPHKV_EINVAL, "%s: page_size times a token stride exceeds 2^28", fn);
+  // (rows and sequences of one call: their workgroups fit a grid)
+  if (num_seqs > (1 << 16) || num_rows > (1 << 26))
+    return fail(SPHKV_EINVAL, "%s: at most 2^16 sequences and 2^26 rows", fn);
+  if (((num_rows >> 4) + 2 * (int64_t)num_seqs) * x.num_kv > (1 << 25))
+    return fail(SPHKV_EINVAL, "%s: (num_rows / 16 + 2 num_seqs) * num_kv exceeds 2^25", fn);
+  if ((int64_t)max_blocks * x.page_size > (1 << 30))
+    return fail(SPHKV_EINVAL, "%s: max_blocks * page_size exceeds 2^30", fn);
+  if (num_seqs > 1 && table_stride < max_blocks)
+    return fail(SPHKV_EINVAL, "%s: table_stride is less than max_blocks", fn);
+  if (((uintptr_t)x.k | (uintptr_t)x.v) & 15) return fail(SPHKV_EINVAL, "%s: k and v of the cache must be 16-byte aligned", fn);
+  if (num_seqs > 0 && x.num_pages > 0 && (!x.k || !x.v)) return fail(SPHKV_EINVAL, "%s: null pointer argument", fn);
+  if (num_seqs > 0 && max_blocks > 0 && !table) return fail(SPHKV_EINVAL, "%s: null pointer argument", fn);
+  int shift = 4;
+  while ((1 << shift) < x.page_size) ++shift;
+  *c = {(uint16_t*)x.k, (uint16_t*)x.v, x.k_page, x.k_head, x.v_page, x.v_head, (int32_t)x.k_token, (int32_t)x.v_token,
+        x.num_pages, x.num_kv, x.dh, shift, x.type};
+  return SPHKV_OK;
+}
+
+// differential attention's weights (NULL: the ordinary one)
+struct Diff16 { const float* lambda; const float* norm_weight; float norm_eps; };
+
+int cache16_attend(const char* fn, bool decode, const Diff16* diff, const sphkv_cache16* cache, const void* q,
+                   int64_t q_row_stride, int64_t q_head_stride, int32_t gqa, int64_t num_rows, const int32_t* cu_rows,
+                   const int32_t* lens, int32_t causal, int32_t window, const int32_t* table, int64_t table_stride,
+                   int32_t max_blocks, int32_t num_seqs, float sm_scale, void* out, float* lse, void* workspace,
+                   int64_t workspace_bytes, void* stream) {
+  sphkv::Cache16 c;
+  if (int rc = cache16_checks(fn, cache, table, table_stride, max_blocks, num_seqs, num_rows, &c)) return rc;
+  const int most = diff ? sphkv::kCache8MaxGqa / 2 : sphkv::kCache8MaxGqa;
+  if (gqa < 1 || gqa > most) return fail(SPHKV_EINVAL, "%s: gqa must be in [1, %d] (got %d)", fn, most, gqa);
+  if (causal != 0 && causal != 1) return fail(SPHKV_EINVAL, "%s: causal must be 0 or 1 (got %d)", fn, causal);
+  if (window < 0 || (window > 0 && !causal))
+    return fail(SPHKV_EINVAL, "%s: window must be non-negative, and 0 without causal (got %d)", fn, window);
+  if (!(sm_scale > 0.f) || !std::isfinite(sm_scale))
+    return fail(SPHKV_EINVAL, "%s: sm_scale must be positive and finite", fn);
+  if (diff && (!(diff->norm_eps >= 0.f) || !std::isfinite(diff->norm_eps)))
+    return fail(SPHKV_EINVAL, "%s: norm_eps must be non-negative and finite", fn);
+  // (a grid holds fewer than 2^32 threads: a merge wave or four per (row, head), 512 per (row tile, kv head))
+  if (decode ? num_rows * c.num_kv * gqa > 1 << 23 : (((num_rows * gqa) >> 7) + num_seqs) * c.num_kv >= 1 << 23)
+    return fail(SPHKV_EINVAL, "%s: too many (row, head) pairs", fn);
+  if (num_seqs == 0 || num_rows == 0) return ok();
+  if (!q || !lens || !out || (!decode && !cu_rows) || (diff && !diff->lambda))
+    return fail(SPHKV_EINVAL, "%s: null pointer argument", fn);
+  const int64_t need = decode ? sphkv::cache16_decode_ws_bytes(num_seqs, c.num_kv, gqa, c.dh, diff)
+                              : sphkv::cache16_prefill_ws_bytes(num_rows, num_seqs, c.num_kv, gqa, c.dh, diff);
+  if (need > 0 && (!workspace || workspace_bytes < need))
+    return fail(SPHKV_EINVAL, "%s: workspace needs %lld bytes (got %lld)", fn, (long long)need,
+                (long long)workspace_bytes);
+  if ((uintptr_t)workspace & 15) return fail(SPHKV_EINVAL, "%s: workspace must be 16-byte aligned", fn);
+  sphkv::Cache16AttendLaunch L{c, {cu_rows, lens, table, table_stride, c.num_pages > 0 ? max_blocks : 0, num_seqs, num_rows},
+                               q, q_row_stride, q_head_stride, gqa, causal, window, sm_scale, out, lse, workspace,
+                               diff ? diff->lambda : nullptr, diff ? diff->norm_weight : nullptr, diff ? diff->norm_eps : 0.f};
+  return launch_status(sphkv::launch_cache16_attend(L, (hipStream_t)stream), fn);
+}
+
 }  // namespace
 
 extern "C" {
@@ -1204,6 +1279,95 @@ int sphkv_cache8_prefill(const void* q, int32_t q_type, int64_t q_row_stride, in
   return cache8_attend("sphkv_cache8_prefill", false, q, q_type, q_row_stride, q_head_stride, num_rows, cu_rows, lens,
                        causal, table, table_stride, max_blocks, num_seqs, k_codes, v_codes, scales, num_pages, num_kv,
                        gqa, dh, page_size, fmt, sm_scale, out, lse, workspace, workspace_bytes, stream);
+}
+
+int sphkv_cache16_append(const sphkv_cache16* cache, const void* k, const void* v, const void* q, int32_t in_type,
+                         int64_t k_row_stride, int64_t k_head_stride, int64_t v_row_stride, int64_t v_head_stride,
+                         int64_t q_row_stride, int64_t q_head_stride, int32_t gqa, void* q_out,
+                         int64_t q_out_row_stride, int64_t q_out_head_stride, int64_t num_rows, const int32_t* cu_rows,
+                         const int32_t* start, const int32_t* table, int64_t table_stride, int32_t max_blocks,
+                         int32_t num_seqs, const void* inv_freq, int32_t freq_type, int32_t num_freqs, int32_t parts,
+                         int32_t interleaved, void* stream) {
+  const char* fn = "sphkv_cache16_append";
+  sphkv::Cache16 c;
+  if (int rc = cache16_checks(fn, cache, table, table_stride, max_blocks, num_seqs, num_rows, &c)) return rc;
+  if (in_type < SPHKV_FP16 || in_type > SPHKV_FP32) return fail(SPHKV_EINVAL, "%s: unknown type %d", fn, in_type);
+  if (gqa < 0 || gqa > sphkv::kCache8MaxGqa)
+    return fail(SPHKV_EINVAL, "%s: gqa must be in [0, %d] (got %d)", fn, sphkv::kCache8MaxGqa, gqa);
+  if ((gqa > 0) != (q != nullptr) && num_rows > 0) return fail(SPHKV_EINVAL, "%s: gqa must be 0 without q, positive with it", fn);
+  if (parts != 1 && parts != 2) return fail(SPHKV_EINVAL, "%s: parts must be 1 or 2 (got %d)", fn, parts);
+  if (interleaved != 0 && interleaved != 1) return fail(SPHKV_EINVAL, "%s: interleaved must be 0 or 1 (got %d)", fn, interleaved);
+  if (num_freqs < 0 || (num_freqs & 7) || 2 * (int64_t)num_freqs > c.dh / parts)
+    return fail(SPHKV_EINVAL, "%s: num_freqs must be a multiple of 8, at most dh / parts / 2 (got %d)", fn, num_freqs);
+  if (num_freqs > 0 && freq_type != SPHKV_FP32 && freq_type != SPHKV_FP64)
+    return fail(SPHKV_EINVAL, "%s: inv_freq must be fp32 or fp64 (type %d)", fn, freq_type);
+  if (!cu_rows && num_rows != num_seqs)
+    return fail(SPHKV_EINVAL, "%s: without cu_rows there is one row per sequence", fn);
+  // (a wave of 64 threads per row: fewer than 2^32 in a grid)
+  if (num_rows >= 1 << 26) return fail(SPHKV_EINVAL, "%s: num_rows must be below 2^26", fn);
+  if (num_seqs == 0 || num_rows == 0) return ok();
+  if (!k || !v || !start || (q && !q_out) || (num_freqs > 0 && !inv_freq))
+    return fail(SPHKV_EINVAL, "%s: null pointer argument", fn);
+  sphkv::Cache16AppendLaunch L{c, {cu_rows, start, table, table_stride, c.num_pages > 0 ? max_blocks : 0, num_seqs, num_rows},
+                               k, v, q, in_type, k_row_stride, k_head_stride, v_row_stride, v_head_stride, q_row_stride,
+                               q_head_stride, gqa, q_out, q_out_row_stride, q_out_head_stride, inv_freq, freq_type,
+                               num_freqs, parts, interleaved};
+  return launch_status(sphkv::launch_cache16_append(L, (hipStream_t)stream), fn);
+}
+
+int64_t sphkv_cache16_decode_workspace_bytes(int32_t num_seqs, int32_t num_kv, int32_t gqa, int32_t dh,
+                                             int32_t differential) {
+  if (num_seqs < 0 || num_kv < 1 || gqa < 1 || gqa > sphkv::kCache8MaxGqa / (differential ? 2 : 1) || !dh_ok(dh)) return -1;
+  return sphkv::cache16_decode_ws_bytes(num_seqs, num_kv, gqa, dh, differential != 0);
+}
+
+int sphkv_cache16_decode(const sphkv_cache16* cache, const void* q, int64_t q_row_stride, int64_t q_head_stride,
+                         int32_t gqa, const int32_t* lens, int32_t window, const int32_t* table, int64_t table_stride,
+                         int32_t max_blocks, int32_t num_seqs, float sm_scale, void* out, float* lse, void* workspace,
+                         int64_t workspace_bytes, void* stream) {
+  return cache16_attend("sphkv_cache16_decode", true, nullptr, cache, q, q_row_stride, q_head_stride, gqa, num_seqs, nullptr,
+                        lens, 1, window, table, table_stride, max_blocks, num_seqs, sm_scale, out, lse, workspace,
+                        workspace_bytes, stream);
+}
+
+int sphkv_cache16_diff_decode(const sphkv_cache16* cache, const void* q, int64_t q_row_stride, int64_t q_head_stride,
+                              int32_t gqa, const float* lambda, const float* norm_weight, float norm_eps,
+                              const int32_t* lens, int32_t window, const int32_t* table, int64_t table_stride,
+                              int32_t max_blocks, int32_t num_seqs, float sm_scale, void* out, float* lse,
+                              void* workspace, int64_t workspace_bytes, void* stream) {
+  const Diff16 diff{lambda, norm_weight, norm_eps};
+  return cache16_attend("sphkv_cache16_diff_decode", true, &diff, cache, q, q_row_stride, q_head_stride, gqa, num_seqs,
+                        nullptr, lens, 1, window, table, table_stride, max_blocks, num_seqs, sm_scale, out, lse, workspace,
+                        workspace_bytes, stream);
+}
+
+int64_t sphkv_cache16_prefill_workspace_bytes(int64_t num_rows, int32_t num_seqs, int32_t num_kv, int32_t gqa,
+                                              int32_t dh, int32_t differential) {
+  if (num_rows < 0 || num_seqs < 0 || num_kv < 1 || gqa < 1 || gqa > sphkv::kCache8MaxGqa / (differential ? 2 : 1) || !dh_ok(dh))
+    return -1;
+  return sphkv::cache16_prefill_ws_bytes(num_rows, num_seqs, num_kv, gqa, dh, differential != 0);
+}
+
+int sphkv_cache16_prefill(const sphkv_cache16* cache, const void* q, int64_t q_row_stride, int64_t q_head_stride,
+                          int32_t gqa, int64_t num_rows, const int32_t* cu_rows, const int32_t* lens, int32_t causal,
+                          int32_t window, const int32_t* table, int64_t table_stride, int32_t max_blocks,
+                          int32_t num_seqs, float sm_scale, void* out, float* lse, void* workspace,
+                          int64_t workspace_bytes, void* stream) {
+  return cache16_attend("sphkv_cache16_prefill", false, nullptr, cache, q, q_row_stride, q_head_stride, gqa, num_rows, cu_rows,
+                        lens, causal, window, table, table_stride, max_blocks, num_seqs, sm_scale, out, lse, workspace,
+                        workspace_bytes, stream);
+}
+
+int sphkv_cache16_diff_prefill(const sphkv_cache16* cache, const void* q, int64_t q_row_stride, int64_t q_head_stride,
+                               int32_t gqa, const float* lambda, const float* norm_weight, float norm_eps,
+                               int64_t num_rows, const int32_t* cu_rows, const int32_t* lens, int32_t causal,
+                               int32_t window, const int32_t* table, int64_t table_stride, int32_t max_blocks,
+                               int32_t num_seqs, float sm_scale, void* out, float* lse, void* workspace,
+                               int64_t workspace_bytes, void* stream) {
+  const Diff16 diff{lambda, norm_weight, norm_eps};
+  return cache16_attend("sphkv_cache16_diff_prefill", false, &diff, cache, q, q_row_stride, q_head_stride, gqa, num_rows,
+                        cu_rows, lens, causal, window, table, table_stride, max_blocks, num_seqs, sm_scale, out, lse,
+                        workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

@@ -251,4 +251,30 @@ int launch_cache8_attend(const Cache8AttendLaunch& L, hipStream_t stream);
 int64_t cache8_decode_ws_bytes(int32_t num_seqs, int32_t num_kv, int32_t gqa, int32_t dh);
 int64_t cache8_prefill_ws_bytes(int64_t num_rows, int32_t num_seqs, int32_t num_kv, int32_t gqa, int32_t dh);
 
+// 16-bit KV cache (sphkv_kv16.hip): fp16 or bf16 numbers in pages of a
+// sequence's tokens, of any page, head and token stride (in elements).
+constexpr int kFp64 = 3;
+struct Cache16 {
+  uint16_t* k; uint16_t* v;
+  int64_t k_page, k_head, v_page, v_head; int32_t k_token, v_token;
+  int64_t num_pages; int32_t num_kv, dh, page_shift, type;
+};
+struct Cache16AppendLaunch {
+  Cache16 c; Cache8Batch b;                // b.at: the first row's position
+  const void* k; const void* v; const void* q; int32_t type;   // q may be null (gqa 0)
+  int64_t k_row, k_head, v_row, v_head, q_row, q_head;
+  int32_t gqa; void* q_out; int64_t o_row, o_head;
+  const void* inv_freq; int32_t freq_type, freqs, parts, interleaved;
+};
+struct Cache16AttendLaunch {
+  Cache16 c; Cache8Batch b;                // b.at: lens; decode: cu null, one query row a sequence
+  const void* q; int64_t q_row, q_head; int32_t gqa, causal, window; float sm_scale;
+  void* out; float* lse; void* ws;
+  const float* lambda; const float* norm_weight; float norm_eps;   // lambda: differential; norm_weight may be null
+};
+int launch_cache16_append(const Cache16AppendLaunch& L, hipStream_t stream);
+int launch_cache16_attend(const Cache16AttendLaunch& L, hipStream_t stream);
+int64_t cache16_decode_ws_bytes(int32_t num_seqs, int32_t num_kv, int32_t gqa, int32_t dh, bool diff);
+int64_t cache16_prefill_ws_bytes(int64_t num_rows, int32_t num_seqs, int32_t num_kv, int32_t gqa, int32_t dh, bool diff);
+
 }  // namespace sphkv

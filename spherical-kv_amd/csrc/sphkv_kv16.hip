@@ -1,0 +1,1194 @@
+// The 16-bit KV cache: append with rotation, attention and differential
+// attention (include/sphkv.h, "16-bit KV cache").  No reference counterpart.
+#include <hip/hip_runtime.h>
+
+#include "sphkv_attend.h"
+
+namespace sphkv {
+namespace {
+
+typedef uint32_t uintx2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float floatx2 __attribute__((ext_vector_type(2)));
+
+// eight 16-bit numbers (four dwords) of a lane as a matrix operand
+template <int TYPE>
+__device__ __forceinline__ floatx4 mfma16(uintx4 a, uintx4 b, floatx4 c) {
+  if constexpr (TYPE == kFp16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+template <int TYPE>
+__device__ __forceinline__ floatx16 mfma32(uintx4 a, uintx4 b, floatx16 c) {
+  if constexpr (TYPE == kFp16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// two numbers, half to even, and the numbers that a pair stands for
+template <int TYPE>
+__device__ __forceinline__ uint32_t pair_of(float x, float y) {
+  if constexpr (TYPE == kFp16) return __builtin_bit_cast(uint32_t, fp16_pair(x, y));
+  else return __builtin_bit_cast(uint32_t, __builtin_convertvector(floatx2{x, y}, bf16x2));
+}
+template <int TYPE>
+__device__ __forceinline__ float low_of(uint32_t p) {
+  if constexpr (TYPE == kFp16) return (float)__builtin_bit_cast(half2v, p)[0];
+  else return __builtin_bit_cast(float, p << 16);
+}
+template <int TYPE>
+__device__ __forceinline__ float high_of(uint32_t p) {
+  if constexpr (TYPE == kFp16) return (float)__builtin_bit_cast(half2v, p)[1];
+  else return __builtin_bit_cast(float, p & 0xFFFF0000u);
+}
+
+// the low or the high halves of two dwords
+__device__ __forceinline__ uint32_t lows(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
+__device__ __forceinline__ uint32_t highs(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
+
+__device__ __forceinline__ int seq_tokens(const Cache16& c, const Cache8Batch& b, int s) {
+  return clampi(b.at[s], 0, (int64_t)b.max_blocks << c.page_shift);
+}
+
+// From this size on a score and the reference are rounded alike before their
+// difference is taken (one multiply-add below it), so that the largest weight is
+// what the reference says at any magnitude.
+constexpr float kPlainScore = 0x1p18f;
+constexpr float kLog2e = 1.44269504088896f, kLn2 = 0.693147180559945f;
+
+// ---- append --------------------------------------------------------------------
+//
+// y_j = x_j cos a - x_j' sin a, y_j' = x_j' cos a + x_j sin a, a = p f: moves bytes.
+// A lane owns 16 elements of a head (the two sides of eight pairs, or 16 that
+// stay) and keeps them for every head that it takes, so their eight angles are
+// formed once per token: the turns p f / 2 pi in 64 bits, less their nearest whole
+// number, then sine and cosine in 32.  A wave takes one token; where a call has
+// few, its heads are spread over waves.
+
+template <int TYPE>
+struct Eight { typename Elem<TYPE>::T x[8]; };
+
+template <int TYPE>
+__device__ __forceinline__ Eight<TYPE> load8(const void* p, int64_t at) {
+  typedef typename Elem<TYPE>::T E;
+  Eight<TYPE> r;
+  *(Unaligned<E, 8>*)&r = *(const Unaligned<E, 8>*)((const E*)p + at);
+  return r;
+}
+
+template <int IN, int OUT, int DH>
+__global__ __launch_bounds__(256) void cache16_append_kernel(Cache16AppendLaunch L, uint32_t items, int splits) {
+  constexpr int UNITS = DH / 16, HEADS = 64 / UNITS;                  // 16-element units of a head, heads at once
+  const Cache16& c = L.c;
+  const Cache8Batch& b = L.b;
+  const uint32_t item = blockIdx.x * 4 + uniform(threadIdx.x >> 6);
+  if (item >= items) return;
+  const int lane = threadIdx.x & 63, unit = lane % UNITS;
+  const int64_t row = item / splits;
+  const int nq = c.num_kv * L.gqa, heads = nq + 2 * c.num_kv;         // q, k, v heads in a row
+  const int first = (item - (uint32_t)row * splits) * HEADS + lane / UNITS, step = splits * HEADS;
+
+  // this lane's elements: o0 .. o0 + 7 and o1 .. o1 + 7, turned (pairs 8 u ..) or not
+  const int width = DH / L.parts, per_part = UNITS / L.parts, part = unit / per_part, u = unit - part * per_part;
+  const bool turns = u < L.freqs / 8;
+  const bool half = turns && !L.interleaved;
+  const int o0 = part * width + (half ? 8 * u : 16 * u), o1 = half ? o0 + L.freqs : o0 + 8;
+
+  auto load = [&](int j, Eight<IN>& x, Eight<IN>& y) {
+    const bool is_q = j < nq, is_k = j < nq + c.num_kv;
+    const void* src = is_q ? L.q : is_k ? L.k : L.v;
+    const int64_t at = is_q ? row * L.q_row + j * L.q_head
+                     : is_k ? row * L.k_row + (j - nq) * L.k_head : row * L.v_row + (j - nq - c.num_kv) * L.v_head;
+    x = load8<IN>(src, at + o0);
+    y = load8<IN>(src, at + o1);
+  };
+  const int s = b.cu ? uniform(seq_of_slot(b, row, 1, 0, 0)) : (int)row;
+  int begin, end;
+  rows_of(b, s, begin, end);
+  if (row < begin || row >= end) return;
+  const int64_t start = b.at[s], pos = start + (row - begin), blk = pos >> c.page_shift;
+  int page = -1;
+  if (start >= 0 && blk < b.max_blocks) {
+    page = b.table[s * b.table_stride + blk];
+    if (page >= c.num_pages) page = -1;
+  }
+  const int slot = (int)(pos & ((1 << c.page_shift) - 1));
+
+  float cs[8], sn[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    cs[i] = 1.f;
+    sn[i] = 0.f;
+  }
+  if (turns) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const double f = L.freq_type == kFp64 ? ((const double*)L.inv_freq)[8 * u + i] : (double)((const float*)L.inv_freq)[8 * u + i];
+      double t = (double)pos * (f * 0.15915494309189535);             // 1 / 2 pi
+      t -= __builtin_rint(t);
+      sincospif(2.0f * (float)t, &sn[i], &cs[i]);
+    }
+  }
+  for (int j = first; j < heads; j += step) {
+    Eight<IN> x, y;
+    load(j, x, y);
+    const bool is_q = j < nq, is_k = j < nq + c.num_kv, turn = turns && is_k;
+    uint32_t xo[4], yo[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float a0 = value_of<IN>(x.x[2 * i]), a1 = value_of<IN>(x.x[2 * i + 1]), b0 = value_of<IN>(y.x[2 * i]), b1 = value_of<IN>(y.x[2 * i + 1]);
+      if (turn) {
+        if (half) {                                                   // pairs (a0, b0), (a1, b1)
+          const float p = a0, q = a1;
+          a0 = fmaf(p, cs[2 * i], -(b0 * sn[2 * i]));
+          a1 = fmaf(q, cs[2 * i + 1], -(b1 * sn[2 * i + 1]));
+          b0 = fmaf(b0, cs[2 * i], p * sn[2 * i]);
+          b1 = fmaf(b1, cs[2 * i + 1], q * sn[2 * i + 1]);
+        } else {                                                      // pairs (a0, a1), (b0, b1)
+          const float p = a0, q = b0;
+          a0 = fmaf(p, cs[i], -(a1 * sn[i]));
+          a1 = fmaf(a1, cs[i], p * sn[i]);
+          b0 = fmaf(q, cs[i + 4], -(b1 * sn[i + 4]));
+          b1 = fmaf(b1, cs[i + 4], q * sn[i + 4]);
+        }
+      }
+      xo[i] = pair_of<OUT>(a0, a1);
+      yo[i] = pair_of<OUT>(b0, b1);
+    }
+    if constexpr (IN == OUT) {                                        // numbers that stay keep their bits
+      if (!turn) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          xo[i] = (uint32_t)x.x[2 * i] | (uint32_t)x.x[2 * i + 1] << 16;
+          yo[i] = (uint32_t)y.x[2 * i] | (uint32_t)y.x[2 * i + 1] << 16;
+        }
+      }
+    }
+    if (is_q) {
+      struct __attribute__((packed, aligned(2))) U4 { uintx4 v; };
+      uint16_t* to = (uint16_t*)L.q_out + row * L.o_row + j * L.o_head;
+      ((U4*)(to + o0))->v = uintx4{xo[0], xo[1], xo[2], xo[3]};
+      ((U4*)(to + o1))->v = uintx4{yo[0], yo[1], yo[2], yo[3]};
+    } else if (page >= 0) {
+      uint16_t* to = is_k ? c.k + page * c.k_page + (j - nq) * c.k_head + slot * c.k_token
+                          : c.v + page * c.v_page + (j - nq - c.num_kv) * c.v_head + slot * c.v_token;
+      *(uintx4*)(to + o0) = uintx4{xo[0], xo[1], xo[2], xo[3]};
+      *(uintx4*)(to + o1) = uintx4{yo[0], yo[1], yo[2], yo[3]};
+    }
+  }
+}
+
+// ---- an output row ---------------------------------------------------------------
+//
+// DH / 64 consecutive elements of a lane, of one map (sums x under reference R with
+// weights' sum l) or of two.
+
+template <int DH>
+struct RowSum { float x[DH / 64], R, l; };
+
+template <int TYPE, int DH, bool DIFF>
+__device__ __forceinline__ void finish_row(const Cache16AttendLaunch& L, int64_t at, int head, const RowSum<DH>& a,
+                                           const RowSum<DH>& b) {
+  constexpr int DPL = DH / 64;
+  const int lane = threadIdx.x & 63;
+  float y[DPL];
+#pragma unroll
+  for (int i = 0; i < DPL; ++i) y[i] = a.l == 0.f ? 0.f : a.x[i] / a.l;
+  if constexpr (DIFF) {
+    const float lam = L.lambda[head];
+    float sq = 0.f;
+#pragma unroll
+    for (int i = 0; i < DPL; ++i) {
+      y[i] = fmaf(-lam, b.l == 0.f ? 0.f : b.x[i] / b.l, y[i]);
+      sq = fmaf(y[i], y[i], sq);
+    }
+    if (L.norm_weight) {
+      const float scale = 1.0f / __builtin_sqrtf(fmaf(wave_sum(sq), 1.0f / DH, L.norm_eps));
+#pragma unroll
+      for (int i = 0; i < DPL; ++i) y[i] *= scale * L.norm_weight[lane * DPL + i];
+      if (a.l == 0.f)                                                 // (no eps: 0 * inf)
+#pragma unroll
+        for (int i = 0; i < DPL; ++i) y[i] = 0.f;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < DPL; ++i) store1<TYPE>(L.out, at * DH + lane * DPL + i, y[i]);
+  if (L.lse && lane == 0) {
+    const float e = a.l == 0.f ? -INFINITY : (a.R + log2_of(a.l)) * kLn2;
+    if constexpr (DIFF) {
+      L.lse[2 * at] = e;
+      L.lse[2 * at + 1] = b.l == 0.f ? -INFINITY : (b.R + log2_of(b.l)) * kLn2;
+    } else {
+      L.lse[at] = e;
+    }
+  }
+}
+
+// ---- decode ------------------------------------------------------------------
+//
+// out = sum_t w_t v_t / sum_t w_t,  w_t = 2^(s_t - R),  s_t = sm_scale log2(e) <q, k_t>,
+// R a reference near the largest s_t.  HBM-bound: every key and value is read once.
+//
+// A tile is 32 tokens, one wave's step: S^T = K Q^T as two 16x16 blocks
+// (v_mfma_f32_16x16x32), O^T += V^T P^T as DH/16 blocks.  Token 8 g + 4 x + r of a
+// tile is row 4 g + r of score block x, so lane (g, column) ends up with the scores
+// of tokens 8 g .. 8 g + 7, in order: its part of the second product's B operand
+// as they stand.  Its part of the A operand is dim d of the same eight tokens: the
+// lane loads DH / 16 consecutive dims of each (16 lanes a whole row), and block j
+// takes the j-th of them, paired by v_perm (one per dword), so that row i of block
+// j is dim DH / 16 i + j.  Nothing passes through LDS.
+//
+// A column is a query head, or one of the two maps of a head in differential
+// attention, whose scores come from half of the dims each.  Up to 8 columns are
+// used twice, the second time for what the first one's 16-bit weight leaves out;
+// more fill the block, and that rest is a product of its own.
+//
+// Work: the tiles of all (sequence, kv head) pairs in a row, cut into equal runs,
+// one per workgroup; its four waves take the tiles of a pair in turn and join their
+// sums in LDS.  A pair that one workgroup holds is written out there; the others
+// leave a partial per workgroup (two at most: its first and its last pair) for the
+// merge kernel.
+constexpr int kDecodeTile = 32, kDecodeWaves = 4;
+__host__ __device__ constexpr int decode_groups(int) { return 512; }
+
+// columns handled together: a kv head's first 16, next 16, ...
+__host__ __device__ __forceinline__ int col_parts(int cols) { return (cols + 15) / 16; }
+__host__ __device__ __forceinline__ int part_cols(int cols, int part) { return cols - part * 16 < 16 ? cols - part * 16 : 16; }
+// floats of one partial: reference and sum per column, then acc[cols][DH]
+__host__ __device__ __forceinline__ int64_t partial_size(int cols, int dh) { return 32 + (int64_t)(cols < 16 ? cols : 16) * dh; }
+__host__ __device__ __forceinline__ int64_t plan_size(int num_seqs) { return (16 + 8 * ((int64_t)num_seqs + 1) + 255) / 256 * 256; }
+
+// what a decoding sequence sees: tokens first .. len - 1, in tiles of 32 from tile `tile` on
+struct Span { int first, len, tile, tiles; };
+__device__ __forceinline__ Span span_of(const Cache16AttendLaunch& L, int s) {
+  const int len = seq_tokens(L.c, L.b, s), first = L.window > 0 && len > L.window ? len - L.window : 0;
+  const int tile = first / kDecodeTile;
+  return {first, len, tile, (len + kDecodeTile - 1) / kDecodeTile - tile};
+}
+
+template <int TYPE, int DH, bool TWIN, bool DIFF>
+__global__ __launch_bounds__(256, 2) void cache16_decode_kernel(Cache16AttendLaunch L, float* partials, int64_t* base_of) {
+  constexpr int KS = DH / 32, VD = DH / 16, DPL = DH / 64;          // k-steps; dims of a lane's value rows; of its output
+  constexpr int MAPS = DIFF ? 2 : 1, KM = KS / MAPS;
+  __shared__ float s_ref[4][16], s_sum[4][16];
+  __shared__ float s_acc[4][16][DH + 4];
+  const Cache16& c = L.c;
+  const Cache8Batch& b = L.b;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
+  const int columns = L.gqa * MAPS, parts = col_parts(columns), HV = c.num_kv * parts, n = b.num_seqs;
+
+  // this workgroup's tiles
+  int64_t total = 0;
+  for (int i = lane; i < n; i += kWave) total += span_of(L, i).tiles;
+  total = uniform64(shfl64(wave_scan(total), 63)) * HV;
+  constexpr int64_t kShare = (int64_t)decode_groups(DH) * kDecodeWaves;
+  const int64_t per = total > kShare ? (total + kShare - 1) / kShare * kDecodeWaves : kDecodeWaves;
+  int64_t p = (int64_t)blockIdx.x * per;
+  const int64_t pend = p + per < total ? p + per : total;
+  const bool writes_plan = blockIdx.x == 0 && wave == 3;
+  int s = 0;
+  int64_t sbase = 0;                                  // tile at which sequence s starts
+  if (p < pend || writes_plan) {
+    int64_t before = 0;
+    bool found = false;
+    for (int i0 = 0; i0 < n && (!found || writes_plan); i0 += kWave) {
+      const int i = i0 + lane;
+      const int64_t t = i < n ? (int64_t)span_of(L, i).tiles * HV : 0;
+      const int64_t incl = before + wave_scan(t);
+      if (writes_plan && i < n) base_of[1 + i] = incl - t;
+      const uint64_t past = __ballot(incl > p);
+      if (!found && past) {
+        const int l = __ffsll((unsigned long long)past) - 1;
+        found = true;
+        s = i0 + l;
+        sbase = uniform64(shfl64(incl - t, l));
+      }
+      before = uniform64(shfl64(incl, 63));
+    }
+    if (writes_plan && lane == 0) {
+      base_of[0] = per;
+      base_of[1 + n] = total;
+    }
+  }
+  const float cq = L.sm_scale * kLog2e;
+  const int ps_mask = (1 << c.page_shift) - 1;
+
+  for (; p < pend && s < n; ++s) {
+    const Span sp = span_of(L, s);
+    const int len = uniform(sp.len), first = uniform(sp.first), tile0 = uniform(sp.tile), T = uniform(sp.tiles);
+    if (T == 0) continue;
+    const int32_t* table = b.table + s * b.table_stride;
+    while (p < pend && p < sbase + (int64_t)T * HV) {
+      const int hv = (int)((p - sbase) / T), h = hv / parts, part = hv - h * parts;
+      const int cols = part_cols(columns, part);
+      const int64_t begin = sbase + (int64_t)hv * T;
+      const int t0 = (int)(p - begin), t1 = pend - begin < T ? (int)(pend - begin) : T;
+      const int mycol = TWIN ? (col & 7) : col;
+
+      // a column's query: dims 32 j + 8 g .. in lane group g
+      uintx4 q[KS];
+      {
+        struct __attribute__((packed, aligned(2))) U4 { uintx4 v; };
+        const int mine = part * 16 + (mycol < cols ? mycol : 0);               // (columns over: the first again, dropped at the end)
+        const uint16_t* src = (const uint16_t*)L.q + s * L.q_row + (int64_t)(h * L.gqa + mine / MAPS) * L.q_head + 8 * g;
+#pragma unroll
+        for (int j = 0; j < KS; ++j) q[j] = ((const U4*)(src + 32 * j))->v;
+        // (used here, so that their wait is here: a wait at the first product, inside
+        // the loop, would in every turn be for the loads of the next tile too)
+#pragma unroll
+        for (int j = 0; j < KS; ++j) asm volatile("" : "+v"(q[j]));
+      }
+
+      // page of run `run` (16 tokens) of tile t, or -1
+      auto page_at = [&](int t, int run) {
+        const int at = (tile0 + t) * kDecodeTile + run * 16, blk = at >> c.page_shift, pg = table[min(blk, b.max_blocks - 1)];
+        const int has = (at < len) & (blk < b.max_blocks) & (pg < (int)c.num_pages);   // (no branch around the load)
+        return pg | (has - 1);
+      };
+      uintx4 kx[2][KS];                               // block x: token 8 (col >> 2) + 4 x + (col & 3), dims 32 j + 8 g ..
+      uint32_t vx[8][VD / 2];                         // token 8 g + e, dims VD col ..
+      int vpage;
+      const uint16_t* kh = c.k + h * c.k_head + 8 * g;
+      const uint16_t* vh = c.v + h * c.v_head + VD * col;
+      auto load_k = [&](int t, int page) {
+        const int slot = (((tile0 + t) * kDecodeTile + 16 * (col >> 3)) & ps_mask) + 8 * ((col >> 2) & 1) + (col & 3);
+        const uint16_t* k = kh + (page < 0 ? 0 : page) * c.k_page + slot * c.k_token;
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int j = 0; j < KS; ++j) kx[x][j] = *(const uintx4*)(k + 4 * x * c.k_token + 32 * j);
+      };
+      auto load_v = [&](int t, int page) {
+        const int slot = (((tile0 + t) * kDecodeTile + 16 * (g >> 1)) & ps_mask) + 8 * (g & 1);
+        const uint16_t* v = vh + (page < 0 ? 0 : page) * c.v_page + slot * c.v_token;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if constexpr (VD == 8) {
+            const uintx4 x = *(const uintx4*)(v + e * c.v_token);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) vx[e][i] = x[i];
+          } else {
+            const uintx2 x = *(const uintx2*)(v + e * c.v_token);
+            vx[e][0] = x[0];
+            vx[e][1] = x[1];
+          }
+        }
+        vpage = page;
+      };
+
+      floatx4 acc[VD];
+#pragma unroll
+      for (int d = 0; d < VD; ++d) acc[d] = floatx4{0, 0, 0, 0};
+      float ref = kNoScore, sum = 0.f;
+
+      int t = t0 + wave;
+      int kp1 = 0, vp1 = 0;                           // the pages of the wave's next tile
+      if (t < t1) {
+        const int kp = page_at(t, col >> 3), vp = page_at(t, g >> 1);
+        kp1 = page_at(t + 4, col >> 3);
+        vp1 = page_at(t + 4, g >> 1);
+        load_k(t, kp);
+        __builtin_amdgcn_sched_barrier(0);            // (in the loop's order, for its waits)
+        load_v(t, vp);
+      }
+      for (; t < t1; t += 4) {
+        const int kp2 = page_at(t + 8, col >> 3), vp2 = page_at(t + 8, g >> 1);
+        // scores
+        floatx4 sc[2];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          floatx4 m[MAPS];
+#pragma unroll
+          for (int i = 0; i < MAPS; ++i) {
+            m[i] = floatx4{0, 0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < KM; ++j) m[i] = mfma16<TYPE>(kx[x][i * KM + j], q[i * KM + j], m[i]);
+          }
+          sc[x] = m[0];
+          if constexpr (DIFF)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sc[x][r] = mycol & 1 ? m[MAPS - 1][r] : m[0][r];
+        }
+        if (t + 4 < t1) load_k(t + 4, kp1);
+        // tokens that are not there: behind the length, before the window, of an absent page
+        const int at = (tile0 + t) * kDecodeTile + 8 * g, have = vpage < 0 ? 0 : len - at, cut = first - at;
+        if (__any((have < 8) | (cut > 0))) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const bool there = e < have && e >= cut;
+            sc[e >> 2][e & 3] = there ? sc[e >> 2][e & 3] : -INFINITY;
+#pragma unroll
+            for (int i = 0; i < VD / 2; ++i) vx[e][i] = there ? vx[e][i] : 0u;
+          }
+        }
+        float top = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3]));
+        top = fmaxf(top, fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3]))) * cq;
+        if (__any(top > ref + (kTopWeight + kSlackWeight))) {                 // (each column by its own scores)
+          top = rows_max(top);
+          const float to = top > ref + (kTopWeight + kSlackWeight) ? top - kTopWeight : ref;
+          const float f = exp2_of(ref - to);
+          ref = to;
+          sum *= f;
+#pragma unroll
+          for (int d = 0; d < VD; ++d) acc[d] *= f;
+        }
+        // weights
+        float cw = cq, off = -ref;
+        if (__any((fabsf(ref) > kPlainScore) & (ref > kNoScore))) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) sc[e >> 2][e & 3] = __fsub_rn(__fmul_rn(sc[e >> 2][e & 3], cq), ref);
+          cw = 1.f;
+          off = 0.f;
+        }
+        uintx4 w, rest;                                                       // 16-bit numbers, and what they leave out
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          const float x = exp2_of(fmaf(sc[e >> 2][e & 3], cw, off)), y = exp2_of(fmaf(sc[e >> 2][(e & 3) + 1], cw, off));
+          sum += x + y;
+          const uint32_t hi = pair_of<TYPE>(x, y), lo = pair_of<TYPE>(x - low_of<TYPE>(hi), y - high_of<TYPE>(hi));
+          w[e / 2] = TWIN && col >= 8 ? lo : hi;
+          rest[e / 2] = lo;
+        }
+#pragma unroll
+        for (int d = 0; d < VD; ++d) {
+          uintx4 a;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            a[i] = d & 1 ? highs(vx[2 * i][d / 2], vx[2 * i + 1][d / 2]) : lows(vx[2 * i][d / 2], vx[2 * i + 1][d / 2]);
+          acc[d] = mfma16<TYPE>(a, w, acc[d]);
+          if constexpr (!TWIN) acc[d] = mfma16<TYPE>(a, rest, acc[d]);
+        }
+        if (t + 4 < t1) load_v(t + 4, vp1);
+        kp1 = kp2;
+        vp1 = vp2;
+      }
+
+      // the waves' sums, joined: reference, sum, then acc under the common reference
+      sum = rows_sum(sum);
+      if (g == 0) {
+        s_ref[wave][col] = ref;
+        s_sum[wave][col] = sum;
+      }
+      __syncthreads();
+      const float R = fmaxf(fmaxf(s_ref[0][col], s_ref[1][col]), fmaxf(s_ref[2][col], s_ref[3][col]));
+      const float f = exp2_of(ref - R);
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int d = 0; d < VD; d += 4)                                       // dims VD (4 g + r) + d ..
+          *(floatx4*)&s_acc[wave][col][VD * (4 * g + r) + d] =
+              floatx4{acc[d][r] * f, acc[d + 1][r] * f, acc[d + 2][r] * f, acc[d + 3][r] * f};
+      __syncthreads();
+      const bool whole = t0 == 0 && t1 == T;
+      float* part_out = partials + (2 * (int64_t)blockIdx.x + (t0 == 0)) * partial_size(columns, DH);
+      auto column = [&](int cc) {
+        RowSum<DH> y;
+#pragma unroll
+        for (int i = 0; i < DPL; ++i) {
+          const int d = lane * DPL + i;
+          float o = s_acc[0][cc][d] + s_acc[1][cc][d] + s_acc[2][cc][d] + s_acc[3][cc][d];
+          if constexpr (TWIN) o += s_acc[0][cc + 8][d] + s_acc[1][cc + 8][d] + s_acc[2][cc + 8][d] + s_acc[3][cc + 8][d];
+          y.x[i] = o;
+        }
+        y.R = fmaxf(fmaxf(s_ref[0][cc], s_ref[1][cc]), fmaxf(s_ref[2][cc], s_ref[3][cc]));
+        y.l = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) y.l = fmaf(s_sum[w][cc], exp2_of(s_ref[w][cc] - y.R), y.l);
+        return y;
+      };
+      if (whole) {
+        for (int o = wave; o < cols / MAPS; o += kDecodeWaves) {
+          const int head = h * L.gqa + part * (16 / MAPS) + o;
+          const RowSum<DH> a = column(o * MAPS), bb = DIFF ? column(o * MAPS + MAPS - 1) : a;
+          finish_row<TYPE, DH, DIFF>(L, (int64_t)s * c.num_kv * L.gqa + head, head, a, bb);
+        }
+      } else {
+        for (int cc = wave; cc < cols; cc += kDecodeWaves) {
+          const RowSum<DH> a = column(cc);
+#pragma unroll
+          for (int i = 0; i < DPL; ++i) part_out[32 + cc * DH + lane * DPL + i] = a.x[i];
+          if (lane == 0) {
+            part_out[cc] = a.R;
+            part_out[16 + cc] = a.l;
+          }
+        }
+      }
+      __syncthreads();
+      p = begin + t1;
+    }
+    sbase += (int64_t)T * HV;
+  }
+}
+
+// Joins the partials of each (sequence, kv head) that several workgroups hold,
+// and writes the rows of sequences without a token.  WAVES waves per query head
+// share its partials: four where there are few pairs and many partials of each,
+// one where there are many pairs of one or two.
+template <int TYPE, int DH, bool DIFF, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void cache16_decode_merge_kernel(Cache16AttendLaunch L, const float* partials,
+                                                                  const int64_t* base_of) {
+  constexpr int DPL = DH / 64, MAPS = DIFF ? 2 : 1;
+  __shared__ float s_r[MAPS][WAVES], s_l[MAPS][WAVES], s_a[MAPS][WAVES][DH];
+  const Cache16& c = L.c;
+  const int heads = c.num_kv * L.gqa, s = blockIdx.x / heads, hq = blockIdx.x % heads;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const int columns = L.gqa * MAPS, h = hq / L.gqa, vh = (hq - h * L.gqa) * MAPS, part = vh / 16, cc = vh % 16, parts = col_parts(columns);
+  const int64_t per = base_of[0], a = base_of[1 + s], T = (base_of[2 + s] - a) / (c.num_kv * parts);
+  const int64_t at = (int64_t)s * heads + hq;
+  RowSum<DH> y[2];
+  if (T == 0) {
+    if (wave != 0) return;
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      y[m].l = y[m].R = 0.f;
+#pragma unroll
+      for (int i = 0; i < DPL; ++i) y[m].x[i] = 0.f;
+    }
+    finish_row<TYPE, DH, DIFF>(L, at, hq, y[0], y[1]);
+    return;
+  }
+  const int64_t first = a + (int64_t)(h * parts + part) * T, g0 = first / per, g1 = (first + T - 1) / per;
+  if (g0 == g1) return;
+  const int64_t floats = partial_size(columns, DH);
+#pragma unroll
+  for (int m = 0; m < MAPS; ++m)
+    join<DPL, WAVES == 4 ? 16 : 4>(g0 + wave, g1 + 1, WAVES, 16, [&](int64_t g) {
+      const float* p = partials + (2 * g + (g == g0)) * floats;
+      return Partial{p + cc + m, p + 32 + (cc + m) * DH};
+    }, y[m].R, y[m].l, y[m].x);
+  if constexpr (WAVES > 1) {
+#pragma unroll
+    for (int m = 0; m < MAPS; ++m) {
+      if (lane == 0) {
+        s_r[m][wave] = y[m].R;
+        s_l[m][wave] = y[m].l;
+      }
+#pragma unroll
+      for (int i = 0; i < DPL; ++i) s_a[m][wave][lane * DPL + i] = y[m].x[i];
+    }
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int m = 0; m < MAPS; ++m) {
+      float M = s_r[m][0];
+#pragma unroll
+      for (int w = 1; w < WAVES; ++w) M = fmaxf(M, s_r[m][w]);
+      y[m].R = M;
+      y[m].l = 0.f;
+#pragma unroll
+      for (int i = 0; i < DPL; ++i) y[m].x[i] = 0.f;
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) {
+        const float f = exp2_of(s_r[m][w] - M);
+        y[m].l = fmaf(s_l[m][w], f, y[m].l);
+#pragma unroll
+        for (int i = 0; i < DPL; ++i) y[m].x[i] = fmaf(s_a[m][w][lane * DPL + i], f, y[m].x[i]);
+      }
+    }
+  }
+  finish_row<TYPE, DH, DIFF>(L, at, hq, y[0], y[MAPS - 1]);
+}
+
+// ---- prefill -----------------------------------------------------------------
+//
+// The same sums for many query rows.  A kv head's rows are its gqa heads of each
+// token in turn: a workgroup takes them in tiles, 32 per wave, and walks the tiles
+// of 64 tokens that any of them sees.  A tile's keys and values go from the pages
+// straight into LDS (16 bytes a lane; two buffers, the next tile's bytes are on the
+// way while this one is multiplied), row by row, the 16-byte chunks of a row
+// exclusive-or'ed with the row so that the rows that a read touches at once lie in
+// different banks.  S^T = K Q^T as two 32x32 blocks per wave (v_mfma_f32_32x32x16),
+// O^T += V^T P^T: lane (h, row) holds scores 8 a + 4 h + r of a block, which is its
+// part of the second product's B operand when its part of the A operand is the
+// same tokens: two transposing LDS reads (ds_read_b64_tr_b16) of four tokens by 16
+// dims each.
+//
+// In differential attention the two maps are two groups of waves over the same
+// rows, each with its half of the dims, whose sums meet in LDS at the end.
+//
+// A masked token's weight is 0, but 0 times an infinity or a NaN is not.  Tokens
+// behind the length or of an absent page are read as zeros.  One that some rows of
+// a tile see and others do not keeps its value; tiles with such tokens are looked
+// through, and where a value is not finite it counts as zero in the product and is
+// put, as an infinity or NaN, on the outputs of the rows that see it.
+constexpr int kTileTokens = 64;
+
+// A workgroup's shape: row waves of 32 rows, groups of them, and whether the groups
+// take the tiles in turn.
+struct PrefillShape {
+  int row_waves, groups, at_once;       // at_once: workgroups that run at the same time
+  __host__ __device__ constexpr int row_shift() const { return row_waves == 8 ? 8 : row_waves == 4 ? 7 : 6; }
+};
+__host__ __device__ __forceinline__ PrefillShape prefill_shape(int64_t num_rows, int num_seqs, int gqa, int dh, bool diff) {
+  if (diff) return {4, 2, dh == 64 ? 512 : 256};
+  if (dh == 64) return {4, 1, 768};
+  return num_rows * gqa <= 128 * (int64_t)num_seqs ? PrefillShape{4, 2, 256} : PrefillShape{8, 1, 256};
+}
+constexpr int kSplitLeast = 4;          // tiles of a split
+constexpr int kSplitMost = 64;
+
+__host__ __device__ __forceinline__ int64_t row_tiles(int64_t num_rows, int num_seqs, int gqa, int row_shift) {
+  return ((num_rows * gqa) >> row_shift) + num_seqs;
+}
+// Splits of each row tile: the workgroups at once over the fewest tiles that the
+// rows can make.  The lengths, which the host does not know, have no part in it.
+__host__ __device__ __forceinline__ int prefill_splits(int64_t num_rows, int num_seqs, int num_kv, int gqa, PrefillShape p) {
+  const int64_t whole = (num_rows * gqa) >> p.row_shift(), s = p.at_once / ((whole > num_seqs ? whole : num_seqs) * num_kv);
+  return (int)(s < 1 ? 1 : (s > kSplitMost ? kSplitMost : s));
+}
+// floats of one split's partial: reference and sum per row, then acc[rows][DH];
+// the rows of the second map behind those of the first
+__host__ __device__ __forceinline__ int64_t split_floats(int dh, int rows) { return (int64_t)(dh + 2) * rows; }
+
+// the tokens [lo, hi) that the row of a sequence's new token `tok` of n sees
+struct Sees { int lo, hi; };
+__device__ __forceinline__ Sees row_sees(const Cache16AttendLaunch& L, int len, int n, int tok) {
+  if (!L.causal) return {0, len};
+  const int64_t end = (int64_t)len - n + tok + 1;
+  const int hi = clampi(end, 0, len);
+  return {L.window > 0 ? clampi(end - L.window, 0, hi) : 0, hi};
+}
+// the tiles [first, first + count) that the rows of tokens a .. b see, and the
+// splits that so many are worth
+struct Tiles { int first, count; };
+__device__ __forceinline__ Tiles tiles_of(const Cache16AttendLaunch& L, int len, int n, int a, int b) {
+  const int lo = row_sees(L, len, n, a).lo / kTileTokens, hi = (row_sees(L, len, n, b).hi + kTileTokens - 1) / kTileTokens;
+  return {lo, hi > lo ? hi - lo : 0};
+}
+__device__ __forceinline__ int splits_of(int tiles, int splits) {
+  const int most = tiles / kSplitLeast;
+  return most < 1 ? 1 : (most < splits ? most : splits);
+}
+
+// 16 bytes that tokens which are not there are read from
+__device__ const uint4 kNothing[1] = {{0, 0, 0, 0}};
+
+// 16 bytes a lane from global memory to LDS: lane i's at to + 16 i (`to` uniform)
+__device__ __forceinline__ void copy_to_lds(const void* from, void* to) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)from,
+                                   (__attribute__((address_space(3))) uint32_t*)to, 16, 0, 0);
+}
+
+typedef short short4v __attribute__((ext_vector_type(4)));
+// column i of four rows of 16 numbers, for lane i of 16; lane i points to row i / 4, column 4 (i & 3)
+__device__ __forceinline__ uintx2 read_columns(const uint16_t* p) {
+  return __builtin_bit_cast(uintx2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)p));
+}
+
+// 1, of a 16-bit type
+template <int TYPE> constexpr uint32_t kOne = TYPE == kFp16 ? 0x3C00u : 0x3F80u;
+template <int TYPE> constexpr uint32_t kExponent = TYPE == kFp16 ? 0x7C00u : 0x7F80u;
+// the numbers of a pair that are +inf, -inf or NaN (kind 0, 1, 2) as ones
+template <int TYPE>
+__device__ __forceinline__ uint32_t are_kind(uint32_t p, int kind) {
+  uint32_t r = 0;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t x = (p >> (16 * i)) & 0xFFFFu, a = x & 0x7FFFu;
+    const bool is = kind == 2 ? a > kExponent<TYPE> : a == kExponent<TYPE> && (x >> 15) == (uint32_t)kind;
+    r |= is ? kOne<TYPE> << (16 * i) : 0u;
+  }
+  return r;
+}
+template <int TYPE>
+__device__ __forceinline__ uint32_t finite_or_zero(uint32_t p) {
+  uint32_t keep = 0;
+  if ((p & kExponent<TYPE>) != kExponent<TYPE>) keep |= 0xFFFFu;
+  if ((p >> 16 & kExponent<TYPE>) != kExponent<TYPE>) keep |= 0xFFFF0000u;
+  return p & keep;
+}
+
+template <int TYPE, int DH, int ROW_WAVES, int GROUPS, bool DIFF>
+__global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_kernel(Cache16AttendLaunch L, int splits, float* partials) {
+  constexpr int KS = DH / 16, DB = DH / 32, KM = DIFF ? KS / 2 : KS;  // k-steps, value blocks, k-steps of a map
+  constexpr int WAVES = ROW_WAVES * GROUPS, kRowTile = 32 * ROW_WAVES, RS = ROW_WAVES == 8 ? 8 : ROW_WAVES == 4 ? 7 : 6;
+  constexpr bool kTurns = GROUPS == 2 && !DIFF;
+  constexpr int STEP = kTurns ? 2 : 1;                                // tiles between two barriers
+  constexpr bool kRest = DIFF || TYPE == kFp16;                       // weights as two numbers
+  constexpr int CH = DH / 8, RPL = 64 / CH, TOK = kTileTokens / WAVES * STEP, NL = TOK / RPL;   // chunks of a row; rows a copy;
+                                                                      // a wave's tokens of a step and copies of each kind
+  __shared__ __align__(16) uint16_t s_k[2][STEP][kTileTokens * DH], s_v[2][STEP][kTileTokens * DH];
+  const Cache16& c = L.c;
+  const Cache8Batch& b = L.b;
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), col = lane & 31, half = lane >> 5;
+  // Neighbours take the splits of one row tile, then different heads (unsplit and
+  // eight of them: one per XCD and its L2, which the row tiles of a head share).  The
+  // longest rows of a sequence come first.
+  const uint32_t pair = blockIdx.x / splits;
+  const int h = pair % c.num_kv, z = blockIdx.x % splits, gqa = L.gqa;
+  const int64_t slot = (gridDim.x / splits - 1 - pair) / c.num_kv;
+  const int s = uniform(seq_of_slot(b, slot, gqa, RS, 1));
+  int begin, end;
+  rows_of(b, s, begin, end);
+  begin = uniform(begin);
+  const int n = uniform(end) - begin;
+  const int64_t r0 = (slot - first_slot(b, s, gqa, RS, 1)) * kRowTile, rows_all = (int64_t)n * gqa;
+  if (r0 < 0 || r0 >= rows_all) return;                             // (r0 < 0: row starts that decrease)
+  const int len = uniform(seq_tokens(c, b, s));
+  const int last = (int)((r0 + kRowTile < rows_all ? r0 + kRowTile : rows_all) - 1);
+  const Tiles tiles = tiles_of(L, len, n, (int)(r0 / gqa), last / gqa);
+  const int parts = splits_of(tiles.count, splits);
+  if (z >= parts) return;
+  const int tbeg = tiles.first + (int)((int64_t)tiles.count * z / parts), tend = tiles.first + (int)((int64_t)tiles.count * (z + 1) / parts);
+
+  // this lane's row
+  const int row_wave = wave % ROW_WAVES, group = wave / ROW_WAVES;
+  const int64_t r = r0 + row_wave * 32 + col;
+  const bool live = r < rows_all;
+  const int tok = live ? (int)(r / gqa) : 0, hd = live ? (int)(r - (int64_t)tok * gqa) : 0;
+  const Sees sees = row_sees(L, len, n, tok);
+  const int lo = live ? sees.lo : 0, lim = live ? sees.hi : 0;
+  // tiles that no row of the wave sees, and tiles that all of them see whole
+  int lim_min = live ? lim : 0x7FFFFFFF, lim_max = lim, lo_min = live && lim > 0 ? lo : 0x7FFFFFFF, lo_max = lo;
+#pragma unroll
+  for (int m = 1; m < 32; m <<= 1) {
+    lim_min = min(lim_min, __shfl_xor(lim_min, m, kWave));
+    lim_max = max(lim_max, __shfl_xor(lim_max, m, kWave));
+    lo_min = min(lo_min, __shfl_xor(lo_min, m, kWave));
+    lo_max = max(lo_max, __shfl_xor(lo_max, m, kWave));
+  }
+  lim_min = uniform(lim_min);
+  lim_max = uniform(lim_max);
+  lo_min = uniform(lo_min);
+  lo_max = uniform(lo_max);
+
+  uintx4 q[KM];
+  const int dim0 = DIFF ? group * (DH / 2) : 0;                     // first dim of this wave's map
+  {
+    struct __attribute__((packed, aligned(2))) U4 { uintx4 v; };
+    const uint16_t* src = (const uint16_t*)L.q + (int64_t)(begin + tok) * L.q_row + (int64_t)(h * gqa + hd) * L.q_head + dim0 + 8 * half;
+#pragma unroll
+    for (int i = 0; i < KM; ++i) q[i] = ((const U4*)(src + 16 * i))->v;   // (a lane without a row takes the first: dropped at the end)
+#pragma unroll
+    for (int i = 0; i < KM; ++i) asm volatile("" : "+v"(q[i]));
+  }
+  const float cq = L.sm_scale * kLog2e;
+
+  // A wave's part of a step's tiles: TOK tokens in copies of RPL rows, all of one
+  // run of 16 tokens, whose page is the same for the wave.
+  const int32_t* table = b.table + s * b.table_stride;
+  const uint16_t* kh = c.k + h * c.k_head;
+  const uint16_t* vh = c.v + h * c.v_head;
+  const int ps_mask = (1 << c.page_shift) - 1, last_blk = b.max_blocks - 1;
+  const int ctile = STEP == 2 ? (wave * TOK) / kTileTokens : 0, ctok = (wave * TOK) % kTileTokens;   // of its copies
+  int koff[NL], voff[NL];                                           // elements from the run's first token
+#pragma unroll
+  for (int i = 0; i < NL; ++i) {
+    const int t = ctok + i * RPL + lane / CH, ch = lane % CH;
+    const int kc = DH == 128 ? ch ^ (t & 15) : ch ^ ((t >> 1) & 7), vc = DH == 128 ? ch ^ ((t & 3) << 2) : ch ^ (((t >> 1) & 1) << 2);
+    koff[i] = (t & 15) * c.k_token + 8 * kc;
+    voff[i] = (t & 15) * c.v_token + 8 * vc;
+  }
+  // pages of the runs of tiles t ..: lane i looks up run i & (4 STEP - 1)
+  auto find = [&](int t) {
+    const int at = t * kTileTokens + 16 * (lane & (4 * STEP - 1)), pg = table[min(at >> c.page_shift, last_blk)];
+    return at < len && pg >= 0 && pg < (int)c.num_pages ? pg : -1;
+  };
+  auto fetch = [&](int t, int bf, int found) {
+    const int run = ctile * 4 + ctok / 16, at = t * kTileTokens + 16 * run;
+    const int pg = __builtin_amdgcn_readlane(found, run), have = pg < 0 ? 0 : len - at;
+    const uint16_t* k = kh + (int64_t)max(pg, 0) * c.k_page + (at & ps_mask) * c.k_token;
+    const uint16_t* v = vh + (int64_t)max(pg, 0) * c.v_page + (at & ps_mask) * c.v_token;
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const bool there = ((ctok & 15) + i * RPL + lane / CH) < have;
+      copy_to_lds(there ? (const void*)(k + koff[i]) : (const void*)kNothing, &s_k[bf][ctile][(ctok + i * RPL) * DH]);
+      copy_to_lds(there ? (const void*)(v + voff[i]) : (const void*)kNothing, &s_v[bf][ctile][(ctok + i * RPL) * DH]);
+    }
+  };
+
+  floatx16 acc[DB];
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
+  float ref = kNoScore, sum = 0.f;
+  // LDS elements: key row col, chunk 2 k + half of the map; value row 4 half + (lane & 15) / 4 and its 4 columns
+  const int krow = col * DH, kswz = DH == 128 ? col & 15 : (col >> 1) & 7;
+  const int vrow = (4 * half + ((lane & 15) >> 2)) * DH + 4 * (lane & 1), vchunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+  const int vswz = DH == 128 ? (lane >> 2) & 3 : (lane >> 3) & 1;
+  auto k_at = [&](const uint16_t* tile, int x, int k) {
+    return *(const uintx4*)&tile[32 * x * DH + krow + 8 * ((dim0 / 8 + 2 * k + half) ^ kswz)];
+  };
+  auto v_at = [&](const uint16_t* tile, int u, int d) {
+    const uint16_t* p = &tile[16 * u * DH + vrow + 8 * (4 * (d ^ vswz) + vchunk)];
+    const uintx2 x = read_columns(p), y = read_columns(p + 8 * DH);
+    return uintx4{x[0], x[1], y[0], y[1]};
+  };
+
+  // tile t by this wave, from its buffer; present: a bit for each run that has a page
+  auto attend = [&](int t, const uint16_t* kt, const uint16_t* vt, uint32_t present) {
+    const int t0 = t * kTileTokens;
+    floatx16 sc[2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sc[x][i] = 0.f;
+#pragma unroll
+      for (int k = 0; k < KM; ++k) sc[x] = mfma32<TYPE>(k_at(kt, x, k), q[k], sc[x]);
+    }
+    const bool masked = t0 + kTileTokens > lim_min || t0 < lo_max || present != 15u;
+    bool odd = false;                                               // a value that is not finite, in such a tile
+    if (masked) {
+#pragma unroll
+      for (int e = 0; e < 32; ++e) {
+        const int at = 32 * (e >> 4) + 8 * ((e >> 2) & 3) + (e & 3), token = t0 + at + 4 * half;
+        const bool there = token < lim && token >= lo && (present >> (at >> 4) & 1);
+        sc[e >> 4][e & 15] = there ? sc[e >> 4][e & 15] : -INFINITY;
+      }
+      uint32_t bad = 0;
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int d = 0; d < DB; ++d) {
+          const uintx4 a = v_at(vt, u, d);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) bad |= finite_or_zero<TYPE>(a[i]) ^ a[i];
+        }
+      odd = __any(bad != 0);
+    }
+    float top = sc[0][0];
+#pragma unroll
+    for (int e = 1; e < 32; ++e) top = fmaxf(top, sc[e >> 4][e & 15]);
+    top *= cq;
+    if (__any(top > ref + (kTopWeight + kSlackWeight))) {           // (each row by its own scores)
+      top = halves_max(top);
+      const float to = top > ref + (kTopWeight + kSlackWeight) ? top - kTopWeight : ref;
+      const float f = exp2_of(ref - to);
+      ref = to;
+      sum *= f;
+#pragma unroll
+      for (int d = 0; d < DB; ++d) acc[d] *= f;
+    }
+    float cw = cq, off = -ref;
+    if (__any((fabsf(ref) > kPlainScore) & (ref > kNoScore))) {
+#pragma unroll
+      for (int e = 0; e < 32; ++e) sc[e >> 4][e & 15] = __fsub_rn(__fmul_rn(sc[e >> 4][e & 15], cq), ref);
+      cw = 1.f;
+      off = 0.f;
+    }
+    uintx4 w[4], rest[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) {
+        const float x = exp2_of(fmaf(sc[u >> 1][8 * (u & 1) + i], cw, off));
+        const float y = exp2_of(fmaf(sc[u >> 1][8 * (u & 1) + i + 1], cw, off));
+        sum += x;
+        sum += y;
+        w[u][i / 2] = pair_of<TYPE>(x, y);
+        if constexpr (kRest) rest[u][i / 2] = pair_of<TYPE>(x - low_of<TYPE>(w[u][i / 2]), y - high_of<TYPE>(w[u][i / 2]));
+      }
+    if (!odd) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int d = 0; d < DB; ++d) {
+          const uintx4 a = v_at(vt, u, d);
+          acc[d] = mfma32<TYPE>(a, w[u], acc[d]);
+          if constexpr (kRest) acc[d] = mfma32<TYPE>(a, rest[u], acc[d]);
+        }
+    } else {
+      // rows that see a token: ones; then how many infinities and NaN each output has
+      uintx4 one[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float x = sc[u >> 1][8 * (u & 1) + 2 * i], y = sc[u >> 1][8 * (u & 1) + 2 * i + 1];
+          one[u][i] = (x == -INFINITY ? 0u : kOne<TYPE>) | (y == -INFINITY ? 0u : kOne<TYPE> << 16);
+        }
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          uintx4 a = v_at(vt, u, d);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) a[i] = finite_or_zero<TYPE>(a[i]);
+          acc[d] = mfma32<TYPE>(a, w[u], acc[d]);
+          if constexpr (kRest) acc[d] = mfma32<TYPE>(a, rest[u], acc[d]);
+        }
+#pragma unroll 1
+        for (int kind = 0; kind < 3; ++kind) {
+          floatx16 count;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) count[i] = 0.f;
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            uintx4 a = v_at(vt, u, d);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) a[i] = are_kind<TYPE>(a[i], kind);
+            count = mfma32<TYPE>(a, one[u], count);
+          }
+          const float what = kind == 0 ? INFINITY : kind == 1 ? -INFINITY : __builtin_nanf("");
+#pragma unroll
+          for (int i = 0; i < 16; ++i) acc[d][i] += count[i] > 0.f ? what : 0.f;
+        }
+      }
+    }
+  };
+
+  if (tbeg < tend) {
+    int found = find(tbeg);
+    fetch(tbeg, 0, found);
+    int next = find(tbeg + STEP);
+    for (int t = tbeg; t < tend; t += 2 * STEP) {
+#pragma unroll
+      for (int bf = 0; bf < 2; ++bf) {
+        const int tt = t + bf * STEP;
+        if (tt < tend) {
+          // this step's bytes have arrived, for every wave; the other buffer is read no more
+          __builtin_amdgcn_s_waitcnt(0x0F70);                       // vmcnt(0)
+          __syncthreads();
+          const uint32_t present = (uint32_t)__ballot(found >= 0) & ((1u << 4 * STEP) - 1);
+          if (tt + STEP < tend) fetch(tt + STEP, 1 - bf, next);
+          found = next;
+          next = find(tt + 2 * STEP);
+          const int mine = kTurns ? group : 0, at = (tt + mine) * kTileTokens;
+          if (tt + mine < tend && at < lim_max && at + kTileTokens > lo_min)
+            attend(tt + mine, s_k[bf][mine], s_v[bf][mine], present >> (4 * mine) & 15u);
+        }
+      }
+    }
+  }
+
+  sum = halves_sum(sum);
+  float lam = 0.f, ref2 = 0.f, sum2 = 0.f;
+  if constexpr (GROUPS == 2) {                                        // the second group's sums, through LDS, to the first
+    float* o = (float*)s_k;                                           // [DH / 4][kRowTile][4]
+    float* rs = (float*)s_v;                                          // references, sums
+    const int row = row_wave * 32 + col;
+    constexpr int ROUNDS = sizeof(s_k) >= sizeof(float) * kRowTile * DH ? 1 : 2, DR = DB / ROUNDS;
+    static_assert(sizeof(s_k) * ROUNDS >= sizeof(float) * kRowTile * DH && sizeof(s_v) >= sizeof(float) * 2 * kRowTile, "");
+    const bool whole = DIFF && parts == 1;
+#pragma unroll
+    for (int round = 0; round < ROUNDS; ++round) {
+      __syncthreads();                                                // (the last tile, or the last round, is read no more)
+      if (group == 1 && (!DIFF || whole)) {
+        if (half == 0) {
+          rs[row] = ref;
+          rs[kRowTile + row] = sum;
+        }
+#pragma unroll
+        for (int d = 0; d < DR; ++d)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const floatx16& x = acc[round * DR + d];
+            *(floatx4*)&o[((8 * d + 2 * i + half) * kRowTile + row) * 4] = floatx4{x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]};
+          }
+      }
+      __syncthreads();
+      if (group == 0 && (!DIFF || whole)) {
+        const float other = rs[row], osum = rs[kRowTile + row];
+        float f, g;
+        if constexpr (DIFF) {
+          lam = L.lambda[h * gqa + hd];
+          f = round > 0 ? 1.f : sum == 0.f ? 0.f : 1.0f / sum;       // (all blocks at once, in the first round)
+          g = osum == 0.f ? 0.f : -lam / osum;
+          ref2 = other;
+          sum2 = osum;
+          if (round == 0)
+#pragma unroll
+            for (int d = 0; d < DB; ++d) acc[d] *= f;
+          f = 1.f;
+        } else {
+          const float R = fmaxf(ref, other);
+          f = exp2_of(ref - R);
+          g = exp2_of(other - R);
+          if (round == ROUNDS - 1) {
+            ref = R;
+            sum = fmaf(sum, f, osum * g);
+          }
+        }
+#pragma unroll
+        for (int d = 0; d < DR; ++d)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const floatx4 x = *(const floatx4*)&o[((8 * d + 2 * i + half) * kRowTile + row) * 4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[round * DR + d][4 * i + e] = fmaf(acc[round * DR + d][4 * i + e], f, x[e] * g);
+          }
+      }
+    }
+    if (group == 1 && (!DIFF || whole)) return;
+  }
+  if (!live) return;
+  const int head = h * gqa + hd;
+  const int64_t at = (int64_t)(begin + tok) * c.num_kv * gqa + head;
+  if (parts == 1) {
+    if constexpr (DIFF) {
+      if (L.norm_weight) {
+        float sq = 0.f;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sq = fmaf(acc[d][i], acc[d][i], sq);
+        const float scale = sum == 0.f ? 0.f : 1.0f / __builtin_sqrtf(fmaf(halves_sum(sq), 1.0f / DH, L.norm_eps));
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) acc[d][i] *= scale * L.norm_weight[32 * d + 8 * (i >> 2) + 4 * half + (i & 3)];
+      }
+    } else {
+      const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+#pragma unroll
+      for (int d = 0; d < DB; ++d) acc[d] *= inv;
+    }
+    const bool none = sum == 0.f;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        struct __attribute__((packed, aligned(2))) U2 { uintx2 v; };
+        const uint32_t x = pair_of<TYPE>(acc[d][4 * i], acc[d][4 * i + 1]), y = pair_of<TYPE>(acc[d][4 * i + 2], acc[d][4 * i + 3]);
+        ((U2*)((uint16_t*)L.out + at * DH + 32 * d + 8 * i + 4 * half))->v = none ? uintx2{0, 0} : uintx2{x, y};
+      }
+    if (L.lse && half == 0) {
+      const float e = none ? -INFINITY : (ref + log2_of(sum)) * kLn2;
+      if constexpr (DIFF) {
+        L.lse[2 * at] = e;
+        L.lse[2 * at + 1] = sum2 == 0.f ? -INFINITY : (ref2 + log2_of(sum2)) * kLn2;
+      } else {
+        L.lse[at] = e;
+      }
+    }
+  } else {
+    constexpr int rows = DIFF ? 2 * kRowTile : kRowTile;
+    float* o = partials + ((slot * c.num_kv + h) * splits + z) * split_floats(DH, rows);
+    const int row = (DIFF ? group * kRowTile : 0) + row_wave * 32 + col;
+    if (half == 0) {
+      o[row] = ref;
+      o[rows + row] = sum;
+    }
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *(floatx4*)&o[2 * rows + row * DH + 32 * d + 8 * i + 4 * half] =
+            floatx4{acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]};
+  }
+}
+
+// Joins the splits of each row; one wave per (row, query head).
+template <int TYPE, int DH, bool DIFF>
+__global__ __launch_bounds__(256) void cache16_prefill_merge_kernel(Cache16AttendLaunch L, int RS, int splits,
+                                                                    const float* partials) {
+  constexpr int DPL = DH / 64, MAPS = DIFF ? 2 : 1;
+  const int kRowTile = 1 << RS, rows = MAPS * kRowTile;
+  const Cache16& c = L.c;
+  const Cache8Batch& b = L.b;
+  const int heads = c.num_kv * L.gqa;
+  const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), row = at / heads;
+  if (row >= b.num_rows) return;
+  const int hq = (int)(at - row * heads), h = hq / L.gqa;
+  const int s = seq_of_slot(b, row, 1, 0, 0);
+  int begin, end;
+  rows_of(b, s, begin, end);
+  if (row < begin || row >= end) return;
+  const int n = end - begin, len = seq_tokens(c, b, s);
+  const int64_t r = (row - begin) * L.gqa + hq - h * L.gqa, rows_all = (int64_t)n * L.gqa, r0 = r & ~(int64_t)(kRowTile - 1);
+  const int last = (int)((r0 + kRowTile < rows_all ? r0 + kRowTile : rows_all) - 1);
+  const int parts = splits_of(tiles_of(L, len, n, (int)(r0 / L.gqa), last / L.gqa).count, splits);
+  if (parts == 1) return;
+  const int64_t slot = first_slot(b, s, L.gqa, RS, 1) + (r >> RS);
+  const int in = (int)(r & (kRowTile - 1));
+  const float* x = partials + (slot * c.num_kv + h) * splits * split_floats(DH, rows);
+  RowSum<DH> y[2];
+#pragma unroll
+  for (int m = 0; m < MAPS; ++m)
+    join<DPL, 16>(0, parts, 1, rows, [&](int64_t z) {
+      const float* p = x + z * split_floats(DH, rows) + m * kRowTile;
+      return Partial{p + in, x + z * split_floats(DH, rows) + 2 * rows + (m * kRowTile + in) * DH};
+    }, y[m].R, y[m].l, y[m].x);
+  finish_row<TYPE, DH, DIFF>(L, at, hq, y[0], y[MAPS - 1]);
+}
+
+// ---- launches ------------------------------------------------------------------
+
+int launched() { return hipPeekAtLastError() == hipSuccess ? 0 : -1; }
+
+template <int IN, int OUT, int DH>
+int append(const Cache16AppendLaunch& L, hipStream_t st) {
+  constexpr int HEADS = 64 / (DH / 16);
+  const int heads = L.c.num_kv * (L.gqa + 2), most = (heads + HEADS - 1) / HEADS;
+  const int64_t want = (2048 + L.b.num_rows - 1) / L.b.num_rows;     // waves of a row: eight per CU in all, if it has as many
+  const int splits = (int)(want < most ? want : most);
+  const uint32_t items = (uint32_t)(L.b.num_rows * splits);
+  cache16_append_kernel<IN, OUT, DH><<<(items + 3) / 4, 256, 0, st>>>(L, items, splits);
+  return launched();
+}
+
+template <int TYPE, int DH, bool DIFF>
+int decode(const Cache16AttendLaunch& L, hipStream_t st) {
+  int64_t* plan = (int64_t*)L.ws;
+  float* partials = (float*)((uint8_t*)L.ws + plan_size(L.b.num_seqs));
+  const int columns = L.gqa * (DIFF ? 2 : 1);
+  if (columns <= 8) cache16_decode_kernel<TYPE, DH, true, DIFF><<<decode_groups(DH), 256, 0, st>>>(L, partials, plan);
+  else cache16_decode_kernel<TYPE, DH, false, DIFF><<<decode_groups(DH), 256, 0, st>>>(L, partials, plan);
+  const int heads = L.b.num_seqs * L.c.num_kv * L.gqa;
+  if (L.b.num_seqs * L.c.num_kv * col_parts(columns) < 128)
+    cache16_decode_merge_kernel<TYPE, DH, DIFF, 4><<<heads, 256, 0, st>>>(L, partials, plan);
+  else
+    cache16_decode_merge_kernel<TYPE, DH, DIFF, 1><<<heads, 64, 0, st>>>(L, partials, plan);
+  return launched();
+}
+
+template <int TYPE, int DH, bool DIFF>
+int prefill(const Cache16AttendLaunch& L, hipStream_t st) {
+  const PrefillShape shape = prefill_shape(L.b.num_rows, L.b.num_seqs, L.gqa, DH, DIFF);
+  const int64_t tiles = row_tiles(L.b.num_rows, L.b.num_seqs, L.gqa, shape.row_shift());
+  const int splits = prefill_splits(L.b.num_rows, L.b.num_seqs, L.c.num_kv, L.gqa, shape);
+  const unsigned grid = (unsigned)(tiles * L.c.num_kv * splits);
+  float* ws = (float*)L.ws;
+  if constexpr (DIFF) {
+    cache16_prefill_kernel<TYPE, DH, 4, 2, true><<<grid, 512, 0, st>>>(L, splits, ws);
+  } else if constexpr (DH == 128) {
+    if (shape.groups == 2) cache16_prefill_kernel<TYPE, DH, 4, 2, false><<<grid, 512, 0, st>>>(L, splits, ws);
+    else cache16_prefill_kernel<TYPE, DH, 8, 1, false><<<grid, 512, 0, st>>>(L, splits, ws);
+  } else {
+    cache16_prefill_kernel<TYPE, DH, 4, 1, false><<<grid, 256, 0, st>>>(L, splits, ws);
+  }
+  if (splits > 1) {
+    const int64_t waves = L.b.num_rows * L.c.num_kv * L.gqa;
+    cache16_prefill_merge_kernel<TYPE, DH, DIFF><<<(unsigned)((waves + 3) / 4), 256, 0, st>>>(L, shape.row_shift(), splits, ws);
+  }
+  return launched();
+}
+
+template <int TYPE, int DH, bool DIFF>
+int attend(const Cache16AttendLaunch& L, hipStream_t st) {
+  return L.b.cu ? prefill<TYPE, DH, DIFF>(L, st) : decode<TYPE, DH, DIFF>(L, st);
+}
+
+}  // namespace
+
+int launch_cache16_append(const Cache16AppendLaunch& L, hipStream_t stream) {
+#define SPHKV_PICK(I, O, D) if (L.type == I && L.c.type == O && L.c.dh == D) return append<I, O, D>(L, stream)
+  SPHKV_PICK(kFp16, kFp16, 64); SPHKV_PICK(kFp16, kFp16, 128); SPHKV_PICK(kFp16, kBf16, 64); SPHKV_PICK(kFp16, kBf16, 128);
+  SPHKV_PICK(kBf16, kFp16, 64); SPHKV_PICK(kBf16, kFp16, 128); SPHKV_PICK(kBf16, kBf16, 64); SPHKV_PICK(kBf16, kBf16, 128);
+  SPHKV_PICK(kFp32, kFp16, 64); SPHKV_PICK(kFp32, kFp16, 128); SPHKV_PICK(kFp32, kBf16, 64); SPHKV_PICK(kFp32, kBf16, 128);
+#undef SPHKV_PICK
+  return -1;
+}
+int launch_cache16_attend(const Cache16AttendLaunch& L, hipStream_t stream) {
+#define SPHKV_PICK(T, D, X) if (L.c.type == T && L.c.dh == D && (L.lambda != nullptr) == X) return attend<T, D, X>(L, stream)
+  SPHKV_PICK(kFp16, 64, false); SPHKV_PICK(kFp16, 128, false); SPHKV_PICK(kBf16, 64, false); SPHKV_PICK(kBf16, 128, false);
+  SPHKV_PICK(kFp16, 64, true); SPHKV_PICK(kFp16, 128, true); SPHKV_PICK(kBf16, 64, true); SPHKV_PICK(kBf16, 128, true);
+#undef SPHKV_PICK
+  return -1;
+}
+int64_t cache16_decode_ws_bytes(int32_t num_seqs, int32_t, int32_t gqa, int32_t dh, bool diff) {
+  return plan_size(num_seqs) + 2 * decode_groups(dh) * 4 * partial_size(gqa * (diff ? 2 : 1), dh);
+}
+int64_t cache16_prefill_ws_bytes(int64_t num_rows, int32_t num_seqs, int32_t num_kv, int32_t gqa, int32_t dh, bool diff) {
+  if (num_rows == 0 || num_seqs == 0) return 0;
+  const PrefillShape p = prefill_shape(num_rows, num_seqs, gqa, dh, diff);
+  const int splits = prefill_splits(num_rows, num_seqs, num_kv, gqa, p);
+  const int rows = (diff ? 2 : 1) << p.row_shift();
+  return splits == 1 ? 0 : row_tiles(num_rows, num_seqs, gqa, p.row_shift()) * num_kv * splits * split_floats(dh, rows) * 4;
+}
+
+}  // namespace sphkv

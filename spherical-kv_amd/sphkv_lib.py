@@ -89,7 +89,24 @@ SIGNATURES = {
     "sphkv_cache8_prefill_workspace_bytes": (I64, [I64, I32, I32, I32, I32]),
     "sphkv_cache8_prefill": (ctypes.c_int, [P, I32, I64, I64, I64, P, P, I32, P, I64, I32, I32, P, P, P, I64, I32, I32,
                                             I32, I32, I32, F32, P, P, P, I64, P]),
+    "sphkv_cache16_append": (ctypes.c_int, [P, P, P, P, I32, I64, I64, I64, I64, I64, I64, I32, P, I64, I64, I64, P, P,
+                                            P, I64, I32, I32, P, I32, I32, I32, I32, P]),
+    "sphkv_cache16_decode_workspace_bytes": (I64, [I32, I32, I32, I32, I32]),
+    "sphkv_cache16_decode": (ctypes.c_int, [P, P, I64, I64, I32, P, I32, P, I64, I32, I32, F32, P, P, P, I64, P]),
+    "sphkv_cache16_diff_decode": (ctypes.c_int, [P, P, I64, I64, I32, P, P, F32, P, I32, P, I64, I32, I32, F32, P, P, P,
+                                                 I64, P]),
+    "sphkv_cache16_prefill_workspace_bytes": (I64, [I64, I32, I32, I32, I32, I32]),
+    "sphkv_cache16_prefill": (ctypes.c_int, [P, P, I64, I64, I32, I64, P, P, I32, I32, P, I64, I32, I32, F32, P, P, P,
+                                             I64, P]),
+    "sphkv_cache16_diff_prefill": (ctypes.c_int, [P, P, I64, I64, I32, P, P, F32, I64, P, P, I32, I32, P, I64, I32, I32,
+                                                  F32, P, P, P, I64, P]),
 }
+
+
+class Cache16Struct(ctypes.Structure):
+    """sphkv_cache16"""
+    _fields_ = [("k", P), ("v", P), ("k_page", I64), ("k_head", I64), ("k_token", I64), ("v_page", I64), ("v_head", I64),
+                ("v_token", I64), ("num_pages", I64), ("num_kv", I32), ("dh", I32), ("page_size", I32), ("type", I32)]
 
 
 class SphkvError(RuntimeError):
