@@ -610,10 +610,9 @@ __global__ __launch_bounds__(64 * WAVES) void cache16_decode_merge_kernel(Cache1
 // rows, each with its half of the dims, whose sums meet in LDS at the end.
 //
 // A masked token's weight is 0, but 0 times an infinity or a NaN is not.  Tokens
-// behind the length or of an absent page are read as zeros.  One that some rows of
-// a tile see and others do not keeps its value; tiles with such tokens are looked
-// through, and where a value is not finite it counts as zero in the product and is
-// put, as an infinity or NaN, on the outputs of the rows that see it.
+// behind the length or of an absent page are read as zeros.  In a tile that some
+// rows see in part, values that are not finite count as zeros in the product, and
+// are added at the end to the outputs of the rows that see them.
 constexpr int kTileTokens = 64;
 
 // A workgroup's shape: row waves of 32 rows, groups of them, and whether the groups
@@ -663,13 +662,16 @@ __device__ __forceinline__ int splits_of(int tiles, int splits) {
   return most < 1 ? 1 : (most < splits ? most : splits);
 }
 
-// 16 bytes that tokens which are not there are read from
-__device__ const uint4 kNothing[1] = {{0, 0, 0, 0}};
-
-// 16 bytes a lane from global memory to LDS: lane i's at to + 16 i (`to` uniform)
-__device__ __forceinline__ void copy_to_lds(const void* from, void* to) {
-  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)from,
-                                   (__attribute__((address_space(3))) uint32_t*)to, 16, 0, 0);
+// 16 bytes a lane from global memory (`base` uniform) to LDS: lane i's at to + 16 i.
+// As an instruction of its own, so that the compiler does not wait for it at the
+// next LDS read, which is of another buffer: whoever reads these bytes waits for
+// vmcnt first.  (M0 is read one wait state after it is written.)
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)p;
+}
+__device__ __forceinline__ void copy_to_lds(const void* base, uint32_t offset, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+               :: "v"(offset), "s"(base), "s"(uniform((int)to)) : "memory", "m0");
 }
 
 typedef short short4v __attribute__((ext_vector_type(4)));
@@ -678,27 +680,26 @@ __device__ __forceinline__ uintx2 read_columns(const uint16_t* p) {
   return __builtin_bit_cast(uintx2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)p));
 }
 
-// 1, of a 16-bit type
-template <int TYPE> constexpr uint32_t kOne = TYPE == kFp16 ? 0x3C00u : 0x3F80u;
-template <int TYPE> constexpr uint32_t kExponent = TYPE == kFp16 ? 0x7C00u : 0x7F80u;
-// the numbers of a pair that are +inf, -inf or NaN (kind 0, 1, 2) as ones
-template <int TYPE>
-__device__ __forceinline__ uint32_t are_kind(uint32_t p, int kind) {
-  uint32_t r = 0;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const uint32_t x = (p >> (16 * i)) & 0xFFFFu, a = x & 0x7FFFu;
-    const bool is = kind == 2 ? a > kExponent<TYPE> : a == kExponent<TYPE> && (x >> 15) == (uint32_t)kind;
-    r |= is ? kOne<TYPE> << (16 * i) : 0u;
-  }
-  return r;
-}
+// the numbers of a pair that are finite, zeros in the place of others
 template <int TYPE>
 __device__ __forceinline__ uint32_t finite_or_zero(uint32_t p) {
+  constexpr uint32_t kExponent = TYPE == kFp16 ? 0x7C00u : 0x7F80u;
   uint32_t keep = 0;
-  if ((p & kExponent<TYPE>) != kExponent<TYPE>) keep |= 0xFFFFu;
-  if ((p >> 16 & kExponent<TYPE>) != kExponent<TYPE>) keep |= 0xFFFF0000u;
+  if ((p & kExponent) != kExponent) keep |= 0xFFFFu;
+  if ((p & kExponent << 16) != kExponent << 16) keep |= 0xFFFF0000u;
   return p & keep;
+}
+
+// N groups of R LDS reads that feed M matrix instructions each: AHEAD groups in flight
+template <int N, int R, int M, int AHEAD>
+__device__ __forceinline__ void groups_ahead() {
+  __builtin_amdgcn_sched_group_barrier(0x100, AHEAD * R, 0);
+#pragma unroll
+  for (int i = 0; i < N - AHEAD; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, M, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, R, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(0x008, AHEAD * M, 0);
 }
 
 template <int TYPE, int DH, int ROW_WAVES, int GROUPS, bool DIFF>
@@ -774,29 +775,43 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
   const uint16_t* vh = c.v + h * c.v_head;
   const int ps_mask = (1 << c.page_shift) - 1, last_blk = b.max_blocks - 1;
   const int ctile = STEP == 2 ? (wave * TOK) / kTileTokens : 0, ctok = (wave * TOK) % kTileTokens;   // of its copies
-  int koff[NL], voff[NL];                                           // elements from the run's first token
+  uint32_t koff[NL], voff[NL];                                      // bytes from the run's first token
 #pragma unroll
   for (int i = 0; i < NL; ++i) {
     const int t = ctok + i * RPL + lane / CH, ch = lane % CH;
     const int kc = DH == 128 ? ch ^ (t & 15) : ch ^ ((t >> 1) & 7), vc = DH == 128 ? ch ^ ((t & 3) << 2) : ch ^ (((t >> 1) & 1) << 2);
-    koff[i] = (t & 15) * c.k_token + 8 * kc;
-    voff[i] = (t & 15) * c.v_token + 8 * vc;
+    koff[i] = 2 * ((t & 15) * c.k_token + 8 * kc);
+    voff[i] = 2 * ((t & 15) * c.v_token + 8 * vc);
   }
-  // pages of the runs of tiles t ..: lane i looks up run i & (4 STEP - 1)
-  auto find = [&](int t) {
-    const int at = t * kTileTokens + 16 * (lane & (4 * STEP - 1)), pg = table[min(at >> c.page_shift, last_blk)];
-    return at < len && pg >= 0 && pg < (int)c.num_pages ? pg : -1;
-  };
+  // pages of the runs of tiles t ..: lane i looks up run i & (4 STEP - 1); what it finds
+  // is looked at a step later, when it has arrived
+  const int my_run = 16 * (lane & (4 * STEP - 1));
+  auto find = [&](int t) { return table[min((t * kTileTokens + my_run) >> c.page_shift, last_blk)]; };
+  auto valid = [&](int t, int pg) { return t * kTileTokens + my_run < len && pg < (int)c.num_pages ? pg : -1; };
   auto fetch = [&](int t, int bf, int found) {
     const int run = ctile * 4 + ctok / 16, at = t * kTileTokens + 16 * run;
     const int pg = __builtin_amdgcn_readlane(found, run), have = pg < 0 ? 0 : len - at;
     const uint16_t* k = kh + (int64_t)max(pg, 0) * c.k_page + (at & ps_mask) * c.k_token;
     const uint16_t* v = vh + (int64_t)max(pg, 0) * c.v_page + (at & ps_mask) * c.v_token;
+    uint16_t* kt = &s_k[bf][ctile][ctok * DH];
+    uint16_t* vt = &s_v[bf][ctile][ctok * DH];
+    if (have >= (ctok & 15) + TOK) {
 #pragma unroll
-    for (int i = 0; i < NL; ++i) {
-      const bool there = ((ctok & 15) + i * RPL + lane / CH) < have;
-      copy_to_lds(there ? (const void*)(k + koff[i]) : (const void*)kNothing, &s_k[bf][ctile][(ctok + i * RPL) * DH]);
-      copy_to_lds(there ? (const void*)(v + voff[i]) : (const void*)kNothing, &s_v[bf][ctile][(ctok + i * RPL) * DH]);
+      for (int i = 0; i < NL; ++i) {
+        copy_to_lds(k, koff[i], lds_address(kt + i * RPL * DH));
+        copy_to_lds(v, voff[i], lds_address(vt + i * RPL * DH));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NL; ++i) {
+        if ((ctok & 15) + i * RPL + lane / CH < have) {
+          copy_to_lds(k, koff[i], lds_address(kt + i * RPL * DH));
+          copy_to_lds(v, voff[i], lds_address(vt + i * RPL * DH));
+        } else {
+          *(uintx4*)(kt + i * RPL * DH + 8 * lane) = uintx4{0, 0, 0, 0};
+          *(uintx4*)(vt + i * RPL * DH + 8 * lane) = uintx4{0, 0, 0, 0};
+        }
+      }
     }
   };
 
@@ -819,6 +834,9 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
     return uintx4{x[0], x[1], y[0], y[1]};
   };
 
+  // a tile that some rows of the wave see in part
+  auto partial = [&](int t) { return (t + 1) * kTileTokens > lim_min || t * kTileTokens < lo_max; };
+  uint32_t odd = 0;                                                 // not 0: such a tile had a value that is not finite
   // tile t by this wave, from its buffer; present: a bit for each run that has a page
   auto attend = [&](int t, const uint16_t* kt, const uint16_t* vt, uint32_t present) {
     const int t0 = t * kTileTokens;
@@ -830,25 +848,19 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
 #pragma unroll
       for (int k = 0; k < KM; ++k) sc[x] = mfma32<TYPE>(k_at(kt, x, k), q[k], sc[x]);
     }
-    const bool masked = t0 + kTileTokens > lim_min || t0 < lo_max || present != 15u;
-    bool odd = false;                                               // a value that is not finite, in such a tile
-    if (masked) {
+    groups_ahead<2 * KM, 1, 1, KM < 6 ? KM : 6>();
+    const bool cut = partial(t);
+    if (cut || present != 15u) {
+      const uint32_t first = t0 + 4 * half - lo, width = lim - lo;
 #pragma unroll
-      for (int e = 0; e < 32; ++e) {
-        const int at = 32 * (e >> 4) + 8 * ((e >> 2) & 3) + (e & 3), token = t0 + at + 4 * half;
-        const bool there = token < lim && token >= lo && (present >> (at >> 4) & 1);
-        sc[e >> 4][e & 15] = there ? sc[e >> 4][e & 15] : -INFINITY;
-      }
-      uint32_t bad = 0;
+      for (int u = 0; u < 4; ++u) {
+        const uint32_t w = present >> u & 1 ? width : 0u;
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
-#pragma unroll
-        for (int d = 0; d < DB; ++d) {
-          const uintx4 a = v_at(vt, u, d);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) bad |= finite_or_zero<TYPE>(a[i]) ^ a[i];
+        for (int i = 0; i < 8; ++i) {
+          const int e = 8 * (u & 1) + i;
+          sc[u >> 1][e] = first + (16 * u + 8 * (i >> 2) + (i & 3)) < w ? sc[u >> 1][e] : -INFINITY;
         }
-      odd = __any(bad != 0);
+      }
     }
     float top = sc[0][0];
 #pragma unroll
@@ -882,7 +894,7 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
         w[u][i / 2] = pair_of<TYPE>(x, y);
         if constexpr (kRest) rest[u][i / 2] = pair_of<TYPE>(x - low_of<TYPE>(w[u][i / 2]), y - high_of<TYPE>(w[u][i / 2]));
       }
-    if (!odd) {
+    if (!cut) {
 #pragma unroll
       for (int u = 0; u < 4; ++u)
 #pragma unroll
@@ -891,50 +903,29 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
           acc[d] = mfma32<TYPE>(a, w[u], acc[d]);
           if constexpr (kRest) acc[d] = mfma32<TYPE>(a, rest[u], acc[d]);
         }
+      groups_ahead<4 * DB, 2, kRest ? 2 : 1, DB < 4 ? DB : 4>();
     } else {
-      // rows that see a token: ones; then how many infinities and NaN each output has
-      uintx4 one[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float x = sc[u >> 1][8 * (u & 1) + 2 * i], y = sc[u >> 1][8 * (u & 1) + 2 * i + 1];
-          one[u][i] = (x == -INFINITY ? 0u : kOne<TYPE>) | (y == -INFINITY ? 0u : kOne<TYPE> << 16);
-        }
-#pragma unroll
-      for (int d = 0; d < DB; ++d) {
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
+        for (int d = 0; d < DB; ++d) {
           uintx4 a = v_at(vt, u, d);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) a[i] = finite_or_zero<TYPE>(a[i]);
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t x = finite_or_zero<TYPE>(a[i]);
+            odd |= x ^ a[i];
+            a[i] = x;
+          }
           acc[d] = mfma32<TYPE>(a, w[u], acc[d]);
           if constexpr (kRest) acc[d] = mfma32<TYPE>(a, rest[u], acc[d]);
         }
-#pragma unroll 1
-        for (int kind = 0; kind < 3; ++kind) {
-          floatx16 count;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) count[i] = 0.f;
-#pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            uintx4 a = v_at(vt, u, d);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) a[i] = are_kind<TYPE>(a[i], kind);
-            count = mfma32<TYPE>(a, one[u], count);
-          }
-          const float what = kind == 0 ? INFINITY : kind == 1 ? -INFINITY : __builtin_nanf("");
-#pragma unroll
-          for (int i = 0; i < 16; ++i) acc[d][i] += count[i] > 0.f ? what : 0.f;
-        }
-      }
     }
   };
 
   if (tbeg < tend) {
-    int found = find(tbeg);
-    fetch(tbeg, 0, found);
-    int next = find(tbeg + STEP);
+    int page = valid(tbeg, find(tbeg));
+    fetch(tbeg, 0, page);
+    int found = find(tbeg + STEP);
     for (int t = tbeg; t < tend; t += 2 * STEP) {
 #pragma unroll
       for (int bf = 0; bf < 2; ++bf) {
@@ -943,14 +934,36 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
           // this step's bytes have arrived, for every wave; the other buffer is read no more
           __builtin_amdgcn_s_waitcnt(0x0F70);                       // vmcnt(0)
           __syncthreads();
-          const uint32_t present = (uint32_t)__ballot(found >= 0) & ((1u << 4 * STEP) - 1);
-          if (tt + STEP < tend) fetch(tt + STEP, 1 - bf, next);
-          found = next;
-          next = find(tt + 2 * STEP);
+          const uint32_t present = (uint32_t)__ballot(page >= 0) & ((1u << 4 * STEP) - 1);
+          page = valid(tt + STEP, found);
+          if (tt + STEP < tend) fetch(tt + STEP, 1 - bf, page);
+          found = find(tt + 2 * STEP);
           const int mine = kTurns ? group : 0, at = (tt + mine) * kTileTokens;
           if (tt + mine < tend && at < lim_max && at + kTileTokens > lo_min)
             attend(tt + mine, s_k[bf][mine], s_v[bf][mine], present >> (4 * mine) & 15u);
         }
+      }
+    }
+  }
+
+  // values that are not finite, of the tiles where they counted as zeros, on the
+  // outputs of the rows that see them
+  if (__any(odd != 0)) {
+#pragma unroll 1
+    for (int t = tbeg; t < tend; ++t) {
+      if (!partial(t) || (kTurns && ((t - tbeg) & 1) != group)) continue;
+#pragma unroll 1
+      for (int token = t * kTileTokens; token < (t + 1) * kTileTokens && token < len; ++token) {
+        const int pg = table[min(token >> c.page_shift, last_blk)];
+        if (pg < 0 || pg >= (int)c.num_pages || token < lo || token >= lim) continue;
+        const uint16_t* v = vh + (int64_t)pg * c.v_page + (token & ps_mask) * c.v_token;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float x = value_of<TYPE>(v[32 * d + 8 * (i >> 2) + 4 * half + (i & 3)]);
+            if (!(fabsf(x) < INFINITY)) acc[d][i] += x;
+          }
       }
     }
   }
