@@ -775,14 +775,13 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
   const uint16_t* vh = c.v + h * c.v_head;
   const int ps_mask = (1 << c.page_shift) - 1, last_blk = b.max_blocks - 1;
   const int ctile = STEP == 2 ? (wave * TOK) / kTileTokens : 0, ctok = (wave * TOK) % kTileTokens;   // of its copies
-  uint32_t koff[NL], voff[NL];                                      // bytes from the run's first token
-#pragma unroll
-  for (int i = 0; i < NL; ++i) {
-    const int t = ctok + i * RPL + lane / CH, ch = lane % CH;
-    const int kc = DH == 128 ? ch ^ (t & 15) : ch ^ ((t >> 1) & 7), vc = DH == 128 ? ch ^ ((t & 3) << 2) : ch ^ (((t >> 1) & 1) << 2);
-    koff[i] = 2 * ((t & 15) * c.k_token + 8 * kc);
-    voff[i] = 2 * ((t & 15) * c.v_token + 8 * vc);
-  }
+  // Bytes of this lane from a copy's first token: its token's, and its chunk's, which
+  // the first token's number turns too (tokens and chunks are exclusive-or'ed bit by bit).
+  const int ltok = lane / CH, lch = lane % CH;
+  auto k_swizzle = [](int t) { return DH == 128 ? t & 15 : (t >> 1) & 7; };
+  auto v_swizzle = [](int t) { return DH == 128 ? (t & 3) << 2 : (t & 2) << 1; };
+  const uint32_t ktok = 2 * ltok * c.k_token, kchunk = 16 * (lch ^ k_swizzle(ltok));
+  const uint32_t voff = 2 * ltok * c.v_token + 16 * (lch ^ v_swizzle(ltok));
   // pages of the runs of tiles t ..: lane i looks up run i & (4 STEP - 1); what it finds
   // is looked at a step later, when it has arrived
   const int my_run = 16 * (lane & (4 * STEP - 1));
@@ -791,29 +790,26 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
   auto fetch = [&](int t, int bf, int found) {
     const int run = ctile * 4 + ctok / 16, at = t * kTileTokens + 16 * run;
     const int pg = __builtin_amdgcn_readlane(found, run), have = pg < 0 ? 0 : len - at;
-    const uint16_t* k = kh + (int64_t)max(pg, 0) * c.k_page + (at & ps_mask) * c.k_token;
-    const uint16_t* v = vh + (int64_t)max(pg, 0) * c.v_page + (at & ps_mask) * c.v_token;
-    uint16_t* kt = &s_k[bf][ctile][ctok * DH];
-    uint16_t* vt = &s_v[bf][ctile][ctok * DH];
-    if (have >= (ctok & 15) + TOK) {
+    const uint16_t* k = kh + (int64_t)max(pg, 0) * c.k_page;
+    const uint16_t* v = vh + (int64_t)max(pg, 0) * c.v_page;
+    const bool all = have >= (ctok & 15) + TOK;
 #pragma unroll
-      for (int i = 0; i < NL; ++i) {
-        copy_to_lds(k, koff[i], lds_address(kt + i * RPL * DH));
-        copy_to_lds(v, voff[i], lds_address(vt + i * RPL * DH));
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < NL; ++i) {
-        if ((ctok & 15) + i * RPL + lane / CH < have) {
-          copy_to_lds(k, koff[i], lds_address(kt + i * RPL * DH));
-          copy_to_lds(v, voff[i], lds_address(vt + i * RPL * DH));
-        } else {
-          *(uintx4*)(kt + i * RPL * DH + 8 * lane) = uintx4{0, 0, 0, 0};
-          *(uintx4*)(vt + i * RPL * DH + 8 * lane) = uintx4{0, 0, 0, 0};
-        }
+    for (int i = 0; i < NL; ++i) {
+      const int first = (ctok & 15) + i * RPL;                      // of the run
+      const uint16_t* kf = k + ((at & ps_mask) + first) * c.k_token;
+      const uint16_t* vf = v + ((at & ps_mask) + first) * c.v_token;
+      uint16_t* kt = &s_k[bf][ctile][(ctok + i * RPL) * DH];
+      uint16_t* vt = &s_v[bf][ctile][(ctok + i * RPL) * DH];
+      if (all || first + ltok < have) {
+        copy_to_lds(kf, ktok + (kchunk ^ 16 * k_swizzle(first)), lds_address(kt));
+        copy_to_lds(vf, voff, lds_address(vt));
+      } else {
+        *(uintx4*)(kt + 8 * lane) = uintx4{0, 0, 0, 0};
+        *(uintx4*)(vt + 8 * lane) = uintx4{0, 0, 0, 0};
       }
     }
   };
+  static_assert(DH == 128 ? RPL % 4 == 0 : RPL % 4 == 0, "the values' chunks turn by a token's low bits");
 
   floatx16 acc[DB];
 #pragma unroll
@@ -821,15 +817,14 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
   float ref = kNoScore, sum = 0.f;
-  // LDS elements: key row col, chunk 2 k + half of the map; value row 4 half + (lane & 15) / 4 and its 4 columns
-  const int krow = col * DH, kswz = DH == 128 ? col & 15 : (col >> 1) & 7;
-  const int vrow = (4 * half + ((lane & 15) >> 2)) * DH + 4 * (lane & 1), vchunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-  const int vswz = DH == 128 ? (lane >> 2) & 3 : (lane >> 3) & 1;
-  auto k_at = [&](const uint16_t* tile, int x, int k) {
-    return *(const uintx4*)&tile[32 * x * DH + krow + 8 * ((dim0 / 8 + 2 * k + half) ^ kswz)];
-  };
+  // LDS elements: key row col, chunk 2 k + half of the map; value row 4 half + (lane & 15)
+  // / 4 and its 4 columns.  A step forms the others from these by exclusive or.
+  int kat = col * DH + 8 * ((dim0 / 8 + half) ^ k_swizzle(col));
+  int vat = (4 * half + ((lane & 15) >> 2)) * DH + 4 * (lane & 1) +
+            8 * ((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ v_swizzle((lane & 15) >> 2));
+  auto k_at = [&](const uint16_t* tile, int x, int k) { return *(const uintx4*)&tile[(kat ^ 16 * k) + 32 * x * DH]; };
   auto v_at = [&](const uint16_t* tile, int u, int d) {
-    const uint16_t* p = &tile[16 * u * DH + vrow + 8 * (4 * (d ^ vswz) + vchunk)];
+    const uint16_t* p = &tile[(vat ^ 32 * d) + 16 * u * DH];
     const uintx2 x = read_columns(p), y = read_columns(p + 8 * DH);
     return uintx4{x[0], x[1], y[0], y[1]};
   };
@@ -840,6 +835,7 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
   // tile t by this wave, from its buffer; present: a bit for each run that has a page
   auto attend = [&](int t, const uint16_t* kt, const uint16_t* vt, uint32_t present) {
     const int t0 = t * kTileTokens;
+    asm volatile("" : "+v"(kat), "+v"(vat));                        // (formed anew in every step: registers are dearer)
     floatx16 sc[2];
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
@@ -883,8 +879,7 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
       off = 0.f;
     }
     uintx4 w[4], rest[4];
-#pragma unroll
-    for (int u = 0; u < 4; ++u)
+    auto weigh = [&](int u) {
 #pragma unroll
       for (int i = 0; i < 8; i += 2) {
         const float x = exp2_of(fmaf(sc[u >> 1][8 * (u & 1) + i], cw, off));
@@ -894,17 +889,30 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
         w[u][i / 2] = pair_of<TYPE>(x, y);
         if constexpr (kRest) rest[u][i / 2] = pair_of<TYPE>(x - low_of<TYPE>(w[u][i / 2]), y - high_of<TYPE>(w[u][i / 2]));
       }
+    };
     if (!cut) {
+      // (two numbers a weight: each four weights' products before the next are formed,
+      // for the registers; one: all weights first, 565 us for an 8K prompt against 590)
+      if constexpr (!kRest)
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
+        for (int u = 0; u < 4; ++u) weigh(u);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if constexpr (kRest) {
+          weigh(u);
+          if (u) __builtin_amdgcn_sched_barrier(0);
+        }
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
           const uintx4 a = v_at(vt, u, d);
           acc[d] = mfma32<TYPE>(a, w[u], acc[d]);
           if constexpr (kRest) acc[d] = mfma32<TYPE>(a, rest[u], acc[d]);
         }
-      groups_ahead<4 * DB, 2, kRest ? 2 : 1, DB < 4 ? DB : 4>();
+      }
+      if constexpr (!kRest) groups_ahead<4 * DB, 2, 1, DB < 4 ? DB : 4>();
     } else {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) weigh(u);
 #pragma unroll
       for (int u = 0; u < 4; ++u)
 #pragma unroll
@@ -918,6 +926,7 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
           }
           acc[d] = mfma32<TYPE>(a, w[u], acc[d]);
           if constexpr (kRest) acc[d] = mfma32<TYPE>(a, rest[u], acc[d]);
+          __builtin_amdgcn_sched_barrier(0);                        // (few such tiles: registers before overlap)
         }
     }
   };
@@ -958,12 +967,14 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
         if (pg < 0 || pg >= (int)c.num_pages || token < lo || token >= lim) continue;
         const uint16_t* v = vh + (int64_t)pg * c.v_page + (token & ps_mask) * c.v_token;
 #pragma unroll
-        for (int d = 0; d < DB; ++d)
+        for (int d = 0; d < DB; ++d) {
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const float x = value_of<TYPE>(v[32 * d + 8 * (i >> 2) + 4 * half + (i & 3)]);
             if (!(fabsf(x) < INFINITY)) acc[d][i] += x;
           }
+          __builtin_amdgcn_sched_barrier(0);
+        }
       }
     }
   }
