@@ -134,10 +134,10 @@ __device__ __forceinline__ float wave_sum(float x) {
 // Partials first, first + step, ... before end of one output row, joined by the
 // wave, CH (up to 16) at a time whose loads are all on the way at once: R, l and
 // the lane's DH / 64 outputs.  `at(i)`: partial i's reference (its sum `sums` floats on) and
-// its row.
+// its row.  A reference times `scale` is a power of two's exponent.
 template <int DPL, int CH, class AT>
 __device__ __forceinline__ void join(int64_t first, int64_t end, int64_t step, int sums, AT at, float& R, float& l,
-                                     float (&acc)[DPL]) {
+                                     float (&acc)[DPL], float scale = 1.0f) {
   const int lane = threadIdx.x & 63;
   R = kNoScore;
   l = 0.f;
@@ -157,7 +157,7 @@ __device__ __forceinline__ void join(int64_t first, int64_t end, int64_t step, i
 #pragma unroll
       for (int d = 0; d < DPL; ++d) a[i][d] = row[d];
     }
-    const float M = fmaxf(R, wave_max(r)), f = exp2_of(r - M), was = exp2_of(R - M);
+    const float M = fmaxf(R, wave_max(r)), f = exp2_of((r - M) * scale), was = exp2_of((R - M) * scale);
     const bool has = lane < CH && g + lane * step < end;
     const float w = has ? f : 0.f;
     l = fmaf(l, was, wave_sum(ls * w));

@@ -614,6 +614,9 @@ __global__ __launch_bounds__(64 * WAVES) void cache16_decode_merge_kernel(Cache1
 // rows see in part, values that are not finite count as zeros in the product, and
 // are added at the end to the outputs of the rows that see them.
 constexpr int kTileTokens = 64;
+// A weight may pass 2^kMostWeight; where a lane's 32 of a tile add up to less than
+// kMostSum none has, or fp16 holds it.
+constexpr float kMostWeight = 10.0f, kMostSum = 0x1p15f;
 
 // A workgroup's shape: row waves of 32 rows, groups of them, and whether the groups
 // take the tiles in turn.
@@ -622,7 +625,7 @@ struct PrefillShape {
   __host__ __device__ constexpr int row_shift() const { return row_waves == 8 ? 8 : row_waves == 4 ? 7 : 6; }
 };
 __host__ __device__ __forceinline__ PrefillShape prefill_shape(int64_t num_rows, int num_seqs, int gqa, int dh, bool diff) {
-  if (diff) return {4, 2, dh == 64 ? 512 : 256};
+  if (diff) return {4, 2, 256};
   if (dh == 64) return {4, 1, 768};
   return num_rows * gqa <= 128 * (int64_t)num_seqs ? PrefillShape{4, 2, 256} : PrefillShape{8, 1, 256};
 }
@@ -707,11 +710,14 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
   constexpr int KS = DH / 16, DB = DH / 32, KM = DIFF ? KS / 2 : KS;  // k-steps, value blocks, k-steps of a map
   constexpr int WAVES = ROW_WAVES * GROUPS, kRowTile = 32 * ROW_WAVES, RS = ROW_WAVES == 8 ? 8 : ROW_WAVES == 4 ? 7 : 6;
   constexpr bool kTurns = GROUPS == 2 && !DIFF;
-  constexpr int STEP = kTurns ? 2 : 1;                                // tiles between two barriers
+  constexpr int STEP = kTurns ? 2 : 1;                                // tiles of a step
+  constexpr bool kPing = WAVES == 8 && !kTurns;                       // two halves of the waves, half a step apart
+  constexpr int NB = kPing ? 4 : 2;                                   // steps in LDS
   constexpr bool kRest = DIFF || TYPE == kFp16;                       // weights as two numbers
   constexpr int CH = DH / 8, RPL = 64 / CH, TOK = kTileTokens / WAVES * STEP, NL = TOK / RPL;   // chunks of a row; rows a copy;
                                                                       // a wave's tokens of a step and copies of each kind
-  __shared__ __align__(16) uint16_t s_k[2][STEP][kTileTokens * DH], s_v[2][STEP][kTileTokens * DH];
+  __shared__ __align__(16) uint16_t s_k[NB][STEP][kTileTokens * DH], s_v[NB][STEP][kTileTokens * DH];
+  __shared__ int s_odd;                                               // a value of a cleaned tile was not finite
   const Cache16& c = L.c;
   const Cache8Batch& b = L.b;
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), col = lane & 31, half = lane >> 5;
@@ -782,32 +788,44 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
   auto v_swizzle = [](int t) { return DH == 128 ? (t & 3) << 2 : (t & 2) << 1; };
   const uint32_t ktok = 2 * ltok * c.k_token, kchunk = 16 * (lch ^ k_swizzle(ltok));
   const uint32_t voff = 2 * ltok * c.v_token + 16 * (lch ^ v_swizzle(ltok));
-  // pages of the runs of tiles t ..: lane i looks up run i & (4 STEP - 1); what it finds
-  // is looked at a step later, when it has arrived
-  const int my_run = 16 * (lane & (4 * STEP - 1));
-  auto find = [&](int t) { return table[min((t * kTileTokens + my_run) >> c.page_shift, last_blk)]; };
-  auto valid = [&](int t, int pg) { return t * kTileTokens + my_run < len && pg < (int)c.num_pages ? pg : -1; };
-  auto fetch = [&](int t, int bf, int found) {
-    const int run = ctile * 4 + ctok / 16, at = t * kTileTokens + 16 * run;
-    const int pg = __builtin_amdgcn_readlane(found, run), have = pg < 0 ? 0 : len - at;
-    const uint16_t* k = kh + (int64_t)max(pg, 0) * c.k_page;
-    const uint16_t* v = vh + (int64_t)max(pg, 0) * c.v_page;
-    const bool all = have >= (ctok & 15) + TOK;
+  // The page of run `run` of tile t, or -1, by scalar loads (whose waits are apart
+  // from those of the copies); a tile's four pages as bits.
+  typedef const __attribute__((address_space(4))) int32_t* constant_t;
+  const constant_t pages = (constant_t)(uintptr_t)table;
+  struct Found { int id[4]; };
+  auto find = [&](int t) {
+    Found f;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) f.id[r] = pages[min((t * kTileTokens + 16 * r) >> c.page_shift, last_blk)];
+    return f;
+  };
+  auto there = [&](int t, const Found& f, int r) {                  // 1 or 0, without branches
+    return (int)(t * kTileTokens + 16 * r < len) & (int)((uint32_t)f.id[r] < (uint32_t)c.num_pages);
+  };
+  auto present_of = [&](int t, const Found& f) {
+    return (uint32_t)(there(t, f, 0) | there(t, f, 1) << 1 | there(t, f, 2) << 2 | there(t, f, 3) << 3);
+  };
+  const int crun = ctok / 16;
+  // this wave's copies' page; page 0 in an absent one's place
+  auto page_of = [&](int t, const Found& f) {
+    const int id = crun == 0 ? f.id[0] : crun == 1 ? f.id[1] : crun == 2 ? f.id[2] : f.id[3];
+    return id & -((int)(t * kTileTokens + 16 * crun < len) & (int)((uint32_t)id < (uint32_t)c.num_pages));
+  };
+  // Every call issues the same copies.  Of an absent page they read page 0, behind the
+  // length what the page holds: the tile is cleaned then.
+  auto copy_k = [&](int t, int page, int bf) {
+    const uint16_t* from = kh + (int64_t)page * c.k_page + ((t * kTileTokens + 16 * crun) & ps_mask) * c.k_token;
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
       const int first = (ctok & 15) + i * RPL;                      // of the run
-      const uint16_t* kf = k + ((at & ps_mask) + first) * c.k_token;
-      const uint16_t* vf = v + ((at & ps_mask) + first) * c.v_token;
-      uint16_t* kt = &s_k[bf][ctile][(ctok + i * RPL) * DH];
-      uint16_t* vt = &s_v[bf][ctile][(ctok + i * RPL) * DH];
-      if (all || first + ltok < have) {
-        copy_to_lds(kf, ktok + (kchunk ^ 16 * k_swizzle(first)), lds_address(kt));
-        copy_to_lds(vf, voff, lds_address(vt));
-      } else {
-        *(uintx4*)(kt + 8 * lane) = uintx4{0, 0, 0, 0};
-        *(uintx4*)(vt + 8 * lane) = uintx4{0, 0, 0, 0};
-      }
+      copy_to_lds(from + first * c.k_token, ktok + (kchunk ^ 16 * k_swizzle(first)), lds_address(&s_k[bf][ctile][(ctok + i * RPL) * DH]));
     }
+  };
+  auto copy_v = [&](int t, int page, int bf) {
+    const uint16_t* from = vh + (int64_t)page * c.v_page + ((t * kTileTokens + 16 * crun) & ps_mask) * c.v_token;
+#pragma unroll
+    for (int i = 0; i < NL; ++i)
+      copy_to_lds(from + ((ctok & 15) + i * RPL) * c.v_token, voff, lds_address(&s_v[bf][ctile][(ctok + i * RPL) * DH]));
   };
   static_assert(DH == 128 ? RPL % 4 == 0 : RPL % 4 == 0, "the values' chunks turn by a token's low bits");
 
@@ -816,156 +834,283 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
   for (int d = 0; d < DB; ++d)
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
-  float ref = kNoScore, sum = 0.f;
-  // LDS elements: key row col, chunk 2 k + half of the map; value row 4 half + (lane & 15)
-  // / 4 and its 4 columns.  A step forms the others from these by exclusive or.
-  int kat = col * DH + 8 * ((dim0 / 8 + half) ^ k_swizzle(col));
-  int vat = (4 * half + ((lane & 15) >> 2)) * DH + 4 * (lane & 1) +
-            8 * ((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ v_swizzle((lane & 15) >> 2));
-  auto k_at = [&](const uint16_t* tile, int x, int k) { return *(const uintx4*)&tile[(kat ^ 16 * k) + 32 * x * DH]; };
+  float ref = 0.f, sum = 0.f;                                       // the reference in units of <q, k>
+  floatx16 minus_ref;                                               // what scores start from: they come out less the reference
+#pragma unroll
+  for (int i = 0; i < 16; ++i) minus_ref[i] = 0.f;
+  // LDS bytes: key row col, chunk 2 k + half of the map; value row 4 half + (lane & 15) / 4
+  // and its 4 columns.  A step forms the others from these by exclusive or.
+  int kat = 2 * (col * DH + 8 * ((dim0 / 8 + half) ^ k_swizzle(col)));
+  int vat = 2 * ((4 * half + ((lane & 15) >> 2)) * DH + 4 * (lane & 1) +
+                 8 * ((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ v_swizzle((lane & 15) >> 2)));
+  auto k_at = [&](const uint16_t* tile, int x, int k) {
+    return *(const uintx4*)((const char*)tile + (kat ^ 32 * k) + 64 * x * DH);
+  };
   auto v_at = [&](const uint16_t* tile, int u, int d) {
-    const uint16_t* p = &tile[(vat ^ 32 * d) + 16 * u * DH];
-    const uintx2 x = read_columns(p), y = read_columns(p + 8 * DH);
+    const char* p = (const char*)tile + (vat ^ 64 * d) + 32 * u * DH;
+    const uintx2 x = read_columns((const uint16_t*)p), y = read_columns((const uint16_t*)(p + 16 * DH));
     return uintx4{x[0], x[1], y[0], y[1]};
   };
 
-  // a tile that some rows of the wave see in part
+  // tile t: rows of the wave that see it; some that see it in part
+  auto visible = [&](int t) { return t < tend && t * kTileTokens < lim_max && (t + 1) * kTileTokens > lo_min; };
   auto partial = [&](int t) { return (t + 1) * kTileTokens > lim_min || t * kTileTokens < lo_max; };
-  uint32_t odd = 0;                                                 // not 0: such a tile had a value that is not finite
-  // tile t by this wave, from its buffer; present: a bit for each run that has a page
-  auto attend = [&](int t, const uint16_t* kt, const uint16_t* vt, uint32_t present) {
-    const int t0 = t * kTileTokens;
-    asm volatile("" : "+v"(kat), "+v"(vat));                        // (formed anew in every step: registers are dearer)
-    floatx16 sc[2];
+  // A tile that some rows of the workgroup see in part, or with an absent page, is
+  // cleaned by the waves that copied it, before any reads it: values of tokens that
+  // are not there and values that are not finite become zeros.
+  const int first_tok = (int)(r0 / gqa), all_lim = row_sees(L, len, n, first_tok).hi, all_lo = row_sees(L, len, n, last / gqa).lo;
+  auto unclean = [&](int t, uint32_t present) {
+    return present != 15u || (t + 1) * kTileTokens > all_lim || t * kTileTokens < all_lo;
+  };
+  auto clean = [&](int t, uint32_t present, uint16_t* vt) {
+    const int have = present >> crun & 1 ? len - t * kTileTokens - 16 * crun : 0;
+    uint32_t bad = 0;
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      uintx4* at = (uintx4*)(vt + (ctok + i * RPL) * DH + 8 * lane);
+      uintx4 x = *at;
+      const bool held = (ctok & 15) + i * RPL + ltok < have;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t y = held ? x[k] : 0u;
+        x[k] = finite_or_zero<TYPE>(y);
+        bad |= x[k] ^ y;
+      }
+      *at = x;
+    }
+    if (__any(bad != 0) && lane == 0) s_odd = 1;
+  };
+
+  floatx16 sc[2];
+  uintx4 w[4], rest[4];
+
+  auto scores = [&](const uint16_t* kt) {
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) sc[x][i] = 0.f;
+      sc[x] = minus_ref;
 #pragma unroll
       for (int k = 0; k < KM; ++k) sc[x] = mfma32<TYPE>(k_at(kt, x, k), q[k], sc[x]);
     }
-    groups_ahead<2 * KM, 1, 1, KM < 6 ? KM : 6>();
-    const bool cut = partial(t);
-    if (cut || present != 15u) {
-      const uint32_t first = t0 + 4 * half - lo, width = lim - lo;
+  };
+  // scores of tile t that do not count; present: a bit for each run that has a page
+  auto mask = [&](int t, uint32_t present) {
+    const uint32_t first = t * kTileTokens + 4 * half - lo, width = lim - lo;
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const uint32_t w = present >> u & 1 ? width : 0u;
+    for (int u = 0; u < 4; ++u) {
+      const uint32_t n = present >> u & 1 ? width : 0u;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int e = 8 * (u & 1) + i;
-          sc[u >> 1][e] = first + (16 * u + 8 * (i >> 2) + (i & 3)) < w ? sc[u >> 1][e] : -INFINITY;
-        }
+      for (int i = 0; i < 8; ++i) {
+        const int e = 8 * (u & 1) + i;
+        sc[u >> 1][e] = first + (16 * u + 8 * (i >> 2) + (i & 3)) < n ? sc[u >> 1][e] : -INFINITY;
       }
     }
-    float top = sc[0][0];
-#pragma unroll
-    for (int e = 1; e < 32; ++e) top = fmaxf(top, sc[e >> 4][e & 15]);
-    top *= cq;
-    if (__any(top > ref + (kTopWeight + kSlackWeight))) {           // (each row by its own scores)
-      top = halves_max(top);
-      const float to = top > ref + (kTopWeight + kSlackWeight) ? top - kTopWeight : ref;
-      const float f = exp2_of(ref - to);
-      ref = to;
-      sum *= f;
-#pragma unroll
-      for (int d = 0; d < DB; ++d) acc[d] *= f;
-    }
-    float cw = cq, off = -ref;
-    if (__any((fabsf(ref) > kPlainScore) & (ref > kNoScore))) {
-#pragma unroll
-      for (int e = 0; e < 32; ++e) sc[e >> 4][e & 15] = __fsub_rn(__fmul_rn(sc[e >> 4][e & 15], cq), ref);
-      cw = 1.f;
-      off = 0.f;
-    }
-    uintx4 w[4], rest[4];
-    auto weigh = [&](int u) {
-#pragma unroll
-      for (int i = 0; i < 8; i += 2) {
-        const float x = exp2_of(fmaf(sc[u >> 1][8 * (u & 1) + i], cw, off));
-        const float y = exp2_of(fmaf(sc[u >> 1][8 * (u & 1) + i + 1], cw, off));
-        sum += x;
-        sum += y;
-        w[u][i / 2] = pair_of<TYPE>(x, y);
-        if constexpr (kRest) rest[u][i / 2] = pair_of<TYPE>(x - low_of<TYPE>(w[u][i / 2]), y - high_of<TYPE>(w[u][i / 2]));
-      }
-    };
-    if (!cut) {
-      // (two numbers a weight: each four weights' products before the next are formed,
-      // for the registers; one: all weights first, 565 us for an 8K prompt against 590)
-      if constexpr (!kRest)
-#pragma unroll
-        for (int u = 0; u < 4; ++u) weigh(u);
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        if constexpr (kRest) {
-          weigh(u);
-          if (u) __builtin_amdgcn_sched_barrier(0);
-        }
-#pragma unroll
-        for (int d = 0; d < DB; ++d) {
-          const uintx4 a = v_at(vt, u, d);
-          acc[d] = mfma32<TYPE>(a, w[u], acc[d]);
-          if constexpr (kRest) acc[d] = mfma32<TYPE>(a, rest[u], acc[d]);
-        }
-      }
-      if constexpr (!kRest) groups_ahead<4 * DB, 2, 1, DB < 4 ? DB : 4>();
-    } else {
-#pragma unroll
-      for (int u = 0; u < 4; ++u) weigh(u);
+  };
+  // The tile's weights, 2^kTopWeight at the reference.  Their largest is not looked
+  // for: where a lane's 32 add up to less than 2^(kMostWeight + 5) none has passed
+  // the bound of the reference.  Otherwise, and at a row's first scores, the reference
+  // becomes the row's largest score (both halves of a row decide alike).
+  auto weigh = [&]() {
+    float ws = 0.f;
+    auto pass = [&](float shift) {
 #pragma unroll
       for (int u = 0; u < 4; ++u)
 #pragma unroll
-        for (int d = 0; d < DB; ++d) {
-          uintx4 a = v_at(vt, u, d);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t x = finite_or_zero<TYPE>(a[i]);
-            odd |= x ^ a[i];
-            a[i] = x;
-          }
-          acc[d] = mfma32<TYPE>(a, w[u], acc[d]);
-          if constexpr (kRest) acc[d] = mfma32<TYPE>(a, rest[u], acc[d]);
-          __builtin_amdgcn_sched_barrier(0);                        // (few such tiles: registers before overlap)
+        for (int i = 0; i < 8; i += 2) {
+          const float x = exp2_of(fmaf(sc[u >> 1][8 * (u & 1) + i] - shift, cq, kTopWeight));
+          const float y = exp2_of(fmaf(sc[u >> 1][8 * (u & 1) + i + 1] - shift, cq, kTopWeight));
+          ws += x;
+          ws += y;
+          w[u][i / 2] = pair_of<TYPE>(x, y);
+          if constexpr (kRest) rest[u][i / 2] = pair_of<TYPE>(x - low_of<TYPE>(w[u][i / 2]), y - high_of<TYPE>(w[u][i / 2]));
         }
+    };
+    pass(0.f);
+    if (__any(!(ws < kMostSum) | (sum == 0.f))) {
+      float top = sc[0][0];
+#pragma unroll
+      for (int e = 1; e < 32; ++e) top = fmaxf(top, sc[e >> 4][e & 15]);
+      top = halves_max(top);
+      const bool fresh = halves_max(sum) == 0.f, moves = top > -INFINITY && (fresh || fmaf(top, cq, kTopWeight) > kMostWeight);
+      const float shift = moves ? top : 0.f, f = fresh ? 1.f : exp2_of(-shift * cq);
+      ref += shift;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) minus_ref[i] = -ref;
+      sum *= f;
+#pragma unroll
+      for (int d = 0; d < DB; ++d) acc[d] *= f;
+      ws = 0.f;
+      pass(shift);
+    }
+    sum += ws;
+  };
+  auto values = [&](const uint16_t* vt) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        const uintx4 a = v_at(vt, u, d);
+        acc[d] = mfma32<TYPE>(a, w[u], acc[d]);
+        if constexpr (kRest) acc[d] = mfma32<TYPE>(a, rest[u], acc[d]);
+      }
+  };
+  // Both, in this order: each product with the reads of the one kAheadReads later
+  // before it (a SIMD's matrix cores have this wave alone then).
+  auto products = [&](const uint16_t* kt, const uint16_t* vt) {
+    constexpr int NK = 2 * KM, N = NK + 4 * DB, kAheadReads = 6;
+    uintx4 a[kAheadReads + 1];
+    auto read = [&](int j) { a[j % (kAheadReads + 1)] = j < NK ? k_at(kt, j / KM, j % KM) : v_at(vt, (j - NK) / DB, (j - NK) % DB); };
+    sc[0] = sc[1] = minus_ref;
+#pragma unroll
+    for (int j = 0; j < kAheadReads; ++j) read(j);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      if (j + kAheadReads < N) read(j + kAheadReads);
+      const uintx4 x = a[j % (kAheadReads + 1)];
+      if (j < NK) {
+        sc[j / KM] = mfma32<TYPE>(x, q[j % KM], sc[j / KM]);
+      } else {
+        const int u = (j - NK) / DB, d = (j - NK) % DB;
+        acc[d] = mfma32<TYPE>(x, w[u], acc[d]);
+        if constexpr (kRest) acc[d] = mfma32<TYPE>(x, rest[u], acc[d]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
+  if (tid == 0) s_odd = 0;
+  __syncthreads();
 
-  if (tbeg < tend) {
-    int page = valid(tbeg, find(tbeg));
-    fetch(tbeg, 0, page);
-    int found = find(tbeg + STEP);
+  if constexpr (kPing) {
+    // The matrix part of a step (scores of the next tile, values of this one) by one
+    // half of the waves while the other half, on the same SIMDs, is at its weights:
+    // a barrier ends each part.  Step i's matrix part reads K(i + 1) and V(i), one half
+    // of the waves a part after the other; its part of weights issues the copies of
+    // K(i + 3) and V(i + 2), over what every wave has read by then.  What the next
+    // matrix parts read has arrived when all but the last steps' copies have (each step
+    // issues 2 NL, and nothing else), and is cleaned, by every wave before the barrier
+    // that the first of them waits at.
+    static_assert(NL == 1 || NL == 2, "copies of a step");
+    constexpr int kOneStep = 0x0F70 | (2 * NL), kTwoSteps = 0x0F70 | (4 * NL);
+    const bool late = wave >= 4;
+    uint32_t present = 0;                                           // of four tiles, the latest in the low bits
+    int page = 0;                                                   // this wave's, of the latest tile
+    Found found = find(tbeg);
+    auto advance = [&](int i) {                                     // `found` is tile i + 3's
+      const int t = tbeg + i + 3;
+      if (i >= -2) copy_v(t - 1, page, (i + 2) & 3);
+      page = page_of(t, found);
+      copy_k(t, page, (i + 3) & 3);
+      present = present << 4 | present_of(t, found);
+      found = find(t + 1);
+    };
+    auto barrier = [&]() {
+      __builtin_amdgcn_sched_barrier(0);
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    // cleans this wave's part of V(i)
+    auto tidy = [&](int i, uint32_t here) {
+      if (i < tend - tbeg && unclean(tbeg + i, here)) {
+        clean(tbeg + i, here, s_v[i & 3][0]);
+        __builtin_amdgcn_s_waitcnt(0xC07F);                         // lgkmcnt(0)
+      }
+    };
+    const int count = tend - tbeg;
+    if (count > 0) {
+#pragma unroll
+      for (int i = -3; i < 0; ++i) advance(i);
+      __builtin_amdgcn_s_waitcnt(kTwoSteps);                        // K(0)
+      barrier();
+      if (late) barrier();
+      scores(s_k[0][0]);
+      if (late) {
+        __builtin_amdgcn_s_waitcnt(kOneStep);
+        tidy(0, present >> 8 & 15u);
+      }
+      barrier();
+      for (int i = 0; i < count; ++i) {
+        const int t = tbeg + i;
+        const uint32_t here = present >> 8 & 15u;
+        // weights
+        advance(i);
+        if (visible(t)) {
+          if (partial(t) || here != 15u) mask(t, here);
+          weigh();
+        } else {
+#pragma unroll
+          for (int u = 0; u < 4; ++u) w[u] = rest[u] = uintx4{0, 0, 0, 0};
+        }
+        if (!late) {
+          __builtin_amdgcn_s_waitcnt(kTwoSteps);
+          tidy(i, here);
+        }
+        barrier();
+        // products (of a tile that this wave's rows do not see: others see it in part, it is clean)
+        asm volatile("" : "+v"(kat), "+v"(vat));                    // (formed anew in every step: registers are dearer)
+        __builtin_amdgcn_s_setprio(1);
+        products(s_k[(i + 1) & 3][0], s_v[i & 3][0]);
+        __builtin_amdgcn_s_setprio(0);
+        if (late) {
+          __builtin_amdgcn_s_waitcnt(kOneStep);
+          tidy(i + 1, present >> 8 & 15u);
+        }
+        barrier();
+      }
+      if (!late) barrier();
+      __builtin_amdgcn_s_waitcnt(0x0F70);                           // vmcnt(0): no copy outlives the wave
+    }
+  } else if (tbeg < tend) {
+    const int mine = kTurns ? group : 0;
+    Found found = find(tbeg + ctile);
+    int page = page_of(tbeg + ctile, found);
+    uint32_t copied = present_of(tbeg + ctile, found);
+    copy_k(tbeg + ctile, page, 0);
+    copy_v(tbeg + ctile, page, 0);
     for (int t = tbeg; t < tend; t += 2 * STEP) {
 #pragma unroll
       for (int bf = 0; bf < 2; ++bf) {
         const int tt = t + bf * STEP;
         if (tt < tend) {
-          // this step's bytes have arrived, for every wave; the other buffer is read no more
+          const int next = tt + STEP + ctile;
+          found = find(next);
+          const uint32_t here = kTurns ? present_of(tt + mine, find(tt + mine)) : copied;
+          // this step's bytes have arrived and are clean, for every wave; the other buffer is read no more
           __builtin_amdgcn_s_waitcnt(0x0F70);                       // vmcnt(0)
+          if (unclean(tt + ctile, copied)) clean(tt + ctile, copied, s_v[bf][ctile]);
           __syncthreads();
-          const uint32_t present = (uint32_t)__ballot(page >= 0) & ((1u << 4 * STEP) - 1);
-          page = valid(tt + STEP, found);
-          if (tt + STEP < tend) fetch(tt + STEP, 1 - bf, page);
-          found = find(tt + 2 * STEP);
-          const int mine = kTurns ? group : 0, at = (tt + mine) * kTileTokens;
-          if (tt + mine < tend && at < lim_max && at + kTileTokens > lo_min)
-            attend(tt + mine, s_k[bf][mine], s_v[bf][mine], present >> (4 * mine) & 15u);
+          copied = present_of(next, found);
+          if (tt + STEP < tend) {
+            page = page_of(next, found);
+            copy_k(next, page, 1 - bf);
+            copy_v(next, page, 1 - bf);
+          }
+          if (visible(tt + mine)) {
+            asm volatile("" : "+v"(kat), "+v"(vat));                // (formed anew in every step: registers are dearer)
+            scores(s_k[bf][mine]);
+            groups_ahead<2 * KM, 1, 1, KM < 6 ? KM : 6>();
+            if (partial(tt + mine) || here != 15u) mask(tt + mine, here);
+            weigh();
+            values(s_v[bf][mine]);
+            groups_ahead<4 * DB, 2, kRest ? 2 : 1, DB < 4 ? DB : 4>();
+          }
         }
       }
     }
   }
-
-  // values that are not finite, of the tiles where they counted as zeros, on the
+  // values that are not finite, of the tiles where they count as zeros, on the
   // outputs of the rows that see them
-  if (__any(odd != 0)) {
+  __syncthreads();
+  if (s_odd) {
 #pragma unroll 1
     for (int t = tbeg; t < tend; ++t) {
-      if (!partial(t) || (kTurns && ((t - tbeg) & 1) != group)) continue;
+      const Found f = find(t);
+      if (!unclean(t, present_of(t, f)) || (kTurns && ((t - tbeg) & 1) != group)) continue;
 #pragma unroll 1
-      for (int token = t * kTileTokens; token < (t + 1) * kTileTokens && token < len; ++token) {
-        const int pg = table[min(token >> c.page_shift, last_blk)];
-        if (pg < 0 || pg >= (int)c.num_pages || token < lo || token >= lim) continue;
-        const uint16_t* v = vh + (int64_t)pg * c.v_page + (token & ps_mask) * c.v_token;
+      for (int token = t * kTileTokens; token < (t + 1) * kTileTokens; ++token) {
+        if (!(present_of(t, f) >> (token >> 4 & 3) & 1) || token < lo || token >= lim) continue;
+        const uint16_t* v = vh + (int64_t)pages[token >> c.page_shift] * c.v_page + (token & ps_mask) * c.v_token;
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
 #pragma unroll
@@ -980,6 +1125,7 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
   }
 
   sum = halves_sum(sum);
+  if (sum == 0.f) ref = kNoScore;
   float lam = 0.f, ref2 = 0.f, sum2 = 0.f;
   if constexpr (GROUPS == 2) {                                        // the second group's sums, through LDS, to the first
     float* o = (float*)s_k;                                           // [DH / 4][kRowTile][4]
@@ -1020,8 +1166,8 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
           f = 1.f;
         } else {
           const float R = fmaxf(ref, other);
-          f = exp2_of(ref - R);
-          g = exp2_of(other - R);
+          f = exp2_of((ref - R) * cq);
+          g = exp2_of((other - R) * cq);
           if (round == ROUNDS - 1) {
             ref = R;
             sum = fmaf(sum, f, osum * g);
@@ -1071,10 +1217,10 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
         ((U2*)((uint16_t*)L.out + at * DH + 32 * d + 8 * i + 4 * half))->v = none ? uintx2{0, 0} : uintx2{x, y};
       }
     if (L.lse && half == 0) {
-      const float e = none ? -INFINITY : (ref + log2_of(sum)) * kLn2;
+      const float e = none ? -INFINITY : (fmaf(ref, cq, -kTopWeight) + log2_of(sum)) * kLn2;
       if constexpr (DIFF) {
         L.lse[2 * at] = e;
-        L.lse[2 * at + 1] = sum2 == 0.f ? -INFINITY : (ref2 + log2_of(sum2)) * kLn2;
+        L.lse[2 * at + 1] = sum2 == 0.f ? -INFINITY : (fmaf(ref2, cq, -kTopWeight) + log2_of(sum2)) * kLn2;
       } else {
         L.lse[at] = e;
       }
@@ -1121,12 +1267,15 @@ __global__ __launch_bounds__(256) void cache16_prefill_merge_kernel(Cache16Atten
   const int in = (int)(r & (kRowTile - 1));
   const float* x = partials + (slot * c.num_kv + h) * splits * split_floats(DH, rows);
   RowSum<DH> y[2];
+  const float cq = L.sm_scale * kLog2e;
 #pragma unroll
-  for (int m = 0; m < MAPS; ++m)
+  for (int m = 0; m < MAPS; ++m) {
     join<DPL, 16>(0, parts, 1, rows, [&](int64_t z) {
       const float* p = x + z * split_floats(DH, rows) + m * kRowTile;
       return Partial{p + in, x + z * split_floats(DH, rows) + 2 * rows + (m * kRowTile + in) * DH};
-    }, y[m].R, y[m].l, y[m].x);
+    }, y[m].R, y[m].l, y[m].x, cq);
+    y[m].R = fmaf(y[m].R, cq, -kTopWeight);
+  }
   finish_row<TYPE, DH, DIFF>(L, at, hq, y[0], y[MAPS - 1]);
 }
 
