@@ -792,40 +792,37 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
   // from those of the copies); a tile's four pages as bits.
   typedef const __attribute__((address_space(4))) int32_t* constant_t;
   const constant_t pages = (constant_t)(uintptr_t)table;
-  struct Found { int id[4]; };
+  const int crun = ctok / 16;                                       // the run of this wave's copies
+  struct Found { int id[4], own; };
   auto find = [&](int t) {
-    Found f;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) f.id[r] = pages[min((t * kTileTokens + 16 * r) >> c.page_shift, last_blk)];
-    return f;
+    auto id = [&](int r) { return pages[min((t * kTileTokens + 16 * r) >> c.page_shift, last_blk)]; };
+    return Found{{id(0), id(1), id(2), id(3)}, id(crun)};
   };
-  auto there = [&](int t, const Found& f, int r) {                  // 1 or 0, without branches
-    return (int)(t * kTileTokens + 16 * r < len) & (int)((uint32_t)f.id[r] < (uint32_t)c.num_pages);
+  auto held = [&](int t, int id, int r) {                           // 1 or 0, without branches
+    return (int)(t * kTileTokens + 16 * r < len) & (int)((uint32_t)id < (uint32_t)c.num_pages);
   };
   auto present_of = [&](int t, const Found& f) {
-    return (uint32_t)(there(t, f, 0) | there(t, f, 1) << 1 | there(t, f, 2) << 2 | there(t, f, 3) << 3);
+    return (uint32_t)(held(t, f.id[0], 0) | held(t, f.id[1], 1) << 1 | held(t, f.id[2], 2) << 2 | held(t, f.id[3], 3) << 3);
   };
-  const int crun = ctok / 16;
-  // this wave's copies' page; page 0 in an absent one's place
-  auto page_of = [&](int t, const Found& f) {
-    const int id = crun == 0 ? f.id[0] : crun == 1 ? f.id[1] : crun == 2 ? f.id[2] : f.id[3];
-    return id & -((int)(t * kTileTokens + 16 * crun < len) & (int)((uint32_t)id < (uint32_t)c.num_pages));
-  };
+  auto page_of = [&](int t, const Found& f) { return f.own & -held(t, f.own, crun); };   // (page 0 in an absent one's place)
   // Every call issues the same copies.  Of an absent page they read page 0, behind the
   // length what the page holds: the tile is cleaned then.
-  auto copy_k = [&](int t, int page, int bf) {
-    const uint16_t* from = kh + (int64_t)page * c.k_page + ((t * kTileTokens + 16 * crun) & ps_mask) * c.k_token;
-#pragma unroll
-    for (int i = 0; i < NL; ++i) {
-      const int first = (ctok & 15) + i * RPL;                      // of the run
-      copy_to_lds(from + first * c.k_token, ktok + (kchunk ^ 16 * k_swizzle(first)), lds_address(&s_k[bf][ctile][(ctok + i * RPL) * DH]));
-    }
+  auto k_from = [&](int t, int page) {
+    return kh + (int64_t)page * c.k_page + (((t * kTileTokens + 16 * crun) & ps_mask) + (ctok & 15)) * c.k_token;
   };
-  auto copy_v = [&](int t, int page, int bf) {
-    const uint16_t* from = vh + (int64_t)page * c.v_page + ((t * kTileTokens + 16 * crun) & ps_mask) * c.v_token;
+  auto v_from = [&](int t, int page) {
+    return vh + (int64_t)page * c.v_page + (((t * kTileTokens + 16 * crun) & ps_mask) + (ctok & 15)) * c.v_token;
+  };
+  auto copy_k = [&](const uint16_t* from, int bf) {
 #pragma unroll
     for (int i = 0; i < NL; ++i)
-      copy_to_lds(from + ((ctok & 15) + i * RPL) * c.v_token, voff, lds_address(&s_v[bf][ctile][(ctok + i * RPL) * DH]));
+      copy_to_lds(from + i * RPL * c.k_token, ktok + (kchunk ^ 16 * k_swizzle((ctok & 15) + i * RPL)),
+                  lds_address(&s_k[bf][ctile][(ctok + i * RPL) * DH]));
+  };
+  auto copy_v = [&](const uint16_t* from, int bf) {
+#pragma unroll
+    for (int i = 0; i < NL; ++i)
+      copy_to_lds(from + i * RPL * c.v_token, voff, lds_address(&s_v[bf][ctile][(ctok + i * RPL) * DH]));
   };
   static_assert(DH == 128 ? RPL % 4 == 0 : RPL % 4 == 0, "the values' chunks turn by a token's low bits");
 
@@ -853,14 +850,14 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
   };
 
   // tile t: rows of the wave that see it; some that see it in part
-  auto visible = [&](int t) { return t < tend && t * kTileTokens < lim_max && (t + 1) * kTileTokens > lo_min; };
-  auto partial = [&](int t) { return (t + 1) * kTileTokens > lim_min || t * kTileTokens < lo_max; };
+  auto visible = [&](int t) { return (int)(t < tend) & (int)(t * kTileTokens < lim_max) & (int)((t + 1) * kTileTokens > lo_min); };
+  auto partial = [&](int t) { return (int)((t + 1) * kTileTokens > lim_min) | (int)(t * kTileTokens < lo_max); };
   // A tile that some rows of the workgroup see in part, or with an absent page, is
   // cleaned by the waves that copied it, before any reads it: values of tokens that
   // are not there and values that are not finite become zeros.
   const int first_tok = (int)(r0 / gqa), all_lim = row_sees(L, len, n, first_tok).hi, all_lo = row_sees(L, len, n, last / gqa).lo;
   auto unclean = [&](int t, uint32_t present) {
-    return present != 15u || (t + 1) * kTileTokens > all_lim || t * kTileTokens < all_lo;
+    return (int)(present != 15u) | (int)((t + 1) * kTileTokens > all_lim) | (int)(t * kTileTokens < all_lo);
   };
   auto clean = [&](int t, uint32_t present, uint16_t* vt) {
     const int have = present >> crun & 1 ? len - t * kTileTokens - 16 * crun : 0;
@@ -869,10 +866,10 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
     for (int i = 0; i < NL; ++i) {
       uintx4* at = (uintx4*)(vt + (ctok + i * RPL) * DH + 8 * lane);
       uintx4 x = *at;
-      const bool held = (ctok & 15) + i * RPL + ltok < have;
+      const bool there = (ctok & 15) + i * RPL + ltok < have;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const uint32_t y = held ? x[k] : 0u;
+        const uint32_t y = there ? x[k] : 0u;
         x[k] = finite_or_zero<TYPE>(y);
         bad |= x[k] ^ y;
       }
@@ -954,8 +951,8 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
       }
   };
   // Both, in this order: each product with the reads of the one kAheadReads later
-  // before it (a SIMD's matrix cores have this wave alone then).
-  auto products = [&](const uint16_t* kt, const uint16_t* vt) {
+  // before it (a SIMD's matrix cores have this wave alone then), and between(j) behind it.
+  auto products = [&](const uint16_t* kt, const uint16_t* vt, auto&& between) {
     constexpr int NK = 2 * KM, N = NK + 4 * DB, kAheadReads = 6;
     uintx4 a[kAheadReads + 1];
     auto read = [&](int j) { a[j % (kAheadReads + 1)] = j < NK ? k_at(kt, j / KM, j % KM) : v_at(vt, (j - NK) / DB, (j - NK) % DB); };
@@ -974,6 +971,7 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
         acc[d] = mfma32<TYPE>(x, w[u], acc[d]);
         if constexpr (kRest) acc[d] = mfma32<TYPE>(x, rest[u], acc[d]);
       }
+      between(j);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
@@ -989,19 +987,41 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
     // matrix parts read has arrived when all but the last steps' copies have (each step
     // issues 2 NL, and nothing else), and is cleaned, by every wave before the barrier
     // that the first of them waits at.
+    // The next step's addresses and cases are worked out among the products, where
+    // the wave has time; pages are looked up a step before that.
     static_assert(NL == 1 || NL == 2, "copies of a step");
     constexpr int kOneStep = 0x0F70 | (2 * NL), kTwoSteps = 0x0F70 | (4 * NL);
     const bool late = wave >= 4;
     uint32_t present = 0;                                           // of four tiles, the latest in the low bits
     int page = 0;                                                   // this wave's, of the latest tile
     Found found = find(tbeg);
-    auto advance = [&](int i) {                                     // `found` is tile i + 3's
-      const int t = tbeg + i + 3;
-      if (i >= -2) copy_v(t - 1, page, (i + 2) & 3);
-      page = page_of(t, found);
-      copy_k(t, page, (i + 3) & 3);
-      present = present << 4 | present_of(t, found);
-      found = find(t + 1);
+    const uint16_t* kfrom = kh;
+    const uint16_t* vfrom = vh;
+    int sees_it = 0, cut = 0, dirty = 0;                            // tile i: rows see it, some in part; cleaned
+    // step i's, in parts; `found` is tile i + 3's
+    auto plan = [&](int i, int part) {
+      const int t = tbeg + i;
+      switch (part) {
+        case 0: vfrom = v_from(t + 2, page); break;
+        case 1: page = page_of(t + 3, found); break;
+        case 2: kfrom = k_from(t + 3, page); break;
+        case 3: present = present << 4 | present_of(t + 3, found); break;
+        case 4: sees_it = visible(t); break;
+        case 5: cut = partial(t) | (int)((present >> 12 & 15u) != 15u); break;
+        default: dirty = (int)(t < tend) & unclean(t, present >> 12 & 15u);
+      }
+    };
+    auto plan_all = [&](int i) {
+#pragma unroll
+      for (int part = 0; part < 7; ++part) plan(i, part);
+    };
+    auto issue = [&](int i) {
+      if (i >= -2) copy_v(vfrom, (i + 2) & 3);
+      copy_k(kfrom, (i + 3) & 3);
+      found = find(tbeg + i + 4);
+    };
+    auto arrived = [&]() {                                          // (waited for here, not among the products)
+      asm volatile("" :: "s"(found.id[0]), "s"(found.id[1]), "s"(found.id[2]), "s"(found.id[3]), "s"(found.own));
     };
     auto barrier = [&]() {
       __builtin_amdgcn_sched_barrier(0);
@@ -1011,50 +1031,58 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
       __builtin_amdgcn_sched_barrier(0);
     };
     // cleans this wave's part of V(i)
-    auto tidy = [&](int i, uint32_t here) {
-      if (i < tend - tbeg && unclean(tbeg + i, here)) {
-        clean(tbeg + i, here, s_v[i & 3][0]);
+    auto tidy = [&](int i) {
+      if (dirty) {
+        clean(tbeg + i, present >> 12 & 15u, s_v[i & 3][0]);
         __builtin_amdgcn_s_waitcnt(0xC07F);                         // lgkmcnt(0)
       }
     };
     const int count = tend - tbeg;
     if (count > 0) {
 #pragma unroll
-      for (int i = -3; i < 0; ++i) advance(i);
+      for (int i = -3; i < 0; ++i) {
+        plan_all(i);
+        issue(i);
+      }
+      arrived();
       __builtin_amdgcn_s_waitcnt(kTwoSteps);                        // K(0)
       barrier();
       if (late) barrier();
       scores(s_k[0][0]);
+      plan_all(0);
       if (late) {
         __builtin_amdgcn_s_waitcnt(kOneStep);
-        tidy(0, present >> 8 & 15u);
+        tidy(0);
       }
       barrier();
       for (int i = 0; i < count; ++i) {
-        const int t = tbeg + i;
-        const uint32_t here = present >> 8 & 15u;
         // weights
-        advance(i);
-        if (visible(t)) {
-          if (partial(t) || here != 15u) mask(t, here);
+        issue(i);
+        if (sees_it) {
+          if (cut) mask(tbeg + i, present >> 12 & 15u);
           weigh();
         } else {
 #pragma unroll
           for (int u = 0; u < 4; ++u) w[u] = rest[u] = uintx4{0, 0, 0, 0};
         }
+        arrived();
         if (!late) {
           __builtin_amdgcn_s_waitcnt(kTwoSteps);
-          tidy(i, here);
+          tidy(i);
         }
         barrier();
         // products (of a tile that this wave's rows do not see: others see it in part, it is clean)
         asm volatile("" : "+v"(kat), "+v"(vat));                    // (formed anew in every step: registers are dearer)
         __builtin_amdgcn_s_setprio(1);
-        products(s_k[(i + 1) & 3][0], s_v[i & 3][0]);
+        products(s_k[(i + 1) & 3][0], s_v[i & 3][0], [&](int j) {
+          constexpr int kParts = 7, kEvery = (2 * KM + 4 * DB - 2) / kParts;
+          static_assert(kEvery >= 1, "every part has a product of its own");
+          if (j >= 1 && (j - 1) % kEvery == 0 && (j - 1) / kEvery < kParts) plan(i + 1, (j - 1) / kEvery);
+        });
         __builtin_amdgcn_s_setprio(0);
         if (late) {
           __builtin_amdgcn_s_waitcnt(kOneStep);
-          tidy(i + 1, present >> 8 & 15u);
+          tidy(i + 1);
         }
         barrier();
       }
@@ -1066,8 +1094,8 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
     Found found = find(tbeg + ctile);
     int page = page_of(tbeg + ctile, found);
     uint32_t copied = present_of(tbeg + ctile, found);
-    copy_k(tbeg + ctile, page, 0);
-    copy_v(tbeg + ctile, page, 0);
+    copy_k(k_from(tbeg + ctile, page), 0);
+    copy_v(v_from(tbeg + ctile, page), 0);
     for (int t = tbeg; t < tend; t += 2 * STEP) {
 #pragma unroll
       for (int bf = 0; bf < 2; ++bf) {
@@ -1083,8 +1111,8 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
           copied = present_of(next, found);
           if (tt + STEP < tend) {
             page = page_of(next, found);
-            copy_k(next, page, 1 - bf);
-            copy_v(next, page, 1 - bf);
+            copy_k(k_from(next, page), 1 - bf);
+            copy_v(v_from(next, page), 1 - bf);
           }
           if (visible(tt + mine)) {
             asm volatile("" : "+v"(kat), "+v"(vat));                // (formed anew in every step: registers are dearer)
