@@ -795,7 +795,10 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
   const int crun = ctok / 16;                                       // the run of this wave's copies
   struct Found { int id[4], own; };
   auto find = [&](int t) {
-    auto id = [&](int r) { return pages[min((t * kTileTokens + 16 * r) >> c.page_shift, last_blk)]; };
+    auto id = [&](int r) {                                          // (32-bit offsets: a table row has less than 2^28 bytes)
+      const uint32_t at = 4 * min((t * kTileTokens + 16 * r) >> c.page_shift, last_blk);
+      return *(constant_t)((const __attribute__((address_space(4))) char*)pages + at);
+    };
     return Found{{id(0), id(1), id(2), id(3)}, id(crun)};
   };
   auto held = [&](int t, int id, int r) {                           // 1 or 0, without branches
@@ -832,9 +835,6 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
   float ref = 0.f, sum = 0.f;                                       // the reference in units of <q, k>
-  floatx16 minus_ref;                                               // what scores start from: they come out less the reference
-#pragma unroll
-  for (int i = 0; i < 16; ++i) minus_ref[i] = 0.f;
   // LDS bytes: key row col, chunk 2 k + half of the map; value row 4 half + (lane & 15) / 4
   // and its 4 columns.  A step forms the others from these by exclusive or.
   int kat = 2 * (col * DH + 8 * ((dim0 / 8 + half) ^ k_swizzle(col)));
@@ -884,7 +884,8 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
   auto scores = [&](const uint16_t* kt) {
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-      sc[x] = minus_ref;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sc[x][i] = -ref;                 // (scores come out less the reference)
 #pragma unroll
       for (int k = 0; k < KM; ++k) sc[x] = mfma32<TYPE>(k_at(kt, x, k), q[k], sc[x]);
     }
@@ -930,8 +931,6 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
       const bool fresh = halves_max(sum) == 0.f, moves = top > -INFINITY && (fresh || fmaf(top, cq, kTopWeight) > kMostWeight);
       const float shift = moves ? top : 0.f, f = fresh ? 1.f : exp2_of(-shift * cq);
       ref += shift;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) minus_ref[i] = -ref;
       sum *= f;
 #pragma unroll
       for (int d = 0; d < DB; ++d) acc[d] *= f;
@@ -956,10 +955,11 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
     constexpr int NK = 2 * KM, N = NK + 4 * DB, kAheadReads = 6;
     uintx4 a[kAheadReads + 1];
     auto read = [&](int j) { a[j % (kAheadReads + 1)] = j < NK ? k_at(kt, j / KM, j % KM) : v_at(vt, (j - NK) / DB, (j - NK) % DB); };
-    sc[0] = sc[1] = minus_ref;
 #pragma unroll
     for (int j = 0; j < kAheadReads; ++j) read(j);
     __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sc[0][i] = sc[1][i] = -ref;        // (scores come out less the reference)
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       if (j + kAheadReads < N) read(j + kAheadReads);
@@ -998,17 +998,29 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
     const uint16_t* kfrom = kh;
     const uint16_t* vfrom = vh;
     int sees_it = 0, cut = 0, dirty = 0;                            // tile i: rows see it, some in part; cleaned
+    // (or they would be worked out where they are used)
+    auto pinned = [](int x) {
+      x = uniform(x);
+      asm volatile("" : "+s"(x));
+      return x;
+    };
+    auto pinned64 = [](int64_t x) {
+      x = uniform64(x);
+      asm volatile("" : "+s"(x));
+      return x;
+    };
     // step i's, in parts; `found` is tile i + 3's
     auto plan = [&](int i, int part) {
       const int t = tbeg + i;
+      const uint32_t here = present >> 12 & 15u;
       switch (part) {
-        case 0: vfrom = v_from(t + 2, page); break;
-        case 1: page = page_of(t + 3, found); break;
-        case 2: kfrom = k_from(t + 3, page); break;
-        case 3: present = present << 4 | present_of(t + 3, found); break;
-        case 4: sees_it = visible(t); break;
-        case 5: cut = partial(t) | (int)((present >> 12 & 15u) != 15u); break;
-        default: dirty = (int)(t < tend) & unclean(t, present >> 12 & 15u);
+        case 0: vfrom = (const uint16_t*)pinned64((int64_t)v_from(t + 2, page)); break;
+        case 1: page = pinned(page_of(t + 3, found)); break;
+        case 2: kfrom = (const uint16_t*)pinned64((int64_t)k_from(t + 3, page)); break;
+        case 3: present = pinned(present << 4 | present_of(t + 3, found)); break;
+        case 4: sees_it = pinned(visible(t)); break;
+        case 5: cut = pinned(partial(t) | (int)(here != 15u)); break;
+        default: dirty = pinned((int)(t < tend) & unclean(t, here));
       }
     };
     auto plan_all = [&](int i) {
