@@ -787,45 +787,18 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
   auto k_swizzle = [](int t) { return DH == 128 ? t & 15 : (t >> 1) & 7; };
   auto v_swizzle = [](int t) { return DH == 128 ? (t & 3) << 2 : (t & 2) << 1; };
   const uint32_t ktok = 2 * ltok * c.k_token, kchunk = 16 * (lch ^ k_swizzle(ltok));
-  const uint32_t voff = 2 * ltok * c.v_token + 16 * (lch ^ v_swizzle(ltok));
-  // The page of run `run` of tile t, or -1, by scalar loads (whose waits are apart
-  // from those of the copies); a tile's four pages as bits.
-  typedef const __attribute__((address_space(4))) int32_t* constant_t;
-  const constant_t pages = (constant_t)(uintptr_t)table;
-  const int crun = ctok / 16;                                       // the run of this wave's copies
-  struct Found { int id[4], own; };
-  auto find = [&](int t) {
-    auto id = [&](int r) {                                          // (32-bit offsets: a table row has less than 2^28 bytes)
-      const uint32_t at = 4 * min((t * kTileTokens + 16 * r) >> c.page_shift, last_blk);
-      return *(constant_t)((const __attribute__((address_space(4))) char*)pages + at);
-    };
-    return Found{{id(0), id(1), id(2), id(3)}, id(crun)};
-  };
-  auto held = [&](int t, int id, int r) {                           // 1 or 0, without branches
-    return (int)(t * kTileTokens + 16 * r < len) & (int)((uint32_t)id < (uint32_t)c.num_pages);
-  };
-  auto present_of = [&](int t, const Found& f) {
-    return (uint32_t)(held(t, f.id[0], 0) | held(t, f.id[1], 1) << 1 | held(t, f.id[2], 2) << 2 | held(t, f.id[3], 3) << 3);
-  };
-  auto page_of = [&](int t, const Found& f) { return f.own & -held(t, f.own, crun); };   // (page 0 in an absent one's place)
-  // Every call issues the same copies.  Of an absent page they read page 0, behind the
-  // length what the page holds: the tile is cleaned then.
-  auto k_from = [&](int t, int page) {
-    return kh + (int64_t)page * c.k_page + (((t * kTileTokens + 16 * crun) & ps_mask) + (ctok & 15)) * c.k_token;
-  };
-  auto v_from = [&](int t, int page) {
-    return vh + (int64_t)page * c.v_page + (((t * kTileTokens + 16 * crun) & ps_mask) + (ctok & 15)) * c.v_token;
-  };
-  auto copy_k = [&](const uint16_t* from, int bf) {
+  const uint32_t vtok = 2 * ltok * c.v_token + 16 * (lch ^ v_swizzle(ltok));
+  // This wave's copies, of run crun of a tile: offsets of a lane, then of the tile.
+  const int crun = ctok / 16;
+  uint32_t koff[NL], voff[NL];
 #pragma unroll
-    for (int i = 0; i < NL; ++i)
-      copy_to_lds(from + i * RPL * c.k_token, ktok + (kchunk ^ 16 * k_swizzle((ctok & 15) + i * RPL)),
-                  lds_address(&s_k[bf][ctile][(ctok + i * RPL) * DH]));
-  };
-  auto copy_v = [&](const uint16_t* from, int bf) {
+  for (int i = 0; i < NL; ++i) {
+    koff[i] = ktok + 2 * i * RPL * c.k_token + (kchunk ^ 16 * k_swizzle((ctok & 15) + i * RPL));
+    voff[i] = vtok + 2 * i * RPL * c.v_token;
+  }
+  auto copy = [&](const uint16_t* from, const uint32_t (&off)[NL], uint16_t* tile) {
 #pragma unroll
-    for (int i = 0; i < NL; ++i)
-      copy_to_lds(from + i * RPL * c.v_token, voff, lds_address(&s_v[bf][ctile][(ctok + i * RPL) * DH]));
+    for (int i = 0; i < NL; ++i) copy_to_lds(from, off[i], lds_address(tile + (ctok + i * RPL) * DH));
   };
   static_assert(DH == 128 ? RPL % 4 == 0 : RPL % 4 == 0, "the values' chunks turn by a token's low bits");
 
@@ -849,18 +822,48 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
     return uintx4{x[0], x[1], y[0], y[1]};
   };
 
-  // tile t: rows of the wave that see it; some that see it in part
-  auto visible = [&](int t) { return (int)(t < tend) & (int)(t * kTileTokens < lim_max) & (int)((t + 1) * kTileTokens > lo_min); };
-  auto partial = [&](int t) { return (int)((t + 1) * kTileTokens > lim_min) | (int)(t * kTileTokens < lo_max); };
-  // A tile that some rows of the workgroup see in part, or with an absent page, is
-  // cleaned by the waves that copied it, before any reads it: values of tokens that
-  // are not there and values that are not finite become zeros.
+  // What the steps need to know of the tiles, 64 at a time, a lane each: where this
+  // wave's copies come from, and the tile's cases.  Of an absent page the copies read
+  // page 0, behind the length what the page holds.  A tile that some rows of the
+  // workgroup see in part, or that is not all there, is cleaned by the waves that
+  // copied it, before any reads it: values of tokens that are not there and values
+  // that are not finite become zeros.
+  enum { kVisible = 16, kCut = 32, kUnclean = 64 };                   // low bits: the runs that have a page
   const int first_tok = (int)(r0 / gqa), all_lim = row_sees(L, len, n, first_tok).hi, all_lo = row_sees(L, len, n, last / gqa).lo;
-  auto unclean = [&](int t, uint32_t present) {
-    return (int)(present != 15u) | (int)((t + 1) * kTileTokens > all_lim) | (int)(t * kTileTokens < all_lo);
+  int64_t kplace = 0, vplace = 0;                                     // elements
+  int cases = 0, batch = 0;                                           // the batch's first tile
+  auto cases_of = [&](int t, int& own) {
+    int f = 0;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int at = t * kTileTokens + 16 * r, id = table[min(at >> c.page_shift, last_blk)];
+      const bool held = at < len && (uint32_t)id < (uint32_t)c.num_pages;
+      f |= held ? 1 << r : 0;
+      if (r == crun) own = held ? id : 0;
+    }
+    const int a = t * kTileTokens, b = a + kTileTokens;
+    if (t < tend && a < lim_max && b > lo_min) f |= kVisible;
+    if (f % 16 != 15 || b > lim_min || a < lo_max) f |= kCut;
+    if (t < tend && (f % 16 != 15 || b > all_lim || a < all_lo)) f |= kUnclean;
+    return f;
   };
-  auto clean = [&](int t, uint32_t present, uint16_t* vt) {
-    const int have = present >> crun & 1 ? len - t * kTileTokens - 16 * crun : 0;
+  auto look_up = [&](int t) {
+    int own = 0;
+    batch = t;
+    cases = cases_of(t + lane, own);
+    const int slot = (((t + lane) * kTileTokens + 16 * crun) & ps_mask) + (ctok & 15);
+    kplace = own * c.k_page + (int64_t)slot * c.k_token;
+    vplace = own * c.v_page + (int64_t)slot * c.v_token;
+  };
+  auto of_tile = [&](int64_t x, int t) {                              // a tile's, from its lane
+    const int lo = __builtin_amdgcn_readlane((int)x, t - batch), hi = __builtin_amdgcn_readlane((int)(x >> 32), t - batch);
+    return ((int64_t)hi << 32) | (uint32_t)lo;
+  };
+  auto k_from = [&](int t) { return kh + of_tile(kplace, t); };
+  auto v_from = [&](int t) { return vh + of_tile(vplace, t); };
+  auto cases_at = [&](int t) { return __builtin_amdgcn_readlane(cases, t - batch); };
+  auto clean = [&](int t, int what, uint16_t* vt) {
+    const int have = what >> crun & 1 ? len - t * kTileTokens - 16 * crun : 0;
     uint32_t bad = 0;
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
@@ -890,12 +893,12 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
       for (int k = 0; k < KM; ++k) sc[x] = mfma32<TYPE>(k_at(kt, x, k), q[k], sc[x]);
     }
   };
-  // scores of tile t that do not count; present: a bit for each run that has a page
-  auto mask = [&](int t, uint32_t present) {
+  // scores of tile t that do not count
+  auto mask = [&](int t, int what) {
     const uint32_t first = t * kTileTokens + 4 * half - lo, width = lim - lo;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const uint32_t n = present >> u & 1 ? width : 0u;
+      const uint32_t n = what >> u & 1 ? width : 0u;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int e = 8 * (u & 1) + i;
@@ -982,58 +985,25 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
     // The matrix part of a step (scores of the next tile, values of this one) by one
     // half of the waves while the other half, on the same SIMDs, is at its weights:
     // a barrier ends each part.  Step i's matrix part reads K(i + 1) and V(i), one half
-    // of the waves a part after the other; its part of weights issues the copies of
-    // K(i + 3) and V(i + 2), over what every wave has read by then.  What the next
-    // matrix parts read has arrived when all but the last steps' copies have (each step
-    // issues 2 NL, and nothing else), and is cleaned, by every wave before the barrier
-    // that the first of them waits at.
-    // The next step's addresses and cases are worked out among the products, where
-    // the wave has time; pages are looked up a step before that.
+    // of the waves a part after the other, and issues the copies of K(i + 4) and
+    // V(i + 3), over what every wave has read by then.  What the next matrix parts read
+    // has arrived when all but the last two steps' copies have (each step issues 2 NL,
+    // and nothing else), and is cleaned, by every wave before the barrier that the
+    // first of them waits at.
     static_assert(NL == 1 || NL == 2, "copies of a step");
-    constexpr int kOneStep = 0x0F70 | (2 * NL), kTwoSteps = 0x0F70 | (4 * NL);
+    constexpr int kTwoSteps = 0x0F70 | (4 * NL), kPrologue = 0x0F70 | (6 * NL);
     const bool late = wave >= 4;
-    uint32_t present = 0;                                           // of four tiles, the latest in the low bits
-    int page = 0;                                                   // this wave's, of the latest tile
-    Found found = find(tbeg);
-    const uint16_t* kfrom = kh;
-    const uint16_t* vfrom = vh;
-    int sees_it = 0, cut = 0, dirty = 0;                            // tile i: rows see it, some in part; cleaned
-    // (or they would be worked out where they are used)
-    auto pinned = [](int x) {
-      x = uniform(x);
-      asm volatile("" : "+s"(x));
-      return x;
-    };
-    auto pinned64 = [](int64_t x) {
-      x = uniform64(x);
-      asm volatile("" : "+s"(x));
-      return x;
-    };
-    // step i's, in parts; `found` is tile i + 3's
-    auto plan = [&](int i, int part) {
+    int what = 0;                                                   // of the next step's tile
+    // what step i does beside its products, in parts
+    auto advance = [&](int i, int part) {
       const int t = tbeg + i;
-      const uint32_t here = present >> 12 & 15u;
       switch (part) {
-        case 0: vfrom = (const uint16_t*)pinned64((int64_t)v_from(t + 2, page)); break;
-        case 1: page = pinned(page_of(t + 3, found)); break;
-        case 2: kfrom = (const uint16_t*)pinned64((int64_t)k_from(t + 3, page)); break;
-        case 3: present = pinned(present << 4 | present_of(t + 3, found)); break;
-        case 4: sees_it = pinned(visible(t)); break;
-        case 5: cut = pinned(partial(t) | (int)(here != 15u)); break;
-        default: dirty = pinned((int)(t < tend) & unclean(t, here));
+        case 0: copy(v_from(t + 3), voff, s_v[(i + 3) & 3][0]); break;
+        case 1: copy(k_from(t + 4), koff, s_k[(i + 4) & 3][0]); break;
+        default:
+          what = cases_at(t + 1);
+          asm volatile("" : "+s"(what));                            // (here, not where it is used)
       }
-    };
-    auto plan_all = [&](int i) {
-#pragma unroll
-      for (int part = 0; part < 7; ++part) plan(i, part);
-    };
-    auto issue = [&](int i) {
-      if (i >= -2) copy_v(vfrom, (i + 2) & 3);
-      copy_k(kfrom, (i + 3) & 3);
-      found = find(tbeg + i + 4);
-    };
-    auto arrived = [&]() {                                          // (waited for here, not among the products)
-      asm volatile("" :: "s"(found.id[0]), "s"(found.id[1]), "s"(found.id[2]), "s"(found.id[3]), "s"(found.own));
     };
     auto barrier = [&]() {
       __builtin_amdgcn_sched_barrier(0);
@@ -1044,56 +1014,54 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
     };
     // cleans this wave's part of V(i)
     auto tidy = [&](int i) {
-      if (dirty) {
-        clean(tbeg + i, present >> 12 & 15u, s_v[i & 3][0]);
+      if (what & kUnclean) {
+        clean(tbeg + i, what, s_v[i & 3][0]);
         __builtin_amdgcn_s_waitcnt(0xC07F);                         // lgkmcnt(0)
       }
     };
     const int count = tend - tbeg;
     if (count > 0) {
+      look_up(tbeg);
+      copy(k_from(tbeg), koff, s_k[0][0]);
 #pragma unroll
-      for (int i = -3; i < 0; ++i) {
-        plan_all(i);
-        issue(i);
+      for (int i = 1; i < 4; ++i) {
+        copy(v_from(tbeg + i - 1), voff, s_v[i - 1][0]);
+        copy(k_from(tbeg + i), koff, s_k[i][0]);
       }
-      arrived();
-      __builtin_amdgcn_s_waitcnt(kTwoSteps);                        // K(0)
+      what = cases_at(tbeg);
+      __builtin_amdgcn_s_waitcnt(kPrologue);                        // K(0)
       barrier();
       if (late) barrier();
       scores(s_k[0][0]);
-      plan_all(0);
       if (late) {
-        __builtin_amdgcn_s_waitcnt(kOneStep);
+        __builtin_amdgcn_s_waitcnt(kTwoSteps);
         tidy(0);
       }
       barrier();
       for (int i = 0; i < count; ++i) {
         // weights
-        issue(i);
-        if (sees_it) {
-          if (cut) mask(tbeg + i, present >> 12 & 15u);
+        if (what & kVisible) {
+          if (what & kCut) mask(tbeg + i, what);
           weigh();
         } else {
 #pragma unroll
           for (int u = 0; u < 4; ++u) w[u] = rest[u] = uintx4{0, 0, 0, 0};
         }
-        arrived();
         if (!late) {
           __builtin_amdgcn_s_waitcnt(kTwoSteps);
           tidy(i);
         }
         barrier();
         // products (of a tile that this wave's rows do not see: others see it in part, it is clean)
+        if (tbeg + i + 4 - batch >= kWave) look_up(tbeg + i + 1);   // (its loads wait for the copies, too)
         asm volatile("" : "+v"(kat), "+v"(vat));                    // (formed anew in every step: registers are dearer)
         __builtin_amdgcn_s_setprio(1);
         products(s_k[(i + 1) & 3][0], s_v[i & 3][0], [&](int j) {
-          constexpr int kParts = 7, kEvery = (2 * KM + 4 * DB - 2) / kParts;
-          static_assert(kEvery >= 1, "every part has a product of its own");
-          if (j >= 1 && (j - 1) % kEvery == 0 && (j - 1) / kEvery < kParts) plan(i + 1, (j - 1) / kEvery);
+          if (j == 1 || j == 4 || j == 7) advance(i, (j - 1) / 3);
         });
         __builtin_amdgcn_s_setprio(0);
         if (late) {
-          __builtin_amdgcn_s_waitcnt(kOneStep);
+          __builtin_amdgcn_s_waitcnt(kTwoSteps);
           tidy(i + 1);
         }
         barrier();
@@ -1103,34 +1071,29 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
     }
   } else if (tbeg < tend) {
     const int mine = kTurns ? group : 0;
-    Found found = find(tbeg + ctile);
-    int page = page_of(tbeg + ctile, found);
-    uint32_t copied = present_of(tbeg + ctile, found);
-    copy_k(k_from(tbeg + ctile, page), 0);
-    copy_v(v_from(tbeg + ctile, page), 0);
+    look_up(tbeg);
+    copy(k_from(tbeg + ctile), koff, s_k[0][ctile]);
+    copy(v_from(tbeg + ctile), voff, s_v[0][ctile]);
     for (int t = tbeg; t < tend; t += 2 * STEP) {
 #pragma unroll
       for (int bf = 0; bf < 2; ++bf) {
         const int tt = t + bf * STEP;
         if (tt < tend) {
-          const int next = tt + STEP + ctile;
-          found = find(next);
-          const uint32_t here = kTurns ? present_of(tt + mine, find(tt + mine)) : copied;
+          const int what = cases_at(tt + mine), copied = cases_at(tt + ctile);
           // this step's bytes have arrived and are clean, for every wave; the other buffer is read no more
           __builtin_amdgcn_s_waitcnt(0x0F70);                       // vmcnt(0)
-          if (unclean(tt + ctile, copied)) clean(tt + ctile, copied, s_v[bf][ctile]);
+          if (copied & kUnclean) clean(tt + ctile, copied, s_v[bf][ctile]);
           __syncthreads();
-          copied = present_of(next, found);
           if (tt + STEP < tend) {
-            page = page_of(next, found);
-            copy_k(k_from(next, page), 1 - bf);
-            copy_v(v_from(next, page), 1 - bf);
+            if (tt + 2 * STEP - 1 - batch >= kWave) look_up(tt + STEP);
+            copy(k_from(tt + STEP + ctile), koff, s_k[1 - bf][ctile]);
+            copy(v_from(tt + STEP + ctile), voff, s_v[1 - bf][ctile]);
           }
-          if (visible(tt + mine)) {
+          if (what & kVisible) {
             asm volatile("" : "+v"(kat), "+v"(vat));                // (formed anew in every step: registers are dearer)
             scores(s_k[bf][mine]);
             groups_ahead<2 * KM, 1, 1, KM < 6 ? KM : 6>();
-            if (partial(tt + mine) || here != 15u) mask(tt + mine, here);
+            if (what & kCut) mask(tt + mine, what);
             weigh();
             values(s_v[bf][mine]);
             groups_ahead<4 * DB, 2, kRest ? 2 : 1, DB < 4 ? DB : 4>();
@@ -1145,12 +1108,13 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
   if (s_odd) {
 #pragma unroll 1
     for (int t = tbeg; t < tend; ++t) {
-      const Found f = find(t);
-      if (!unclean(t, present_of(t, f)) || (kTurns && ((t - tbeg) & 1) != group)) continue;
+      int own = 0;
+      const int what = uniform(cases_of(t, own));
+      if (!(what & kUnclean) || (kTurns && ((t - tbeg) & 1) != group)) continue;
 #pragma unroll 1
       for (int token = t * kTileTokens; token < (t + 1) * kTileTokens; ++token) {
-        if (!(present_of(t, f) >> (token >> 4 & 3) & 1) || token < lo || token >= lim) continue;
-        const uint16_t* v = vh + (int64_t)pages[token >> c.page_shift] * c.v_page + (token & ps_mask) * c.v_token;
+        if (!(what >> (token >> 4 & 3) & 1) || token < lo || token >= lim) continue;
+        const uint16_t* v = vh + (int64_t)table[token >> c.page_shift] * c.v_page + (token & ps_mask) * c.v_token;
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
 #pragma unroll
