@@ -796,9 +796,12 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
     koff[i] = ktok + 2 * i * RPL * c.k_token + (kchunk ^ 16 * k_swizzle((ctok & 15) + i * RPL));
     voff[i] = vtok + 2 * i * RPL * c.v_token;
   }
+  auto copy_one = [&](const uint16_t* from, const uint32_t (&off)[NL], uint16_t* tile, int i) {
+    copy_to_lds(from, off[i], lds_address(tile + (ctok + i * RPL) * DH));
+  };
   auto copy = [&](const uint16_t* from, const uint32_t (&off)[NL], uint16_t* tile) {
 #pragma unroll
-    for (int i = 0; i < NL; ++i) copy_to_lds(from, off[i], lds_address(tile + (ctok + i * RPL) * DH));
+    for (int i = 0; i < NL; ++i) copy_one(from, off, tile, i);
   };
   static_assert(DH == 128 ? RPL % 4 == 0 : RPL % 4 == 0, "the values' chunks turn by a token's low bits");
 
@@ -953,20 +956,24 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
       }
   };
   // Both, in this order: each product with the reads of the one kAheadReads later
-  // before it (a SIMD's matrix cores have this wave alone then), and between(j) behind it.
-  auto products = [&](const uint16_t* kt, const uint16_t* vt, auto&& between) {
-    constexpr int NK = 2 * KM, N = NK + 4 * DB, kAheadReads = 6;
-    uintx4 a[kAheadReads + 1];
-    auto read = [&](int j) { a[j % (kAheadReads + 1)] = j < NK ? k_at(kt, j / KM, j % KM) : v_at(vt, (j - NK) / DB, (j - NK) % DB); };
+  // before it (a SIMD's matrix cores have this wave alone then), and between(j) behind
+  // it.  The first reads come before, by read_ahead.
+  constexpr int NK = 2 * KM, kProducts = NK + 4 * DB, kAheadReads = 6;
+  uintx4 part[kAheadReads + 1];
+  auto read_ahead = [&](const uint16_t* kt) {
 #pragma unroll
-    for (int j = 0; j < kAheadReads; ++j) read(j);
-    __builtin_amdgcn_sched_barrier(0);
+    for (int j = 0; j < kAheadReads; ++j) part[j] = j < NK ? k_at(kt, j / KM, j % KM) : uintx4{0, 0, 0, 0};
+  };
+  auto products = [&](const uint16_t* kt, const uint16_t* vt, auto&& between) {
+    auto read = [&](int j) { return j < NK ? k_at(kt, j / KM, j % KM) : v_at(vt, (j - NK) / DB, (j - NK) % DB); };
+#pragma unroll
+    for (int j = NK; j < kAheadReads; ++j) part[j] = read(j);
 #pragma unroll
     for (int i = 0; i < 16; ++i) sc[0][i] = sc[1][i] = -ref;        // (scores come out less the reference)
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      if (j + kAheadReads < N) read(j + kAheadReads);
-      const uintx4 x = a[j % (kAheadReads + 1)];
+    for (int j = 0; j < kProducts; ++j) {
+      if (j + kAheadReads < kProducts) part[(j + kAheadReads) % (kAheadReads + 1)] = read(j + kAheadReads);
+      const uintx4 x = part[j % (kAheadReads + 1)];
       if (j < NK) {
         sc[j / KM] = mfma32<TYPE>(x, q[j % KM], sc[j / KM]);
       } else {
@@ -986,23 +993,33 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
     // half of the waves while the other half, on the same SIMDs, is at its weights:
     // a barrier ends each part.  Step i's matrix part reads K(i + 1) and V(i), one half
     // of the waves a part after the other, and issues the copies of K(i + 4) and
-    // V(i + 3), over what every wave has read by then.  What the next matrix parts read
-    // has arrived when all but the last two steps' copies have (each step issues 2 NL,
-    // and nothing else), and is cleaned, by every wave before the barrier that the
-    // first of them waits at.
+    // V(i + 3), over what every wave has read by then.  The first keys are read before
+    // the barrier that the part starts at; so K(i + 1) and V(i) have to arrive a part
+    // earlier than the first half reads them: the first half waits behind its products
+    // i - 1, for all but the last two steps' copies (each step issues 2 NL, and nothing
+    // else), the second behind its weights i - 1, for all but the last step's.  V(i) is
+    // cleaned before the barrier that the first half's products i start at.
     static_assert(NL == 1 || NL == 2, "copies of a step");
-    constexpr int kTwoSteps = 0x0F70 | (4 * NL), kPrologue = 0x0F70 | (6 * NL);
+    constexpr int kOneStep = 0x0F70 | (2 * NL), kTwoSteps = 0x0F70 | (4 * NL), kPrologue = 0x0F70 | (6 * NL);
     const bool late = wave >= 4;
     int what = 0;                                                   // of the next step's tile
-    // what step i does beside its products, in parts
+    const uint16_t* from = kh;
+    // what step i does beside its products, in parts (a copy takes as long to issue as
+    // a product, and the scores' part has less time to spare)
+    constexpr int kParts = 3 + 2 * NL;
     auto advance = [&](int i, int part) {
       const int t = tbeg + i;
-      switch (part) {
-        case 0: copy(v_from(t + 3), voff, s_v[(i + 3) & 3][0]); break;
-        case 1: copy(k_from(t + 4), koff, s_k[(i + 4) & 3][0]); break;
-        default:
-          what = cases_at(t + 1);
-          asm volatile("" : "+s"(what));                            // (here, not where it is used)
+      if (part == 0) {
+        what = cases_at(t + 1);
+        asm volatile("" : "+s"(what));                              // (here, not where it is used)
+      } else if (part == 1) {
+        from = v_from(t + 3);
+      } else if (part < 2 + NL) {
+        copy_one(from, voff, s_v[(i + 3) & 3][0], part - 2);
+      } else if (part == 2 + NL) {
+        from = k_from(t + 4);
+      } else {
+        copy_one(from, koff, s_k[(i + 4) & 3][0], part - 3 - NL);
       }
     };
     auto barrier = [&]() {
@@ -1031,12 +1048,13 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
       what = cases_at(tbeg);
       __builtin_amdgcn_s_waitcnt(kPrologue);                        // K(0)
       barrier();
-      if (late) barrier();
-      scores(s_k[0][0]);
       if (late) {
         __builtin_amdgcn_s_waitcnt(kTwoSteps);
-        tidy(0);
+        barrier();
       }
+      scores(s_k[0][0]);
+      if (!late) __builtin_amdgcn_s_waitcnt(kTwoSteps);
+      if (late) tidy(0);
       barrier();
       for (int i = 0; i < count; ++i) {
         // weights
@@ -1047,23 +1065,22 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
 #pragma unroll
           for (int u = 0; u < 4; ++u) w[u] = rest[u] = uintx4{0, 0, 0, 0};
         }
-        if (!late) {
-          __builtin_amdgcn_s_waitcnt(kTwoSteps);
-          tidy(i);
-        }
+        asm volatile("" : "+v"(kat), "+v"(vat));                    // (formed anew in every step: registers are dearer)
+        read_ahead(s_k[(i + 1) & 3][0]);
+        if (!late) tidy(i);
+        if (late) __builtin_amdgcn_s_waitcnt(kOneStep);
         barrier();
         // products (of a tile that this wave's rows do not see: others see it in part, it is clean)
-        if (tbeg + i + 4 - batch >= kWave) look_up(tbeg + i + 1);   // (its loads wait for the copies, too)
-        asm volatile("" : "+v"(kat), "+v"(vat));                    // (formed anew in every step: registers are dearer)
         __builtin_amdgcn_s_setprio(1);
         products(s_k[(i + 1) & 3][0], s_v[i & 3][0], [&](int j) {
-          if (j == 1 || j == 4 || j == 7) advance(i, (j - 1) / 3);
+          constexpr int kFirst = kProducts / 2 - 1, kEvery = (kProducts - kFirst) / kParts;
+          static_assert(kEvery >= 1, "every part has a product of its own");
+          if (j == 0 && tbeg + i + 4 - batch >= kWave) look_up(tbeg + i + 1);   // (its loads wait for the copies, too)
+          if (j >= kFirst && (j - kFirst) % kEvery == 0 && (j - kFirst) / kEvery < kParts) advance(i, (j - kFirst) / kEvery);
         });
         __builtin_amdgcn_s_setprio(0);
-        if (late) {
-          __builtin_amdgcn_s_waitcnt(kTwoSteps);
-          tidy(i + 1);
-        }
+        if (!late) __builtin_amdgcn_s_waitcnt(kTwoSteps);
+        if (late) tidy(i + 1);
         barrier();
       }
       if (!late) barrier();
