@@ -752,7 +752,8 @@ int sphkv_cache8_prefill(const void* q, int32_t q_type, int64_t q_row_stride, in
  * 16, 32, 64 or 128, num_kv at most 1024.  The struct is read during the call.
  *
  * table, cu_rows, start, lens, num_rows, num_seqs, workspace, stream and their
- * limits are those of the 8-bit cache above: a page outside [0, num_pages) holds
+ * limits (an append: fewer than 2^26 - 3 rows, and none of its page limit) are those
+ * of the 8-bit cache above: a page outside [0, num_pages) holds
  * no token.  Rows of k, v, q and q_out may have any row and head stride and the
  * alignment of their elements, their dh elements are contiguous.
  */

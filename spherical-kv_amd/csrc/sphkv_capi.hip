@@ -1303,8 +1303,8 @@ int sphkv_cache16_append(const sphkv_cache16* cache, const void* k, const void* 
     return fail(SPHKV_EINVAL, "%s: inv_freq must be fp32 or fp64 (type %d)", fn, freq_type);
   if (!cu_rows && num_rows != num_seqs)
     return fail(SPHKV_EINVAL, "%s: without cu_rows there is one row per sequence", fn);
-  // (a wave of 64 threads per row: fewer than 2^32 in a grid)
-  if (num_rows >= 1 << 26) return fail(SPHKV_EINVAL, "%s: num_rows must be below 2^26", fn);
+  // (a wave of 64 threads per row, four to a workgroup: fewer than 2^32 in a grid)
+  if (num_rows > (1 << 26) - 4) return fail(SPHKV_EINVAL, "%s: num_rows must be below 2^26 - 3", fn);
   if (num_seqs == 0 || num_rows == 0) return ok();
   if (!k || !v || !start || (q && !q_out) || (num_freqs > 0 && !inv_freq))
     return fail(SPHKV_EINVAL, "%s: null pointer argument", fn);

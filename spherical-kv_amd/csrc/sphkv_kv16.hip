@@ -252,7 +252,11 @@ __device__ __forceinline__ void finish_row(const Cache16AttendLaunch& L, int64_t
 // leave a partial per workgroup (two at most: its first and its last pair) for the
 // merge kernel.
 constexpr int kDecodeTile = 32, kDecodeWaves = 4;
-__host__ __device__ constexpr int decode_groups(int) { return 512; }
+// Workgroups: as many as run at once by their registers, two per CU at dh 128 and
+// three at 64.  (64 contexts of 150 to 2,100 tokens, 8 kv heads of 8 query heads, dh
+// 64: 31.5 us with 768, 32.5 with 512.  dh 128 in the registers of three per CU
+// spills: 32K tokens in 31.7 us, 27.3 with two.)
+__host__ __device__ constexpr int decode_groups(int dh) { return dh == 128 ? 512 : 768; }
 
 // columns handled together: a kv head's first 16, next 16, ...
 __host__ __device__ __forceinline__ int col_parts(int cols) { return (cols + 15) / 16; }

@@ -51,7 +51,7 @@ class Cache16:
     another Cache16."""
 
     __slots__ = ("_k", "_v", "_num_pages", "_num_kv", "_page_size", "_dh", "_device", "_dtype", "_index", "_type", "_struct",
-                 "_ref", "_sm")
+                 "_ref", "_at", "_sm")
     k, v, dtype, device = (property(attrgetter(n)) for n in ("_k", "_v", "_dtype", "_device"))
     num_pages, num_kv = property(attrgetter("_num_pages")), property(attrgetter("_num_kv"))
     page_size, dh = property(attrgetter("_page_size")), property(attrgetter("_dh"))
@@ -84,7 +84,8 @@ class Cache16:
         self._k, self._v, self._dtype, self._device, self._index = k, v, k.dtype, k.device, k.device.index
         self._num_pages, self._num_kv, self._page_size, self._dh = num_pages, num_kv, page_size, dh
         self._type, self._sm = _TYPES[k.dtype], 1.0 / math.sqrt(dh)
-        self._struct = sphkv_lib.Cache16Struct(k.data_ptr(), v.data_ptr(), *strides, num_pages, num_kv, dh, page_size, self._type)
+        self._at = k.data_ptr(), v.data_ptr()
+        self._struct = sphkv_lib.Cache16Struct(*self._at, *strides, num_pages, num_kv, dh, page_size, self._type)
         self._ref = ctypes.addressof(self._struct)
 
     @staticmethod
@@ -96,7 +97,9 @@ class Cache16:
 
     def _address(self) -> int:
         """The struct's address, over what the tensors are now."""
-        self._struct.k, self._struct.v = self._k.data_ptr(), self._v.data_ptr()
+        at = self._k.data_ptr(), self._v.data_ptr()
+        if at != self._at:
+            self._struct.k, self._struct.v = self._at = at
         return self._ref
 
     def _call(self, fn, *args) -> None:
@@ -133,6 +136,8 @@ def cache16_append(cache: Cache16, k: torch.Tensor, v: torch.Tensor, table: torc
     Keys and values past the table, of a sequence with a negative start or of a
     page outside the cache are dropped; rows behind the last sequence are left as
     they were in q_out.  A written page belongs to one sequence."""
+    if parts not in (1, 2):
+        raise ValueError(f"parts must be 1 or 2, got {parts}")
     tab, stride, blocks, n = _seq_args(cache, table, start, cu_rows, "start")
     if not isinstance(k, torch.Tensor) or k.dtype not in _TYPES:
         raise TypeError("k must be an fp16, bf16 or fp32 tensor")
@@ -156,12 +161,17 @@ def cache16_append(cache: Cache16, k: torch.Tensor, v: torch.Tensor, table: torc
         gqa = shape[1] // heads
         q_row, q_head = _rows(q, "q", shape[1], dh)
         if q_out is None:
-            q_out = torch.empty(shape, dtype=cache._dtype, device=dev)
+            q_out = _like(q, cache._dtype)
         else:
             _need(q_out, cache._dtype, "q_out", dev)
             if q_out.shape != shape:
                 raise ValueError(f"q_out must be {tuple(shape)}")
         o_row, o_head = _rows(q_out, "q_out", shape[1], dh)
+        size = dh
+        for st, count in sorted(x for x in ((o_row, rows), (o_head, shape[1])) if x[1] > 1):
+            if st < size:
+                raise ValueError("rows and heads of q_out overlap")
+            size += st * (count - 1)
         q_ptr, o_ptr = q.data_ptr(), q_out.data_ptr()
     elif q_out is not None:
         raise ValueError("q_out goes with q")
@@ -177,6 +187,13 @@ def cache16_append(cache: Cache16, k: torch.Tensor, v: torch.Tensor, table: torc
                 v_row, v_head, q_row, q_head, gqa, o_ptr, o_row, o_head, rows, None if cu_rows is None else cu_rows.data_ptr(),
                 start.data_ptr(), tab, stride, blocks, n, f_ptr, f_type, freqs, parts, 1 if interleaved else 0)
     return q_out
+
+
+def _like(q: torch.Tensor, dtype) -> torch.Tensor:
+    """A contiguous tensor of q's shape."""
+    if q.dtype is dtype and q.is_contiguous():
+        return torch.empty_like(q)
+    return q.new_empty(tuple(q.shape), dtype=dtype)
 
 
 def _query(cache: Cache16, q: torch.Tensor):
@@ -226,6 +243,13 @@ def _diff_args(cache: Cache16, lam: torch.Tensor, heads: int, norm_weight: Optio
     return lam.data_ptr(), None if norm_weight is None else norm_weight.data_ptr(), float(norm_eps)
 
 
+def _window(window) -> int:
+    w = int(window)
+    if not 0 <= w < 2 ** 31 or w != window:
+        raise ValueError(f"window must be a non-negative int32, got {window}")
+    return w
+
+
 def _decode(cache, q, table, lens, window, sm_scale, out, return_lse, lse, workspace, diff):
     tab, stride, blocks, n = _seq_args(cache, table, lens, None, "lens")
     shape, gqa, q_row, q_head = _query(cache, q)
@@ -235,11 +259,11 @@ def _decode(cache, q, table, lens, window, sm_scale, out, return_lse, lse, works
         fn, more, scale, maps = _lib.sphkv_cache16_decode, (), cache._sm, ()
     else:
         fn, more, scale, maps = _lib.sphkv_cache16_diff_decode, _diff_args(cache, diff[0], shape[1], *diff[1:]), math.sqrt(2.0) * cache._sm, (2,)
-    out = _out(out, shape, cache._dtype, "out", cache)
+    out = _like(q, cache._dtype) if out is None else _out(out, shape, cache._dtype, "out", cache)
     if return_lse or lse is not None:
-        lse = _out(lse, (*shape[:2], *maps), _FLOAT, "lse", cache)
+        lse = _out(lse, (shape[0], shape[1], *maps), _FLOAT, "lse", cache)
     ws, nbytes, _keep = _workspace(cache, decode_workspace_bytes(cache, n, gqa, diff is not None), workspace)
-    cache._call(fn, cache._address(), q.data_ptr(), q_row, q_head, gqa, *more, lens.data_ptr(), int(window), tab, stride, blocks, n,
+    cache._call(fn, cache._address(), q.data_ptr(), q_row, q_head, gqa, *more, lens.data_ptr(), _window(window), tab, stride, blocks, n,
                 scale if sm_scale is None else float(sm_scale), out.data_ptr(), None if lse is None else lse.data_ptr(), ws,
                 nbytes)
     return (out, lse) if return_lse else out
@@ -254,12 +278,12 @@ def _prefill(cache, q, cu_rows, table, lens, causal, window, sm_scale, out, retu
         fn, more, scale, maps = _lib.sphkv_cache16_prefill, (), cache._sm, ()
     else:
         fn, more, scale, maps = _lib.sphkv_cache16_diff_prefill, _diff_args(cache, diff[0], shape[1], *diff[1:]), math.sqrt(2.0) * cache._sm, (2,)
-    out = _out(out, shape, cache._dtype, "out", cache)
+    out = _like(q, cache._dtype) if out is None else _out(out, shape, cache._dtype, "out", cache)
     if return_lse or lse is not None:
-        lse = _out(lse, (*shape[:2], *maps), _FLOAT, "lse", cache)
+        lse = _out(lse, (shape[0], shape[1], *maps), _FLOAT, "lse", cache)
     ws, nbytes, _keep = _workspace(cache, prefill_workspace_bytes(cache, shape[0], n, gqa, diff is not None), workspace)
     cache._call(fn, cache._address(), q.data_ptr(), q_row, q_head, gqa, *more, shape[0], cu_rows.data_ptr(), lens.data_ptr(),
-                1 if causal else 0, int(window), tab, stride, blocks, n, scale if sm_scale is None else float(sm_scale),
+                1 if causal else 0, _window(window), tab, stride, blocks, n, scale if sm_scale is None else float(sm_scale),
                 out.data_ptr(), None if lse is None else lse.data_ptr(), ws, nbytes)
     return (out, lse) if return_lse else out
 

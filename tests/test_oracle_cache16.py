@@ -7,6 +7,7 @@ import pytest
 import torch
 
 import sphkv_kv16 as kv16
+import sphkv_kv8 as kv8
 import sphkv_lib
 from oracle import cache16 as o16
 
@@ -281,3 +282,124 @@ def test_default_frequencies():
     f = kv16.rope_inv_freq(128, 500000.0, "cpu")
     assert f.dtype is torch.float64 and f.shape == (64,) and f[0] == 1.0
     assert abs(f[1].item() - 500000.0 ** (-2 / 128)) < 1e-15
+
+
+@pytest.fixture
+def on_cpu(monkeypatch):
+    """CPU tensors pass for the GPU's; a call that would be launched says so."""
+    def need(t, dtype, name, device=None):
+        if not isinstance(t, torch.Tensor) or t.dtype != dtype:
+            raise TypeError(name)
+
+    def launched(self, fn, *args):
+        raise AssertionError("launched")
+
+    for module in (kv8, kv16):
+        monkeypatch.setattr(module, "_need", need)
+    monkeypatch.setattr(kv16.Cache16, "_call", launched)
+
+
+def half(*shape):
+    return torch.zeros(shape, dtype=torch.float16)
+
+
+def ints(*x):
+    return torch.tensor(x, dtype=torch.int32)
+
+
+@pytest.mark.parametrize("k, v, msg", [
+    (half(2, 1, 16, 64), half(2, 1, 16, 128), "v must be"),
+    (half(1, 16, 64), half(1, 16, 64), "k must be"),
+    (half(2, 1, 24, 64), half(2, 1, 24, 64), "page_size must be"),
+    (half(2, 1, 16, 96), half(2, 1, 16, 96), "dh must be"),
+    (half(1, 1025, 16, 64), half(1, 1025, 16, 64), "num_kv must be"),
+    (half(2, 1, 16, 68)[..., :64], half(2, 1, 16, 64), "multiples of 8"),
+    (half(2, 1, 64, 16).transpose(2, 3)[:, :, :16], half(2, 1, 16, 64), "k must be|page_size|dh must be|contiguous"),
+    (half(4, 1, 16, 64).view(-1)[1:2049].view(2, 1, 16, 64), half(2, 1, 16, 64), "16-byte aligned"),
+])
+def test_python_refuses_caches(on_cpu, k, v, msg):
+    with pytest.raises(ValueError, match=msg):
+        kv16.Cache16(k, v)
+
+
+APPEND_ARGS = dict(k=half(2, 1, 64), v=half(2, 1, 64), table=torch.zeros((2, 1), dtype=torch.int32), start=ints(0, 0))
+
+
+@pytest.mark.parametrize("kw, error, msg", [
+    (dict(), AssertionError, "launched"),
+    (dict(q=half(2, 3, 64), q_out=half(3, 2, 64).transpose(0, 1)), AssertionError, "launched"),
+    (dict(q=half(2, 3, 64), q_out=half(2, 1, 64).expand(2, 3, 64)), ValueError, "overlap"),
+    (dict(q=half(2, 3, 64), q_out=half(1, 3, 64).expand(2, 3, 64)), ValueError, "overlap"),
+    (dict(q=half(2, 1, 64), q_out=half(100).as_strided((2, 1, 64), (32, 64, 1))), ValueError, "overlap"),
+    (dict(q=half(2, 2, 64), q_out=half(300).as_strided((2, 2, 64), (100, 64, 1))), ValueError, "overlap"),
+    (dict(q=half(2, 2, 64), q_out=half(300).as_strided((2, 2, 64), (64, 100, 1))), ValueError, "overlap"),
+    (dict(q=half(2, 2, 64), q_out=half(2, 1, 64)), ValueError, "q_out must be"),
+    (dict(q_out=half(2, 1, 64)), ValueError, "goes with q"),
+    (dict(q=half(3, 1, 64)), ValueError, "q must be"),
+    (dict(q=half(2, 0, 64)), ValueError, "q must be"),
+    (dict(q=half(2, 1, 64).float()), TypeError, "q"),
+    (dict(k=half(2, 1, 64).double()), TypeError, "k must be"),
+    (dict(v=half(3, 1, 64)), ValueError, "as many rows"),
+    (dict(v=half(2, 64, 2).transpose(1, 2)[:, :1]), ValueError, "contiguous"),
+    (dict(start=ints(0, 0, 0)), ValueError, "table must be"),
+    (dict(start=ints(0, 0).long()), TypeError, "start"),
+    (dict(table=torch.zeros((2, 2), dtype=torch.int32).t()), ValueError, "contiguous"),
+    (dict(table=torch.zeros((1, 2), dtype=torch.int32).expand(2, 2)), ValueError, "overlap"),
+    (dict(cu_rows=ints(0, 2)), ValueError, "cu_rows must be"),
+    (dict(k=half(3, 1, 64), v=half(3, 1, 64)), ValueError, "one row per sequence"),
+    (dict(parts=3), ValueError, "parts must be"),
+    (dict(parts=2 ** 32 + 1), ValueError, "parts must be"),
+    (dict(inv_freq=half(32)), TypeError, "inv_freq must be"),
+    (dict(inv_freq=torch.zeros(64)[::2]), ValueError, "inv_freq must be"),
+])
+def test_python_refuses_appends(on_cpu, kw, error, msg):
+    cache = kv16.Cache16(half(2, 1, 16, 64), half(2, 1, 16, 64))
+    with pytest.raises(error, match=msg):
+        kv16.cache16_append(cache, **{**APPEND_ARGS, **kw})
+
+
+@pytest.mark.parametrize("name", ["decode", "prefill", "diff_decode", "diff_prefill"])
+@pytest.mark.parametrize("kw, error, msg", [
+    (dict(), AssertionError, "launched"),
+    (dict(window=2 ** 31 - 1), AssertionError, "launched"),
+    (dict(window=2 ** 31), ValueError, "window must be"),
+    (dict(window=2 ** 32 + 5), ValueError, "window must be"),
+    (dict(window=-1), ValueError, "window must be"),
+    (dict(window=2.5), ValueError, "window must be"),
+    (dict(q=half(2, 0, 64)), ValueError, "q must be"),
+    (dict(q=half(2, 2, 32)), ValueError, "q must be"),
+    (dict(q=half(2, 65, 64)), ValueError, "bad num"),
+    (dict(q=half(2, 2, 64).bfloat16()), TypeError, "q"),
+    (dict(out=half(2, 4, 64)[:, ::2]), ValueError, "out must be"),
+    (dict(lse=torch.zeros(1)), ValueError, "lse must be"),
+    (dict(lens=ints(1)), ValueError, "table must be"),
+    (dict(workspace=torch.zeros(4, dtype=torch.uint8)), ValueError, "workspace"),
+])
+def test_python_refuses_attention(on_cpu, name, kw, error, msg):
+    cache = kv16.Cache16(half(2, 1, 16, 64), half(2, 1, 16, 64))
+    args = dict(q=half(2, 2, 64), table=torch.zeros((2, 1), dtype=torch.int32), lens=ints(1, 1))
+    if "prefill" in name:
+        args["cu_rows"] = ints(0, 1, 2)
+    if "diff" in name:
+        args["lam"] = torch.zeros(kw["q"].shape[1] if "q" in kw else 2)
+    with pytest.raises(error, match=msg):
+        getattr(kv16, "cache16_" + name)(cache, **{**args, **kw})
+
+
+@pytest.mark.parametrize("kw, error, msg", [
+    (dict(lam=torch.zeros(3)), ValueError, "lam must be"),
+    (dict(lam=torch.zeros(4)[::2]), ValueError, "lam must be"),
+    (dict(lam=torch.zeros(1).expand(2)), ValueError, "lam must be"),
+    (dict(lam=half(2)), TypeError, "lam"),
+    (dict(norm_weight=torch.zeros(128)[::2]), ValueError, "norm_weight must be"),
+    (dict(norm_weight=half(64)), TypeError, "norm_weight"),
+])
+def test_python_refuses_differential_weights(on_cpu, kw, error, msg):
+    cache = kv16.Cache16(half(2, 1, 16, 64), half(2, 1, 16, 64))
+    args = dict(q=half(2, 2, 64), lam=torch.zeros(2), table=torch.zeros((2, 1), dtype=torch.int32), lens=ints(1, 1))
+    with pytest.raises(error, match=msg):
+        kv16.cache16_diff_decode(cache, **{**args, **kw})
+    with pytest.raises(error, match=msg):
+        kv16.cache16_diff_prefill(cache, cu_rows=ints(0, 1, 2), **{**args, **kw})
+    with pytest.raises(TypeError, match="cu_rows"):
+        kv16.cache16_diff_prefill(cache, cu_rows=None, **args)
