@@ -253,7 +253,7 @@ __device__ __forceinline__ void finish_row(const Cache16AttendLaunch& L, int64_t
 // merge kernel.
 constexpr int kDecodeTile = 32, kDecodeWaves = 4;
 // Workgroups: as many as run at once by their registers, two per CU at dh 128 and
-// three at 64.  (64 contexts of 150 to 2,100 tokens, 8 kv heads of 8 query heads, dh
+// three at 64.  (64 contexts of 150 to 2,100 tokens, 8 kv heads of 4 query heads, dh
 // 64: 31.5 us with 768, 32.5 with 512.  dh 128 in the registers of three per CU
 // spills: 32K tokens in 31.7 us, 27.3 with two.)
 __host__ __device__ constexpr int decode_groups(int dh) { return dh == 128 ? 512 : 768; }
@@ -653,9 +653,8 @@ __host__ __device__ __forceinline__ int64_t split_floats(int dh, int rows) { ret
 struct Sees { int lo, hi; };
 __device__ __forceinline__ Sees row_sees(const Cache16AttendLaunch& L, int len, int n, int tok) {
   if (!L.causal) return {0, len};
-  const int64_t end = (int64_t)len - n + tok + 1;
-  const int hi = clampi(end, 0, len);
-  return {L.window > 0 ? clampi(end - L.window, 0, hi) : 0, hi};
+  const int end = len - n + tok + 1, hi = end < 0 ? 0 : end;         // (at most len)
+  return {L.window > 0 && hi > L.window ? hi - L.window : 0, hi};
 }
 // the tiles [first, first + count) that the rows of tokens a .. b see, and the
 // splits that so many are worth
@@ -667,6 +666,27 @@ __device__ __forceinline__ Tiles tiles_of(const Cache16AttendLaunch& L, int len,
 __device__ __forceinline__ int splits_of(int tiles, int splits) {
   const int most = tiles / kSplitLeast;
   return most < 1 ? 1 : (most < splits ? most : splits);
+}
+
+// The sequence of a slot (as seq_of_slot, one slot extra), its rows and its length.
+// Of the last 64 that it may be, a lane holds one's: nothing is loaded for the one
+// that it is.
+struct Seq { int s, first, begin, end, len; };
+__device__ __forceinline__ Seq seq_at(const Cache16& c, const Cache8Batch& b, int slot, int gqa, int shift) {
+  const int lane = threadIdx.x & (kWave - 1);
+  int lo = 0, hi = b.num_seqs;
+  while (hi - lo > kWave) {
+    const int step = (hi - lo + kWave - 1) / kWave, p = lo + lane * step;
+    const bool le = p < hi && first_slot(b, p < hi ? p : lo, gqa, shift, 1) <= slot;
+    const int cnt = __popcll(__ballot(le));
+    lo += (cnt > 0 ? cnt - 1 : 0) * step;
+    hi = lo + step < hi ? lo + step : hi;
+  }
+  const int p = lo + lane < hi ? lo + lane : lo, from = b.cu[p], to = b.cu[p + 1], len = seq_tokens(c, b, p);
+  const int begin = clampi(from, 0, b.num_rows), end = clampi(to, begin, b.num_rows), first = (begin * gqa >> shift) + p;
+  const int cnt = __popcll(__ballot(lo + lane < hi && first <= slot)), l = cnt > 0 ? cnt - 1 : 0;
+  return {lo + l, __builtin_amdgcn_readlane(first, l), __builtin_amdgcn_readlane(begin, l), __builtin_amdgcn_readlane(end, l),
+          __builtin_amdgcn_readlane(len, l)};
 }
 
 // 16 bytes a lane from global memory (`base` uniform) to LDS: lane i's at to + 16 i.
@@ -710,7 +730,8 @@ __device__ __forceinline__ void groups_ahead() {
 }
 
 template <int TYPE, int DH, int ROW_WAVES, int GROUPS, bool DIFF>
-__global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_kernel(Cache16AttendLaunch L, int splits, float* partials) {
+__global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_kernel(Cache16AttendLaunch L, int tiles_all, int splits,
+                                                                                       float* partials) {
   constexpr int KS = DH / 16, DB = DH / 32, KM = DIFF ? KS / 2 : KS;  // k-steps, value blocks, k-steps of a map
   constexpr int WAVES = ROW_WAVES * GROUPS, kRowTile = 32 * ROW_WAVES, RS = ROW_WAVES == 8 ? 8 : ROW_WAVES == 4 ? 7 : 6;
   constexpr bool kTurns = GROUPS == 2 && !DIFF;
@@ -728,43 +749,55 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
   // Neighbours take the splits of one row tile, then different heads (unsplit and
   // eight of them: one per XCD and its L2, which the row tiles of a head share).  The
   // longest rows of a sequence come first.
-  const uint32_t pair = blockIdx.x / splits;
-  const int h = pair % c.num_kv, z = blockIdx.x % splits, gqa = L.gqa;
-  const int64_t slot = (gridDim.x / splits - 1 - pair) / c.num_kv;
-  const int s = uniform(seq_of_slot(b, slot, gqa, RS, 1));
-  int begin, end;
-  rows_of(b, s, begin, end);
-  begin = uniform(begin);
-  const int n = uniform(end) - begin;
-  const int64_t r0 = (slot - first_slot(b, s, gqa, RS, 1)) * kRowTile, rows_all = (int64_t)n * gqa;
+  // (The rows of a call times gqa are fewer than 2^30.)
+  const uint32_t pair = splits == 1 ? blockIdx.x : blockIdx.x / (uint32_t)splits, z = blockIdx.x - pair * splits;
+  const uint32_t turn = pair / (uint32_t)c.num_kv;
+  const int h = pair - turn * c.num_kv, slot = tiles_all - 1 - (int)turn, gqa = L.gqa;
+  if (tid == 0) s_odd = 0;
+  const Seq seq = seq_at(c, b, slot, gqa, RS);
+  const int s = seq.s, begin = seq.begin, n = seq.end - seq.begin, len = seq.len;
+  const int r0 = (slot - seq.first) * kRowTile, rows_all = n * gqa;
   if (r0 < 0 || r0 >= rows_all) return;                             // (r0 < 0: row starts that decrease)
-  const int len = uniform(seq_tokens(c, b, s));
-  const int last = (int)((r0 + kRowTile < rows_all ? r0 + kRowTile : rows_all) - 1);
-  const Tiles tiles = tiles_of(L, len, n, (int)(r0 / gqa), last / gqa);
+  const int last = (r0 + kRowTile < rows_all ? r0 + kRowTile : rows_all) - 1;
+  const int first_tok = (uint32_t)r0 / (uint32_t)gqa, last_tok = (uint32_t)last / (uint32_t)gqa;
+  const Tiles tiles = tiles_of(L, len, n, first_tok, last_tok);
   const int parts = splits_of(tiles.count, splits);
-  if (z >= parts) return;
-  const int tbeg = tiles.first + (int)((int64_t)tiles.count * z / parts), tend = tiles.first + (int)((int64_t)tiles.count * (z + 1) / parts);
+  if ((int)z >= parts) return;
+  int tbeg = tiles.first, tend = tiles.first + tiles.count;
+  if (parts > 1) {                                                  // (a count is at most 2^24, parts 64)
+    tend = tiles.first + (uint32_t)(tiles.count * (z + 1)) / (uint32_t)parts;
+    tbeg = tiles.first + (uint32_t)(tiles.count * z) / (uint32_t)parts;
+  }
 
   // this lane's row
   const int row_wave = wave % ROW_WAVES, group = wave / ROW_WAVES;
-  const int64_t r = r0 + row_wave * 32 + col;
+  const int r = r0 + row_wave * 32 + col;
   const bool live = r < rows_all;
-  const int tok = live ? (int)(r / gqa) : 0, hd = live ? (int)(r - (int64_t)tok * gqa) : 0;
+  const int tok = live ? (int)((uint32_t)r / (uint32_t)gqa) : 0, hd = live ? r - tok * gqa : 0;
   const Sees sees = row_sees(L, len, n, tok);
   const int lo = live ? sees.lo : 0, lim = live ? sees.hi : 0;
-  // tiles that no row of the wave sees, and tiles that all of them see whole
-  int lim_min = live ? lim : 0x7FFFFFFF, lim_max = lim, lo_min = live && lim > 0 ? lo : 0x7FFFFFFF, lo_max = lo;
-#pragma unroll
-  for (int m = 1; m < 32; m <<= 1) {
-    lim_min = min(lim_min, __shfl_xor(lim_min, m, kWave));
-    lim_max = max(lim_max, __shfl_xor(lim_max, m, kWave));
-    lo_min = min(lo_min, __shfl_xor(lo_min, m, kWave));
-    lo_max = max(lo_max, __shfl_xor(lo_max, m, kWave));
+  // Tiles that no row of the wave sees, and tiles that all of them see whole: by its
+  // first and last row, for both ends grow with the row.
+  const int rows_wave = rows_all - r0 - row_wave * 32, end_row = (rows_wave < 32 ? rows_wave : 32) - 1;
+  int lim_min = 0x7FFFFFFF, lim_max = 0, lo_min = 0x7FFFFFFF, lo_max = 0;
+  if (end_row >= 0) {
+    lim_min = __builtin_amdgcn_readlane(lim, 0);
+    lo_min = __builtin_amdgcn_readlane(lo, 0);
+    lim_max = __builtin_amdgcn_readlane(lim, end_row);
+    lo_max = __builtin_amdgcn_readlane(lo, end_row);
   }
-  lim_min = uniform(lim_min);
-  lim_max = uniform(lim_max);
-  lo_min = uniform(lo_min);
-  lo_max = uniform(lo_max);
+
+  // The pages of the first 64 tiles are asked for before the queries, and used before
+  // the queries are.
+  const int32_t* table = b.table + s * b.table_stride;
+  const int last_blk = b.max_blocks - 1;
+  int ids[4] = {0, 0, 0, 0};
+  auto ask = [&](int t) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) ids[r] = table[min((t * kTileTokens + 16 * r) >> c.page_shift, last_blk)];
+  };
+  if (tbeg < tend) ask(tbeg + lane);
+  __builtin_amdgcn_sched_barrier(0);
 
   uintx4 q[KM];
   const int dim0 = DIFF ? group * (DH / 2) : 0;                     // first dim of this wave's map
@@ -773,17 +806,14 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
     const uint16_t* src = (const uint16_t*)L.q + (int64_t)(begin + tok) * L.q_row + (int64_t)(h * gqa + hd) * L.q_head + dim0 + 8 * half;
 #pragma unroll
     for (int i = 0; i < KM; ++i) q[i] = ((const U4*)(src + 16 * i))->v;   // (a lane without a row takes the first: dropped at the end)
-#pragma unroll
-    for (int i = 0; i < KM; ++i) asm volatile("" : "+v"(q[i]));
   }
   const float cq = L.sm_scale * kLog2e;
 
   // A wave's part of a step's tiles: TOK tokens in copies of RPL rows, all of one
   // run of 16 tokens, whose page is the same for the wave.
-  const int32_t* table = b.table + s * b.table_stride;
   const uint16_t* kh = c.k + h * c.k_head;
   const uint16_t* vh = c.v + h * c.v_head;
-  const int ps_mask = (1 << c.page_shift) - 1, last_blk = b.max_blocks - 1;
+  const int ps_mask = (1 << c.page_shift) - 1;
   const int ctile = STEP == 2 ? (wave * TOK) / kTileTokens : 0, ctok = (wave * TOK) % kTileTokens;   // of its copies
   // Bytes of this lane from a copy's first token: its token's, and its chunk's, which
   // the first token's number turns too (tokens and chunks are exclusive-or'ed bit by bit).
@@ -836,14 +866,14 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
   // copied it, before any reads it: values of tokens that are not there and values
   // that are not finite become zeros.
   enum { kVisible = 16, kCut = 32, kUnclean = 64 };                   // low bits: the runs that have a page
-  const int first_tok = (int)(r0 / gqa), all_lim = row_sees(L, len, n, first_tok).hi, all_lo = row_sees(L, len, n, last / gqa).lo;
+  const int all_lim = row_sees(L, len, n, first_tok).hi, all_lo = row_sees(L, len, n, last_tok).lo;
   int64_t kplace = 0, vplace = 0;                                     // elements
   int cases = 0, batch = 0;                                           // the batch's first tile
-  auto cases_of = [&](int t, int& own) {
+  auto cases_of = [&](int t, int& own) {                             // (of the pages in ids)
     int f = 0;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int at = t * kTileTokens + 16 * r, id = table[min(at >> c.page_shift, last_blk)];
+      const int at = t * kTileTokens + 16 * r, id = ids[r];
       const bool held = at < len && (uint32_t)id < (uint32_t)c.num_pages;
       f |= held ? 1 << r : 0;
       if (r == crun) own = held ? id : 0;
@@ -854,13 +884,17 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
     if (t < tend && (f % 16 != 15 || b > all_lim || a < all_lo)) f |= kUnclean;
     return f;
   };
-  auto look_up = [&](int t) {
+  auto place = [&](int t) {
     int own = 0;
     batch = t;
     cases = cases_of(t + lane, own);
     const int slot = (((t + lane) * kTileTokens + 16 * crun) & ps_mask) + (ctok & 15);
     kplace = own * c.k_page + (int64_t)slot * c.k_token;
     vplace = own * c.v_page + (int64_t)slot * c.v_token;
+  };
+  auto look_up = [&](int t) {
+    ask(t + lane);
+    place(t);
   };
   auto of_tile = [&](int64_t x, int t) {                              // a tile's, from its lane
     const int lo = __builtin_amdgcn_readlane((int)x, t - batch), hi = __builtin_amdgcn_readlane((int)(x >> 32), t - batch);
@@ -989,8 +1023,18 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  if (tid == 0) s_odd = 0;
-  __syncthreads();
+  auto barrier = [&]() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  if (tbeg < tend) place(tbeg);
+#pragma unroll
+  for (int i = 0; i < KM; ++i) asm volatile("" : "+v"(q[i]));       // (arrived here, before any copy that a wait would be for too)
+  __builtin_amdgcn_s_waitcnt(0xC07F);                               // lgkmcnt(0): s_odd is 0 for every wave
+  barrier();
 
   if constexpr (kPing) {
     // The matrix part of a step (scores of the next tile, values of this one) by one
@@ -1026,13 +1070,6 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
         copy_one(from, koff, s_k[(i + 4) & 3][0], part - 3 - NL);
       }
     };
-    auto barrier = [&]() {
-      __builtin_amdgcn_sched_barrier(0);
-      asm volatile("" ::: "memory");
-      __builtin_amdgcn_s_barrier();
-      asm volatile("" ::: "memory");
-      __builtin_amdgcn_sched_barrier(0);
-    };
     // cleans this wave's part of V(i)
     auto tidy = [&](int i) {
       if (what & kUnclean) {
@@ -1042,7 +1079,6 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
     };
     const int count = tend - tbeg;
     if (count > 0) {
-      look_up(tbeg);
       copy(k_from(tbeg), koff, s_k[0][0]);
 #pragma unroll
       for (int i = 1; i < 4; ++i) {
@@ -1092,7 +1128,6 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
     }
   } else if (tbeg < tend) {
     const int mine = kTurns ? group : 0;
-    look_up(tbeg);
     copy(k_from(tbeg + ctile), koff, s_k[0][ctile]);
     copy(v_from(tbeg + ctile), voff, s_v[0][ctile]);
     for (int t = tbeg; t < tend; t += 2 * STEP) {
@@ -1130,6 +1165,7 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
 #pragma unroll 1
     for (int t = tbeg; t < tend; ++t) {
       int own = 0;
+      ask(t);
       const int what = uniform(cases_of(t, own));
       if (!(what & kUnclean) || (kTurns && ((t - tbeg) & 1) != group)) continue;
 #pragma unroll 1
@@ -1252,7 +1288,7 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
     }
   } else {
     constexpr int rows = DIFF ? 2 * kRowTile : kRowTile;
-    float* o = partials + ((slot * c.num_kv + h) * splits + z) * split_floats(DH, rows);
+    float* o = partials + (((int64_t)slot * c.num_kv + h) * splits + z) * split_floats(DH, rows);
     const int row = (DIFF ? group * kRowTile : 0) + row_wave * 32 + col;
     if (half == 0) {
       o[row] = ref;
@@ -1342,12 +1378,12 @@ int prefill(const Cache16AttendLaunch& L, hipStream_t st) {
   const unsigned grid = (unsigned)(tiles * L.c.num_kv * splits);
   float* ws = (float*)L.ws;
   if constexpr (DIFF) {
-    cache16_prefill_kernel<TYPE, DH, 4, 2, true><<<grid, 512, 0, st>>>(L, splits, ws);
+    cache16_prefill_kernel<TYPE, DH, 4, 2, true><<<grid, 512, 0, st>>>(L, (int)tiles, splits, ws);
   } else if constexpr (DH == 128) {
-    if (shape.groups == 2) cache16_prefill_kernel<TYPE, DH, 4, 2, false><<<grid, 512, 0, st>>>(L, splits, ws);
-    else cache16_prefill_kernel<TYPE, DH, 8, 1, false><<<grid, 512, 0, st>>>(L, splits, ws);
+    if (shape.groups == 2) cache16_prefill_kernel<TYPE, DH, 4, 2, false><<<grid, 512, 0, st>>>(L, (int)tiles, splits, ws);
+    else cache16_prefill_kernel<TYPE, DH, 8, 1, false><<<grid, 512, 0, st>>>(L, (int)tiles, splits, ws);
   } else {
-    cache16_prefill_kernel<TYPE, DH, 4, 1, false><<<grid, 256, 0, st>>>(L, splits, ws);
+    cache16_prefill_kernel<TYPE, DH, 4, 1, false><<<grid, 256, 0, st>>>(L, (int)tiles, splits, ws);
   }
   if (splits > 1) {
     const int64_t waves = L.b.num_rows * L.c.num_kv * L.gqa;
