@@ -1246,9 +1246,7 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
     }
     if (group == 1 && (!DIFF || whole)) return;
   }
-  if (!live) return;
-  const int head = h * gqa + hd;
-  const int64_t at = (int64_t)(begin + tok) * c.num_kv * gqa + head;
+  const int at = (begin + tok) * c.num_kv * gqa + h * gqa + hd;      // (below 2^30: rows * gqa * num_kv is)
   if (parts == 1) {
     if constexpr (DIFF) {
       if (L.norm_weight) {
@@ -1269,24 +1267,35 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
       for (int d = 0; d < DB; ++d) acc[d] *= inv;
     }
     const bool none = sum == 0.f;
+    // The rows pass through LDS (their chunks exclusive-or'ed with the row), so that a
+    // store writes whole rows: it takes as long per row that it touches as for 64 bytes
+    // of one.
+    char* mine = (char*)s_v + (GROUPS == 2 ? 8 * kRowTile : 0) + 2 * DH * 32 * row_wave;
+    static_assert(sizeof(s_v) >= (GROUPS == 2 ? 8 * kRowTile : 0) + 2 * DH * kRowTile, "");
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        struct __attribute__((packed, aligned(2))) U2 { uintx2 v; };
         const uint32_t x = pair_of<TYPE>(acc[d][4 * i], acc[d][4 * i + 1]), y = pair_of<TYPE>(acc[d][4 * i + 2], acc[d][4 * i + 3]);
-        ((U2*)((uint16_t*)L.out + at * DH + 32 * d + 8 * i + 4 * half))->v = none ? uintx2{0, 0} : uintx2{x, y};
+        *(uintx2*)(mine + 2 * DH * col + 16 * ((4 * d + i) ^ (col & (CH - 1))) + 8 * half) = none ? uintx2{0, 0} : uintx2{x, y};
       }
-    if (L.lse && half == 0) {
+#pragma unroll
+    for (int i = 0; i < 32; i += RPL) {
+      const int row = i + lane / CH, to = __shfl(at, row, kWave);
+      const uintx4 x = *(const uintx4*)(mine + 2 * DH * row + 16 * ((lane % CH) ^ (row & (CH - 1))));
+      struct __attribute__((packed, aligned(2))) U4 { uintx4 v; };
+      if (row <= end_row) ((U4*)((uint16_t*)L.out + (int64_t)to * DH + 8 * (lane % CH)))->v = x;
+    }
+    if (L.lse && half == 0 && live) {
       const float e = none ? -INFINITY : (fmaf(ref, cq, -kTopWeight) + log2_of(sum)) * kLn2;
       if constexpr (DIFF) {
-        L.lse[2 * at] = e;
-        L.lse[2 * at + 1] = sum2 == 0.f ? -INFINITY : (fmaf(ref2, cq, -kTopWeight) + log2_of(sum2)) * kLn2;
+        L.lse[2 * (int64_t)at] = e;
+        L.lse[2 * (int64_t)at + 1] = sum2 == 0.f ? -INFINITY : (fmaf(ref2, cq, -kTopWeight) + log2_of(sum2)) * kLn2;
       } else {
         L.lse[at] = e;
       }
     }
-  } else {
+  } else if (live) {
     constexpr int rows = DIFF ? 2 * kRowTile : kRowTile;
     float* o = partials + (((int64_t)slot * c.num_kv + h) * splits + z) * split_floats(DH, rows);
     const int row = (DIFF ? group * kRowTile : 0) + row_wave * 32 + col;
