@@ -830,10 +830,12 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
     koff[i] = ktok + 2 * i * RPL * c.k_token + (kchunk ^ 16 * k_swizzle((ctok & 15) + i * RPL));
     voff[i] = vtok + 2 * i * RPL * c.v_token;
   }
-  auto copy_one = [&](const uint16_t* from, const uint32_t (&off)[NL], uint16_t* tile, int i) {
-    copy_to_lds(from, off[i], lds_address(tile + (ctok + i * RPL) * DH));
+  constexpr int kTileBytes = 2 * kTileTokens * DH;
+  const uint32_t k_lds = lds_address(s_k), v_lds = lds_address(s_v);
+  auto copy_one = [&](const uint16_t* from, const uint32_t (&off)[NL], uint32_t tile, int i) {
+    copy_to_lds(from, off[i], tile + 2 * (ctok + i * RPL) * DH);
   };
-  auto copy = [&](const uint16_t* from, const uint32_t (&off)[NL], uint16_t* tile) {
+  auto copy = [&](const uint16_t* from, const uint32_t (&off)[NL], uint32_t tile) {
 #pragma unroll
     for (int i = 0; i < NL; ++i) copy_one(from, off, tile, i);
   };
@@ -1063,11 +1065,11 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
       } else if (part == 1) {
         from = v_from(t + 3);
       } else if (part < 2 + NL) {
-        copy_one(from, voff, s_v[(i + 3) & 3][0], part - 2);
+        copy_one(from, voff, v_lds + ((i + 3) & 3) * kTileBytes, part - 2);
       } else if (part == 2 + NL) {
         from = k_from(t + 4);
       } else {
-        copy_one(from, koff, s_k[(i + 4) & 3][0], part - 3 - NL);
+        copy_one(from, koff, k_lds + (i & 3) * kTileBytes, part - 3 - NL);
       }
     };
     // cleans this wave's part of V(i)
@@ -1079,11 +1081,11 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
     };
     const int count = tend - tbeg;
     if (count > 0) {
-      copy(k_from(tbeg), koff, s_k[0][0]);
+      copy(k_from(tbeg), koff, k_lds);
 #pragma unroll
       for (int i = 1; i < 4; ++i) {
-        copy(v_from(tbeg + i - 1), voff, s_v[i - 1][0]);
-        copy(k_from(tbeg + i), koff, s_k[i][0]);
+        copy(v_from(tbeg + i - 1), voff, v_lds + (i - 1) * kTileBytes);
+        copy(k_from(tbeg + i), koff, k_lds + i * kTileBytes);
       }
       what = cases_at(tbeg);
       __builtin_amdgcn_s_waitcnt(kPrologue);                        // K(0)
@@ -1128,8 +1130,8 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
     }
   } else if (tbeg < tend) {
     const int mine = kTurns ? group : 0;
-    copy(k_from(tbeg + ctile), koff, s_k[0][ctile]);
-    copy(v_from(tbeg + ctile), voff, s_v[0][ctile]);
+    copy(k_from(tbeg + ctile), koff, k_lds + ctile * kTileBytes);
+    copy(v_from(tbeg + ctile), voff, v_lds + ctile * kTileBytes);
     for (int t = tbeg; t < tend; t += 2 * STEP) {
 #pragma unroll
       for (int bf = 0; bf < 2; ++bf) {
@@ -1142,8 +1144,8 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
           __syncthreads();
           if (tt + STEP < tend) {
             if (tt + 2 * STEP - 1 - batch >= kWave) look_up(tt + STEP);
-            copy(k_from(tt + STEP + ctile), koff, s_k[1 - bf][ctile]);
-            copy(v_from(tt + STEP + ctile), voff, s_v[1 - bf][ctile]);
+            copy(k_from(tt + STEP + ctile), koff, k_lds + ((1 - bf) * STEP + ctile) * kTileBytes);
+            copy(v_from(tt + STEP + ctile), voff, v_lds + ((1 - bf) * STEP + ctile) * kTileBytes);
           }
           if (what & kVisible) {
             asm volatile("" : "+v"(kat), "+v"(vat));                // (formed anew in every step: registers are dearer)
@@ -1185,6 +1187,10 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
     }
   }
 
+  // (the arguments that only the end uses, read again: scalar registers are scarce)
+  const __attribute__((address_space(4))) Cache16AttendLaunch* late =
+      (const __attribute__((address_space(4))) Cache16AttendLaunch*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(late));
   sum = halves_sum(sum);
   if (sum == 0.f) ref = kNoScore;
   float lam = 0.f, ref2 = 0.f, sum2 = 0.f;
@@ -1216,7 +1222,7 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
         const float other = rs[row], osum = rs[kRowTile + row];
         float f, g;
         if constexpr (DIFF) {
-          lam = L.lambda[h * gqa + hd];
+          lam = late->lambda[h * gqa + hd];
           f = round > 0 ? 1.f : sum == 0.f ? 0.f : 1.0f / sum;       // (all blocks at once, in the first round)
           g = osum == 0.f ? 0.f : -lam / osum;
           ref2 = other;
@@ -1249,17 +1255,17 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
   const int at = (begin + tok) * c.num_kv * gqa + h * gqa + hd;      // (below 2^30: rows * gqa * num_kv is)
   if (parts == 1) {
     if constexpr (DIFF) {
-      if (L.norm_weight) {
+      if (late->norm_weight) {
         float sq = 0.f;
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
           for (int i = 0; i < 16; ++i) sq = fmaf(acc[d][i], acc[d][i], sq);
-        const float scale = sum == 0.f ? 0.f : 1.0f / __builtin_sqrtf(fmaf(halves_sum(sq), 1.0f / DH, L.norm_eps));
+        const float scale = sum == 0.f ? 0.f : 1.0f / __builtin_sqrtf(fmaf(halves_sum(sq), 1.0f / DH, late->norm_eps));
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) acc[d][i] *= scale * L.norm_weight[32 * d + 8 * (i >> 2) + 4 * half + (i & 3)];
+          for (int i = 0; i < 16; ++i) acc[d][i] *= scale * late->norm_weight[32 * d + 8 * (i >> 2) + 4 * half + (i & 3)];
       }
     } else {
       const float inv = sum == 0.f ? 0.f : 1.0f / sum;
@@ -1284,15 +1290,15 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
       const int row = i + lane / CH, to = __shfl(at, row, kWave);
       const uintx4 x = *(const uintx4*)(mine + 2 * DH * row + 16 * ((lane % CH) ^ (row & (CH - 1))));
       struct __attribute__((packed, aligned(2))) U4 { uintx4 v; };
-      if (row <= end_row) ((U4*)((uint16_t*)L.out + (int64_t)to * DH + 8 * (lane % CH)))->v = x;
+      if (row <= end_row) ((U4*)((uint16_t*)late->out + (int64_t)to * DH + 8 * (lane % CH)))->v = x;
     }
-    if (L.lse && half == 0 && live) {
+    if (late->lse && half == 0 && live) {
       const float e = none ? -INFINITY : (fmaf(ref, cq, -kTopWeight) + log2_of(sum)) * kLn2;
       if constexpr (DIFF) {
-        L.lse[2 * (int64_t)at] = e;
-        L.lse[2 * (int64_t)at + 1] = sum2 == 0.f ? -INFINITY : (fmaf(ref2, cq, -kTopWeight) + log2_of(sum2)) * kLn2;
+        late->lse[2 * (int64_t)at] = e;
+        late->lse[2 * (int64_t)at + 1] = sum2 == 0.f ? -INFINITY : (fmaf(ref2, cq, -kTopWeight) + log2_of(sum2)) * kLn2;
       } else {
-        L.lse[at] = e;
+        late->lse[at] = e;
       }
     }
   } else if (live) {
