@@ -186,11 +186,24 @@ __global__ __launch_bounds__(256) void cache16_append_kernel(Cache16AppendLaunch
 // DH / 64 consecutive elements of a lane, of one map (sums x under reference R with
 // weights' sum l) or of two.
 
+// The launch's arguments read again, where only the end of a kernel uses them:
+// scalar registers are scarce before it.  (They are a kernel's first argument.)
+typedef const __attribute__((address_space(4))) Cache16AttendLaunch* LateArgs;
+__device__ __forceinline__ LateArgs late_args() {
+  LateArgs p = (LateArgs)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return p;
+}
+
+struct RowOut { const float *lambda, *norm_weight; float norm_eps; void* out; float* lse; };
+template <class ARGS>
+__device__ __forceinline__ RowOut row_out(ARGS p) { return {p->lambda, p->norm_weight, p->norm_eps, p->out, p->lse}; }
+
 template <int DH>
 struct RowSum { float x[DH / 64], R, l; };
 
 template <int TYPE, int DH, bool DIFF>
-__device__ __forceinline__ void finish_row(const Cache16AttendLaunch& L, int64_t at, int head, const RowSum<DH>& a,
+__device__ __forceinline__ void finish_row(const RowOut& L, int64_t at, int head, const RowSum<DH>& a,
                                            const RowSum<DH>& b) {
   constexpr int DPL = DH / 64;
   const int lane = threadIdx.x & 63;
@@ -267,10 +280,25 @@ __host__ __device__ __forceinline__ int64_t plan_size(int num_seqs) { return (16
 
 // what a decoding sequence sees: tokens first .. len - 1, in tiles of 32 from tile `tile` on
 struct Span { int first, len, tile, tiles; };
-__device__ __forceinline__ Span span_of(const Cache16AttendLaunch& L, int s) {
-  const int len = seq_tokens(L.c, L.b, s), first = L.window > 0 && len > L.window ? len - L.window : 0;
+__device__ __forceinline__ Span span_of(const Cache16AttendLaunch& L, int len) {
+  const int first = L.window > 0 && len > L.window ? len - L.window : 0;
   const int tile = first / kDecodeTile;
   return {first, len, tile, (len + kDecodeTile - 1) / kDecodeTile - tile};
+}
+
+// inclusive scan over the wave: within rows of 16, then a row's last to those behind
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t moved(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xF, false);
+}
+__device__ __forceinline__ uint32_t scan32(uint32_t x) {
+  x += moved<0x111, 0xF>(x);
+  x += moved<0x112, 0xF>(x);
+  x += moved<0x114, 0xF>(x);
+  x += moved<0x118, 0xF>(x);
+  x += moved<0x142, 0xA>(x);
+  x += moved<0x143, 0xC>(x);
+  return x;
 }
 
 template <int TYPE, int DH, bool TWIN, bool DIFF>
@@ -284,10 +312,15 @@ __global__ __launch_bounds__(256, 2) void cache16_decode_kernel(Cache16AttendLau
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
   const int columns = L.gqa * MAPS, parts = col_parts(columns), HV = c.num_kv * parts, n = b.num_seqs;
 
-  // this workgroup's tiles
-  int64_t total = 0;
-  for (int i = lane; i < n; i += kWave) total += span_of(L, i).tiles;
-  total = uniform64(shfl64(wave_scan(total), 63)) * HV;
+  // This workgroup's tiles.  The first 64 sequences' lengths stay with the lanes (the
+  // tiles of 64 are at most 2^31).
+  auto tiles_of_lane = [&](int len) { return (uint32_t)span_of(L, len).tiles; };
+  const int len0 = lane < n ? seq_tokens(c, b, lane) : 0;
+  const uint32_t scan0 = scan32(tiles_of_lane(len0));
+  auto last_of = [](uint32_t scan) { return (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)scan, 63); };
+  int64_t total = last_of(scan0);
+  for (int i = kWave + lane; i - lane < n; i += kWave) total += last_of(scan32(i < n ? tiles_of_lane(seq_tokens(c, b, i)) : 0));
+  total *= HV;
   constexpr int64_t kShare = (int64_t)decode_groups(DH) * kDecodeWaves;
   const int64_t per = total > kShare ? (total + kShare - 1) / kShare * kDecodeWaves : kDecodeWaves;
   int64_t p = (int64_t)blockIdx.x * per;
@@ -300,17 +333,16 @@ __global__ __launch_bounds__(256, 2) void cache16_decode_kernel(Cache16AttendLau
     bool found = false;
     for (int i0 = 0; i0 < n && (!found || writes_plan); i0 += kWave) {
       const int i = i0 + lane;
-      const int64_t t = i < n ? (int64_t)span_of(L, i).tiles * HV : 0;
-      const int64_t incl = before + wave_scan(t);
-      if (writes_plan && i < n) base_of[1 + i] = incl - t;
-      const uint64_t past = __ballot(incl > p);
+      const uint32_t t = tiles_of_lane(i0 == 0 ? len0 : i < n ? seq_tokens(c, b, i) : 0), scan = i0 == 0 ? scan0 : scan32(t);
+      if (writes_plan && i < n) base_of[1 + i] = before + (int64_t)(scan - t) * HV;
+      const uint64_t past = __ballot(before + (int64_t)scan * HV > p);
       if (!found && past) {
         const int l = __ffsll((unsigned long long)past) - 1;
         found = true;
         s = i0 + l;
-        sbase = uniform64(shfl64(incl - t, l));
+        sbase = before + (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)(scan - t), l) * HV;
       }
-      before = uniform64(shfl64(incl, 63));
+      before += last_of(scan) * HV;
     }
     if (writes_plan && lane == 0) {
       base_of[0] = per;
@@ -321,7 +353,7 @@ __global__ __launch_bounds__(256, 2) void cache16_decode_kernel(Cache16AttendLau
   const int ps_mask = (1 << c.page_shift) - 1;
 
   for (; p < pend && s < n; ++s) {
-    const Span sp = span_of(L, s);
+    const Span sp = span_of(L, s < kWave ? __builtin_amdgcn_readlane(len0, s) : seq_tokens(c, b, s));
     const int len = uniform(sp.len), first = uniform(sp.first), tile0 = uniform(sp.tile), T = uniform(sp.tiles);
     if (T == 0) continue;
     const int32_t* table = b.table + s * b.table_stride;
@@ -332,6 +364,17 @@ __global__ __launch_bounds__(256, 2) void cache16_decode_kernel(Cache16AttendLau
       const int t0 = (int)(p - begin), t1 = pend - begin < T ? (int)(pend - begin) : T;
       const int mycol = TWIN ? (col & 7) : col;
 
+      // page of run `run` (16 tokens) of tile t, or -1
+      auto page_at = [&](int t, int run) {
+        const int at = (tile0 + t) * kDecodeTile + run * 16, blk = at >> c.page_shift, pg = table[min(blk, b.max_blocks - 1)];
+        const int has = (at < len) & (blk < b.max_blocks) & (pg < (int)c.num_pages);   // (no branch around the load)
+        return pg | (has - 1);
+      };
+      // the first tiles' pages, asked for before the queries (a wave without a tile takes
+      // the last one's and drops them)
+      int t = t0 + wave;
+      const int tl = min(t, t1 - 1), kp = page_at(tl, col >> 3), vp = page_at(tl, g >> 1);
+      int kp1 = page_at(t + 4, col >> 3), vp1 = page_at(t + 4, g >> 1);        // of the wave's next tile
       // a column's query: dims 32 j + 8 g .. in lane group g
       uintx4 q[KS];
       {
@@ -340,18 +383,8 @@ __global__ __launch_bounds__(256, 2) void cache16_decode_kernel(Cache16AttendLau
         const uint16_t* src = (const uint16_t*)L.q + s * L.q_row + (int64_t)(h * L.gqa + mine / MAPS) * L.q_head + 8 * g;
 #pragma unroll
         for (int j = 0; j < KS; ++j) q[j] = ((const U4*)(src + 32 * j))->v;
-        // (used here, so that their wait is here: a wait at the first product, inside
-        // the loop, would in every turn be for the loads of the next tile too)
-#pragma unroll
-        for (int j = 0; j < KS; ++j) asm volatile("" : "+v"(q[j]));
       }
 
-      // page of run `run` (16 tokens) of tile t, or -1
-      auto page_at = [&](int t, int run) {
-        const int at = (tile0 + t) * kDecodeTile + run * 16, blk = at >> c.page_shift, pg = table[min(blk, b.max_blocks - 1)];
-        const int has = (at < len) & (blk < b.max_blocks) & (pg < (int)c.num_pages);   // (no branch around the load)
-        return pg | (has - 1);
-      };
       uintx4 kx[2][KS];                               // block x: token 8 (col >> 2) + 4 x + (col & 3), dims 32 j + 8 g ..
       uint32_t vx[8][VD / 2];                         // token 8 g + e, dims VD col ..
       int vpage;
@@ -388,18 +421,22 @@ __global__ __launch_bounds__(256, 2) void cache16_decode_kernel(Cache16AttendLau
       for (int d = 0; d < VD; ++d) acc[d] = floatx4{0, 0, 0, 0};
       float ref = kNoScore, sum = 0.f;
 
-      int t = t0 + wave;
-      int kp1 = 0, vp1 = 0;                           // the pages of the wave's next tile
-      if (t < t1) {
-        const int kp = page_at(t, col >> 3), vp = page_at(t, g >> 1);
-        kp1 = page_at(t + 4, col >> 3);
-        vp1 = page_at(t + 4, g >> 1);
-        load_k(t, kp);
-        __builtin_amdgcn_sched_barrier(0);            // (in the loop's order, for its waits)
-        load_v(t, vp);
-      }
-      for (; t < t1; t += 4) {
-        const int kp2 = page_at(t + 8, col >> 3), vp2 = page_at(t + 8, g >> 1);
+      load_k(tl, kp);
+      __builtin_amdgcn_sched_barrier(0);              // (in the loop's order, for its waits)
+      load_v(tl, vp);
+      // (used here, so that their wait is here: a wait at the first product, inside
+      // the loop, would in every turn be for the loads of the next tile too)
+#pragma unroll
+      for (int j = 0; j < KS; ++j) asm volatile("" : "+v"(q[j]));
+      // One tile.  The next one's loads are on the way meanwhile, issued without a
+      // condition: a path past them would make every wait one for all loads.
+      auto step = [&](auto more) {
+        constexpr bool kMore = decltype(more)::value != 0;
+        int kp2 = 0, vp2 = 0;
+        if constexpr (kMore) {
+          kp2 = page_at(t + 8, col >> 3);
+          vp2 = page_at(t + 8, g >> 1);
+        }
         // scores
         floatx4 sc[2];
 #pragma unroll
@@ -416,7 +453,7 @@ __global__ __launch_bounds__(256, 2) void cache16_decode_kernel(Cache16AttendLau
 #pragma unroll
             for (int r = 0; r < 4; ++r) sc[x][r] = mycol & 1 ? m[MAPS - 1][r] : m[0][r];
         }
-        if (t + 4 < t1) load_k(t + 4, kp1);
+        if constexpr (kMore) load_k(t + 4, kp1);
         // tokens that are not there: behind the length, before the window, of an absent page
         const int at = (tile0 + t) * kDecodeTile + 8 * g, have = vpage < 0 ? 0 : len - at, cut = first - at;
         if (__any((have < 8) | (cut > 0))) {
@@ -465,10 +502,12 @@ __global__ __launch_bounds__(256, 2) void cache16_decode_kernel(Cache16AttendLau
           acc[d] = mfma16<TYPE>(a, w, acc[d]);
           if constexpr (!TWIN) acc[d] = mfma16<TYPE>(a, rest, acc[d]);
         }
-        if (t + 4 < t1) load_v(t + 4, vp1);
+        if constexpr (kMore) load_v(t + 4, vp1);
         kp1 = kp2;
         vp1 = vp2;
-      }
+      };
+      for (; t + 4 < t1; t += 4) step(Int<1>{});
+      if (t < t1) step(Int<0>{});
 
       // the waves' sums, joined: reference, sum, then acc under the common reference
       sum = rows_sum(sum);
@@ -504,10 +543,11 @@ __global__ __launch_bounds__(256, 2) void cache16_decode_kernel(Cache16AttendLau
         return y;
       };
       if (whole) {
+        const RowOut to = row_out(late_args());
         for (int o = wave; o < cols / MAPS; o += kDecodeWaves) {
           const int head = h * L.gqa + part * (16 / MAPS) + o;
           const RowSum<DH> a = column(o * MAPS), bb = DIFF ? column(o * MAPS + MAPS - 1) : a;
-          finish_row<TYPE, DH, DIFF>(L, (int64_t)s * c.num_kv * L.gqa + head, head, a, bb);
+          finish_row<TYPE, DH, DIFF>(to, (int64_t)s * c.num_kv * L.gqa + head, head, a, bb);
         }
       } else {
         for (int cc = wave; cc < cols; cc += kDecodeWaves) {
@@ -551,7 +591,7 @@ __global__ __launch_bounds__(64 * WAVES) void cache16_decode_merge_kernel(Cache1
 #pragma unroll
       for (int i = 0; i < DPL; ++i) y[m].x[i] = 0.f;
     }
-    finish_row<TYPE, DH, DIFF>(L, at, hq, y[0], y[1]);
+    finish_row<TYPE, DH, DIFF>(row_out(&L), at, hq, y[0], y[1]);
     return;
   }
   const int64_t first = a + (int64_t)(h * parts + part) * T, g0 = first / per, g1 = (first + T - 1) / per;
@@ -593,7 +633,7 @@ __global__ __launch_bounds__(64 * WAVES) void cache16_decode_merge_kernel(Cache1
       }
     }
   }
-  finish_row<TYPE, DH, DIFF>(L, at, hq, y[0], y[MAPS - 1]);
+  finish_row<TYPE, DH, DIFF>(row_out(&L), at, hq, y[0], y[MAPS - 1]);
 }
 
 // ---- prefill -----------------------------------------------------------------
@@ -1237,10 +1277,7 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
     }
   }
 
-  // (the arguments that only the end uses, read again: scalar registers are scarce)
-  const __attribute__((address_space(4))) Cache16AttendLaunch* late =
-      (const __attribute__((address_space(4))) Cache16AttendLaunch*)__builtin_amdgcn_kernarg_segment_ptr();
-  asm volatile("" : "+s"(late));
+  const LateArgs late = late_args();
   sum = halves_sum(sum);
   if (sum == 0.f) ref = kNoScore;
   float lam = 0.f, ref2 = 0.f, sum2 = 0.f;
@@ -1402,7 +1439,7 @@ __global__ __launch_bounds__(256) void cache16_prefill_merge_kernel(Cache16Atten
     }, y[m].R, y[m].l, y[m].x, cq);
     y[m].R = fmaf(y[m].R, cq, -kTopWeight);
   }
-  finish_row<TYPE, DH, DIFF>(L, at, hq, y[0], y[MAPS - 1]);
+  finish_row<TYPE, DH, DIFF>(row_out(&L), at, hq, y[0], y[MAPS - 1]);
 }
 
 // ---- launches ------------------------------------------------------------------
