@@ -61,12 +61,15 @@ constexpr float kLog2e = 1.44269504088896f, kLn2 = 0.693147180559945f;
 
 // ---- append --------------------------------------------------------------------
 //
-// y_j = x_j cos a - x_j' sin a, y_j' = x_j' cos a + x_j sin a, a = p f: moves bytes.
+// y_j = x_j cos a - x_j' sin a, y_j' = x_j' cos a + x_j sin a, a = p f: HBM-bound (16
+// prompts of 500 to 12,000 tokens, 8 kv heads of 4 query heads, dim 128, in fp16: 2.5
+// GB in 475 us, 5.3 TB/s), a chain of dependent loads for few tokens (one: 4.5 us).
 // A lane owns 16 elements of a head (the two sides of eight pairs, or 16 that
 // stay) and keeps them for every head that it takes, so their eight angles are
 // formed once per token: the turns p f / 2 pi in 64 bits, less their nearest whole
 // number, then sine and cosine in 32.  A wave takes one token; where a call has
-// few, its heads are spread over waves.
+// fewer than eight per CU, its heads are spread over waves (one token 4.5 us, by one
+// wave 6.9; 256 tokens 6.0 and 8.6).
 
 template <int TYPE>
 struct Eight { typename Elem<TYPE>::T x[8]; };
@@ -243,7 +246,10 @@ __device__ __forceinline__ void finish_row(const RowOut& L, int64_t at, int head
 // ---- decode ------------------------------------------------------------------
 //
 // out = sum_t w_t v_t / sum_t w_t,  w_t = 2^(s_t - R),  s_t = sm_scale log2(e) <q, k_t>,
-// R a reference near the largest s_t.  HBM-bound: every key and value is read once.
+// R a reference near the largest s_t.  HBM-bound: every key and value is read once
+// (64 contexts of 2K to 32K tokens, 8 kv heads of 8 query heads, dim 128: 4.6 GB in
+// 757 us, 6.0 TB/s; below some hundred MB the start, the joins and the merge show:
+// 32K tokens of one context, 134 MB, in 30.7 us, 4.4 TB/s, from HBM).
 //
 // A tile is 32 tokens, one wave's step: S^T = K Q^T as two 16x16 blocks
 // (v_mfma_f32_16x16x32), O^T += V^T P^T as DH/16 blocks.  Token 8 g + 4 x + r of a
@@ -255,9 +261,10 @@ __device__ __forceinline__ void finish_row(const RowOut& L, int64_t at, int head
 // j is dim DH / 16 i + j.  Nothing passes through LDS.
 //
 // A column is a query head, or one of the two maps of a head in differential
-// attention, whose scores come from half of the dims each.  Up to 8 columns are
-// used twice, the second time for what the first one's 16-bit weight leaves out;
-// more fill the block, and that rest is a product of its own.
+// attention, whose scores come from half of the dims each.  A weight meets its value
+// as two 16-bit numbers, a product each.  (Up to 8 columns could take the second in
+// the idle ones: one product less, and no faster, 116.0 us against 114.7 for 256
+// contexts of 100 to 900 tokens, for the products wait for the loads.)
 //
 // Work: the tiles of all (sequence, kv head) pairs in a row, cut into equal runs,
 // one per workgroup; its four waves take the tiles of a pair in turn and join their
@@ -267,8 +274,8 @@ __device__ __forceinline__ void finish_row(const RowOut& L, int64_t at, int head
 constexpr int kDecodeTile = 32, kDecodeWaves = 4;
 // Workgroups: as many as run at once by their registers, two per CU at dh 128 and
 // three at 64.  (64 contexts of 150 to 2,100 tokens, 8 kv heads of 4 query heads, dh
-// 64: 31.5 us with 768, 32.5 with 512.  dh 128 in the registers of three per CU
-// spills: 32K tokens in 31.7 us, 27.3 with two.)
+// 64: 29.8 us with 768, 31.6 with 512, 29.9 with 1,024.  dh 128 in the registers of
+// three per CU spills: 32K tokens in 27.7 us, 25.7 with two.)
 __host__ __device__ constexpr int decode_groups(int dh) { return dh == 128 ? 512 : 768; }
 
 // columns handled together: a kv head's first 16, next 16, ...
@@ -301,7 +308,7 @@ __device__ __forceinline__ uint32_t scan32(uint32_t x) {
   return x;
 }
 
-template <int TYPE, int DH, bool TWIN, bool DIFF>
+template <int TYPE, int DH, bool DIFF>
 __global__ __launch_bounds__(256, 2) void cache16_decode_kernel(Cache16AttendLaunch L, float* partials, int64_t* base_of) {
   constexpr int KS = DH / 32, VD = DH / 16, DPL = DH / 64;          // k-steps; dims of a lane's value rows; of its output
   constexpr int MAPS = DIFF ? 2 : 1, KM = KS / MAPS;
@@ -362,7 +369,6 @@ __global__ __launch_bounds__(256, 2) void cache16_decode_kernel(Cache16AttendLau
       const int cols = part_cols(columns, part);
       const int64_t begin = sbase + (int64_t)hv * T;
       const int t0 = (int)(p - begin), t1 = pend - begin < T ? (int)(pend - begin) : T;
-      const int mycol = TWIN ? (col & 7) : col;
 
       // page of run `run` (16 tokens) of tile t, or -1
       auto page_at = [&](int t, int run) {
@@ -379,7 +385,7 @@ __global__ __launch_bounds__(256, 2) void cache16_decode_kernel(Cache16AttendLau
       uintx4 q[KS];
       {
         struct __attribute__((packed, aligned(2))) U4 { uintx4 v; };
-        const int mine = part * 16 + (mycol < cols ? mycol : 0);               // (columns over: the first again, dropped at the end)
+        const int mine = part * 16 + (col < cols ? col : 0);                   // (columns over: the first again, dropped at the end)
         const uint16_t* src = (const uint16_t*)L.q + s * L.q_row + (int64_t)(h * L.gqa + mine / MAPS) * L.q_head + 8 * g;
 #pragma unroll
         for (int j = 0; j < KS; ++j) q[j] = ((const U4*)(src + 32 * j))->v;
@@ -451,7 +457,7 @@ __global__ __launch_bounds__(256, 2) void cache16_decode_kernel(Cache16AttendLau
           sc[x] = m[0];
           if constexpr (DIFF)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) sc[x][r] = mycol & 1 ? m[MAPS - 1][r] : m[0][r];
+            for (int r = 0; r < 4; ++r) sc[x][r] = col & 1 ? m[MAPS - 1][r] : m[0][r];
         }
         if constexpr (kMore) load_k(t + 4, kp1);
         // tokens that are not there: behind the length, before the window, of an absent page
@@ -490,7 +496,7 @@ __global__ __launch_bounds__(256, 2) void cache16_decode_kernel(Cache16AttendLau
           const float x = exp2_of(fmaf(sc[e >> 2][e & 3], cw, off)), y = exp2_of(fmaf(sc[e >> 2][(e & 3) + 1], cw, off));
           sum += x + y;
           const uint32_t hi = pair_of<TYPE>(x, y), lo = pair_of<TYPE>(x - low_of<TYPE>(hi), y - high_of<TYPE>(hi));
-          w[e / 2] = TWIN && col >= 8 ? lo : hi;
+          w[e / 2] = hi;
           rest[e / 2] = lo;
         }
 #pragma unroll
@@ -500,7 +506,7 @@ __global__ __launch_bounds__(256, 2) void cache16_decode_kernel(Cache16AttendLau
           for (int i = 0; i < 4; ++i)
             a[i] = d & 1 ? highs(vx[2 * i][d / 2], vx[2 * i + 1][d / 2]) : lows(vx[2 * i][d / 2], vx[2 * i + 1][d / 2]);
           acc[d] = mfma16<TYPE>(a, w, acc[d]);
-          if constexpr (!TWIN) acc[d] = mfma16<TYPE>(a, rest, acc[d]);
+          acc[d] = mfma16<TYPE>(a, rest, acc[d]);
         }
         if constexpr (kMore) load_v(t + 4, vp1);
         kp1 = kp2;
@@ -532,9 +538,7 @@ __global__ __launch_bounds__(256, 2) void cache16_decode_kernel(Cache16AttendLau
 #pragma unroll
         for (int i = 0; i < DPL; ++i) {
           const int d = lane * DPL + i;
-          float o = s_acc[0][cc][d] + s_acc[1][cc][d] + s_acc[2][cc][d] + s_acc[3][cc][d];
-          if constexpr (TWIN) o += s_acc[0][cc + 8][d] + s_acc[1][cc + 8][d] + s_acc[2][cc + 8][d] + s_acc[3][cc + 8][d];
-          y.x[i] = o;
+          y.x[i] = s_acc[0][cc][d] + s_acc[1][cc][d] + s_acc[2][cc][d] + s_acc[3][cc][d];
         }
         y.R = fmaxf(fmaxf(s_ref[0][cc], s_ref[1][cc]), fmaxf(s_ref[2][cc], s_ref[3][cc]));
         y.l = 0.f;
@@ -569,8 +573,9 @@ __global__ __launch_bounds__(256, 2) void cache16_decode_kernel(Cache16AttendLau
 
 // Joins the partials of each (sequence, kv head) that several workgroups hold,
 // and writes the rows of sequences without a token.  WAVES waves per query head
-// share its partials: four where there are few pairs and many partials of each,
-// one where there are many pairs of one or two.
+// share its partials: four where there are few pairs and many partials of each (8
+// pairs of 32K tokens: 25.9 us in all, 34.0 with one), one where there are many pairs
+// of one or two (2,048 of 100 to 900 tokens: 115.7 us, 123.4 with four).
 template <int TYPE, int DH, bool DIFF, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void cache16_decode_merge_kernel(Cache16AttendLaunch L, const float* partials,
                                                                   const int64_t* base_of) {
@@ -641,14 +646,25 @@ __global__ __launch_bounds__(64 * WAVES) void cache16_decode_merge_kernel(Cache1
 // The same sums for many query rows.  A kv head's rows are its gqa heads of each
 // token in turn: a workgroup takes them in tiles, 32 per wave, and walks the tiles
 // of 64 tokens that any of them sees.  A tile's keys and values go from the pages
-// straight into LDS (16 bytes a lane; two buffers, the next tile's bytes are on the
-// way while this one is multiplied), row by row, the 16-byte chunks of a row
-// exclusive-or'ed with the row so that the rows that a read touches at once lie in
-// different banks.  S^T = K Q^T as two 32x32 blocks per wave (v_mfma_f32_32x32x16),
-// O^T += V^T P^T: lane (h, row) holds scores 8 a + 4 h + r of a block, which is its
-// part of the second product's B operand when its part of the A operand is the
-// same tokens: two transposing LDS reads (ds_read_b64_tr_b16) of four tokens by 16
-// dims each.
+// straight into LDS (16 bytes a lane), one to four tiles ahead, row by row, the
+// 16-byte chunks of a row exclusive-or'ed with the row so that the rows that a read
+// touches at once lie in different banks.  S^T = K Q^T as two 32x32 blocks per wave
+// (v_mfma_f32_32x32x16), O^T += V^T P^T: lane (h, row) holds scores 8 a + 4 h + r of
+// a block, which is its part of the second product's B operand when its part of the
+// A operand is the same tokens: two transposing LDS reads (ds_read_b64_tr_b16) of
+// four tokens by 16 dims each.
+//
+// Bound by the matrix cores' rate under load: a prompt of 8,192 tokens, 8 kv heads of
+// 4 query heads, dim 128, bf16, in 480 to 500 us, 1.1 PFLOP/s, where a library product
+// of 8192^3 reaches 1.31.  In eight waves of one step the weights would alternate
+// with the products; half a step apart, the one half's weights run beside the other
+// half's products (524 us for the same prompt when it came, 570 before).
+//
+// A weight meets its value as two 16-bit numbers in fp16 and in differential
+// attention, whose outputs would show one number's rounding (fp16 2^-11 against the
+// output's own; a difference of two maps can be much smaller than either), and as
+// one in bf16: outputs are off by 1.7e-3 (relative norm, against 64 bits), 1.6e-3 of
+// it their own rounding, and two cost that prompt 673 us for 498.
 //
 // In differential attention the two maps are two groups of waves over the same
 // rows, each with its half of the dims, whose sums meet in LDS at the end.
@@ -662,8 +678,11 @@ constexpr int kTileTokens = 64;
 // kMostSum none has, or fp16 holds it.
 constexpr float kMostWeight = 10.0f, kMostSum = 0x1p15f;
 
-// A workgroup's shape: row waves of 32 rows, groups of them, and whether the groups
-// take the tiles in turn.
+// A workgroup's shape: row waves of 32 rows, and groups of them: the two maps, or,
+// where the rows of a sequence are 128 at most on average, two that take its tiles in
+// turn, so that eight waves have work.  (dim 128; 4 times 5 to 24 tokens of 4 heads on
+// 20K to 32K, fp16: 92.0 us, 132.9 without turns; 64 times 4 tokens on 2K 82.6 and 94.0;
+// at 256 rows, 4 times 64 tokens on 16K, 88.9 in turn, 85.9 without.)
 struct PrefillShape {
   int row_waves, groups, at_once;       // at_once: workgroups that run at the same time
   __host__ __device__ constexpr int row_shift() const { return row_waves == 8 ? 8 : row_waves == 4 ? 7 : 6; }
@@ -673,14 +692,15 @@ __host__ __device__ __forceinline__ PrefillShape prefill_shape(int64_t num_rows,
   if (dh == 64) return {4, 1, 768};
   return num_rows * gqa <= 128 * (int64_t)num_seqs ? PrefillShape{4, 2, 256} : PrefillShape{8, 1, 256};
 }
-constexpr int kSplitLeast = 4;          // tiles of a split
+constexpr int kSplitLeast = 4;          // tiles of a split (2 to 8: no difference)
 constexpr int kSplitMost = 64;
 
 __host__ __device__ __forceinline__ int64_t row_tiles(int64_t num_rows, int num_seqs, int gqa, int row_shift) {
   return ((num_rows * gqa) >> row_shift) + num_seqs;
 }
 // Splits of each row tile: the workgroups at once over the fewest tiles that the
-// rows can make.  The lengths, which the host does not know, have no part in it.
+// rows can make (twice as many: 98.7 us for those 92.0, 72.2 for 60.5 with 8 times 64
+// tokens on 4K).  The lengths, which the host does not know, have no part in it.
 __host__ __device__ __forceinline__ int prefill_splits(int64_t num_rows, int num_seqs, int num_kv, int gqa, PrefillShape p) {
   const int64_t whole = (num_rows * gqa) >> p.row_shift(), s = p.at_once / ((whole > num_seqs ? whole : num_seqs) * num_kv);
   return (int)(s < 1 ? 1 : (s > kSplitMost ? kSplitMost : s));
@@ -1462,8 +1482,7 @@ int decode(const Cache16AttendLaunch& L, hipStream_t st) {
   int64_t* plan = (int64_t*)L.ws;
   float* partials = (float*)((uint8_t*)L.ws + plan_size(L.b.num_seqs));
   const int columns = L.gqa * (DIFF ? 2 : 1);
-  if (columns <= 8) cache16_decode_kernel<TYPE, DH, true, DIFF><<<decode_groups(DH), 256, 0, st>>>(L, partials, plan);
-  else cache16_decode_kernel<TYPE, DH, false, DIFF><<<decode_groups(DH), 256, 0, st>>>(L, partials, plan);
+  cache16_decode_kernel<TYPE, DH, DIFF><<<decode_groups(DH), 256, 0, st>>>(L, partials, plan);
   const int heads = L.b.num_seqs * L.c.num_kv * L.gqa;
   if (L.b.num_seqs * L.c.num_kv * col_parts(columns) < 128)
     cache16_decode_merge_kernel<TYPE, DH, DIFF, 4><<<heads, 256, 0, st>>>(L, partials, plan);
