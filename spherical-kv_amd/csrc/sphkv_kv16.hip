@@ -685,7 +685,7 @@ constexpr float kMostWeight = 10.0f, kMostSum = 0x1p15f;
 // at 256 rows, 4 times 64 tokens on 16K, 88.9 in turn, 85.9 without.)
 struct PrefillShape {
   int row_waves, groups, at_once;       // at_once: workgroups that run at the same time
-  __host__ __device__ constexpr int row_shift() const { return row_waves == 8 ? 8 : row_waves == 4 ? 7 : 6; }
+  __host__ __device__ constexpr int row_shift() const { return row_waves == 8 ? 8 : 7; }
 };
 __host__ __device__ __forceinline__ PrefillShape prefill_shape(int64_t num_rows, int num_seqs, int gqa, int dh, bool diff) {
   if (diff) return {4, 2, 256};
@@ -843,7 +843,7 @@ template <int TYPE, int DH, int ROW_WAVES, int GROUPS, bool DIFF>
 __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_kernel(Cache16AttendLaunch L, int turns, int splits,
                                                                                        float* partials) {
   constexpr int KS = DH / 16, DB = DH / 32, KM = DIFF ? KS / 2 : KS;  // k-steps, value blocks, k-steps of a map
-  constexpr int WAVES = ROW_WAVES * GROUPS, kRowTile = 32 * ROW_WAVES, RS = ROW_WAVES == 8 ? 8 : ROW_WAVES == 4 ? 7 : 6;
+  constexpr int WAVES = ROW_WAVES * GROUPS, kRowTile = 32 * ROW_WAVES, RS = ROW_WAVES == 8 ? 8 : 7;
   constexpr bool kTurns = GROUPS == 2 && !DIFF;
   constexpr int STEP = kTurns ? 2 : 1;                                // tiles of a step
   constexpr bool kPing = WAVES == 8 && !kTurns;                       // two halves of the waves, half a step apart
@@ -949,7 +949,7 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
 #pragma unroll
     for (int i = 0; i < NL; ++i) copy_one(from, off, tile, i);
   };
-  static_assert(DH == 128 ? RPL % 4 == 0 : RPL % 4 == 0, "the values' chunks turn by a token's low bits");
+  static_assert(RPL % 4 == 0, "the values' chunks turn by a token's low bits");
 
   floatx16 acc[DB];
 #pragma unroll

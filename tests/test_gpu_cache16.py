@@ -537,6 +537,8 @@ def rows_on_gpu(cache, q, table, lens, cu, window, dims=None):
         there = torch.as_tensor(there, device=q.device).repeat_interleave(ps)[:n]
         k, v = (torch.where(there[:, None, None], x[pages].transpose(1, 2).reshape(-1, H, dh)[:n], 0).double() for x in (cache.k, cache.v))
         a, b = int(cu[s]), int(cu[s + 1])
+        if n <= 0 or a == b:
+            continue
         pos = torch.arange(n - (b - a), n, device=q.device)[:, None]
         t = torch.arange(n, device=q.device)[None]
         sees = (t <= pos) & there[None] & ((t > pos - window) if window else True)
@@ -545,7 +547,7 @@ def rows_on_gpu(cache, q, table, lens, cu, window, dims=None):
                 rows = q[a:b, g, dims].double()
                 x = (rows @ k[:, h, dims].T * sm).masked_fill(~sees, -math.inf)
                 l = torch.logsumexp(x, 1)
-                p = torch.exp(x - l[:, None])
+                p = torch.exp(x - l[:, None]).masked_fill(~sees, 0)
                 reach = (rows.abs() @ k[:, h, dims].abs().T * sm).masked_fill(~sees, 0).amax(1)
                 under = p.amax(1)[:, None] * (sees.double() @ v[:, h].abs())
                 for to, x in zip(res, (p @ v[:, h], l, p @ v[:, h].abs(), reach, under)):
@@ -571,6 +573,37 @@ def test_prefill_many_tiles(gpu, dtype, dh, ps, num_kv, gqa, seqs, window):
     out, lse = kv16.cache16_diff_prefill(cache, q, lam, *args, norm_weight=weight, window=window, return_lse=True)
     maps = [rows_on_gpu(cache, q, table, lens, cu, window, d) for d in (slice(0, dh // 2), slice(dh // 2, dh))]
     check_diff(out, lse, maps, lam, weight, 1e-5, lens, dh, weight_bits(dtype, True, True), f"diff many tiles {dtype} {dh}")
+
+
+# more row tiles than run at once, of 2 to 9 sequences (up to 8 are taken by how far their tiles reach): equal ones, empty
+# ones, ones without rows, rows before the first token, a tile that two share the reach of, one reach of its own
+ORDERS = [
+    [(1024, 1024)] * 2,
+    [(700, 600), (0, 0), (300, 300), (1200, 37), (90, 500), (64, 64), (2000, 256), (1, 1)],
+    [(0, 0), (900, 0), (1500, 1500), (40000, 70), (0, 90)],
+    [(5, 5), (1337, 1337), (257, 257), (3, 3)],
+    [(600, 300)] * 7 + [(1, 1)] * 2,
+]
+
+
+@pytest.mark.parametrize("window", [0, 300])
+@pytest.mark.parametrize("dtype, dh, gqa", [("bf16", 128, 4), ("fp16", 64, 7), ("fp16", 128, 3)])
+@pytest.mark.parametrize("seqs", ORDERS)
+def test_prefill_order(gpu, dtype, dh, gqa, seqs, window):
+    lens, new, H = [a for a, _ in seqs], [b for _, b in seqs], 8
+    cache, _, table = setup(gpu, 33, dtype, dh, 32, H, lens)
+    cu = np.cumsum([0] + new)
+    rows = int(cu[-1])
+    q = torch.randn((rows + 3, H * gqa, dh), device=gpu, generator=torch.Generator(device=gpu).manual_seed(9)).to(TYPES[dtype])
+    args = (i32(cu, gpu), i32(table, gpu), i32(lens, gpu))
+    lam, _ = diff_weights(gpu, 5, H * gqa, dh)
+    out, lse = torch.full_like(q, 7.0), torch.full(q.shape[:2], 7.0, device=gpu)
+    kv16.cache16_prefill(cache, q, *args, window=window, out=out, lse=lse)
+    check(out[:rows], lse[:rows], rows_on_gpu(cache, q[:rows], table, lens, cu, window), lens, dh, weight_bits(dtype, True, False), f"order {seqs}")
+    assert (out[rows:] == 7.0).all() and (lse[rows:] == 7.0).all()
+    out, lse = kv16.cache16_diff_prefill(cache, q, lam, *args, window=window, return_lse=True)
+    maps = [rows_on_gpu(cache, q[:rows], table, lens, cu, window, d) for d in (slice(0, dh // 2), slice(dh // 2, dh))]
+    check_diff(out[:rows], lse[:rows], maps, lam, None, 1e-5, lens, dh, weight_bits(dtype, True, True), f"diff order {seqs}")
 
 
 @pytest.mark.parametrize("diff", [False, True])
