@@ -33,6 +33,7 @@ from sphkv_lib import check
 
 _lib = sphkv_lib.load()
 
+_Tensor = torch.Tensor
 _FREQ_TYPES = {torch.float32: 2, torch.float64: 3}         # SPHKV_FP32, SPHKV_FP64
 
 
@@ -112,6 +113,26 @@ class Cache16:
             check(rc, fn.__name__)
 
 
+# A plain tensor of the right type on the cache's device passes by three comparisons;
+# anything else goes through _need, _seq_args and _rows, which say what is wrong, or
+# that nothing is (one token's append 8.9 us of the host, 10.4 with those alone).
+
+def _seqs(cache: Cache16, table: torch.Tensor, at: torch.Tensor, cu_rows: Optional[torch.Tensor], name: str):
+    """_seq_args of the ordinary case; (table, row stride, blocks, sequences) for the call."""
+    index = cache._index
+    if (type(table) is _Tensor and type(at) is _Tensor and table.dtype is _INT and at.dtype is _INT
+            and table.get_device() == index and at.get_device() == index):
+        shape = table.shape
+        if len(shape) == 2 and at.shape == shape[:1]:
+            n, blocks = shape
+            row, one = table.stride()
+            if (one == 1 or blocks <= 1) and (n == 1 or (row >= blocks and at.is_contiguous())) and (
+                    cu_rows is None or (type(cu_rows) is _Tensor and cu_rows.dtype is _INT and cu_rows.get_device() == index
+                                        and cu_rows.shape == (n + 1,) and cu_rows.is_contiguous())):
+                return table.data_ptr(), row, blocks, n
+    return _seq_args(cache, table, at, cu_rows, name)
+
+
 def cache16_append(cache: Cache16, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, start: torch.Tensor,
                    cu_rows: Optional[torch.Tensor] = None, inv_freq: Optional[torch.Tensor] = None,
                    interleaved: bool = False, parts: int = 1, q: Optional[torch.Tensor] = None,
@@ -138,51 +159,62 @@ def cache16_append(cache: Cache16, k: torch.Tensor, v: torch.Tensor, table: torc
     they were in q_out.  A written page belongs to one sequence."""
     if parts not in (1, 2):
         raise ValueError(f"parts must be 1 or 2, got {parts}")
-    tab, stride, blocks, n = _seq_args(cache, table, start, cu_rows, "start")
-    if not isinstance(k, torch.Tensor) or k.dtype not in _TYPES:
+    tab, stride, blocks, n = _seqs(cache, table, start, cu_rows, "start")
+    if not isinstance(k, _Tensor) or k.dtype not in _TYPES:
         raise TypeError("k must be an fp16, bf16 or fp32 tensor")
-    dtype, dev, heads, dh = k.dtype, cache._device, cache._num_kv, cache._dh
-    _need(k, dtype, "k", dev)
-    _need(v, dtype, "v", dev)
+    dtype, dev, index, heads, dh = k.dtype, cache._device, cache._index, cache._num_kv, cache._dh
+    if k.get_device() != index:
+        _need(k, dtype, "k", dev)
+    if type(v) is not _Tensor or v.dtype is not dtype or v.get_device() != index:
+        _need(v, dtype, "v", dev)
+    shape = k.shape
+    rows = shape[0] if shape else 0
     k_row, k_head = _rows(k, "k", heads, dh)
-    v_row, v_head = _rows(v, "v", heads, dh)
-    rows = k.shape[0]
-    if v.shape[0] != rows:
+    if v.shape == shape:
+        v_row, v_head, one = v.stride()
+        if one != 1:
+            _rows(v, "v", heads, dh)
+    else:
+        _rows(v, "v", heads, dh)
         raise ValueError("k and v must have as many rows")
     if cu_rows is None and rows != n:
         raise ValueError("without cu_rows there is one row per sequence")
     q_ptr = o_ptr = None
     q_row = q_head = o_row = o_head = gqa = 0
     if q is not None:
-        _need(q, dtype, "q", dev)
-        if q.dim() != 3 or q.shape[0] != rows or q.shape[1] == 0 or q.shape[1] % heads:
-            raise ValueError("q must be [rows, num_kv * gqa, dh], as many rows as k")
+        if type(q) is not _Tensor or q.dtype is not dtype or q.get_device() != index:
+            _need(q, dtype, "q", dev)
         shape = q.shape
+        if len(shape) != 3 or shape[0] != rows or shape[1] == 0 or shape[1] % heads:
+            raise ValueError("q must be [rows, num_kv * gqa, dh], as many rows as k")
         gqa = shape[1] // heads
         q_row, q_head = _rows(q, "q", shape[1], dh)
         if q_out is None:
             q_out = _like(q, cache._dtype)
+            o_row, o_head = shape[1] * dh, dh
         else:
             _need(q_out, cache._dtype, "q_out", dev)
             if q_out.shape != shape:
                 raise ValueError(f"q_out must be {tuple(shape)}")
-        o_row, o_head = _rows(q_out, "q_out", shape[1], dh)
-        size = dh
-        for st, count in sorted(x for x in ((o_row, rows), (o_head, shape[1])) if x[1] > 1):
-            if st < size:
-                raise ValueError("rows and heads of q_out overlap")
-            size += st * (count - 1)
+            o_row, o_head = _rows(q_out, "q_out", shape[1], dh)
+            size = dh
+            for st, count in sorted(x for x in ((o_row, rows), (o_head, shape[1])) if x[1] > 1):
+                if st < size:
+                    raise ValueError("rows and heads of q_out overlap")
+                size += st * (count - 1)
         q_ptr, o_ptr = q.data_ptr(), q_out.data_ptr()
     elif q_out is not None:
         raise ValueError("q_out goes with q")
     f_ptr, f_type, freqs = None, 0, 0
     if inv_freq is not None:
-        if not isinstance(inv_freq, torch.Tensor) or inv_freq.dtype not in _FREQ_TYPES:
+        if not isinstance(inv_freq, _Tensor) or inv_freq.dtype not in _FREQ_TYPES:
             raise TypeError("inv_freq must be an fp32 or fp64 tensor")
-        _need(inv_freq, inv_freq.dtype, "inv_freq", dev)
-        if inv_freq.dim() != 1 or (inv_freq.shape[0] > 1 and inv_freq.stride(0) != 1):
+        if inv_freq.get_device() != index:
+            _need(inv_freq, inv_freq.dtype, "inv_freq", dev)
+        shape = inv_freq.shape
+        if len(shape) != 1 or not inv_freq.is_contiguous():
             raise ValueError("inv_freq must be a contiguous [n]")
-        f_ptr, f_type, freqs = inv_freq.data_ptr(), _FREQ_TYPES[inv_freq.dtype], inv_freq.shape[0]
+        f_ptr, f_type, freqs = inv_freq.data_ptr(), _FREQ_TYPES[inv_freq.dtype], shape[0]
     cache._call(_lib.sphkv_cache16_append, cache._address(), k.data_ptr(), v.data_ptr(), q_ptr, _TYPES[dtype], k_row, k_head,
                 v_row, v_head, q_row, q_head, gqa, o_ptr, o_row, o_head, rows, None if cu_rows is None else cu_rows.data_ptr(),
                 start.data_ptr(), tab, stride, blocks, n, f_ptr, f_type, freqs, parts, 1 if interleaved else 0)
@@ -198,7 +230,8 @@ def _like(q: torch.Tensor, dtype) -> torch.Tensor:
 
 def _query(cache: Cache16, q: torch.Tensor):
     """Checks of q; (shape, q heads per kv head, row stride, head stride)."""
-    _need(q, cache._dtype, "q", cache._device)
+    if type(q) is not _Tensor or q.dtype is not cache._dtype or q.get_device() != cache._index:
+        _need(q, cache._dtype, "q", cache._device)
     shape = q.shape
     if len(shape) != 3 or shape[1] == 0 or shape[1] % cache._num_kv:
         raise ValueError("q must be [rows, num_kv * gqa, dh]")
@@ -245,13 +278,13 @@ def _diff_args(cache: Cache16, lam: torch.Tensor, heads: int, norm_weight: Optio
 
 def _window(window) -> int:
     w = int(window)
-    if not 0 <= w < 2 ** 31 or w != window:
+    if w != window or not 0 <= w < 2 ** 31:
         raise ValueError(f"window must be a non-negative int32, got {window}")
     return w
 
 
 def _decode(cache, q, table, lens, window, sm_scale, out, return_lse, lse, workspace, diff):
-    tab, stride, blocks, n = _seq_args(cache, table, lens, None, "lens")
+    tab, stride, blocks, n = _seqs(cache, table, lens, None, "lens")
     shape, gqa, q_row, q_head = _query(cache, q)
     if shape[0] != n:
         raise ValueError("q must have one row per sequence")
@@ -262,7 +295,10 @@ def _decode(cache, q, table, lens, window, sm_scale, out, return_lse, lse, works
     out = _like(q, cache._dtype) if out is None else _out(out, shape, cache._dtype, "out", cache)
     if return_lse or lse is not None:
         lse = _out(lse, (shape[0], shape[1], *maps), _FLOAT, "lse", cache)
-    ws, nbytes, _keep = _workspace(cache, decode_workspace_bytes(cache, n, gqa, diff is not None), workspace)
+    need = _decode_bytes(n, cache._num_kv, gqa, cache._dh, 0 if diff is None else 1)
+    if need < 0:
+        decode_workspace_bytes(cache, n, gqa, diff is not None)
+    ws, nbytes, _keep = _workspace(cache, need, workspace)
     cache._call(fn, cache._address(), q.data_ptr(), q_row, q_head, gqa, *more, lens.data_ptr(), _window(window), tab, stride, blocks, n,
                 scale if sm_scale is None else float(sm_scale), out.data_ptr(), None if lse is None else lse.data_ptr(), ws,
                 nbytes)
@@ -272,7 +308,7 @@ def _decode(cache, q, table, lens, window, sm_scale, out, return_lse, lse, works
 def _prefill(cache, q, cu_rows, table, lens, causal, window, sm_scale, out, return_lse, lse, workspace, diff):
     if cu_rows is None:
         raise TypeError("cu_rows must be a torch.Tensor")
-    tab, stride, blocks, n = _seq_args(cache, table, lens, cu_rows, "lens")
+    tab, stride, blocks, n = _seqs(cache, table, lens, cu_rows, "lens")
     shape, gqa, q_row, q_head = _query(cache, q)
     if diff is None:
         fn, more, scale, maps = _lib.sphkv_cache16_prefill, (), cache._sm, ()

@@ -366,6 +366,11 @@ def test_python_refuses_appends(on_cpu, kw, error, msg):
     (dict(window=2 ** 32 + 5), ValueError, "window must be"),
     (dict(window=-1), ValueError, "window must be"),
     (dict(window=2.5), ValueError, "window must be"),
+    (dict(window=0.4), ValueError, "window must be"),
+    (dict(q=torch.nn.Parameter(half(2, 2, 64))), AssertionError, "launched"),
+    (dict(lens=ints(1, 7, 1, 7)[::2]), ValueError, "contiguous"),
+    (dict(table=torch.zeros((2, 4), dtype=torch.int32)[:, ::2]), ValueError, "contiguous"),
+    (dict(lens=None), TypeError, "lens"),
     (dict(q=half(2, 0, 64)), ValueError, "q must be"),
     (dict(q=half(2, 2, 32)), ValueError, "q must be"),
     (dict(q=half(2, 65, 64)), ValueError, "bad num"),
