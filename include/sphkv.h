@@ -833,9 +833,7 @@ int sphkv_cache16_diff_decode(const sphkv_cache16* cache, const void* q, int64_t
  * positions up to p (causal = 1; with a window w > 0 those above p - w) or all
  * lens[s] (causal = 0, window 0).  A row that attends nothing gets zeros and
  * -inf; rows from cu_rows[num_seqs] on keep their contents.  q, out [num_rows,
- * num_kv*gqa, dh], lse [num_rows, num_kv*gqa].  A weight meets its value as two
- * numbers of the cache's type in fp16 and in differential attention, as one bf16
- * number otherwise.  The rest as the calls above.
+ * num_kv*gqa, dh], lse [num_rows, num_kv*gqa].  The rest as the calls above.
  */
 int64_t sphkv_cache16_prefill_workspace_bytes(int64_t num_rows, int32_t num_seqs, int32_t num_kv, int32_t gqa,
                                               int32_t dh, int32_t differential);

@@ -655,16 +655,15 @@ __global__ __launch_bounds__(64 * WAVES) void cache16_decode_merge_kernel(Cache1
 // four tokens by 16 dims each.
 //
 // Bound by the matrix cores' rate under load: a prompt of 8,192 tokens, 8 kv heads of
-// 4 query heads, dim 128, bf16, in 480 to 500 us, 1.1 PFLOP/s, where a library product
-// of 8192^3 reaches 1.31.  In eight waves of one step the weights would alternate
-// with the products; half a step apart, the one half's weights run beside the other
-// half's products (524 us for the same prompt when it came, 570 before).
+// 4 query heads, dim 128, bf16, in 653 us, 1.26 PFLOP/s of the products below, where a
+// library product of 8192^3 reaches 1.31.  In eight waves of one step the weights would
+// alternate with the products; half a step apart, the one half's weights run beside the
+// other half's products (with one product a weight 524 us when it came, 570 before).
 //
-// A weight meets its value as two 16-bit numbers in fp16 and in differential
-// attention, whose outputs would show one number's rounding (fp16 2^-11 against the
-// output's own; a difference of two maps can be much smaller than either), and as
-// one in bf16: outputs are off by 1.7e-3 (relative norm, against 64 bits), 1.6e-3 of
-// it their own rounding, and two cost that prompt 673 us for 498.
+// A weight meets its value as two 16-bit numbers, a product each: outputs show one
+// number's rounding.  (In bf16 they were 5 % further from 64 bits with one, 1.73e-3
+// relative norm for 1.65e-3, of which 1.64e-3 is their own rounding, and where values
+// cancel by 2^-9 of what cancels.  One number took 478 us for those 653.)
 //
 // In differential attention the two maps are two groups of waves over the same
 // rows, each with its half of the dims, whose sums meet in LDS at the end.
@@ -848,7 +847,6 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
   constexpr int STEP = kTurns ? 2 : 1;                                // tiles of a step
   constexpr bool kPing = WAVES == 8 && !kTurns;                       // two halves of the waves, half a step apart
   constexpr int NB = kPing ? 4 : 2;                                   // steps in LDS
-  constexpr bool kRest = DIFF || TYPE == kFp16;                       // weights as two numbers
   constexpr int CH = DH / 8, RPL = 64 / CH, TOK = kTileTokens / WAVES * STEP, NL = TOK / RPL;   // chunks of a row; rows a copy;
                                                                       // a wave's tokens of a step and copies of each kind
   __shared__ __align__(16) uint16_t s_k[NB][STEP][kTileTokens * DH], s_v[NB][STEP][kTileTokens * DH];
@@ -1075,7 +1073,7 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
           ws += x;
           ws += y;
           w[u][i / 2] = pair_of<TYPE>(x, y);
-          if constexpr (kRest) rest[u][i / 2] = pair_of<TYPE>(x - low_of<TYPE>(w[u][i / 2]), y - high_of<TYPE>(w[u][i / 2]));
+          rest[u][i / 2] = pair_of<TYPE>(x - low_of<TYPE>(w[u][i / 2]), y - high_of<TYPE>(w[u][i / 2]));
         }
     };
     pass(0.f);
@@ -1102,7 +1100,7 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
       for (int d = 0; d < DB; ++d) {
         const uintx4 a = v_at(vt, u, d);
         acc[d] = mfma32<TYPE>(a, w[u], acc[d]);
-        if constexpr (kRest) acc[d] = mfma32<TYPE>(a, rest[u], acc[d]);
+        acc[d] = mfma32<TYPE>(a, rest[u], acc[d]);
       }
   };
   // Both, in this order: each product with the reads of the one kAheadReads later
@@ -1129,7 +1127,7 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
       } else {
         const int u = (j - NK) / DB, d = (j - NK) % DB;
         acc[d] = mfma32<TYPE>(x, w[u], acc[d]);
-        if constexpr (kRest) acc[d] = mfma32<TYPE>(x, rest[u], acc[d]);
+        acc[d] = mfma32<TYPE>(x, rest[u], acc[d]);
       }
       between(j);
       __builtin_amdgcn_sched_barrier(0);
@@ -1264,7 +1262,7 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
             if (what & kCut) mask(tt + mine, what);
             weigh();
             values(s_v[bf][mine]);
-            groups_ahead<4 * DB, 2, kRest ? 2 : 1, DB < 4 ? DB : 4>();
+            groups_ahead<4 * DB, 2, 2, DB < 4 ? DB : 4>();
           }
         }
       }

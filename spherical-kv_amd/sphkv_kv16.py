@@ -330,7 +330,8 @@ def cache16_decode(cache: Cache16, q: torch.Tensor, table: torch.Tensor, lens: t
     """Attention of one query token per sequence over the first lens[s] tokens of
     its pages, or the last `window` of them (sphkv_cache16_decode).  q [num_seqs,
     num_kv * gqa, dh] of the cache's type, gqa up to 64; lens int32 [num_seqs];
-    window 0: no window; sm_scale 1 / sqrt(dh) unless given.  Returns out (q's
+    window 0: no window; sm_scale 1 / sqrt(dh) unless given.  A softmax weight
+    meets its value with 22 bits in fp16, with 16 in bf16.  Returns out (q's
     shape and type), with return_lse (out, lse): lse fp32 [num_seqs, num_kv *
     gqa] is the natural log of the softmax's sum.  A sequence without tokens gets
     zeros and -inf."""
@@ -361,8 +362,7 @@ def cache16_prefill(cache: Cache16, q: torch.Tensor, cu_rows: torch.Tensor, tabl
     * gqa, dh] is at position p = lens[s] - n_s + i and attends the tokens up to
     its own (causal; with a window those after p - window) or all lens[s].  Append
     the tokens first.  Rows that attend nothing get zeros and -inf; rows behind
-    the last sequence are left as they were in out and lse.  A softmax weight
-    meets its value with 22 bits in fp16, with 8 in bf16.  Few tokens on a long
+    the last sequence are left as they were in out and lse.  Few tokens on a long
     context are slow beside many short sequences (the keys are split evenly over a
     batch): give them a call of their own.  The rest as cache16_decode."""
     return _prefill(cache, q, cu_rows, table, lens, causal, window, sm_scale, out, return_lse, lse, workspace, None)
@@ -375,7 +375,6 @@ def cache16_diff_prefill(cache: Cache16, q: torch.Tensor, lam: torch.Tensor, cu_
                          lse: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None):
     """Differential attention of several query tokens per sequence
     (sphkv_cache16_diff_prefill): rows as cache16_prefill's, maps, lam and
-    norm_weight as cache16_diff_decode's, lse [rows, num_kv * gqa, 2].  A weight
-    meets its value with 22 bits in fp16, with 16 in bf16."""
+    norm_weight as cache16_diff_decode's, lse [rows, num_kv * gqa, 2]."""
     return _prefill(cache, q, cu_rows, table, lens, causal, window, sm_scale, out, return_lse, lse, workspace,
                     (lam, norm_weight, norm_eps))

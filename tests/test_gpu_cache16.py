@@ -705,6 +705,18 @@ def test_prefill_weights_are_two_numbers(gpu, dtype, dh, diff):
         check(out, lse, oracle_of(cache).attend(f64(q), table.cpu().numpy(), [64]), [64], dh, 22, "prefill")
 
 
+@pytest.mark.parametrize("dh, rows, gqa", [(128, 1, 8), (128, 40, 4), (64, 40, 4)])
+def test_prefill_bf16_weights_are_two_numbers(gpu, dh, rows, gqa):
+    """Tiles taken in turn and by row tiles: outputs far below their terms, to which a weight of 8 bits would show."""
+    n = 128
+    cache, table, _ = cancelling(gpu, "bf16", dh, n, 1, gqa)
+    q = (0.3 * torch.randn((rows, gqa, dh), generator=torch.Generator(device=gpu).manual_seed(4), device=gpu)).bfloat16()
+    cu = [0, rows]
+    out, lse = kv16.cache16_prefill(cache, q, i32(cu, gpu), table, i32([n], gpu), causal=False, return_lse=True)
+    parts = oracle_of(cache).attend(f64(q), table.cpu().numpy(), [n], cu, causal=False)
+    check(out, lse, parts, [n], dh, 16, f"bf16 prefill dh {dh} rows {rows}")
+
+
 def test_nan_query_and_key_stay_in_their_rows(gpu):
     lens = [50, 70]
     cache, want, table = setup(gpu, 22, "fp16", 128, 16, 2, lens)
