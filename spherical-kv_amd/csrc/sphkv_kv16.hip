@@ -655,7 +655,7 @@ __global__ __launch_bounds__(64 * WAVES) void cache16_decode_merge_kernel(Cache1
 // four tokens by 16 dims each.
 //
 // Bound by the matrix cores' rate under load: a prompt of 8,192 tokens, 8 kv heads of
-// 4 query heads, dim 128, bf16, in 653 us, 1.26 PFLOP/s of the products below, where a
+// 4 query heads, dim 128, bf16, in 638 us, 1.29 PFLOP/s of the products below, where a
 // library product of 8192^3 reaches 1.31.  In eight waves of one step the weights would
 // alternate with the products; half a step apart, the one half's weights run beside the
 // other half's products (with one product a weight 524 us when it came, 570 before).
@@ -676,6 +676,7 @@ constexpr int kTileTokens = 64;
 // A weight may pass 2^kMostWeight; where a lane's 32 of a tile add up to less than
 // kMostSum none has, or fp16 holds it.
 constexpr float kMostWeight = 10.0f, kMostSum = 0x1p15f;
+constexpr float kNearScore = 64.f;
 
 // A workgroup's shape: row waves of 32 rows, and groups of them: the two maps, or,
 // where the rows of a sequence are 128 at most on average, two that take its tiles in
@@ -1039,7 +1040,7 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) sc[x][i] = -ref;                 // (scores come out less the reference)
+      for (int i = 0; i < 16; ++i) sc[x][i] = 0.f;
 #pragma unroll
       for (int k = 0; k < KM; ++k) sc[x] = mfma32<TYPE>(k_at(kt, x, k), q[k], sc[x]);
     }
@@ -1060,36 +1061,43 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
   // The tile's weights, 2^kTopWeight at the reference.  Their largest is not looked
   // for: where a lane's 32 add up to less than 2^(kMostWeight + 5) none has passed
   // the bound of the reference.  Otherwise, and at a row's first scores, the reference
-  // becomes the row's largest score (both halves of a row decide alike).
+  // becomes the row's largest score (both halves of a row decide alike).  Every score is
+  // a sum from zero, less the reference, so that equal ones weigh the same in any tile
+  // and at any magnitude.  The difference is part of the exponent's one multiply-add up to
+  // kNearScore, whose rounding is 2^-19 of a weight there (always apart: 661 us for that
+  // prompt's 638, differential prompts of 1,000 to 2,000 tokens 198 for 193).
   auto weigh = [&]() {
     float ws = 0.f;
-    auto pass = [&](float shift) {
+    auto pass = [&](auto exponent) {
 #pragma unroll
       for (int u = 0; u < 4; ++u)
 #pragma unroll
         for (int i = 0; i < 8; i += 2) {
-          const float x = exp2_of(fmaf(sc[u >> 1][8 * (u & 1) + i] - shift, cq, kTopWeight));
-          const float y = exp2_of(fmaf(sc[u >> 1][8 * (u & 1) + i + 1] - shift, cq, kTopWeight));
+          const float x = exp2_of(exponent(sc[u >> 1][8 * (u & 1) + i]));
+          const float y = exp2_of(exponent(sc[u >> 1][8 * (u & 1) + i + 1]));
           ws += x;
           ws += y;
           w[u][i / 2] = pair_of<TYPE>(x, y);
           rest[u][i / 2] = pair_of<TYPE>(x - low_of<TYPE>(w[u][i / 2]), y - high_of<TYPE>(w[u][i / 2]));
         }
     };
-    pass(0.f);
+    auto plain = [&](float x) { return fmaf(x - ref, cq, kTopWeight); };
+    const float off = fmaf(-ref, cq, kTopWeight);
+    if (__any(fabsf(off) > kNearScore)) pass(plain);
+    else pass([&](float x) { return fmaf(x, cq, off); });
     if (__any(!(ws < kMostSum) | (sum == 0.f))) {
       float top = sc[0][0];
 #pragma unroll
       for (int e = 1; e < 32; ++e) top = fmaxf(top, sc[e >> 4][e & 15]);
       top = halves_max(top);
-      const bool fresh = halves_max(sum) == 0.f, moves = top > -INFINITY && (fresh || fmaf(top, cq, kTopWeight) > kMostWeight);
-      const float shift = moves ? top : 0.f, f = fresh ? 1.f : exp2_of(-shift * cq);
-      ref += shift;
+      const bool fresh = halves_max(sum) == 0.f, moves = top > -INFINITY && (fresh || fmaf(top - ref, cq, kTopWeight) > kMostWeight);
+      const float to = moves ? top : ref, f = fresh ? 1.f : exp2_of((ref - to) * cq);
+      ref = to;
       sum *= f;
 #pragma unroll
       for (int d = 0; d < DB; ++d) acc[d] *= f;
       ws = 0.f;
-      pass(shift);
+      pass(plain);
     }
     sum += ws;
   };
@@ -1117,7 +1125,7 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
 #pragma unroll
     for (int j = NK; j < kAheadReads; ++j) part[j] = read(j);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) sc[0][i] = sc[1][i] = -ref;        // (scores come out less the reference)
+    for (int i = 0; i < 16; ++i) sc[0][i] = sc[1][i] = 0.f;
 #pragma unroll
     for (int j = 0; j < kProducts; ++j) {
       if (j + kAheadReads < kProducts) part[(j + kAheadReads) % (kAheadReads + 1)] = read(j + kAheadReads);

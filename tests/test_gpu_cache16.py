@@ -717,6 +717,60 @@ def test_prefill_bf16_weights_are_two_numbers(gpu, dh, rows, gqa):
     check(out, lse, parts, [n], dh, 16, f"bf16 prefill dh {dh} rows {rows}")
 
 
+# rows of a call and kv heads: prefill's tiles in turn, split and not; row tiles, split and not
+SHAPES = [("prefill", 2, 2), ("prefill", 2, 400), ("prefill", 140, 2), ("prefill", 140, 400)]
+
+
+@pytest.mark.parametrize("diff", [False, True])
+@pytest.mark.parametrize("late", [False, True])
+@pytest.mark.parametrize("dtype, dh", [("fp16", 128), ("bf16", 128), ("fp16", 64)])
+@pytest.mark.parametrize("kind, rows, H", SHAPES)
+def test_equal_scores_share_in_any_tile(gpu, kind, rows, H, dtype, dh, late, diff):
+    """A few equal keys far above all others, in different tiles (late: larger ones behind them): their values' mean, at any
+    magnitude of the scores.  Equal numbers meet the same roundings, so an output is off by the weights' bits, a few fp32
+    sums and its own rounding alone; 3,600 makes scores whose fp32 step is 16 in the exponent of two."""
+    n, ps = 1000, 16
+    first, behind = [5, 70, 333, 400], [600, 990]
+    top = behind if late else first
+    table = np.random.default_rng(5).permutation(-(-n // ps))[None].astype(np.int32)
+    pages = torch.as_tensor(table[0].astype(np.int64), device=gpu)
+    for size in (6.0, 64.0, 512.0, 3600.0):
+        g = torch.Generator(device=gpu).manual_seed(7)
+        key = size * torch.exp(0.2 * torch.randn((H, dh), generator=g, device=gpu))          # (all positive)
+        k = 0.25 * size * torch.randn((n, H, dh), generator=g, device=gpu)
+        k[first] = key
+        if late:
+            k[behind] = 1.5 * key
+        v = torch.randn((n, H, dh), generator=g, device=gpu)
+        cache = kv16.Cache16.allocate(table.size, H, dh, ps, TYPES[dtype], gpu)
+        k, v = (torch.cat([x, x.new_zeros((table.size * ps - n, H, dh))]).to(TYPES[dtype]).view(-1, ps, H, dh).transpose(1, 2) for x in (k, v))
+        cache.k[pages], cache.v[pages] = k, v
+        q = (size * torch.exp(0.2 * torch.randn((rows, H, dh), generator=g, device=gpu))).to(TYPES[dtype])
+        lam = torch.full((H,), 0.5, device=gpu)
+        args = (i32(table, gpu), i32([n], gpu))
+        if kind == "decode":
+            out, lse = kv16.cache16_diff_decode(cache, q, lam, *args, return_lse=True) if diff else kv16.cache16_decode(cache, q, *args, return_lse=True)
+        else:
+            cu, more = i32([0, rows], gpu), dict(causal=False, return_lse=True)
+            out, lse = kv16.cache16_diff_prefill(cache, q, lam, cu, *args, **more) if diff else kv16.cache16_prefill(cache, q, cu, *args, **more)
+        kk, vv = (x.transpose(1, 2).reshape(-1, H, dh)[:n].double() for x in (k, v))
+        for i, d in enumerate((slice(0, dh // 2), slice(dh // 2, dh)) if diff else (slice(0, dh),)):
+            s = torch.bmm(q[..., d].double().transpose(0, 1).contiguous(), kk[..., d].permute(1, 2, 0).contiguous())
+            s = s.transpose(0, 1) / math.sqrt(d.stop - d.start)
+            others = s.clone()
+            others[..., top] = -math.inf
+            most = s[..., top[0]]
+            assert (most - others.amax(-1) > 40).all()                   # (e^-40 of the others)
+            want = f64(most) + math.log(len(top))
+            check_lse(lse[..., i] if diff else lse, want, f64(q[..., d].double().mul(kk[top[0], :, d]).sum(-1) / math.sqrt(d.stop - d.start)), dh, f"size {size}")
+        want = vv[top].mean(0)[None].expand(rows, -1, -1) * (0.5 if diff else 1.0)
+        mass = vv[top].abs().mean(0)[None] * (1.5 if diff else 1.0)
+        tol = (2.0 ** (-22 if dtype == "fp16" else -16) + 2.0 ** -19) * f64(mass) + last_rounding(f64(want), TYPES[dtype]) * 1.01
+        err = np.abs(f64(out) - f64(want))
+        log(f"  {kind} {rows} x {H} {dtype} dh {dh} size {size}: {np.nan_to_num(err / tol, nan=9e9).max():.3f} of the bound")
+        assert (err <= tol).all(), f"size {size}: {(~(err <= tol)).sum()} outputs off"
+
+
 def test_nan_query_and_key_stay_in_their_rows(gpu):
     lens = [50, 70]
     cache, want, table = setup(gpu, 22, "fp16", 128, 16, 2, lens)
