@@ -122,6 +122,19 @@ __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2
 constexpr float kTopWeight = 8.0f;      // log2 of the weight at the reference, ...
 constexpr float kSlackWeight = 4.0f;    // ... which moves once a weight passes 2^4 times that
 constexpr float kNoScore = -3.0e38f;    // reference before the first score
+// A row's reference for the largest exponent `top` that it has seen, and whether it is
+// to move there: by the difference, for past 2^27 an fp32 step is 16 and more, and
+// a weight of 2^16 is no fp16 number.  top - kTopWeight, or top where that would round
+// further down.  (Not contracted: `top` may be a product, and its rounded value counts.)
+__device__ __forceinline__ bool moves_to(float top, float ref) {
+#pragma clang fp contract(off)
+  return top - ref > kTopWeight + kSlackWeight;
+}
+__device__ __forceinline__ float reference_at(float top) {
+#pragma clang fp contract(off)
+  const float to = top - kTopWeight;
+  return top - to > kTopWeight ? top : to;
+}
 
 __device__ __forceinline__ float wave_sum(float x) {
   x += row_rotated<8>(x);

@@ -57,6 +57,11 @@ __device__ __forceinline__ int seq_tokens(const Cache16& c, const Cache8Batch& b
 // difference is taken (one multiply-add below it), so that the largest weight is
 // what the reference says at any magnitude.
 constexpr float kPlainScore = 0x1p18f;
+__device__ __forceinline__ float score_less(float x, float cq, float ref) {
+#pragma clang fp contract(off)                                       // (__fmul_rn and __fsub_rn are contracted)
+  const float s = x * cq;
+  return s - ref;
+}
 constexpr float kLog2e = 1.44269504088896f, kLn2 = 0.693147180559945f;
 
 // ---- append --------------------------------------------------------------------
@@ -473,9 +478,9 @@ __global__ __launch_bounds__(256, 2) void cache16_decode_kernel(Cache16AttendLau
         }
         float top = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3]));
         top = fmaxf(top, fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3]))) * cq;
-        if (__any(top > ref + (kTopWeight + kSlackWeight))) {                 // (each column by its own scores)
+        if (__any(moves_to(top, ref))) {                                      // (each column by its own scores)
           top = rows_max(top);
-          const float to = top > ref + (kTopWeight + kSlackWeight) ? top - kTopWeight : ref;
+          const float to = moves_to(top, ref) ? reference_at(top) : ref;
           const float f = exp2_of(ref - to);
           ref = to;
           sum *= f;
@@ -486,7 +491,7 @@ __global__ __launch_bounds__(256, 2) void cache16_decode_kernel(Cache16AttendLau
         float cw = cq, off = -ref;
         if (__any((fabsf(ref) > kPlainScore) & (ref > kNoScore))) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) sc[e >> 2][e & 3] = __fsub_rn(__fmul_rn(sc[e >> 2][e & 3], cq), ref);
+          for (int e = 0; e < 8; ++e) sc[e >> 2][e & 3] = score_less(sc[e >> 2][e & 3], cq, ref);
           cw = 1.f;
           off = 0.f;
         }

@@ -717,8 +717,8 @@ def test_prefill_bf16_weights_are_two_numbers(gpu, dh, rows, gqa):
     check(out, lse, parts, [n], dh, 16, f"bf16 prefill dh {dh} rows {rows}")
 
 
-# rows of a call and kv heads: prefill's tiles in turn, split and not; row tiles, split and not
-SHAPES = [("prefill", 2, 2), ("prefill", 2, 400), ("prefill", 140, 2), ("prefill", 140, 400)]
+# rows of a call and kv heads: decode; prefill's tiles in turn, split and not; row tiles, split and not
+SHAPES = [("decode", 1, 4), ("decode", 1, 300), ("prefill", 2, 2), ("prefill", 2, 400), ("prefill", 140, 2), ("prefill", 140, 400)]
 
 
 @pytest.mark.parametrize("diff", [False, True])
