@@ -688,9 +688,9 @@ __global__ __launch_bounds__(256, 2) void cache8_decode_kernel(Cache8AttendLaunc
 #pragma unroll
         for (int i = 1; i < 4; ++i) top = fmaxf(top, fmaxf(fmaxf(sc[i][0], sc[i][1]), fmaxf(sc[i][2], sc[i][3])));
         top = fmaf(top, ck, lsv);
-        if (__any(top > ref + (kTopWeight + kSlackWeight))) {                 // (each column by its own scores)
+        if (__any(moves_to(top, ref))) {                                      // (each column by its own scores)
           top = rows_max(top);
-          const float to = top > ref + (kTopWeight + kSlackWeight) ? top - kTopWeight : ref;
+          const float to = moves_to(top, ref) ? reference_at(top) : ref;
           const float f = exp2_of(ref - to);
           ref = to;
           sum *= f;
@@ -1072,9 +1072,9 @@ __global__ __launch_bounds__(DH == 128 ? 512 : 256, 2) void cache8_prefill_kerne
         for (int i = 1; i < 8; ++i) m = fmaxf(m, sc[u >> 1][8 * (u & 1) + i]);
         top = fmaxf(top, fmaf(m, ck[u], lsv[u]));
       }
-      if (__any(top > ref + (kTopWeight + kSlackWeight))) {           // (each row by its own scores)
+      if (__any(moves_to(top, ref))) {                                // (each row by its own scores)
         top = halves_max(top);
-        const float to = top > ref + (kTopWeight + kSlackWeight) ? top - kTopWeight : ref;
+        const float to = moves_to(top, ref) ? reference_at(top) : ref;
         const float f = exp2_of(ref - to);
         ref = to;
         sum *= f;

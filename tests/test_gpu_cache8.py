@@ -391,6 +391,32 @@ def test_scores_of_any_size(gpu, dh):
                 assert abs(lse[row, head].item() - score) <= 2.0 ** -21 * abs(score)
 
 
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("dh", [64, 128])
+def test_scores_whose_step_is_sixteen(gpu, dh, dtype):
+    """Exponents of two from 2^27 to 2^28, where 8 below a number is a tie between it and 16 below: the largest takes all."""
+    n, ps, heads = 100, 16, 16
+    table = tables(70, 8, [7])
+    cache = random_cache(gpu, 71, 8, 1, dh, ps, "int8")
+    cache.k_codes.zero_()
+    for t in range(n):
+        cache.k_codes[int(table[0, t // ps]), 0, t % ps, 0] = t + 1
+    cache.scales[..., 0] = 512.0
+    q = torch.zeros(1, heads, dh, dtype=TYPES[dtype], device=gpu)
+    q[0, :, 0] = torch.linspace(2.0 ** 27.1, 2.0 ** 27.9, heads) * (math.sqrt(dh) * math.log(2) / 512 / n)
+    score = rows_np(q)[0, :, 0] * 512 * n / math.sqrt(dh)
+    assert (score / math.log(2) > 2 ** 27).all() and (score / math.log(2) < 2 ** 28).all()
+    _, v, _ = oracle_of(cache).tokens(table, 0, 0, n)
+    td, lens = i32(table, gpu), i32([n], gpu)
+    for out, lse in (kv8.cache8_decode(cache, q, td, lens, return_lse=True),
+                     kv8.cache8_prefill(cache, q, i32([0, 1], gpu), td, lens, return_lse=True)):
+        got = rows_np(out)[0]
+        # one weight, rounded in the product and not in the sum (2^-11), and the output's own rounding
+        tol = 2.0 ** -11 + torch.finfo(TYPES[dtype]).eps / 2 * 1.001
+        assert (np.abs(got - v[n - 1, 0]) <= tol * np.abs(v[n - 1, 0]) + 2.0 ** -24).all()
+        assert (np.abs(rows_np(lse)[0] - score) <= 2.0 ** -21 * score).all()
+
+
 def test_empty_caches_and_tables(gpu):
     """A cache of no page, tables of no block, no sequence at all: zeros and -inf, and nothing written."""
     q = torch.randn(2, 4, 64, device=gpu).half()
