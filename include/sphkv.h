@@ -785,7 +785,9 @@ typedef struct sphkv_cache16 {
  * Keys and values of a token past the table, of a sequence with a negative start
  * or of an absent page are dropped (its queries are rotated all the same); rows
  * from cu_rows[num_seqs] on are not read, and keep their contents in q_out.  A
- * written page belongs to one sequence.
+ * written page belongs to one sequence.  Tokens, heads and pages of the cache, its k
+ * and v, rows and heads of q_out, and q_out and the inputs (but for q itself) that
+ * share memory are refused; attention reads such a cache.
  */
 int sphkv_cache16_append(const sphkv_cache16* cache, const void* k, const void* v, const void* q, int32_t in_type,
                          int64_t k_row_stride, int64_t k_head_stride, int64_t v_row_stride, int64_t v_head_stride,

@@ -12,6 +12,7 @@
 
 #include "../../include/sphkv.h"
 #include "sphkv_internal.h"
+#include "sphkv_overlap.h"
 
 namespace {
 
@@ -1162,6 +1163,18 @@ int cache16_checks(const char* fn, const sphkv_cache16* cache, const int32_t* ta
   return SPHKV_OK;
 }
 
+// rows [rows, heads, dh] of elements of `size` bytes
+sphkv::Rows rows_in(const void* at, int64_t rows, int64_t row, int64_t heads, int64_t head, int32_t dh, int64_t size) {
+  const int64_t most = (int64_t)1 << 60;                             // (in bytes they stay within 64 bits)
+  return {(int64_t)(uintptr_t)at, dh * size, 2, {rows, heads, 1},
+          {std::clamp(row, -most, most) * size, std::clamp(head, -most, most) * size, 0}};
+}
+sphkv::Rows tokens_in(const void* at, const sphkv_cache16& x, int64_t page, int64_t head, int64_t token) {
+  const int64_t most = (int64_t)1 << 60;
+  return {(int64_t)(uintptr_t)at, x.dh * 2, 3, {x.num_pages, x.num_kv, x.page_size},
+          {std::min(page, most) * 2, std::min(head, most) * 2, token * 2}};
+}
+
 // differential attention's weights (NULL: the ordinary one)
 struct Diff16 { const float* lambda; const float* norm_weight; float norm_eps; };
 
@@ -1308,6 +1321,24 @@ int sphkv_cache16_append(const sphkv_cache16* cache, const void* k, const void* 
   if (num_seqs == 0 || num_rows == 0) return ok();
   if (!k || !v || !start || (q && !q_out) || (num_freqs > 0 && !inv_freq))
     return fail(SPHKV_EINVAL, "%s: null pointer argument", fn);
+  // what is written, by threads in any order, is written once and not read as something else
+  if (c.num_pages > 0 && max_blocks > 0) {
+    const sphkv::Rows ck = tokens_in(cache->k, *cache, cache->k_page, cache->k_head, cache->k_token);
+    const sphkv::Rows cv = tokens_in(cache->v, *cache, cache->v_page, cache->v_head, cache->v_token);
+    if (sphkv::shares_itself(ck) || sphkv::shares_itself(cv) || sphkv::share(ck, cv))
+      return fail(SPHKV_EINVAL, "%s: tokens of the cache, or its k and v, share memory", fn);
+  }
+  if (q) {
+    const int64_t heads = (int64_t)c.num_kv * gqa, size = in_type == SPHKV_FP32 ? 4 : 2;
+    const sphkv::Rows in = rows_in(q, num_rows, q_row_stride, heads, q_head_stride, c.dh, size);
+    const sphkv::Rows out = rows_in(q_out, num_rows, q_out_row_stride, heads, q_out_head_stride, c.dh, 2);
+    if (sphkv::shares_itself(out)) return fail(SPHKV_EINVAL, "%s: rows and heads of q_out overlap", fn);
+    if (!(in_type == c.type && sphkv::same(in, out)) && sphkv::share(in, out))
+      return fail(SPHKV_EINVAL, "%s: q_out must be q itself, of its type and strides, or share no memory with it", fn);
+    if (sphkv::share(rows_in(k, num_rows, k_row_stride, c.num_kv, k_head_stride, c.dh, size), out) ||
+        sphkv::share(rows_in(v, num_rows, v_row_stride, c.num_kv, v_head_stride, c.dh, size), out))
+      return fail(SPHKV_EINVAL, "%s: q_out shares memory with k or v", fn);
+  }
   sphkv::Cache16AppendLaunch L{c, {cu_rows, start, table, table_stride, c.num_pages > 0 ? max_blocks : 0, num_seqs, num_rows},
                                k, v, q, in_type, k_row_stride, k_head_stride, v_row_stride, v_head_stride, q_row_stride,
                                q_head_stride, gqa, q_out, q_out_row_stride, q_out_head_stride, inv_freq, freq_type,

@@ -47,8 +47,9 @@ class Cache16:
     page_size, dh], both fp16 or both bf16, 16-byte aligned, the dh elements of a
     token contiguous.  Pages, heads and tokens may lie in any order, their
     strides multiples of 8 elements: a tensor of [num_pages, page_size, num_kv,
-    dh] comes in as x.transpose(1, 2), one of two as kv[:, 0] and kv[:, 1].  The
-    tensors and what follows from them are read-only: a cache over others is
+    dh] comes in as x.transpose(1, 2), one of two as kv[:, 0] and kv[:, 1].  A
+    cache whose tokens share memory (an expanded view, one tensor as k and v) is
+    for attention alone, an append to it is refused.  The tensors and what follows from them are read-only: a cache over others is
     another Cache16."""
 
     __slots__ = ("_k", "_v", "_num_pages", "_num_kv", "_page_size", "_dh", "_device", "_dtype", "_index", "_type", "_struct",
@@ -153,7 +154,8 @@ def cache16_append(cache: Cache16, k: torch.Tensor, v: torch.Tensor, table: torc
     rest stays (None: all).  Two parts: the two maps of differential attention.
 
     Returns the rotated queries [rows, num_kv * gqa, dh] of the cache's type (None
-    without q), in q_out if that is given: any row and head stride, q itself too.
+    without q), in q_out if that is given: any row and head stride, q itself too
+    (other memory of q, k or v is refused).
     Keys and values past the table, of a sequence with a negative start or of a
     page outside the cache are dropped; rows behind the last sequence are left as
     they were in q_out.  A written page belongs to one sequence."""

@@ -7,6 +7,7 @@ import pytest
 import torch
 
 import sphkv_kv16 as kv16
+import sphkv_lib
 from gpu_helpers import log
 from oracle import cache16 as o16
 
@@ -213,6 +214,42 @@ def test_append_strides_alignment_and_queries_in_place(gpu):
     for s in range(T):
         p, i = [2, 0][(3 + s) // ps], (3 + s) % ps
         assert torch.equal(first[0][p, :, i], cache.k[p, :, i]) and torch.equal(first[1][p, :, i], cache.v[p, :, i])
+
+
+def test_memory_that_tensors_share(gpu):
+    """Keys and values, queries and outputs beside each other in one buffer are appended as into buffers of their own; over
+    each other they are refused, and attention reads such a cache."""
+    P, H, ps, dh, T = 4, 3, 16, 64, 40
+    g = torch.Generator(device=gpu).manual_seed(3)
+    k, v, q = (torch.randn((T, h, dh), generator=g, device=gpu).half() for h in (H, H, 2 * H))
+    args = (i32([[2, 0, 3]], gpu), i32([5], gpu), i32([0, T], gpu))
+    f = kv16.rope_inv_freq(dh, device=gpu)
+    own = kv16.Cache16.allocate(P, H, dh, ps, device=gpu)
+    ref = kv16.cache16_append(own, k, v, *args, inv_freq=f, q=q)
+    pair = torch.zeros((P, ps, H, 2, dh), dtype=torch.float16, device=gpu).transpose(1, 2)           # a token's keys, then its values
+    mixed = torch.zeros((P, 2, H * ps * dh), dtype=torch.float16, device=gpu)                         # heads first, tokens first
+    both = torch.empty((T, 2, 2 * H, dh), dtype=torch.float16, device=gpu)
+    both[:, 0] = q
+    for cache in (kv16.Cache16(pair[..., 0, :], pair[..., 1, :]),
+                  kv16.Cache16(mixed[:, 0].unflatten(1, (H, ps, dh)), mixed[:, 1].unflatten(1, (ps, H, dh)).transpose(1, 2))):
+        got = kv16.cache16_append(cache, k, v, *args, inv_freq=f, q=both[:, 0], q_out=both[:, 1])
+        assert torch.equal(got, ref) and torch.equal(cache.k, own.k) and torch.equal(cache.v, own.v)
+    assert torch.equal(both[:, 0], q)
+    lens = i32([45], gpu)
+    tied, alike = kv16.Cache16(own.k, own.k), kv16.Cache16(own.k, own.k.clone())
+    views = kv16.Cache16(own.k[:1].expand(P, -1, -1, -1), own.v[:, :1].expand(-1, H, -1, -1))
+    copies = kv16.Cache16(views.k.contiguous(), views.v.contiguous())
+    for x, y in ((tied, alike), (views, copies)):
+        before = x.k.clone()
+        with pytest.raises(sphkv_lib.SphkvError, match="share memory"):
+            kv16.cache16_append(x, k, v, *args, inv_freq=f)
+        assert torch.equal(x.k, before)
+        assert torch.equal(kv16.cache16_decode(x, q[:1], args[0], lens), kv16.cache16_decode(y, q[:1], args[0], lens))
+        assert torch.equal(kv16.cache16_prefill(x, q, args[2], args[0], lens), kv16.cache16_prefill(y, q, args[2], args[0], lens))
+    flat = torch.zeros(T * 2 * H * dh + 8, dtype=torch.float16, device=gpu)
+    over = [flat[a:a + T * 2 * H * dh].view(T, 2 * H, dh) for a in (0, 8)]
+    with pytest.raises(sphkv_lib.SphkvError, match="q_out must be q itself"):
+        kv16.cache16_append(own, k, v, *args, inv_freq=f, q=over[0], q_out=over[1])
 
 
 # ---- attention -------------------------------------------------------------------

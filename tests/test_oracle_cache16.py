@@ -181,6 +181,89 @@ def test_append_refusals(kw, msg):
     assert rc == -1 and msg in text, text
 
 
+# what an append writes is written once and not read as something else.  Caches that are in order, and the other way
+# round queries' outputs that are, are shown by the refusal of what is looked at next
+A, B, Q, O, K, V = (i << 32 for i in range(1, 7))
+ONE = dict(num_seqs=1, num_rows=1, ck=A, cv=B, q=Q, q_out=O, k=K, v=V)
+GOOD_CACHES = [
+    dict(),
+    dict(num_kv=3, k_head=16 * 64, v_head=16 * 64, k_page=3 * 16 * 64, v_page=3 * 16 * 64),
+    dict(num_kv=3, k_head=64, v_head=64, k_token=3 * 64, v_token=3 * 64, k_page=3 * 16 * 64, v_page=3 * 16 * 64),
+    dict(cv=A + 2 * 16 * 64, k_page=2 * 16 * 64, v_page=2 * 16 * 64),                             # a page's keys, then its values
+    dict(cv=A + 2 * 64, k_token=128, v_token=128, k_page=16 * 128, v_page=16 * 128),              # a token's
+    dict(cv=A + 2 * 64, num_kv=3, k_head=128, v_head=128, k_token=3 * 128, v_token=3 * 128, k_page=3 * 16 * 128, v_page=3 * 16 * 128),
+    dict(num_pages=1, k_page=0, v_page=0),
+    dict(cv=A + 2 * 4 * 16 * 64),                                                                  # behind each other
+]
+BAD_CACHES = [
+    dict(cv=A),
+    dict(cv=A + 2 * 64),
+    dict(cv=A + 2 * 4 * 16 * 64 - 16),
+    dict(k_page=0),
+    dict(v_page=0),
+    dict(v_token=0),
+    dict(k_token=56),
+    dict(num_kv=2),                                                                                # (head strides 0)
+    dict(num_kv=2, k_head=16 * 64, v_head=16 * 64),                                                # (page strides for one head)
+    dict(k_page=16 * 64 - 8),
+]
+
+
+@pytest.mark.parametrize("kw", GOOD_CACHES)
+def test_append_takes_caches_in_order(kw):
+    rc, text = call(*ENTRIES["append"], {**ONE, "q_out": Q + 2, **kw})
+    assert rc == -1 and "q_out must be q itself" in text, text
+
+
+@pytest.mark.parametrize("kw", BAD_CACHES)
+def test_append_refuses_caches_that_share_memory(kw):
+    rc, text = call(*ENTRIES["append"], {**ONE, **kw})
+    assert rc == -1 and "the cache, or its k and v, share memory" in text, text
+    rc, text = call(*ENTRIES["append"], {**ONE, "q": None, "gqa": 0, **kw})
+    assert rc == -1 and "the cache, or its k and v, share memory" in text, text
+
+
+ROWS = dict(num_seqs=3, num_rows=3, gqa=2, q_row=128, q_head=64, o_row=128, o_head=64)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(),
+    dict(q_out=Q),
+    dict(q_out=Q + 2 * 128, q_row=256, o_row=256),                                                 # halves of a row
+    dict(q_out=Q + 2 * 64, q_row=256, q_head=128, o_row=256, o_head=128),                          # every other head
+    dict(q_out=Q, q_row=-200, o_row=-200),
+    dict(q=K - 2 * 128, q_out=K - 2 * 128, q_row=320, o_row=320, k_row=320, v=K + 128, v_row=320),  # q, k, v of one row
+], ids=range(6))
+def test_append_takes_outputs_in_order(kw):
+    """(The keys or values are laid over the outputs then.)"""
+    good = {**ONE, **ROWS, **kw}
+    if "v" not in kw:
+        rc, text = call(*ENTRIES["append"], {**good, "v": good["q_out"] + 2})
+    else:
+        rc, text = call(*ENTRIES["append"], {**good, "v": good["q_out"] + 4})
+    assert rc == -1 and "shares memory with k or v" in text, text
+
+
+@pytest.mark.parametrize("kw, msg", [
+    (dict(o_row=64), "rows and heads of q_out overlap"),
+    (dict(o_row=0), "rows and heads of q_out overlap"),
+    (dict(o_head=63), "rows and heads of q_out overlap"),
+    (dict(o_row=-127), "rows and heads of q_out overlap"),
+    (dict(q_out=Q + 2), "q_out must be q itself"),
+    (dict(q_out=Q + 2 * 64), "q_out must be q itself"),
+    (dict(q_out=Q, o_row=192), "q_out must be q itself"),
+    (dict(q_out=Q, o_row=64, o_head=192), "q_out must be q itself"),
+    (dict(q_out=Q, in_type=2), "q_out must be q itself"),
+    (dict(q_out=Q, in_type=1), "q_out must be q itself"),
+    (dict(q_out=Q - 2 * 383), "q_out must be q itself"),
+    (dict(q_out=K), "shares memory with k or v"),
+    (dict(q_out=V + 2 * 191), "shares memory with k or v"),
+])
+def test_append_refuses_outputs_that_share_memory(kw, msg):
+    rc, text = call(*ENTRIES["append"], {**ONE, **ROWS, **kw})
+    assert rc == -1 and msg in text, text
+
+
 @pytest.mark.parametrize("kw, msg", [
     (dict(gqa=0), "gqa must be"),
     (dict(gqa=65), "gqa must be"),
