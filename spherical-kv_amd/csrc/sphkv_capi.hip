@@ -1206,6 +1206,12 @@ int cache16_attend(const char* fn, bool decode, const Diff16* diff, const sphkv_
     return fail(SPHKV_EINVAL, "%s: workspace needs %lld bytes (got %lld)", fn, (long long)need,
                 (long long)workspace_bytes);
   if ((uintptr_t)workspace & 15) return fail(SPHKV_EINVAL, "%s: workspace must be 16-byte aligned", fn);
+  // (a row's output is written when its queries have been read, and not when another row's have)
+  const int64_t heads = (int64_t)c.num_kv * gqa;
+  const sphkv::Rows in = rows_in(q, num_rows, q_row_stride, heads, q_head_stride, c.dh, 2);
+  const sphkv::Rows to = rows_in(out, num_rows, heads * c.dh, heads, c.dh, c.dh, 2);
+  if (!sphkv::same(in, to) && sphkv::share(in, to))
+    return fail(SPHKV_EINVAL, "%s: out must be q itself, of its strides, or share no memory with it", fn);
   sphkv::Cache16AttendLaunch L{c, {cu_rows, lens, table, table_stride, c.num_pages > 0 ? max_blocks : 0, num_seqs, num_rows},
                                q, q_row_stride, q_head_stride, gqa, causal, window, sm_scale, out, lse, workspace,
                                diff ? diff->lambda : nullptr, diff ? diff->norm_weight : nullptr, diff ? diff->norm_eps : 0.f};

@@ -880,6 +880,23 @@ def test_outputs_over_their_queries(gpu):
             assert run(x, out=x) is x and torch.equal(x, ref)
 
 
+def test_outputs_beside_their_queries(gpu):
+    """Queries and outputs in one buffer without a common byte, as in buffers of their own; a shifted output is refused."""
+    lens = [70, 300, 1]
+    cache, want, table = setup(gpu, 36, "fp16", 64, 16, 2, lens)
+    flat = torch.randn(2 * 3 * 8 * 64 + 64, device=gpu).half()
+    q, out = flat[:3 * 8 * 64].view(3, 8, 64), flat[3 * 8 * 64:2 * 3 * 8 * 64].view(3, 8, 64)
+    near = flat[64:3 * 8 * 64 + 64].view(3, 8, 64)
+    lam = torch.full((8,), 0.5, device=gpu)
+    args, cu = (i32(table, gpu), i32(lens, gpu)), i32([0, 1, 2, 3], gpu)
+    for run in (lambda **kw: kv16.cache16_decode(cache, q, *args, **kw), lambda **kw: kv16.cache16_diff_decode(cache, q, lam, *args, **kw),
+                lambda **kw: kv16.cache16_prefill(cache, q, cu, *args, **kw), lambda **kw: kv16.cache16_diff_prefill(cache, q, lam, cu, *args, **kw)):
+        ref = run()
+        assert torch.equal(run(out=out), ref)
+        with pytest.raises(sphkv_lib.SphkvError, match="out must be q itself"):
+            run(out=near)
+
+
 def test_graphs_that_share_a_workspace(gpu):
     """Two captured graphs over one workspace, replayed in turn with eager calls between."""
     lens = [900, 70, 4000]

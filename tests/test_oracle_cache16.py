@@ -294,6 +294,21 @@ def test_attention_refusals_of_work(entry, kw, msg):
     assert rc == -1 and msg in text
 
 
+@pytest.mark.parametrize("kw", [
+    dict(out=Q + 2),
+    dict(out=Q, q_row=192),
+    dict(out=Q, q_row=64, q_head=192),
+    dict(out=Q, q_head=0),
+    dict(out=Q + 2 * 128, q_row=200),
+    dict(out=Q - 2 * 127),
+])
+@pytest.mark.parametrize("entry", ATTENTION)
+def test_attention_refuses_outputs_over_other_queries(entry, kw):
+    more = dict(num_rows=3, cu_rows=P) if "prefill" in entry else {}
+    rc, text = call(*ENTRIES[entry], dict(dict(num_seqs=3, gqa=2, q=Q, q_row=128, q_head=64, **more), **kw))
+    assert rc == -1 and "out must be q itself" in text, text
+
+
 @pytest.mark.parametrize("kw, msg", [
     (dict(gqa=33), "gqa must be"),
     (dict(norm_eps=-1e-9), "norm_eps"),
