@@ -643,6 +643,63 @@ def test_prefill_order(gpu, dtype, dh, gqa, seqs, window):
     check_diff(out[:rows], lse[:rows], maps, lam, None, 1e-5, lens, dh, weight_bits(dtype, True, True), f"diff order {seqs}")
 
 
+# contexts of up to 625 tiles: row tiles of 256 and 128 rows, tiles in turn, splits
+EACH_TILE = [
+    ("bf16", 128, 16, 8, 4, [(9000, 1100)]),
+    ("fp16", 128, 32, 8, 3, [(0, 0), (900, 0), (1500, 1500), (40000, 70), (0, 90)]),
+    ("bf16", 64, 32, 8, 4, [(9000, 1600)]),
+    ("fp16", 128, 128, 8, 4, [(9000, 3), (20, 3), (5000, 4)] + [(100, 1)] * 29),
+    ("bf16", 128, 16, 2, 4, [(30000, 9)]),
+    ("fp16", 64, 16, 2, 4, [(30000, 33), (3000, 2)]),
+]
+
+
+@pytest.mark.parametrize("diff", [False, True])
+@pytest.mark.parametrize("dtype, dh, ps, num_kv, gqa, seqs", EACH_TILE)
+def test_every_tile_of_a_long_context_counts(gpu, dtype, dh, ps, num_kv, gqa, seqs, diff):
+    """A tile's values lie in one element, so that an output is the sum of a few tiles: keys or values of one of hundreds
+    taken from another tile are far past the bound, as the oracle with such a tile in it shows."""
+    lens, new = [a for a, _ in seqs], [b for _, b in seqs]
+    cache, _, table = setup(gpu, 35, dtype, dh, ps, num_kv, lens)
+    long = int(np.argmax(lens))
+    v = torch.zeros_like(cache.v)
+    for s, n in enumerate(lens):
+        token = torch.arange(n, device=gpu)
+        page = torch.as_tensor(table[s].astype(np.int64), device=gpu)[token // ps]
+        d = (token // 64) % dh
+        v[page, :, token % ps, d] = cache.v[page, :, token % ps, d].abs() + 1
+    cache = kv16.Cache16(cache.k, v)
+    bad = kv16.Cache16(cache.k.clone(), v.clone())                        # a late tile's keys and values are the next one's
+    tile = lens[long] // 64 - 3
+    at = [[(int(table[long, t // ps]), t % ps) for t in range(64 * i, 64 * i + 64)] for i in (tile, tile + 1)]
+    to, of = (torch.as_tensor(x, device=gpu).T for x in at)
+    bad.k[to[0], :, to[1]], bad.v[to[0], :, to[1]] = cache.k[of[0], :, of[1]], cache.v[of[0], :, of[1]]
+    bits = 22 if dtype == "fp16" else 16
+    cu = np.cumsum([0] + new)
+    rows = int(cu[-1])
+    q = (0.5 * torch.randn((rows, num_kv * gqa, dh), device=gpu, generator=torch.Generator(device=gpu).manual_seed(9))).to(TYPES[dtype])
+    args = (i32(cu, gpu), i32(table, gpu), i32(lens, gpu))
+    last = slice(int(cu[long + 1]) - 1, int(cu[long + 1]))
+    few = [0] * long + [lens[long]] + [0] * (len(lens) - long - 1)        # the last row of the long context alone
+    one = [0] * (long + 1) + [1] * (len(lens) - long)
+    if diff:
+        lam = torch.full((num_kv * gqa,), 0.5, device=gpu)
+        out, lse = kv16.cache16_diff_prefill(cache, q, lam, *args, return_lse=True)
+        halves = (slice(0, dh // 2), slice(dh // 2, dh))
+        maps = [rows_on_gpu(cache, q, table, lens, cu, 0, d) for d in halves]
+        check_diff(out, lse, maps, lam, None, 0, lens, dh, bits, f"each tile {dtype} {dh}")
+        wrong = [rows_on_gpu(bad, q[last], table, few, one, 0, d) for d in halves]
+        tol = x_bound([x[last] for x in maps[0]], lens, TYPES[dtype], dh, bits) + 0.5 * x_bound([x[last] for x in maps[1]], lens, TYPES[dtype], dh, bits)
+        want, other = maps[0][0][last] - 0.5 * maps[1][0][last], wrong[0][0] - 0.5 * wrong[1][0]
+    else:
+        out, lse = kv16.cache16_prefill(cache, q, *args, return_lse=True)
+        parts = rows_on_gpu(cache, q, table, lens, cu, 0)
+        check(out, lse, parts, lens, dh, bits, f"each tile {dtype} {dh}")
+        other = rows_on_gpu(bad, q[last], table, few, one, 0)[0]
+        want, tol = parts[0][last], x_bound([x[last] for x in parts], lens, TYPES[dtype], dh, bits)
+    assert (np.abs(other - want) > 4 * (tol + last_rounding(want, TYPES[dtype]))).any(-1).all()
+
+
 @pytest.mark.parametrize("diff", [False, True])
 @pytest.mark.parametrize("dtype", ["fp16", "bf16"])
 @pytest.mark.parametrize("dh", [64, 128])
