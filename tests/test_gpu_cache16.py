@@ -687,14 +687,18 @@ def test_every_tile_of_a_long_context_counts(gpu, dtype, dh, ps, num_kv, gqa, se
         out, lse = kv16.cache16_diff_prefill(cache, q, lam, *args, return_lse=True)
         halves = (slice(0, dh // 2), slice(dh // 2, dh))
         maps = [rows_on_gpu(cache, q, table, lens, cu, 0, d) for d in halves]
-        check_diff(out, lse, maps, lam, None, 0, lens, dh, bits, f"each tile {dtype} {dh}")
+        for s, n in enumerate(lens):                                      # (each by its own length)
+            of = slice(int(cu[s]), int(cu[s + 1]))
+            check_diff(out[of], lse[of], [[x[of] for x in m] for m in maps], lam, None, 0, [n], dh, bits, f"each tile {dtype} {dh} {n}")
         wrong = [rows_on_gpu(bad, q[last], table, few, one, 0, d) for d in halves]
         tol = x_bound([x[last] for x in maps[0]], lens, TYPES[dtype], dh, bits) + 0.5 * x_bound([x[last] for x in maps[1]], lens, TYPES[dtype], dh, bits)
         want, other = maps[0][0][last] - 0.5 * maps[1][0][last], wrong[0][0] - 0.5 * wrong[1][0]
     else:
         out, lse = kv16.cache16_prefill(cache, q, *args, return_lse=True)
         parts = rows_on_gpu(cache, q, table, lens, cu, 0)
-        check(out, lse, parts, lens, dh, bits, f"each tile {dtype} {dh}")
+        for s, n in enumerate(lens):
+            of = slice(int(cu[s]), int(cu[s + 1]))
+            check(out[of], lse[of], [x[of] for x in parts], [n], dh, bits, f"each tile {dtype} {dh} {n}")
         other = rows_on_gpu(bad, q[last], table, few, one, 0)[0]
         want, tol = parts[0][last], x_bound([x[last] for x in parts], lens, TYPES[dtype], dh, bits)
     assert (np.abs(other - want) > 4 * (tol + last_rounding(want, TYPES[dtype]))).any(-1).all()
