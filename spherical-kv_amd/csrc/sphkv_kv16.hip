@@ -1316,57 +1316,46 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
     float* o = (float*)s_k;                                           // [DH / 4][kRowTile][4]
     float* rs = (float*)s_v;                                          // references, sums
     const int row = row_wave * 32 + col;
-    constexpr int ROUNDS = sizeof(s_k) >= sizeof(float) * kRowTile * DH ? 1 : 2, DR = DB / ROUNDS;
-    static_assert(sizeof(s_k) * ROUNDS >= sizeof(float) * kRowTile * DH && sizeof(s_v) >= sizeof(float) * 2 * kRowTile, "");
+    static_assert(sizeof(s_k) >= sizeof(float) * kRowTile * DH && sizeof(s_v) >= sizeof(float) * 2 * kRowTile, "");
     const bool whole = DIFF && parts == 1;
-#pragma unroll
-    for (int round = 0; round < ROUNDS; ++round) {
-      __syncthreads();                                                // (the last tile, or the last round, is read no more)
-      if (group == 1 && (!DIFF || whole)) {
-        if (half == 0) {
-          rs[row] = ref;
-          rs[kRowTile + row] = sum;
-        }
-#pragma unroll
-        for (int d = 0; d < DR; ++d)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const floatx16& x = acc[round * DR + d];
-            *(floatx4*)&o[((8 * d + 2 * i + half) * kRowTile + row) * 4] = floatx4{x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]};
-          }
+    __syncthreads();                                                  // (the last tile is read no more)
+    if (group == 1 && (!DIFF || whole)) {
+      if (half == 0) {
+        rs[row] = ref;
+        rs[kRowTile + row] = sum;
       }
-      __syncthreads();
-      if (group == 0 && (!DIFF || whole)) {
-        const float other = rs[row], osum = rs[kRowTile + row];
-        float f, g;
-        if constexpr (DIFF) {
-          lam = late->lambda[h * gqa + hd];
-          f = round > 0 ? 1.f : sum == 0.f ? 0.f : 1.0f / sum;       // (all blocks at once, in the first round)
-          g = osum == 0.f ? 0.f : -lam / osum;
-          ref2 = other;
-          sum2 = osum;
-          if (round == 0)
 #pragma unroll
-            for (int d = 0; d < DB; ++d) acc[d] *= f;
-          f = 1.f;
-        } else {
-          const float R = fmaxf(ref, other);
-          f = exp2_of((ref - R) * cq);
-          g = exp2_of((other - R) * cq);
-          if (round == ROUNDS - 1) {
-            ref = R;
-            sum = fmaf(sum, f, osum * g);
-          }
-        }
+      for (int d = 0; d < DB; ++d)
 #pragma unroll
-        for (int d = 0; d < DR; ++d)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const floatx4 x = *(const floatx4*)&o[((8 * d + 2 * i + half) * kRowTile + row) * 4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[round * DR + d][4 * i + e] = fmaf(acc[round * DR + d][4 * i + e], f, x[e] * g);
-          }
+        for (int i = 0; i < 4; ++i)
+          *(floatx4*)&o[((8 * d + 2 * i + half) * kRowTile + row) * 4] =
+              floatx4{acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]};
+    }
+    __syncthreads();
+    if (group == 0 && (!DIFF || whole)) {
+      const float other = rs[row], osum = rs[kRowTile + row];
+      float f, g;
+      if constexpr (DIFF) {
+        lam = late->lambda[h * gqa + hd];
+        f = sum == 0.f ? 0.f : 1.0f / sum;
+        g = osum == 0.f ? 0.f : -lam / osum;
+        ref2 = other;
+        sum2 = osum;
+      } else {
+        const float R = fmaxf(ref, other);
+        f = exp2_of((ref - R) * cq);
+        g = exp2_of((other - R) * cq);
+        ref = R;
+        sum = fmaf(sum, f, osum * g);
       }
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const floatx4 x = *(const floatx4*)&o[((8 * d + 2 * i + half) * kRowTile + row) * 4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[d][4 * i + e] = fmaf(acc[d][4 * i + e], f, x[e] * g);
+        }
     }
     if (group == 1 && (!DIFF || whole)) return;
   }
