@@ -802,11 +802,12 @@ int sphkv_cache16_append(const sphkv_cache16* cache, const void* k, const void* 
  * last `window` of its first lens[s] tokens (0: all of them), its own among them:
  *   out = sum_t softmax_t(sm_scale <q, k_t>) v_t,  lse = ln sum_t exp(sm_scale <q, k_t>)
  * q [num_seqs, num_kv*gqa, dh] and out (contiguous, q itself or none of its memory) of
- * the cache's type, lse fp32 [num_seqs, num_kv*gqa] or NULL, gqa 1..64.  A sequence without a token gets zeros
- * and -inf.  Scores, sums and outputs are held in fp32; a weight meets its value as
- * two numbers of the cache's type (22 bits for fp16, 16 for bf16).  A value that
- * is not finite makes that element of the rows that see its token an infinity or
- * NaN, and of no other row.
+ * the cache's type, lse fp32 [num_seqs, num_kv*gqa] or NULL, gqa 1..64.  A sequence
+ * without a token gets zeros and -inf.  Scores, sums and outputs are held in fp32; a
+ * weight meets its value as two numbers of the cache's type: 16 bits for bf16, 22 for
+ * fp16 (and, for weights below 2^-10 of the row's largest, whose second number is
+ * subnormal, to within 2^-33 of the largest).  A value that is not finite makes that
+ * element of the rows that see its token an infinity or NaN, and of no other row.
  */
 int64_t sphkv_cache16_decode_workspace_bytes(int32_t num_seqs, int32_t num_kv, int32_t gqa, int32_t dh,
                                              int32_t differential);

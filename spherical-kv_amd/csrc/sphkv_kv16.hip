@@ -678,8 +678,8 @@ __global__ __launch_bounds__(64 * WAVES) void cache16_decode_merge_kernel(Cache1
 // rows see in part, values that are not finite count as zeros in the product, and
 // are added at the end to the outputs of the rows that see them.
 constexpr int kTileTokens = 64;
-// A weight may pass 2^kMostWeight; where a lane's 32 of a tile add up to less than
-// kMostSum none has, or fp16 holds it.
+// The reference moves where a weight has passed 2^kMostWeight and a lane's 32 of a
+// tile add up to kMostSum or more: with less each is below kMostSum, which fp16 holds.
 constexpr float kMostWeight = 10.0f, kMostSum = 0x1p15f;
 constexpr float kNearScore = 64.f;
 
@@ -1064,9 +1064,9 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
     }
   };
   // The tile's weights, 2^kTopWeight at the reference.  Their largest is not looked
-  // for: where a lane's 32 add up to less than 2^(kMostWeight + 5) none has passed
-  // the bound of the reference.  Otherwise, and at a row's first scores, the reference
-  // becomes the row's largest score (both halves of a row decide alike).  Every score is
+  // for where a lane's 32 add up to less than kMostSum.  Otherwise, and at a row's first
+  // scores, the reference becomes the row's largest score if that one's weight passes
+  // 2^kMostWeight (both halves of a row decide alike).  Every score is
   // a sum from zero, less the reference, so that equal ones weigh the same in any tile
   // and at any magnitude.  The difference is part of the exponent's one multiply-add up to
   // kNearScore, whose rounding is 2^-19 of a weight there (always apart: 661 us for that

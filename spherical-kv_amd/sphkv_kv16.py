@@ -333,10 +333,11 @@ def cache16_decode(cache: Cache16, q: torch.Tensor, table: torch.Tensor, lens: t
     its pages, or the last `window` of them (sphkv_cache16_decode).  q [num_seqs,
     num_kv * gqa, dh] of the cache's type, gqa up to 64; lens int32 [num_seqs];
     window 0: no window; sm_scale 1 / sqrt(dh) unless given.  A softmax weight
-    meets its value with 22 bits in fp16, with 16 in bf16.  Returns out (q's
-    shape and type), with return_lse (out, lse): lse fp32 [num_seqs, num_kv *
-    gqa] is the natural log of the softmax's sum.  A sequence without tokens gets
-    zeros and -inf."""
+    meets its value with 16 bits in bf16, with 22 in fp16 (to within 2^-33 of the
+    row's largest weight, if it is small beside it).  Returns out (q's shape and
+    type), with return_lse (out, lse): lse fp32 [num_seqs, num_kv * gqa] is the
+    natural log of the softmax's sum.  A sequence without tokens gets zeros and
+    -inf."""
     return _decode(cache, q, table, lens, window, sm_scale, out, return_lse, lse, workspace, None)
 
 
