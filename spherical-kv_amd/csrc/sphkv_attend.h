@@ -66,13 +66,6 @@ __device__ __forceinline__ float value_of(typename Elem<TYPE>::T x) {
   else if constexpr (TYPE == kBf16) return __builtin_bit_cast(float, (uint32_t)x << 16);
   else return x;
 }
-template <int TYPE>
-__device__ __forceinline__ typename Elem<TYPE>::T element_of(float x) {
-  if constexpr (TYPE == kFp16) return __builtin_bit_cast(uint16_t, (_Float16)x);
-  else if constexpr (TYPE == kBf16) return __builtin_bit_cast(uint16_t, (__bf16)x);
-  else return x;
-}
-
 // N consecutive elements at any alignment that theirs allows
 template <class T, int N>
 struct __attribute__((packed, aligned(sizeof(T)))) Unaligned { T x[N]; };
@@ -88,26 +81,6 @@ __device__ __forceinline__ float wave_max(float x) {
   x = fmaxf(x, row_rotated<2>(x));
   x = fmaxf(x, row_rotated<1>(x));
   return rows_max(x);
-}
-
-__device__ __forceinline__ int64_t shfl64(int64_t x, int lane) {
-  const int lo = __shfl((int)x, lane, kWave), hi = __shfl((int)(x >> 32), lane, kWave);
-  return ((int64_t)hi << 32) | (uint32_t)lo;
-}
-
-// inclusive scan over the wave
-__device__ __forceinline__ int64_t wave_scan(int64_t x) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int d = 1; d < kWave; d <<= 1) {
-    const int64_t y = shfl64(x, lane - d);
-    if (lane >= d) x += y;
-  }
-  return x;
-}
-
-__device__ __forceinline__ int64_t uniform64(int64_t x) {
-  return ((int64_t)uniform((int)(x >> 32)) << 32) | (uint32_t)uniform((int)x);
 }
 
 // two numbers as fp16, half to even
@@ -201,19 +174,6 @@ __device__ __forceinline__ float halves_sum(float x) {
 
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 template <int N> struct Int { static constexpr int value = N; };
-
-// N LDS reads that feed M matrix instructions each: kAhead of them in flight
-constexpr int kAhead = 6;
-template <int N, int M>
-__device__ __forceinline__ void reads_ahead() {
-  __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
-#pragma unroll
-  for (int i = 0; i < N - kAhead; ++i) {
-    __builtin_amdgcn_sched_group_barrier(0x008, M, 0);
-    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-  }
-  __builtin_amdgcn_sched_group_barrier(0x008, kAhead * M, 0);
-}
 
 }  // namespace
 }  // namespace sphkv

@@ -101,6 +101,13 @@ __device__ __forceinline__ uint8_t recode(uint8_t c, float s, float t) {
 // 8 heads x 128 are written as int8 in 136 us and read back in 122 (626 MB each way:
 // 4.6 and 5.1 TB/s, a large copy has 4.9).
 
+template <int TYPE>
+__device__ __forceinline__ typename Elem<TYPE>::T element_of(float x) {
+  if constexpr (TYPE == kFp16) return __builtin_bit_cast(uint16_t, (_Float16)x);
+  else if constexpr (TYPE == kBf16) return __builtin_bit_cast(uint16_t, (__bf16)x);
+  else return x;
+}
+
 // |x|, or 0 where x is not finite
 __device__ __forceinline__ float finite_abs(float x) {
   x = fabsf(x);
@@ -464,6 +471,26 @@ __host__ __device__ __forceinline__ int64_t plan_bytes(int num_seqs) { return (1
 
 __device__ __forceinline__ int seq_tokens(const Cache8& c, const Cache8Batch& b, int s) {
   return clampi(b.at[s], 0, (int64_t)b.max_blocks << c.page_shift);
+}
+
+__device__ __forceinline__ int64_t shfl64(int64_t x, int lane) {
+  const int lo = __shfl((int)x, lane, kWave), hi = __shfl((int)(x >> 32), lane, kWave);
+  return ((int64_t)hi << 32) | (uint32_t)lo;
+}
+
+// inclusive scan over the wave
+__device__ __forceinline__ int64_t wave_scan(int64_t x) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1) {
+    const int64_t y = shfl64(x, lane - d);
+    if (lane >= d) x += y;
+  }
+  return x;
+}
+
+__device__ __forceinline__ int64_t uniform64(int64_t x) {
+  return ((int64_t)uniform((int)(x >> 32)) << 32) | (uint32_t)uniform((int)x);
 }
 
 // Four codes as two pairs of fp16 (exact).  int8: the byte + 128 below 1024,
@@ -916,6 +943,19 @@ __device__ __forceinline__ int k_at(int token, int chunk) {        // fp16 eleme
   return token * DH + 8 * (DH == 128 ? (chunk ^ (token & 15)) : (chunk ^ ((token >> 1) & 7)));
 }
 __device__ __forceinline__ int v_at(int d, int chunk) { return d * kTileTokens + 8 * (chunk ^ ((d >> 1) & 7)); }
+
+// N LDS reads that feed M matrix instructions each: kAhead of them in flight
+constexpr int kAhead = 6;
+template <int N, int M>
+__device__ __forceinline__ void reads_ahead() {
+  __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+#pragma unroll
+  for (int i = 0; i < N - kAhead; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, M, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(0x008, kAhead * M, 0);
+}
 
 template <int FMT, int TYPE, int DH, int TURNS>
 __global__ __launch_bounds__(DH == 128 ? 512 : 256, 2) void cache8_prefill_kernel(Cache8AttendLaunch L, int splits, float* partials) {
