@@ -11,7 +11,8 @@ namespace sphkv {
 // Rows of `bytes` consecutive bytes, one at `at` plus a multiple of each stride (in
 // bytes, of either sign) below its count.
 struct Rows {
-  int64_t at, bytes;
+  __int128 at;
+  int64_t bytes;
   int dims;
   int64_t count[3], stride[3];
 };
@@ -65,7 +66,7 @@ inline Rows positive(Rows r) {
     if (r.count[i] <= 1) continue;
     int64_t s = r.stride[i];
     if (s < 0) {
-      r.at += s * (r.count[i] - 1);
+      r.at += (__int128)s * (r.count[i] - 1);
       s = -s;
     }
     r.count[n] = r.count[i];
@@ -113,7 +114,7 @@ inline bool share(const Rows& one, const Rows& two) {
   const Rows a = positive(one), b = positive(two);
   // (a's offset + b's offset from its end back) in the interval
   Sums s;
-  __int128 off = (__int128)a.at - b.at;
+  __int128 off = a.at - b.at;
   for (int i = 0; i < a.dims; ++i) s.add(a.stride[i], a.count[i] - 1);
   for (int i = 0; i < b.dims; ++i) {
     s.add(b.stride[i], b.count[i] - 1);
