@@ -660,15 +660,15 @@ __global__ __launch_bounds__(64 * WAVES) void cache16_decode_merge_kernel(Cache1
 // four tokens by 16 dims each.
 //
 // Bound by the matrix cores' rate under load: a prompt of 8,192 tokens, 8 kv heads of
-// 4 query heads, dim 128, bf16, in 638 us, 1.29 PFLOP/s of the products below, where a
-// library product of 8192^3 reaches 1.31.  In eight waves of one step the weights would
+// 4 query heads, dim 128, bf16, in 638 to 660 us, 1.29 to 1.25 PFLOP/s of the products
+// below, where a library product of 8192^3 reaches 1.31.  In eight waves of one step the weights would
 // alternate with the products; half a step apart, the one half's weights run beside the
 // other half's products (with one product a weight 524 us when it came, 570 before).
 //
 // A weight meets its value as two 16-bit numbers, a product each: outputs show one
 // number's rounding.  (In bf16 they were 5 % further from 64 bits with one, 1.73e-3
-// relative norm for 1.65e-3, of which 1.64e-3 is their own rounding, and where values
-// cancel by 2^-9 of what cancels.  One number took 478 us for those 653.)
+// relative norm for 1.65e-3, nearly all of that their own rounding, and where values
+// cancel by 2^-9 of what cancels.  One number took 478 us for that prompt.)
 //
 // In differential attention the two maps are two groups of waves over the same
 // rows, each with its half of the dims, whose sums meet in LDS at the end.
@@ -686,8 +686,8 @@ constexpr float kNearScore = 64.f;
 // A workgroup's shape: row waves of 32 rows, and groups of them: the two maps, or,
 // where the rows of a sequence are 128 at most on average, two that take its tiles in
 // turn, so that eight waves have work.  (dim 128; 4 times 5 to 24 tokens of 4 heads on
-// 20K to 32K, fp16: 92.0 us, 132.9 without turns; 64 times 4 tokens on 2K 82.6 and 94.0;
-// at 256 rows, 4 times 64 tokens on 16K, 88.9 in turn, 85.9 without.)
+// 20K to 32K, fp16: 94.1 us, 130.7 without turns; 64 times 4 tokens on 2K 94.1 and 113.9;
+// at 256 rows, 4 times 64 tokens on 16K, 111.6 in turn, 107.3 without.)
 struct PrefillShape {
   int row_waves, groups, at_once;       // at_once: workgroups that run at the same time
   __host__ __device__ constexpr int row_shift() const { return row_waves == 8 ? 8 : 7; }
@@ -704,7 +704,7 @@ __host__ __device__ __forceinline__ int64_t row_tiles(int64_t num_rows, int num_
   return ((num_rows * gqa) >> row_shift) + num_seqs;
 }
 // Splits of each row tile: the workgroups at once over the fewest tiles that the
-// rows can make (twice as many: 98.7 us for those 92.0, 72.2 for 60.5 with 8 times 64
+// rows can make (twice as many: 100.1 us for those 94.1, 82.6 for 69.5 with 8 times 64
 // tokens on 4K).  The lengths, which the host does not know, have no part in it.
 __host__ __device__ __forceinline__ int prefill_splits(int64_t num_rows, int num_seqs, int num_kv, int gqa, PrefillShape p) {
   const int64_t whole = (num_rows * gqa) >> p.row_shift(), s = p.at_once / ((whole > num_seqs ? whole : num_seqs) * num_kv);
@@ -737,10 +737,10 @@ __device__ __forceinline__ int splits_of(int tiles, int splits) {
 // rows, length and first slot (as first_slot, one extra), and the tile's number in
 // it (none: -1 or past its rows).  A sequence's tiles come last one first, for they
 // see most; `ordered`: those of 2 to 8 sequences by the tokens that they see, so
-// that the last workgroups are short ones.  (4 prompts of 1,024 tokens 51.1 us,
-// sequence by sequence 55.4.  Where all run at once, or with 16 sequences, finding
-// the tile costs more than it gives: 8 times 64 rows on 4,096 tokens 62.1 against
-// 59.9, 16 sequences of 750 to 5,000 tokens, a window of 2,000, 128.8 against 124.7.)
+// that the last workgroups are short ones.  (4 prompts of 1,024 tokens 61.2 us,
+// sequence by sequence 68.4.  Where all run at once, or with 16 sequences, finding
+// the tile costs more than it gives: 8 times 64 rows on 4,096 tokens 73.2 against
+// 69.5, 16 sequences of 750 to 5,000 tokens, a window of 2,000, 171.9 against 168.2.)
 struct Turn { int s, first, begin, end, len, tile; };
 constexpr int kOrdered = 8;
 __device__ __forceinline__ Turn turn_of(const Cache16& c, const Cache8Batch& b, int turn, int turns, int gqa, int shift,
