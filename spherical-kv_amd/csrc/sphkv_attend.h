@@ -66,6 +66,7 @@ __device__ __forceinline__ float value_of(typename Elem<TYPE>::T x) {
   else if constexpr (TYPE == kBf16) return __builtin_bit_cast(float, (uint32_t)x << 16);
   else return x;
 }
+
 // N consecutive elements at any alignment that theirs allows
 template <class T, int N>
 struct __attribute__((packed, aligned(sizeof(T)))) Unaligned { T x[N]; };

@@ -661,9 +661,10 @@ __global__ __launch_bounds__(64 * WAVES) void cache16_decode_merge_kernel(Cache1
 //
 // Bound by the matrix cores' rate under load: a prompt of 8,192 tokens, 8 kv heads of
 // 4 query heads, dim 128, bf16, in 638 to 660 us, 1.29 to 1.25 PFLOP/s of the products
-// below, where a library product of 8192^3 reaches 1.31.  In eight waves of one step the weights would
-// alternate with the products; half a step apart, the one half's weights run beside the
-// other half's products (with one product a weight 524 us when it came, 570 before).
+// below, where a library product of 8192^3 reaches 1.31.  In eight waves of one step
+// the weights would alternate with the products; half a step apart, the one half's
+// weights run beside the other half's products (with one product a weight 524 us when
+// it came, 570 before).
 //
 // A weight meets its value as two 16-bit numbers, a product each: outputs show one
 // number's rounding.  (In bf16 they were 5 % further from 64 bits with one, 1.73e-3
@@ -1066,11 +1067,12 @@ __global__ __launch_bounds__(64 * ROW_WAVES * GROUPS, 2) void cache16_prefill_ke
   // The tile's weights, 2^kTopWeight at the reference.  Their largest is not looked
   // for where a lane's 32 add up to less than kMostSum.  Otherwise, and at a row's first
   // scores, the reference becomes the row's largest score if that one's weight passes
-  // 2^kMostWeight (both halves of a row decide alike).  Every score is
-  // a sum from zero, less the reference, so that equal ones weigh the same in any tile
-  // and at any magnitude.  The difference is part of the exponent's one multiply-add up to
-  // kNearScore, whose rounding is 2^-19 of a weight there (always apart: 661 us for that
-  // prompt's 638, differential prompts of 1,000 to 2,000 tokens 198 for 193).
+  // 2^kMostWeight (both halves of a row decide alike).  Every score is a sum from zero,
+  // less the reference, so that equal ones weigh the same in any tile and at any
+  // magnitude.  Up to exponents of kNearScore the difference is part of the exponent's
+  // one multiply-add, whose rounding is at most 2^-19 of a weight there (always apart:
+  // an 8K prompt 661 us for 638, differential prompts of 1,000 to 2,000 tokens 198 for
+  // 193).
   auto weigh = [&]() {
     float ws = 0.f;
     auto pass = [&](auto exponent) {
